@@ -21,6 +21,7 @@ _i = ctypes.c_int
 _f = ctypes.c_float
 _sz = ctypes.c_size_t
 _u64 = ctypes.c_uint64
+_ll = ctypes.c_longlong
 
 # name -> (restype, argtypes); must list every symbol include/dgnn_hip.h declares.
 SIGNATURES = {
@@ -78,6 +79,15 @@ SIGNATURES = {
     "dgnn_gat_epilogue": (_i, [_i, _i, _i, _f] + [_vp] * 4 + [_vp]),
     "dgnn_gat_epilogue_backward_workspace_bytes": (_sz, [_i, _i]),
     "dgnn_gat_epilogue_backward": (_i, [_i, _i, _i, _f] + [_vp] * 4 + [_vp, _sz, _vp]),
+    "dgnn_embedding_forward": (_i, [_i] * 5 + [_f] + [_vp] * 3 + [_vp]),
+    "dgnn_embedding_backward_workspace_bytes": (_sz, [_i, _i, _i]),
+    "dgnn_embedding_backward": (_i, [_i] * 5 + [_f] + [_vp] * 3 + [_vp, _sz, _vp]),
+    "dgnn_attn_forward": (_i, [_i] * 8 + [_f] + [_vp] * 8 + [_vp]),
+    "dgnn_attn_backward_workspace_bytes": (_sz, [_i, _i]),
+    "dgnn_attn_backward": (_i, [_i] * 8 + [_f] + [_vp] * 12 + [_vp, _sz, _vp]),
+    "dgnn_linear_ce_workspace_bytes": (_sz, [_i] * 5),
+    "dgnn_linear_ce_forward": (_i, [_i] * 5 + [_ll, _i] + [_vp] * 5 + [_vp, _sz, _vp]),
+    "dgnn_linear_ce_backward": (_i, [_i] * 5 + [_ll, _i] + [_vp] * 7 + [_vp, _sz, _vp]),
 }
 
 _lib = None

@@ -1,0 +1,120 @@
+// Packed attention: what the forward and the backward kernels share.
+#pragma once
+#include <string.h>
+
+#include "mma.hpp"
+
+namespace dgnn {
+
+struct AttnArgs {
+  const void *q, *k, *v, *out, *grad;         // grad: of the output
+  void *o, *dq, *dk, *dv;
+  float *lse;                                 // [hq, tq], natural logarithm
+  float *stat;                                // backward: [2, hq, tq] = lse log2(e) (+inf for an empty row), <grad, out>
+  const int *row_ptr, *col_ptr;
+  int nseq, tq, tk, hq, hk, g, d, causal;     // g = hq / hk
+  long long q_tok, q_head, k_tok, k_head, v_tok, v_head;   // strides in elements; o, grad, dq, dk, dv are contiguous
+  float scale;
+};
+
+// Boundaries of the segments of `total` packed rows: 0, ptr[0], ..., ptr[nseq], total.  Segment 0 and
+// segment nseq + 1 are the rows in front of the first and behind the last sequence, which belong to none.
+__device__ __forceinline__ int seg_bound(const int *__restrict__ ptr, int nseq, int total, int s) {
+  if (s <= 0) return 0;
+  if (s >= nseq + 2) return total;
+  return min(max(ptr[s - 1], 0), total);       // whatever ptr holds, no access leaves the tensors
+}
+
+struct Segment {
+  int seq;                 // sequence, or -1 / nseq for rows that belong to none
+  int start, len;          // first row and rows
+  int tile;                // which tile of the segment, in units of `rows_per_tile` rows x g
+};
+
+// Workgroup -> tile without a list of tiles: segment s owns the tile slots from
+// floor(bound(s) g / rows) + s up to the next segment's, at least as many as it has tiles (the spare
+// ones find nothing to do).  The segment of a slot is searched with 64 probes a step.
+__device__ __forceinline__ Segment find_segment(const int *__restrict__ ptr, int nseq, int total, int g, int rows,
+                                                int slot, bool last_first) {
+  int lo = 0, hi = nseq + 2;
+  const int lane = lane_id();
+  while (hi - lo > 1) {
+    const int step = (hi - lo + 63) >> 6, s = lo + lane * step;
+    const bool below = s < hi && seg_bound(ptr, nseq, total, s) * (long long)g / rows + s <= slot;
+    const int n = __popcll(__ballot(below));
+    lo += max(n - 1, 0) * step;
+    hi = min(hi, lo + step);
+  }
+  lo = uniform_i32(lo);
+  Segment r;
+  r.seq = lo - 1;
+  r.start = uniform_i32(seg_bound(ptr, nseq, total, lo));
+  const int end = uniform_i32(seg_bound(ptr, nseq, total, lo + 1));
+  r.len = max(end - r.start, 0);
+  r.tile = slot - (int)(r.start * (long long)g / rows + lo);
+  const int tiles = (int)((r.len * (long long)g + rows - 1) / rows);
+  if (r.tile < 0 || r.tile >= tiles) r.tile = -1;
+  else if (last_first) r.tile = tiles - 1 - r.tile;
+  return r;
+}
+static inline long long tile_slots(int total, int nseq, int g, int rows) {
+  return (long long)total * g / rows + nseq + 2;
+}
+// rows of a sequence in the other index (keys of a query's sequence and the other way round)
+__device__ __forceinline__ void other_side(const int *__restrict__ ptr, int nseq, int total, int seq, int *start, int *len) {
+  *start = 0;
+  *len = 0;
+  if (seq < 0 || seq >= nseq) return;
+  const int s = uniform_i32(seg_bound(ptr, nseq, total, seq + 1)), e = uniform_i32(seg_bound(ptr, nseq, total, seq + 2));
+  *start = s;
+  *len = max(e - s, 0);
+}
+
+// A query row's (or key row's) DP / 16 fragments straight from global memory; columns behind d are zeros.
+template <class T, int DP>
+__device__ __forceinline__ void load_row_frags(frag8<T> (&f)[DP / 16], const T *row, int d, int h, bool valid) {
+#pragma unroll
+  for (int s = 0; s < DP / 16; ++s) {
+    const int c = 16 * s + 8 * h;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f[s][j] = (T)0.f;
+    if constexpr (sizeof(T) == 2) {
+      if (valid && c < d) f[s] = *(const frag8<T> *)(row + c);
+    } else {
+      if (valid && c < d) {
+        const vec4<T> a = *(const vec4<T> *)(row + c);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) f[s][j] = a[j];
+      }
+      if (valid && c + 4 < d) {
+        const vec4<T> a = *(const vec4<T> *)(row + c + 4);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) f[s][4 + j] = a[j];
+      }
+    }
+  }
+}
+// The transposed result blocks of a lane's row, times `by`, to global memory (d is a multiple of four).
+template <class T, int DP>
+__device__ __forceinline__ void store_row(T *row, const acc16 (&c)[DP / 32], float by, int d, int h) {
+#pragma unroll
+  for (int b = 0; b < DP / 32; ++b)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int at = 32 * b + 8 * i + 4 * h;
+      vec4<T> v;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] = (T)(c[b][4 * i + j] * by);
+      if (at < d) *(vec4<T> *)(row + at) = v;
+    }
+}
+
+int attn_args(int dtype, int nseq, int tq, int tk, int hq, int hk, int d, int causal, float scale, const void *q,
+              const void *k, const void *v, const int *row_ptr, const int *col_ptr, const long long *strides,
+              AttnArgs *a);
+
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+#define DGNN_LOG2E 1.44269504088896340736f
+#define DGNN_LN2 0.69314718055994530942f
+
+}  // namespace dgnn

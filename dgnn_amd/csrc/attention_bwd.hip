@@ -1,0 +1,299 @@
+// Packed attention, backward (formulas of the forward: attention.hip).
+//
+//   delta_i = <do_i, o_i>,  dv_j = sum_i p_ij do_i,  ds_ij = p_ij (<do_i, v_j> - delta_i),
+//   dq_i = scale sum_j ds_ij k_j,  dk_j = scale sum_i ds_ij q_i
+//
+// p is rebuilt from the saved lse.  Two kernels, each owning its outputs, so nothing is summed through
+// atomics and results do not depend on the order of workgroups: k_attn_bwd_kv keeps 32 keys a wave
+// with dk^T and dv^T in accumulators and walks the query tiles of all heads that share the key head;
+// k_attn_bwd_q keeps 32 packed query rows a wave and walks the key tiles.  The price is forming z and
+// do v^T twice: seven products instead of five.
+#include "attention.hpp"
+
+using namespace dgnn;
+
+namespace dgnn {
+
+// stat[0] = lse log2(e), +inf where the row saw no key (p = exp2(z - inf) = 0); stat[1] = <do, o>.
+// One thread per 16-byte chunk, lanes of a row joined by shuffles.
+template <class T, int LPR>
+__global__ __launch_bounds__(DGNN_BLOCK) void k_attn_bwd_stat(long long rows, int d, int tq, int hq,
+                                                              const T *__restrict__ out, const T *__restrict__ grad,
+                                                              const float *__restrict__ lse, float *__restrict__ stat) {
+  constexpr int VEC = 16 / sizeof(T);
+  const long long r = (blockIdx.x * (long long)DGNN_BLOCK + threadIdx.x) / LPR;
+  const int c = (threadIdx.x % LPR) * VEC;
+  float sum = 0.f;
+  if (r < rows && c < d) {
+    T o[VEC], g[VEC];
+    *(u32x4 *)o = *(const u32x4 *)(out + r * d + c);
+    *(u32x4 *)g = *(const u32x4 *)(grad + r * d + c);
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) sum = fmaf((float)o[j], (float)g[j], sum);
+  }
+#pragma unroll
+  for (int w = LPR / 2; w > 0; w >>= 1) sum += __shfl_xor(sum, w, 64);
+  if (r < rows && threadIdx.x % LPR == 0) {
+    const long long tok = r / hq, head = r % hq, at = head * tq + tok;
+    const float x = lse[at];
+    stat[at] = x == -INFINITY ? INFINITY : x * DGNN_LOG2E;
+    stat[rows + at] = sum;
+  }
+}
+
+template <class T, int DP, int NW>
+__global__ __launch_bounds__(64 * NW) void k_attn_bwd_kv(const AttnArgs a) {
+  constexpr int BK = 32 * NW, BQ = 32, THREADS = 64 * NW;
+  using TL = Tile<T, DP>;
+  __shared__ __align__(16) char lds_q[2][BQ * TL::ROW_BYTES];
+  __shared__ __align__(16) char lds_g[2][BQ * TL::ROW_BYTES];
+  __shared__ __align__(16) float lds_s[2][2 * BQ];
+  const int lane = lane_id(), h = lane >> 5, wave = uniform_i32(wave_in_block());
+  const int kvh = blockIdx.x % a.hk, slot = blockIdx.x / a.hk;
+  const Segment seg = find_segment(a.col_ptr, a.nseq, a.tk, 1, BK, slot, false);
+  if (seg.tile < 0) return;
+  int qs, lq;
+  other_side(a.row_ptr, a.nseq, a.tq, seg.seq, &qs, &lq);
+  const int lk = seg.len;
+
+  const int key0 = seg.tile * BK + wave * 32, key = key0 + (lane & 31);
+  const bool valid = key < lk;
+  const long long tok = seg.start + (long long)key;
+  // first query that sees a key: query i sees key j when j <= i + lk - lq
+  const int first = a.causal ? key - (lk - lq) : 0;
+  const int wave_first = a.causal ? key0 - (lk - lq) : 0, wave_all = a.causal ? key0 + 31 - (lk - lq) : 0;
+  const int t0 = a.causal ? max(0, seg.tile * BK - (lk - lq)) / BQ : 0;
+  const int tiles = (lq + BQ - 1) / BQ, per_head = max(0, tiles - t0), total = per_head * a.g;
+
+  frag8<T> kf[DP / 16], vf[DP / 16];
+  load_row_frags<T, DP>(kf, (const T *)a.k + tok * a.k_tok + (long long)kvh * a.k_head, a.d, h, valid);
+  load_row_frags<T, DP>(vf, (const T *)a.v + tok * a.v_tok + (long long)kvh * a.v_head, a.d, h, valid);
+  const float c = a.scale * DGNN_LOG2E;
+
+  const unsigned q_stride = (unsigned)(a.q_tok * sizeof(T)), g_stride = (unsigned)((long long)a.hq * a.d * sizeof(T));
+  const unsigned row_bytes = a.d * (unsigned)sizeof(T);
+  Stager<T, DP, BQ, THREADS> st_q, st_g;
+  st_q.init(q_stride, a.d);
+  st_g.init(g_stride, a.d);
+  auto stage = [&](int u, char *qt, char *gt, float *stt) {
+    const int head = kvh * a.g + u / per_head, t = t0 + u % per_head;
+    const int n = min(BQ, lq - t * BQ);
+    const long long tq0 = qs + (long long)t * BQ;
+    st_q.load(qt, buffer_over((const T *)a.q + tq0 * a.q_tok + (long long)head * a.q_head, span_bytes(n, q_stride, row_bytes)));
+    st_g.load(gt, buffer_over((const T *)a.grad + (tq0 * a.hq + head) * a.d, span_bytes(n, g_stride, row_bytes)));
+    if (threadIdx.x < 2 * BQ) {
+      const int i = threadIdx.x % BQ;
+      const float *src = a.stat + (threadIdx.x < BQ ? 0 : (long long)a.hq * a.tq) + (long long)head * a.tq + tq0;
+      stt[threadIdx.x] = i < n ? src[i] : (threadIdx.x < BQ ? INFINITY : 0.f);     // rows behind the end: p = 0
+    }
+  };
+
+  acc16 dk[DP / 32], dv[DP / 32];
+#pragma unroll
+  for (int b = 0; b < DP / 32; ++b) dk[b] = acc_zero(), dv[b] = acc_zero();
+
+  auto work = [&](int u, const char *qt, const char *gt, const float *stt) {
+    const int q0 = (t0 + u % per_head) * BQ;
+    if (q0 + BQ - 1 < wave_first || key0 >= lk) return;
+    acc16 s = acc_zero(), dp = acc_zero();
+#pragma unroll
+    for (int i = 0; i < DP / 16; ++i) {
+      s = mma(TL::row_frag(qt, lane & 31, 16 * i + 8 * h), kf[i], s);
+      dp = mma(TL::row_frag(gt, lane & 31, 16 * i + 8 * h), vf[i], dp);
+    }
+    const bool masked = q0 < wave_all;
+#pragma unroll
+    for (int r4 = 0; r4 < 4; ++r4) {
+      const float4 lse = *(const float4 *)(stt + 8 * r4 + 4 * h);
+      const float4 dl = *(const float4 *)(stt + BQ + 8 * r4 + 4 * h);
+      const float ls[4] = {lse.x, lse.y, lse.z, lse.w}, de[4] = {dl.x, dl.y, dl.z, dl.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int r = 4 * r4 + j;
+        const bool seen = !masked || q0 + acc_row(r, h) >= first;
+        const float p = seen ? exp2_fast(fmaf(s[r], c, -ls[j])) : 0.f;
+        s[r] = p;
+        dp[r] = seen ? p * (dp[r] - de[j]) : 0.f;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const frag8<T> p = frag_of<T>(s, 8 * i), ds = frag_of<T>(dp, 8 * i);
+#pragma unroll
+      for (int b = 0; b < DP / 32; ++b) {
+        dv[b] = mma(TL::col_frag(gt, 16 * i, 32 * b, lane), p, dv[b]);
+        dk[b] = mma(TL::col_frag(qt, 16 * i, 32 * b, lane), ds, dk[b]);
+      }
+    }
+  };
+
+  if (total > 0) stage(0, lds_q[0], lds_g[0], lds_s[0]);
+  for (int u = 0; u < total; u += 2) {
+    __syncthreads();
+    if (u + 1 < total) stage(u + 1, lds_q[1], lds_g[1], lds_s[1]);
+    work(u, lds_q[0], lds_g[0], lds_s[0]);
+    if (u + 1 < total) {
+      __syncthreads();
+      if (u + 2 < total) stage(u + 2, lds_q[0], lds_g[0], lds_s[0]);
+      work(u + 1, lds_q[1], lds_g[1], lds_s[1]);
+    }
+  }
+
+  if (!valid) return;
+  const long long at = (tok * a.hk + kvh) * a.d;
+  store_row<T, DP>((T *)a.dk + at, dk, a.scale, a.d, h);
+  store_row<T, DP>((T *)a.dv + at, dv, 1.f, a.d, h);
+}
+
+template <class T, int DP, int NW>
+__global__ __launch_bounds__(64 * NW) void k_attn_bwd_q(const AttnArgs a) {
+  constexpr int BM = 32 * NW, BN = 32, THREADS = 64 * NW;
+  using TL = Tile<T, DP>;
+  __shared__ __align__(16) char lds_k[2][BN * TL::ROW_BYTES];
+  __shared__ __align__(16) char lds_v[2][BN * TL::ROW_BYTES];
+  const int lane = lane_id(), h = lane >> 5, wave = uniform_i32(wave_in_block());
+  const int kvh = blockIdx.x % a.hk, slot = blockIdx.x / a.hk;
+  const Segment seg = find_segment(a.row_ptr, a.nseq, a.tq, a.g, BM, slot, a.causal != 0);
+  if (seg.tile < 0) return;
+  int ks, lk;
+  other_side(a.col_ptr, a.nseq, a.tk, seg.seq, &ks, &lk);
+
+  const long long rows = (long long)seg.len * a.g;
+  const long long row = (long long)seg.tile * BM + wave * 32 + (lane & 31);
+  const bool valid = row < rows;
+  const int qi = (int)(row / a.g), head = kvh * a.g + (int)(row % a.g);
+  const long long tok = seg.start + (long long)qi;
+  const int limit = !valid ? -1 : a.causal ? qi + (lk - seg.len) : lk - 1;
+  const long long last_row = min(rows, (long long)(seg.tile + 1) * BM) - 1;
+  const int seen = a.causal ? max(0, min(lk, (int)(last_row / a.g) + (lk - seg.len) + 1)) : lk;
+  const int tiles = (seen + BN - 1) / BN;
+  const long long wrow = (long long)seg.tile * BM + wave * 32;
+  const int wave_all = a.causal ? (int)(min(wrow, last_row) / a.g) + (lk - seg.len) : lk - 1;
+  const int wave_any = wrow > last_row ? -1
+                       : a.causal ? (int)(min(wrow + 31, last_row) / a.g) + (lk - seg.len) : lk - 1;
+
+  frag8<T> qf[DP / 16], gf[DP / 16];
+  load_row_frags<T, DP>(qf, (const T *)a.q + tok * a.q_tok + (long long)head * a.q_head, a.d, h, valid);
+  load_row_frags<T, DP>(gf, (const T *)a.grad + (tok * a.hq + head) * a.d, a.d, h, valid);
+  const long long at = (long long)head * a.tq + tok;
+  const float lse = valid ? a.stat[at] : INFINITY, delta = valid ? a.stat[(long long)a.hq * a.tq + at] : 0.f;
+  const float c = a.scale * DGNN_LOG2E;
+
+  const unsigned k_stride = (unsigned)(a.k_tok * sizeof(T)), v_stride = (unsigned)(a.v_tok * sizeof(T));
+  const unsigned row_bytes = a.d * (unsigned)sizeof(T);
+  const T *kbase = (const T *)a.k + (long long)ks * a.k_tok + (long long)kvh * a.k_head;
+  const T *vbase = (const T *)a.v + (long long)ks * a.v_tok + (long long)kvh * a.v_head;
+  Stager<T, DP, BN, THREADS> st_k, st_v;
+  st_k.init(k_stride, a.d);
+  st_v.init(v_stride, a.d);
+  auto stage = [&](int t, char *kt, char *vt) {
+    const int n = min(BN, lk - t * BN);
+    st_k.load(kt, buffer_over(kbase + (long long)t * BN * a.k_tok, span_bytes(n, k_stride, row_bytes)));
+    st_v.load(vt, buffer_over(vbase + (long long)t * BN * a.v_tok, span_bytes(n, v_stride, row_bytes)));
+  };
+
+  acc16 dq[DP / 32];
+#pragma unroll
+  for (int b = 0; b < DP / 32; ++b) dq[b] = acc_zero();
+
+  auto work = [&](int t, const char *kt, const char *vt) {
+    if (t * BN > wave_any) return;
+    acc16 s = acc_zero(), dp = acc_zero();
+#pragma unroll
+    for (int i = 0; i < DP / 16; ++i) {
+      s = mma(TL::row_frag(kt, lane & 31, 16 * i + 8 * h), qf[i], s);
+      dp = mma(TL::row_frag(vt, lane & 31, 16 * i + 8 * h), gf[i], dp);
+    }
+    const bool masked = t * BN + BN - 1 > wave_all;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const bool on = !masked || t * BN + acc_row(r, h) <= limit;
+      const float p = exp2_fast(fmaf(s[r], c, -lse));
+      dp[r] = on ? p * (dp[r] - delta) : 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const frag8<T> ds = frag_of<T>(dp, 8 * i);
+#pragma unroll
+      for (int b = 0; b < DP / 32; ++b) dq[b] = mma(TL::col_frag(kt, 16 * i, 32 * b, lane), ds, dq[b]);
+    }
+  };
+
+  if (tiles > 0) stage(0, lds_k[0], lds_v[0]);
+  for (int t = 0; t < tiles; t += 2) {
+    __syncthreads();
+    if (t + 1 < tiles) stage(t + 1, lds_k[1], lds_v[1]);
+    work(t, lds_k[0], lds_v[0]);
+    if (t + 1 < tiles) {
+      __syncthreads();
+      if (t + 2 < tiles) stage(t + 2, lds_k[0], lds_v[0]);
+      work(t + 1, lds_k[1], lds_v[1]);
+    }
+  }
+
+  if (valid) store_row<T, DP>((T *)a.dq + (tok * a.hq + head) * a.d, dq, a.scale, a.d, h);
+}
+
+template <class T, int DP>
+static int launch_bwd(const AttnArgs &a, const float *lse, hipStream_t st) {
+  constexpr int NW = 4;
+  const long long rows = (long long)a.tq * a.hq;
+  if (rows > 0) {
+    constexpr int LPR = DP * (int)sizeof(T) / 16;
+    hipLaunchKernelGGL((k_attn_bwd_stat<T, LPR>), dim3((unsigned)((rows * LPR + DGNN_BLOCK - 1) / DGNN_BLOCK)),
+                       dim3(DGNN_BLOCK), 0, st, rows, a.d, a.tq, a.hq, (const T *)a.out, (const T *)a.grad, lse, a.stat);
+    DGNN_LAUNCH_CHECK();
+  }
+  if (a.tk > 0) {
+    const long long slots = tile_slots(a.tk, a.nseq, 1, 32 * NW) * a.hk;
+    if (slots > 0x7fffffffLL) return DGNN_ERR_UNSUPPORTED;
+    hipLaunchKernelGGL((k_attn_bwd_kv<T, DP, NW>), dim3((unsigned)slots), dim3(64 * NW), 0, st, a);
+    DGNN_LAUNCH_CHECK();
+  }
+  if (a.tq > 0) {
+    const long long slots = tile_slots(a.tq, a.nseq, a.g, 32 * NW) * a.hk;
+    if (slots > 0x7fffffffLL) return DGNN_ERR_UNSUPPORTED;
+    hipLaunchKernelGGL((k_attn_bwd_q<T, DP, NW>), dim3((unsigned)slots), dim3(64 * NW), 0, st, a);
+    DGNN_LAUNCH_CHECK();
+  }
+  return DGNN_OK;
+}
+template <class T>
+static int launch_bwd_d(const AttnArgs &a, const float *lse, hipStream_t st) {
+  if (a.d <= 32) return launch_bwd<T, 32>(a, lse, st);
+  if (a.d <= 64) return launch_bwd<T, 64>(a, lse, st);
+  return launch_bwd<T, 128>(a, lse, st);
+}
+
+}  // namespace dgnn
+
+extern "C" {
+
+size_t dgnn_attn_backward_workspace_bytes(int tq, int hq) {
+  if (tq <= 0 || hq <= 0) return 0;
+  return 2 * sizeof(float) * (size_t)tq * (size_t)hq;
+}
+
+int dgnn_attn_backward(int dtype, int nseq, int tq, int tk, int hq, int hk, int d, int causal, float scale,
+                       const void *q, const void *k, const void *v, const long long *strides, const int *row_ptr,
+                       const int *col_ptr, const void *out, const float *lse, const void *grad, void *dq, void *dk,
+                       void *dv, void *workspace, size_t workspace_bytes, void *stream) {
+  AttnArgs a;
+  const int rc = attn_args(dtype, nseq, tq, tk, hq, hk, d, causal, scale, q, k, v, row_ptr, col_ptr, strides, &a);
+  if (rc != DGNN_OK) return rc;
+  if (tq > 0 && (!out || !lse || !grad || !dq)) return DGNN_ERR_BAD_ARG;
+  if (tk > 0 && (!dk || !dv)) return DGNN_ERR_BAD_ARG;
+  for (const void *p : {out, grad, (const void *)dq, (const void *)dk, (const void *)dv})
+    if ((uintptr_t)p & 15) return DGNN_ERR_ALIGNMENT;
+  if (workspace_bytes < dgnn_attn_backward_workspace_bytes(tq, hq) || (tq > 0 && !workspace)) return DGNN_ERR_WORKSPACE;
+  if ((((uintptr_t)workspace) | ((uintptr_t)lse)) & 3) return DGNN_ERR_ALIGNMENT;
+  if ((long long)hq * d * (dtype == DGNN_F32 ? 4 : 2) >= (1LL << 31) / 128) return DGNN_ERR_UNSUPPORTED;
+  a.out = out, a.grad = grad, a.dq = dq, a.dk = dk, a.dv = dv;
+  a.stat = (float *)workspace;
+  hipStream_t st = (hipStream_t)stream;
+  if (dtype == DGNN_F32) return launch_bwd_d<float>(a, lse, st);
+  if (dtype == DGNN_BF16) return launch_bwd_d<bf16_t>(a, lse, st);
+  return launch_bwd_d<half_t>(a, lse, st);
+}
+
+}  // extern "C"

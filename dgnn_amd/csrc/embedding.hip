@@ -1,0 +1,411 @@
+// Node (token) embedding: lookup with scaling, and the gradient of the table by sorted ids.
+//
+//   out_i = scale * table[id_i],   dtable_r = scale * sum over i with id_i = r of grad_i
+//
+// An id outside [0, rows) names no row: zeros out, no gradient.  Both directions are bound by memory.
+// The gradient sorts (id, i) with a stable radix sort, eight bits a pass, so that every row of the
+// table is written exactly once, by the sum of its own run in ascending i: no atomics on floats, no
+// zeroed table, the same bits every time.  Runs longer than RUN (frequent tokens, hub nodes) are
+// summed in pieces first.
+#include "common.hpp"
+
+using namespace dgnn;
+
+namespace dgnn {
+
+typedef _Float16 half_t;
+typedef __bf16 bf16_t;
+
+// N elements of a row in one access of N * sizeof(T) bytes
+template <class T, int N>
+struct __align__(sizeof(T) * N) Pack {
+  T v[N];
+};
+
+template <class I>
+__device__ __forceinline__ int row_of_id(const I *ids, long long i, int rows) {
+  const I x = ids[i];
+  return x >= 0 && x < (I)rows ? (int)x : rows;           // rows: names none
+}
+
+// lanes = threads that share a row (a power of two up to 256)
+template <class T, int N, class I>
+__global__ __launch_bounds__(DGNN_BLOCK) void k_embed_fwd(int n, int rows, int dim, int lanes, float scale,
+                                                          const I *__restrict__ ids, const T *__restrict__ table,
+                                                          T *__restrict__ out) {
+  const int per = DGNN_BLOCK / lanes;
+  const long long i = (long long)blockIdx.x * per + threadIdx.x / lanes;
+  if (i >= n) return;
+  const int r = row_of_id(ids, i, rows);
+  for (int c = (threadIdx.x & (lanes - 1)) * N; c < dim; c += lanes * N) {
+    Pack<T, N> p;
+    if (r < rows) {
+      p = *(const Pack<T, N> *)(table + (long long)r * dim + c);
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        // a float product, then the type: left alone the compiler merges both into v_fma_mixlo_f16, whose
+        // single rounding differs from float16's table * scale in the last place now and then
+        float y = (float)p.v[j] * scale;
+        asm("" : "+v"(y));
+        p.v[j] = (T)y;
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < N; ++j) p.v[j] = (T)0.f;
+    }
+    *(Pack<T, N> *)(out + i * dim + c) = p;
+  }
+}
+
+// ------------------------------------------------------------------ stable radix sort of (row, i)
+constexpr int SORT_TILE = 4096, SORT_BINS = 256;
+static inline int sort_tiles(int n) { return (n + SORT_TILE - 1) / SORT_TILE; }
+
+template <class I>
+struct SortSrc {                       // the first pass reads the ids, later ones the previous pass's pairs
+  const I *ids;
+  const int *key, *val;
+  int rows;
+  __device__ __forceinline__ int k(int i) const { return ids ? row_of_id(ids, i, rows) : key[i]; }
+  __device__ __forceinline__ int v(int i) const { return ids ? i : val[i]; }
+};
+
+// counts[bin * tiles + tile]
+template <class I>
+__global__ __launch_bounds__(DGNN_BLOCK) void k_sort_count(int n, int shift, SortSrc<I> src, int *__restrict__ counts) {
+  __shared__ int bins[SORT_BINS];
+  bins[threadIdx.x] = 0;
+  __syncthreads();
+  const int lo = blockIdx.x * SORT_TILE, hi = min(n, lo + SORT_TILE);
+  for (int i = lo + threadIdx.x; i < hi; i += DGNN_BLOCK) atomicAdd(&bins[(src.k(i) >> shift) & (SORT_BINS - 1)], 1);
+  __syncthreads();
+  counts[(long long)threadIdx.x * gridDim.x + blockIdx.x] = bins[threadIdx.x];
+}
+
+// exclusive sums in place, one workgroup
+__global__ __launch_bounds__(1024) void k_sort_scan(int total, int *__restrict__ x) {
+  __shared__ int part[1024];
+  int carry = 0;
+  for (int base = 0; base < total; base += 4096) {
+    const int i = base + threadIdx.x * 4;
+    int v[4], s = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      v[j] = i + j < total ? x[i + j] : 0;
+      s += v[j];
+    }
+    part[threadIdx.x] = s;
+    __syncthreads();
+    for (int w = 1; w < 1024; w <<= 1) {
+      const int add = threadIdx.x >= (unsigned)w ? part[threadIdx.x - w] : 0;
+      __syncthreads();
+      part[threadIdx.x] += add;
+      __syncthreads();
+    }
+    int run = carry + part[threadIdx.x] - s;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (i + j < total) x[i + j] = run;
+      run += v[j];
+    }
+    carry += part[1023];
+    __syncthreads();
+  }
+}
+
+// Every wave owns a quarter of the tile; it counts its digits, then walks it again in order: the rank
+// of a key among the 64 of a step is the number of lower lanes with its digit.
+template <class I>
+__global__ __launch_bounds__(DGNN_BLOCK) void k_sort_scatter(int n, int shift, SortSrc<I> src,
+                                                             const int *__restrict__ offs, int *__restrict__ key,
+                                                             int *__restrict__ val) {
+  __shared__ int at[DGNN_WAVES_PER_BLOCK][SORT_BINS];
+  const int lane = lane_id(), wave = wave_in_block();
+  for (int w = 0; w < DGNN_WAVES_PER_BLOCK; ++w) at[w][threadIdx.x] = 0;
+  __syncthreads();
+  constexpr int PART = SORT_TILE / DGNN_WAVES_PER_BLOCK;
+  const int lo = blockIdx.x * SORT_TILE + wave * PART, hi = min(n, lo + PART);
+  for (int i = lo + lane; i < hi; i += DGNN_WAVE) atomicAdd(&at[wave][(src.k(i) >> shift) & (SORT_BINS - 1)], 1);
+  __syncthreads();
+  int run = offs[(long long)threadIdx.x * gridDim.x + blockIdx.x];
+  for (int w = 0; w < DGNN_WAVES_PER_BLOCK; ++w) {
+    const int c = at[w][threadIdx.x];
+    at[w][threadIdx.x] = run;
+    run += c;
+  }
+  __syncthreads();
+  for (int base = lo; base < hi; base += DGNN_WAVE) {
+    const int i = base + lane;
+    const bool on = i < hi;
+    const int k = on ? src.k(i) : 0, digit = (k >> shift) & (SORT_BINS - 1);
+    unsigned long long same = __ballot(on);
+#pragma unroll
+    for (int b = 0; b < 8; ++b) {
+      const unsigned long long set = __ballot((digit >> b) & 1);
+      same &= (digit >> b) & 1 ? set : ~set;
+    }
+    const int rank = __popcll(same & ((1ULL << lane) - 1)), count = __popcll(same);
+    const int to = on ? at[wave][digit] + rank : 0;
+    wave_lds_sync();
+    if (on && rank == 0) at[wave][digit] += count;
+    wave_lds_sync();
+    if (on) {
+      key[to] = k;
+      val[to] = src.v(i);
+    }
+  }
+}
+
+// ------------------------------------------------------------------ sums of the runs
+__device__ __forceinline__ int first_not_below(const int *__restrict__ key, int n, int k) {
+  int lo = 0, hi = n;
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (key[mid] < k) lo = mid + 1; else hi = mid;
+  }
+  return lo;
+}
+
+// Sorted positions are cut into pieces of `run`.  A row whose run is longer than that gets one partial
+// sum per piece it touches: slot 2 p when its run holds the first position of piece p, slot 2 p + 1
+// when it begins inside (a piece holds the beginning of at most one such run).
+template <class T, int N>
+__global__ __launch_bounds__(DGNN_BLOCK) void k_embed_long(int n, int rows, int dim, int run,
+                                                           const int *__restrict__ key, const int *__restrict__ val,
+                                                           const T *__restrict__ grad, float *__restrict__ part) {
+  __shared__ float sums[DGNN_WAVES_PER_BLOCK][DGNN_WAVE * N];
+  const int lane = lane_id(), wave = wave_in_block();
+  const int lo = blockIdx.x * run, hi = min(n, lo + run);
+  const int c = (blockIdx.y * DGNN_WAVE + lane) * N;
+  const int ends[2] = {key[lo], key[hi - 1]};
+  for (int which = 0; which < 2; ++which) {
+    const int k = ends[which];
+    if (k >= rows || (which == 1 && k == ends[0])) continue;
+    const int s = first_not_below(key, n, k), e = first_not_below(key, n, k + 1);
+    if (e - s <= run) continue;
+    const int a = max(s, lo), b = min(e, hi);
+    float acc[N];
+#pragma unroll
+    for (int j = 0; j < N; ++j) acc[j] = 0.f;
+    if (c < dim) {
+#pragma unroll 4
+      for (int i = a + wave; i < b; i += DGNN_WAVES_PER_BLOCK) {
+        const Pack<T, N> p = *(const Pack<T, N> *)(grad + (long long)val[i] * dim + c);
+#pragma unroll
+        for (int j = 0; j < N; ++j) acc[j] += (float)p.v[j];
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < N; ++j) sums[wave][lane * N + j] = acc[j];
+    __syncthreads();
+    if (wave == 0 && c < dim)
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        float t = 0.f;
+        for (int w = 0; w < DGNN_WAVES_PER_BLOCK; ++w) t += sums[w][lane * N + j];
+        part[((long long)(2 * blockIdx.x + (s < lo || s == lo ? 0 : 1))) * dim + c + j] = t;
+      }
+    __syncthreads();
+  }
+}
+
+constexpr int EMBED_ROWS = 64;       // rows of the table a workgroup writes
+
+template <class T, int N>
+__global__ __launch_bounds__(DGNN_BLOCK) void k_embed_rows(int n, int rows, int dim, int lanes, int run, float scale,
+                                                           const int *__restrict__ key, const int *__restrict__ val,
+                                                           const T *__restrict__ grad, const float *__restrict__ part,
+                                                           T *__restrict__ out) {
+  __shared__ int start[EMBED_ROWS + 1];
+  const int row0 = blockIdx.x * EMBED_ROWS;
+  if (threadIdx.x <= EMBED_ROWS) start[threadIdx.x] = first_not_below(key, n, (int)min((long long)rows, row0 + (long long)threadIdx.x));
+  __syncthreads();
+  const int per = DGNN_BLOCK / lanes, group = threadIdx.x / lanes, lane = threadIdx.x & (lanes - 1);
+  for (int rr = group; rr < EMBED_ROWS && row0 + rr < rows; rr += per) {
+    const int s = start[rr], e = start[rr + 1];
+    T *to = out + (long long)(row0 + rr) * dim;
+    for (int c = lane * N; c < dim; c += lanes * N) {
+      float acc[N];
+#pragma unroll
+      for (int j = 0; j < N; ++j) acc[j] = 0.f;
+      if (e - s <= run) {
+#pragma unroll 4
+        for (int i = s; i < e; ++i) {
+          const Pack<T, N> p = *(const Pack<T, N> *)(grad + (long long)val[i] * dim + c);
+#pragma unroll
+          for (int j = 0; j < N; ++j) acc[j] += (float)p.v[j];
+        }
+      } else {
+        const int p0 = s / run, p1 = (e - 1) / run;
+#pragma unroll 4
+        for (int p = p0; p <= p1; ++p) {
+          const float *src = part + (long long)(2 * p + (p == p0 && s != p * run ? 1 : 0)) * dim + c;
+#pragma unroll
+          for (int j = 0; j < N; ++j) acc[j] += src[j];
+        }
+      }
+      Pack<T, N> p;
+#pragma unroll
+      for (int j = 0; j < N; ++j) p.v[j] = (T)(acc[j] * scale);
+      *(Pack<T, N> *)(to + c) = p;
+    }
+  }
+}
+
+// pieces of about sqrt(n): a run of all n ids is summed in two balanced steps
+static inline int embed_run(int n) {
+  int r = 64;
+  while ((long long)r * r < n) r <<= 1;
+  return r;
+}
+static inline size_t align256(size_t x) { return (x + 255) / 256 * 256; }
+struct EmbedPlan {
+  int passes, run, pieces;
+  size_t pairs, counts, part, total;      // bytes
+};
+static EmbedPlan embed_plan(int n, int rows, int dim) {
+  EmbedPlan p;
+  int bits = 1;
+  while ((1LL << bits) <= (long long)rows) ++bits;           // keys 0 .. rows
+  p.passes = (bits + 7) / 8;
+  p.run = embed_run(n);
+  p.pieces = (n + p.run - 1) / p.run;
+  p.pairs = align256(sizeof(int) * (size_t)n);
+  p.counts = align256(sizeof(int) * (size_t)SORT_BINS * sort_tiles(n));
+  p.part = align256(sizeof(float) * 2 * (size_t)p.pieces * dim);
+  p.total = 4 * p.pairs + p.counts + p.part;
+  return p;
+}
+
+// widest access every row's bytes and all pointers allow: 16, 8, 4 or 2 bytes
+static int access_bytes(int dim, int size, const void *a, const void *b) {
+  const uintptr_t x = (uintptr_t)a | (uintptr_t)b | (uintptr_t)((size_t)dim * size);
+  for (int w = 16; w > size; w >>= 1)
+    if (x % w == 0) return w;
+  return size;
+}
+static int row_lanes(int dim, int per) {
+  int l = 1;
+  while (l < DGNN_BLOCK && l * per < dim) l <<= 1;
+  return l;
+}
+
+template <class T, int N, class I>
+static int launch_embed_fwd(int n, int rows, int dim, float scale, const void *ids, const void *table, void *out,
+                            hipStream_t st) {
+  const int lanes = row_lanes(dim, N), per = DGNN_BLOCK / lanes;
+  hipLaunchKernelGGL((k_embed_fwd<T, N, I>), dim3((unsigned)((n + (long long)per - 1) / per)), dim3(DGNN_BLOCK), 0, st, n, rows,
+                     dim, lanes, scale, (const I *)ids, (const T *)table, (T *)out);
+  DGNN_LAUNCH_CHECK();
+  return DGNN_OK;
+}
+template <class T, int N>
+static int launch_embed_sums(int n, int rows, int dim, float scale, const EmbedPlan &p, const int *key, const int *val,
+                             const void *grad, float *part, void *out, hipStream_t st) {
+  if (n > p.run) {
+    hipLaunchKernelGGL((k_embed_long<T, N>), dim3((unsigned)p.pieces, (unsigned)((dim + DGNN_WAVE * N - 1) / (DGNN_WAVE * N))),
+                       dim3(DGNN_BLOCK), 0, st, n, rows, dim, p.run, key, val, (const T *)grad, part);
+    DGNN_LAUNCH_CHECK();
+  }
+  hipLaunchKernelGGL((k_embed_rows<T, N>), dim3((unsigned)((rows + (long long)EMBED_ROWS - 1) / EMBED_ROWS)), dim3(DGNN_BLOCK), 0, st, n,
+                     rows, dim, row_lanes(dim, N), p.run, scale, key, val, (const T *)grad, part, (T *)out);
+  DGNN_LAUNCH_CHECK();
+  return DGNN_OK;
+}
+template <class I>
+static int sort_ids(int n, int rows, const void *ids, const EmbedPlan &p, char *ws, const int **key, const int **val,
+                    hipStream_t st) {
+  int *k[2] = {(int *)ws, (int *)(ws + p.pairs)}, *v[2] = {(int *)(ws + 2 * p.pairs), (int *)(ws + 3 * p.pairs)};
+  int *counts = (int *)(ws + 4 * p.pairs);
+  const int tiles = sort_tiles(n);
+  for (int i = 0; i < p.passes; ++i) {
+    const SortSrc<I> src = {i == 0 ? (const I *)ids : nullptr, k[(i + 1) & 1], v[(i + 1) & 1], rows};
+    hipLaunchKernelGGL(k_sort_count<I>, dim3(tiles), dim3(DGNN_BLOCK), 0, st, n, 8 * i, src, counts);
+    DGNN_LAUNCH_CHECK();
+    hipLaunchKernelGGL(k_sort_scan, dim3(1), dim3(1024), 0, st, SORT_BINS * tiles, counts);
+    DGNN_LAUNCH_CHECK();
+    hipLaunchKernelGGL(k_sort_scatter<I>, dim3(tiles), dim3(DGNN_BLOCK), 0, st, n, 8 * i, src, (const int *)counts,
+                       k[i & 1], v[i & 1]);
+    DGNN_LAUNCH_CHECK();
+  }
+  *key = k[(p.passes - 1) & 1];
+  *val = v[(p.passes - 1) & 1];
+  return DGNN_OK;
+}
+
+static int embed_check(int dtype, int idx_bytes, int n, int rows, int dim) {
+  if (dtype < 0 || dtype > 2 || (idx_bytes != 4 && idx_bytes != 8) || n < 0 || rows < 0 || dim < 0) return DGNN_ERR_BAD_ARG;
+  return DGNN_OK;
+}
+static bool aligned_to(const void *p, int bytes) { return (uintptr_t)p % bytes == 0; }
+
+}  // namespace dgnn
+
+// one call per element type and access width: EXPR may use T (the element) and N (elements an access)
+#define DGNN_EMBED_DISPATCH(dtype, bytes, EXPR)                                   \
+  do {                                                                            \
+    if ((dtype) == DGNN_F32) {                                                    \
+      typedef float T;                                                            \
+      if ((bytes) == 16) { constexpr int N = 4; return EXPR; }                    \
+      if ((bytes) == 8) { constexpr int N = 2; return EXPR; }                     \
+      { constexpr int N = 1; return EXPR; }                                       \
+    }                                                                             \
+    if ((dtype) == DGNN_BF16) {                                                   \
+      typedef bf16_t T;                                                           \
+      if ((bytes) == 16) { constexpr int N = 8; return EXPR; }                    \
+      if ((bytes) >= 4) { constexpr int N = 2; return EXPR; }                     \
+      { constexpr int N = 1; return EXPR; }                                       \
+    }                                                                             \
+    typedef half_t T;                                                             \
+    if ((bytes) == 16) { constexpr int N = 8; return EXPR; }                      \
+    if ((bytes) >= 4) { constexpr int N = 2; return EXPR; }                       \
+    { constexpr int N = 1; return EXPR; }                                         \
+  } while (0)
+
+extern "C" {
+
+int dgnn_embedding_forward(int dtype, int idx_bytes, int n, int rows, int dim, float scale, const void *ids,
+                           const void *table, void *out, void *stream) {
+  const int rc = embed_check(dtype, idx_bytes, n, rows, dim);
+  if (rc != DGNN_OK) return rc;
+  if (n == 0 || dim == 0) return DGNN_OK;
+  if (!ids || !out || (rows > 0 && !table)) return DGNN_ERR_BAD_ARG;
+  const int size = dtype == DGNN_F32 ? 4 : 2;
+  if (!aligned_to(ids, idx_bytes) || !aligned_to(table, size) || !aligned_to(out, size)) return DGNN_ERR_ALIGNMENT;
+  const int bytes = access_bytes(dim, size, table, out);
+  hipStream_t st = (hipStream_t)stream;
+  if (idx_bytes == 8)
+    DGNN_EMBED_DISPATCH(dtype, bytes, (launch_embed_fwd<T, N, long long>(n, rows, dim, scale, ids, table, out, st)));
+  DGNN_EMBED_DISPATCH(dtype, bytes, (launch_embed_fwd<T, N, int>(n, rows, dim, scale, ids, table, out, st)));
+}
+
+size_t dgnn_embedding_backward_workspace_bytes(int n, int rows, int dim) {
+  if (n <= 0 || rows <= 0 || dim <= 0) return 0;
+  return embed_plan(n, rows, dim).total;
+}
+
+int dgnn_embedding_backward(int dtype, int idx_bytes, int n, int rows, int dim, float scale, const void *ids,
+                            const void *grad, void *grad_table, void *workspace, size_t workspace_bytes, void *stream) {
+  int rc = embed_check(dtype, idx_bytes, n, rows, dim);
+  if (rc != DGNN_OK) return rc;
+  if (rows == 0 || dim == 0) return DGNN_OK;
+  if (!grad_table || (n > 0 && (!ids || !grad))) return DGNN_ERR_BAD_ARG;
+  const int size = dtype == DGNN_F32 ? 4 : 2;
+  if (!aligned_to(ids, idx_bytes) || !aligned_to(grad, size) || !aligned_to(grad_table, size)) return DGNN_ERR_ALIGNMENT;
+  const EmbedPlan p = embed_plan(n > 0 ? n : 1, rows, dim);
+  if (n > 0 && (!workspace || workspace_bytes < p.total)) return DGNN_ERR_WORKSPACE;
+  if (n > 0 && !aligned_to(workspace, 16)) return DGNN_ERR_ALIGNMENT;
+  hipStream_t st = (hipStream_t)stream;
+  const int *key = nullptr, *val = nullptr;
+  float *part = nullptr;
+  if (n > 0) {
+    rc = idx_bytes == 8 ? sort_ids<long long>(n, rows, ids, p, (char *)workspace, &key, &val, st)
+                        : sort_ids<int>(n, rows, ids, p, (char *)workspace, &key, &val, st);
+    if (rc != DGNN_OK) return rc;
+    part = (float *)((char *)workspace + 4 * p.pairs + p.counts);
+  }
+  const int bytes = access_bytes(dim, size, grad, grad_table);
+  DGNN_EMBED_DISPATCH(dtype, bytes, (launch_embed_sums<T, N>(n, rows, dim, scale, p, key, val, grad, part, grad_table, st)));
+}
+
+}  // extern "C"

@@ -1,0 +1,154 @@
+// Matrix-core building blocks of the dense operators (attention.hip, attention_bwd.hip, linear_ce.hip).
+//
+// Everything is built from one product, C[32 x 32] += A[32 x 16] B[16 x 32], on 64 lanes.  Lane l
+// holds eight elements of A's row l % 32 and eight of B's column l % 32, those of k-half l / 32; the
+// result puts column l % 32 of C into lane l, rows 8 (r / 4) + 4 (l / 32) + r % 4 for r = 0 .. 15.
+// For 16-bit types that is one v_mfma_f32_32x32x16; for float it is eight v_mfma_f32_32x32x2, where
+// element j of both operands feeds product j.  Which k an element stands for does not matter
+// as long as A and B agree, so the rows a lane holds of one product are, unmoved, the k elements of
+// its column in the next: element j of half h stands for k = 8 (j / 4) + 4 h + j % 4 there.
+#pragma once
+#include "common.hpp"
+
+namespace dgnn {
+
+typedef _Float16 half_t;
+typedef __bf16 bf16_t;
+typedef float acc16 __attribute__((ext_vector_type(16)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+
+template <class T> struct frag8_of;
+template <> struct frag8_of<bf16_t> { typedef bf16_t type __attribute__((ext_vector_type(8))); };
+template <> struct frag8_of<half_t> { typedef half_t type __attribute__((ext_vector_type(8))); };
+template <> struct frag8_of<float> { typedef float type __attribute__((ext_vector_type(8))); };
+template <class T> using frag8 = typename frag8_of<T>::type;
+template <class T> struct vec4_of;
+template <> struct vec4_of<bf16_t> { typedef bf16_t type __attribute__((ext_vector_type(4))); };
+template <> struct vec4_of<half_t> { typedef half_t type __attribute__((ext_vector_type(4))); };
+template <> struct vec4_of<float> { typedef float type __attribute__((ext_vector_type(4))); };
+template <class T> using vec4 = typename vec4_of<T>::type;
+
+__device__ __forceinline__ acc16 mma(frag8<bf16_t> a, frag8<bf16_t> b, acc16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ acc16 mma(frag8<half_t> a, frag8<half_t> b, acc16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ acc16 mma(frag8<float> a, frag8<float> b, acc16 c) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[j], b[j], c, 0, 0, 0);
+  return c;
+}
+__device__ __forceinline__ acc16 acc_zero() {
+  acc16 c;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) c[r] = 0.f;
+  return c;
+}
+// row of C that element r of the lane half `h` holds
+__device__ __forceinline__ int acc_row(int r, int h) { return 8 * (r >> 2) + 4 * h + (r & 3); }
+
+// eight consecutive result rows-of-a-lane as the k elements of the next product (round to nearest even)
+template <class T>
+__device__ __forceinline__ frag8<T> frag_of(const acc16 &c, int first) {
+  frag8<T> f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) f[j] = (T)c[first + j];
+  return f;
+}
+
+// ------------------------------------------------------------------ global -> LDS tiles
+// A tile is ROWS rows of COLS elements, row major, its 16-byte chunks permuted inside each row by
+// chunk ^ swizzle(row): sixteen consecutive rows then put the same chunk into different banks (the
+// row reads), and four consecutive rows the same pair of chunks (the transposing reads).
+template <class T, int COLS>
+struct Tile {
+  static constexpr int CHUNK = 16 / (int)sizeof(T);          // elements of a 16-byte chunk
+  static constexpr int CPR = COLS / CHUNK;                   // chunks of a row
+  static constexpr int ROW_BYTES = COLS * (int)sizeof(T);
+  static_assert(CPR == 4 || CPR == 8 || CPR >= 16, "rows of at least four chunks");
+  __device__ static __forceinline__ int swizzle(int row) {
+    if (CPR >= 16) return ((row & 7) << 1) | ((row >> 3) & 1);
+    if (CPR == 8) return (((row >> 1) & 3) << 1) | ((row >> 3) & 1);
+    return (((row >> 2) & 1) << 1) | ((row >> 3) & 1);
+  }
+  __device__ static __forceinline__ int chunk_addr(int row, int chunk) {
+    return row * ROW_BYTES + ((chunk ^ swizzle(row)) << 4);
+  }
+  // eight consecutive elements (a lane's k elements of a product that sums over the columns)
+  __device__ static __forceinline__ frag8<T> row_frag(const char *tile, int row, int k0) {
+    if constexpr (sizeof(T) == 2) {
+      return *(const frag8<T> *)(tile + chunk_addr(row, k0 / 8));
+    } else {
+      const vec4<T> a = *(const vec4<T> *)(tile + chunk_addr(row, k0 / 4));
+      const vec4<T> b = *(const vec4<T> *)(tile + chunk_addr(row, k0 / 4 + 1));
+      return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+  }
+  // a lane's k elements of a product that sums over the rows, for column col0 + lane % 32: rows
+  // row0 + 8 (j / 4) + 4 (lane / 32) + j % 4.  16-bit: ds_read_b64_tr_b16 hands each lane of a group of
+  // sixteen one column of a 4 x 16 block, lane i supplying the address of row i / 4, columns 4 (i % 4) ..
+  __device__ static __forceinline__ frag8<T> col_frag(const char *tile, int row0, int col0, int lane) {
+    const int h = lane >> 5;
+    if constexpr (sizeof(T) == 2) {
+      typedef __attribute__((address_space(3))) s16x4 *lds_p;
+      const int row = row0 + 4 * h + ((lane & 15) >> 2), chunk = col0 / 8 + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+      const char *p0 = tile + chunk_addr(row, chunk) + (lane & 1) * 8;
+      const char *p1 = tile + chunk_addr(row + 8, chunk) + (lane & 1) * 8;
+      union { s16x4 s[2]; frag8<T> f; } u;
+      u.s[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p)p0);
+      u.s[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p)p1);
+      return u.f;
+    } else {
+      const int col = col0 + (lane & 31);
+      frag8<T> f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        f[j] = *(const T *)(tile + chunk_addr(row0 + acc_row(j, h), col / 4) + (col & 3) * 4);
+      return f;
+    }
+  }
+};
+
+// 128-bit buffer descriptor over `bytes` bytes at p: reads behind them give zeros.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_over(const void *p, unsigned bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc((void *)p, 0, (int)bytes, 0x00020000);
+}
+#define DGNN_OOB 0x80000000u                       // an offset behind every descriptor used here
+
+// Stages ROWS x COLS elements into a tile with direct loads to LDS (16 bytes a lane, no registers).  A
+// wave's load fills 1024 consecutive bytes of LDS, so the permutation is applied to the address each
+// lane reads.  Offsets are relative to the tile's first row and the same for every tile of a
+// matrix; `bytes` of the descriptor ends with the last valid row, `cols` (elements) with the last
+// valid column: what lies behind either arrives as zeros.
+template <class T, int COLS, int ROWS, int THREADS>
+struct Stager {
+  using TL = Tile<T, COLS>;
+  static constexpr int LOADS = (ROWS * TL::CPR + THREADS - 1) / THREADS;
+  static_assert(ROWS * TL::CPR % 64 == 0, "whole waves");
+  unsigned off[LOADS];
+  __device__ __forceinline__ void init(unsigned row_stride_bytes, int cols) {
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      const int c = i * THREADS + threadIdx.x, row = c / TL::CPR, chunk = (c % TL::CPR) ^ TL::swizzle(row);
+      off[i] = chunk * TL::CHUNK < cols ? row * row_stride_bytes + chunk * 16u : DGNN_OOB;
+    }
+  }
+  __device__ __forceinline__ void load(char *tile, __amdgpu_buffer_rsrc_t src) const {
+    typedef __attribute__((address_space(3))) void *lds_p;
+    const int wave = uniform_i32(threadIdx.x >> 6);
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i)
+      if (ROWS * TL::CPR % THREADS == 0 || i * THREADS + wave * 64 < ROWS * TL::CPR)
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(src, (lds_p)(tile + (i * THREADS + wave * 64) * 16), 16, (int)off[i], 0, 0, 0);
+  }
+};
+
+// bytes a descriptor over `rows` rows spans (0 rows: nothing is readable)
+__device__ __forceinline__ unsigned span_bytes(int rows, unsigned row_stride_bytes, unsigned row_bytes) {
+  return rows > 0 ? (unsigned)(rows - 1) * row_stride_bytes + row_bytes : 0u;
+}
+
+}  // namespace dgnn

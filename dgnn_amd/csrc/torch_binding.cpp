@@ -945,6 +945,214 @@ std::tuple<Tensor, py::object> epilogue_backward(const Tensor &out, const Tensor
   return std::make_tuple(grad_pre, want_bias ? py::cast(grad_bias) : py::object(py::none()));
 }
 
+// ================================================================== sequence operators
+// float32, bfloat16 or float16 -> the element type of the C ABI
+int dense_type(const Tensor &t, const char *name) {
+  if (!t.defined() || !t.is_cuda()) fail(name, " must be a GPU tensor (dgnn_amd has no CPU path)");
+  switch (t.scalar_type()) {
+    case at::kFloat: return DGNN_F32;
+    case at::kBFloat16: return DGNN_BF16;
+    case at::kHalf: return DGNN_F16;
+    default: fail(name, " must be float32, bfloat16 or float16, got ", t.scalar_type());
+  }
+}
+// another tensor of the same call: same type, same device
+const Tensor &like(const Tensor &t, const Tensor &ref, const char *name, const char *ref_name) {
+  dense_type(t, name);
+  if (t.scalar_type() != ref.scalar_type() || t.device() != ref.device())
+    fail(name, " must have ", ref_name, "'s type and device (", ref.scalar_type(), " on ", ref.device(), "), got ",
+         t.scalar_type(), " on ", t.device());
+  return t;
+}
+int index_bytes(const Tensor &t, const Tensor &ref, const char *name) {
+  if (!t.defined() || t.device() != ref.device()) fail(name, " must be on ", ref.device());
+  if (t.scalar_type() != at::kInt && t.scalar_type() != at::kLong) fail(name, " must be int32 or int64, got ", t.scalar_type());
+  if (!t.is_contiguous()) fail(name, " must be contiguous");
+  return t.scalar_type() == at::kInt ? 4 : 8;
+}
+const Tensor &contiguous(const Tensor &t, const char *name) {
+  if (!t.is_contiguous()) fail(name, " must be contiguous");
+  return t;
+}
+const void *cv(const Tensor &t) { return ptr<const void>(t); }
+void *vo(const Tensor &t) { return ptr<void>(t); }
+
+// -> out [*ids.shape, dim]
+Tensor embedding_forward(const Tensor &ids, const Tensor &table, double scale) {
+  const int dtype = dense_type(table, "table"), ib = index_bytes(ids, table, "ids");
+  if (table.dim() != 2) fail("table must be [rows, dim], got shape ", table.sizes());
+  contiguous(table, "table");
+  std::vector<int64_t> sizes = ids.sizes().vec();
+  sizes.push_back(table.size(1));
+  c10::DeviceGuard guard(table.device());
+  Tensor out = at::empty(sizes, table.options());
+  check_rc(API(dgnn_embedding_forward)(dtype, ib, as_int(ids.numel(), "ids"), as_int(table.size(0), "table rows"),
+                                       as_int(table.size(1), "table dim"), (float)scale, cv(ids), cv(table), vo(out),
+                                       stream_of(table)),
+           "dgnn_embedding_forward");
+  return out;
+}
+
+// -> grad_table [rows, dim]
+Tensor embedding_backward(const Tensor &ids, const Tensor &grad_out, int64_t rows, double scale) {
+  const int dtype = dense_type(grad_out, "grad_out"), ib = index_bytes(ids, grad_out, "ids");
+  contiguous(grad_out, "grad_out");
+  if (grad_out.dim() != ids.dim() + 1 || grad_out.sizes().slice(0, ids.dim()) != ids.sizes())
+    fail("grad_out must be [*ids.shape, dim], got ", grad_out.sizes(), " for ids of shape ", ids.sizes());
+  const int n = as_int(ids.numel(), "ids"), r = as_int(rows, "table rows"), dim = as_int(grad_out.size(-1), "table dim");
+  c10::DeviceGuard guard(grad_out.device());
+  Tensor out = at::empty({rows, dim}, grad_out.options());
+  const size_t nb = API(dgnn_embedding_backward_workspace_bytes)(n, r, dim);
+  Tensor ws = workspace(nb, grad_out);
+  check_rc(API(dgnn_embedding_backward)(dtype, ib, n, r, dim, (float)scale, cv(ids), cv(grad_out), vo(out), vo(ws), nb,
+                                        stream_of(grad_out)),
+           "dgnn_embedding_backward");
+  return out;
+}
+
+// The tensors of an attention call in the form the kernels read: rows of whole, aligned 16-byte chunks.
+// Anything else (odd head widths, a last dimension with a stride, expanded tensors) is copied once.
+struct AttnCall {
+  Tensor q, k, v;
+  long long strides[6];
+  int dtype, nseq, tq, tk, hq, hk, d, width;       // width: d rounded up to whole chunks
+};
+bool rows_readable(const Tensor &t, int64_t vec) {
+  if (t.numel() == 0) return true;
+  if (t.size(2) % vec != 0 || t.stride(2) != 1 || (uintptr_t)t.data_ptr() % 16 != 0) return false;
+  const int64_t tok = t.size(0) > 1 ? t.stride(0) : t.size(2), head = t.size(1) > 1 ? t.stride(1) : 0;
+  if (tok < t.size(2) || tok % vec != 0 || head % vec != 0) return false;
+  return tok * (int64_t)t.element_size() < ((int64_t)1 << 31) / 128;
+}
+Tensor padded(const Tensor &t, int64_t width) {
+  if (t.size(2) == width) return t.clone(at::MemoryFormat::Contiguous);
+  Tensor out = at::zeros({t.size(0), t.size(1), width}, t.options());
+  out.narrow(2, 0, t.size(2)).copy_(t);
+  return out;
+}
+AttnCall attn_call(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &row_ptr, const Tensor &col_ptr) {
+  AttnCall c;
+  c.dtype = dense_type(q, "q");
+  like(k, q, "k", "q"), like(v, q, "v", "q");
+  if (q.dim() != 3 || k.dim() != 3) fail("q must be [rows, heads, dim] and k [keys, key heads, dim], got ", q.sizes(), " and ", k.sizes());
+  if (v.sizes() != k.sizes()) fail("v must have k's shape ", k.sizes(), ", got ", v.sizes());
+  if (q.size(2) != k.size(2)) fail("q and k disagree on the head dim: ", q.size(2), " and ", k.size(2));
+  if (k.size(1) < 1 || q.size(1) < 1 || q.size(1) % k.size(1) != 0)
+    fail("the key heads (", k.size(1), ") must divide the query heads (", q.size(1), ")");
+  i32(row_ptr, "row_ptr"), i32(col_ptr, "col_ptr");
+  if (row_ptr.device() != q.device() || col_ptr.device() != q.device()) fail("row_ptr and col_ptr must be on ", q.device());
+  if (row_ptr.size(0) < 1 || row_ptr.size(0) != col_ptr.size(0))
+    fail("row_ptr and col_ptr must hold sequences + 1 offsets each, got ", row_ptr.size(0), " and ", col_ptr.size(0));
+  if (q.size(2) < 1 || q.size(2) > 128) fail("head dims of 1 to 128 are supported, got ", q.size(2));
+  c.nseq = as_int(row_ptr.size(0) - 1, "sequences");
+  c.tq = as_int(q.size(0), "rows"), c.tk = as_int(k.size(0), "keys");
+  c.hq = as_int(q.size(1), "heads"), c.hk = as_int(k.size(1), "key heads");
+  const int vec = 16 / (int)q.element_size();
+  c.width = ((int)q.size(2) + vec - 1) / vec * vec;
+  c.d = c.width;
+  const Tensor *in[3] = {&q, &k, &v};
+  Tensor *to[3] = {&c.q, &c.k, &c.v};
+  for (int i = 0; i < 3; ++i) {
+    *to[i] = rows_readable(*in[i], vec) ? *in[i] : padded(*in[i], c.width);
+    c.strides[2 * i] = to[i]->stride(0), c.strides[2 * i + 1] = to[i]->stride(1);
+  }
+  return c;
+}
+Tensor cut(const Tensor &t, int64_t d) { return t.size(2) == d ? t : t.narrow(2, 0, d).contiguous(); }
+
+// -> (out [rows, heads, dim], lse [heads, rows])
+std::tuple<Tensor, Tensor> attention_forward(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &row_ptr,
+                                             const Tensor &col_ptr, double scale, bool causal) {
+  c10::DeviceGuard guard(q.device());
+  const AttnCall c = attn_call(q, k, v, row_ptr, col_ptr);
+  Tensor out = at::empty({c.tq, c.hq, c.width}, q.options()), lse = new_f32({c.hq, c.tq}, q);
+  check_rc(API(dgnn_attn_forward)(c.dtype, c.nseq, c.tq, c.tk, c.hq, c.hk, c.d, causal, (float)scale, cv(c.q), cv(c.k),
+                                  cv(c.v), c.strides, ip(row_ptr), ip(col_ptr), vo(out), fo(lse), stream_of(q)),
+           "dgnn_attn_forward");
+  return std::make_tuple(cut(out, q.size(2)), lse);
+}
+
+// -> (dq, dk, dv)
+std::tuple<Tensor, Tensor, Tensor> attention_backward(const Tensor &q, const Tensor &k, const Tensor &v,
+                                                      const Tensor &row_ptr, const Tensor &col_ptr, double scale,
+                                                      bool causal, const Tensor &out, const Tensor &lse,
+                                                      const Tensor &grad) {
+  c10::DeviceGuard guard(q.device());
+  const AttnCall c = attn_call(q, k, v, row_ptr, col_ptr);
+  like(out, q, "out", "q"), like(grad, q, "grad", "q"), f32(lse, "lse", 2);
+  if (out.sizes() != q.sizes() || grad.sizes() != q.sizes()) fail("out and grad must have q's shape ", q.sizes());
+  if (lse.size(0) != c.hq || lse.size(1) != c.tq || lse.device() != q.device()) fail("lse must be the forward's [heads, rows]");
+  const int64_t d = q.size(2);
+  auto dense = [&](const Tensor &t) {
+    return d == c.width && t.is_contiguous() && (uintptr_t)t.data_ptr() % 16 == 0 ? t : padded(t, c.width);
+  };
+  const Tensor o = dense(out), g = dense(grad);
+  Tensor dq = at::empty({c.tq, c.hq, c.width}, q.options()), dk = at::empty({c.tk, c.hk, c.width}, q.options()),
+         dv = at::empty({c.tk, c.hk, c.width}, q.options());
+  const size_t nb = API(dgnn_attn_backward_workspace_bytes)(c.tq, c.hq);
+  Tensor ws = workspace(nb, q);
+  check_rc(API(dgnn_attn_backward)(c.dtype, c.nseq, c.tq, c.tk, c.hq, c.hk, c.d, causal, (float)scale, cv(c.q), cv(c.k),
+                                   cv(c.v), c.strides, ip(row_ptr), ip(col_ptr), cv(o), fp(lse), cv(g), vo(dq), vo(dk),
+                                   vo(dv), vo(ws), nb, stream_of(q)),
+           "dgnn_attn_backward");
+  return std::make_tuple(cut(dq, d), cut(dk, d), cut(dv, d));
+}
+
+struct CeCall {
+  int dtype, label_bytes, n, classes, d;
+};
+CeCall ce_call(const Tensor &feat, const Tensor &weight, const Tensor &label, int64_t reduction) {
+  CeCall c;
+  c.dtype = dense_type(feat, "feat");
+  like(weight, feat, "weight", "feat");
+  if (feat.dim() != 2 || weight.dim() != 2 || feat.size(1) != weight.size(1))
+    fail("feat must be [rows, dim] and weight [classes, dim], got ", feat.sizes(), " and ", weight.sizes());
+  contiguous(feat, "feat"), contiguous(weight, "weight");
+  c.label_bytes = index_bytes(label, feat, "label");
+  if (label.dim() != 1 || label.size(0) != feat.size(0)) fail("label must be [rows], got ", label.sizes());
+  if (weight.size(0) < 1 || weight.size(1) < 1) fail("weight must have at least one class and one column, got ", weight.sizes());
+  if (reduction < 0 || reduction > 2) fail("reduction must be 0 (none), 1 (mean) or 2 (sum)");
+  c.n = as_int(feat.size(0), "rows"), c.classes = as_int(weight.size(0), "classes"), c.d = as_int(feat.size(1), "dim");
+  return c;
+}
+
+// -> (loss [rows] or [], lse [rows])
+std::tuple<Tensor, Tensor> linear_ce_forward(const Tensor &feat, const Tensor &weight, const Tensor &label,
+                                             int64_t ignore_index, int64_t reduction) {
+  const CeCall c = ce_call(feat, weight, label, reduction);
+  c10::DeviceGuard guard(feat.device());
+  Tensor loss = reduction == 0 ? new_f32({c.n}, feat) : new_f32({}, feat), lse = new_f32({c.n}, feat);
+  const size_t nb = API(dgnn_linear_ce_workspace_bytes)(c.dtype, c.n, c.classes, c.d, 0);
+  Tensor ws = workspace(nb, feat);
+  check_rc(API(dgnn_linear_ce_forward)(c.dtype, c.label_bytes, c.n, c.classes, c.d, ignore_index, (int)reduction, cv(feat),
+                                       cv(weight), cv(label), fo(loss), fo(lse), vo(ws), nb, stream_of(feat)),
+           "dgnn_linear_ce_forward");
+  return std::make_tuple(loss, lse);
+}
+
+// -> (grad_feat or None, grad_weight or None)
+std::tuple<py::object, py::object> linear_ce_backward(const Tensor &feat, const Tensor &weight, const Tensor &label,
+                                                      int64_t ignore_index, int64_t reduction, const Tensor &lse,
+                                                      const Tensor &grad, bool want_feat, bool want_weight) {
+  const CeCall c = ce_call(feat, weight, label, reduction);
+  f32(lse, "lse", 1), f32(grad, "grad");
+  if (lse.size(0) != c.n || lse.device() != feat.device()) fail("lse must be the forward's [rows]");
+  if (grad.numel() != (reduction == 0 ? c.n : 1) || grad.device() != feat.device())
+    fail("grad must be the gradient of the loss, got shape ", grad.sizes());
+  c10::DeviceGuard guard(feat.device());
+  Tensor dx = want_feat ? at::empty_like(feat) : Tensor();
+  Tensor dw = !want_weight ? Tensor() : c.n == 0 ? at::zeros_like(weight) : at::empty_like(weight);
+  if (c.n > 0) {
+    const size_t nb = API(dgnn_linear_ce_workspace_bytes)(c.dtype, c.n, c.classes, c.d, 1);
+    Tensor ws = workspace(nb, feat);
+    check_rc(API(dgnn_linear_ce_backward)(c.dtype, c.label_bytes, c.n, c.classes, c.d, ignore_index, (int)reduction,
+                                          cv(feat), cv(weight), cv(label), fp(lse), fp(grad), vo(dx), vo(dw), vo(ws), nb,
+                                          stream_of(feat)),
+             "dgnn_linear_ce_backward");
+  }
+  return std::make_tuple(want_feat ? py::cast(dx) : py::object(py::none()), want_weight ? py::cast(dw) : py::object(py::none()));
+}
+
 // ------------------------------------------------------------------ module plumbing
 // DgnnError surfaces as dgnn_amd._lib.DgnnError (a RuntimeError), the class the ctypes users raise.
 void translate_errors() {
@@ -1191,4 +1399,40 @@ PYBIND11_MODULE(gat_layer_ops, m) {
   def(m, "epilogue_backward", &epilogue_backward, "out, grad, activation, act_param, want_bias",
       "-> (grad_pre, grad_bias or None)", arg("out"), arg("grad"), arg("activation"), arg("act_param"),
       arg("want_bias"));
+}
+
+PYBIND11_MODULE(fused_embedding, m) {
+  py::options options;
+  options.disable_function_signatures();
+  init(m, "Node-id embedding with scaling, gradient by sorted ids (no reference module).");
+  def(m, "embedding_forward", &embedding_forward, "ids, table, scale=1.0",
+      "-> scale * table[ids] [*ids.shape, dim]; ids (int32 or int64) outside [0, rows): zeros", arg("ids"), arg("table"),
+      arg("scale") = 1.0);
+  def(m, "embedding_backward", &embedding_backward, "ids, grad_out, rows, scale=1.0",
+      "-> grad_table [rows, dim], deterministic", arg("ids"), arg("grad_out"), arg("rows"), arg("scale") = 1.0);
+}
+
+PYBIND11_MODULE(fused_attention, m) {
+  py::options options;
+  options.disable_function_signatures();
+  init(m, "Packed attention: every row to every key of its own sequence (no reference module).");
+  def(m, "attention_forward", &attention_forward, "q, k, v, row_ptr, col_ptr, scale, causal",
+      "-> (out [rows, heads, dim], lse [heads, rows])", arg("q"), arg("k"), arg("v"), arg("row_ptr"), arg("col_ptr"),
+      arg("scale"), arg("causal"));
+  def(m, "attention_backward", &attention_backward, "q, k, v, row_ptr, col_ptr, scale, causal, out, lse, grad",
+      "-> (dq, dk, dv), deterministic", arg("q"), arg("k"), arg("v"), arg("row_ptr"), arg("col_ptr"), arg("scale"),
+      arg("causal"), arg("out"), arg("lse"), arg("grad"));
+}
+
+PYBIND11_MODULE(fused_cross_entropy, m) {
+  py::options options;
+  options.disable_function_signatures();
+  init(m, "Cross entropy of a linear layer without its logits (no reference module).");
+  def(m, "linear_ce_forward", &linear_ce_forward, "feat, weight, label, ignore_index=-100, reduction=1",
+      "-> (loss, lse [rows]); reduction 0: loss [rows], 1: mean over the labelled rows, 2: sum", arg("feat"),
+      arg("weight"), arg("label"), arg("ignore_index") = -100, arg("reduction") = 1);
+  def(m, "linear_ce_backward", &linear_ce_backward,
+      "feat, weight, label, ignore_index, reduction, lse, grad, want_feat=True, want_weight=True",
+      "-> (grad_feat or None, grad_weight or None), deterministic", arg("feat"), arg("weight"), arg("label"),
+      arg("ignore_index"), arg("reduction"), arg("lse"), arg("grad"), arg("want_feat") = true, arg("want_weight") = true);
 }

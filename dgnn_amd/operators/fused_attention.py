@@ -1,0 +1,42 @@
+"""Autograd operator of packed attention (new API surface: the reference's attention runs over given
+edges, dgNN/operators/fused_gatconv.py; this one over all pairs of a graph, a walk or a prompt)."""
+import torch
+
+from ..native import fused_attention
+
+
+def PackedAttentionFuse(q, k, v, row_ptr, col_ptr=None, causal=False, scale=None):
+    """softmax(scale q k^T) v inside every sequence of a packed batch; [rows, heads, dim] in q's type.
+
+    q [rows, heads, dim], k and v [keys, key_heads, dim], float32, bfloat16 or float16, dim 1 to 128;
+    key_heads divides heads, query head i reads key head i // (heads // key_heads).  Views with
+    strides (slices of one projection's output) are read where they lie if their rows are whole
+    16-byte chunks, otherwise copied once.
+    row_ptr (int32, sequences + 1 ascending offsets) bounds the rows of every sequence, col_ptr (default:
+    row_ptr) its keys: one row a sequence and all of its nodes as keys is an attention pooling, or
+    the step of a single token.  causal: row i of a sequence sees its keys j <= i + keys - rows.
+    scale defaults to dim ** -0.5.
+
+    A row that sees no key (masked, empty sequence, in front of or behind the sequences) gives zeros and no
+    gradient.  Values do not cross sequences, not even NaN; inside one, a NaN or infinity in a key or
+    value may reach rows that the causal mask keeps from it, as a weight of zero times it does."""
+    if scale is None:
+        scale = q.size(-1) ** -0.5
+    return PackedAttentionFunction.apply(q, k, v, row_ptr, row_ptr if col_ptr is None else col_ptr, causal, scale)
+
+
+class PackedAttentionFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, row_ptr, col_ptr, causal, scale):
+        out, lse = fused_attention.attention_forward(q, k, v, row_ptr, col_ptr, scale, causal)
+        ctx.save_for_backward(q, k, v, row_ptr, col_ptr, out, lse)
+        ctx.causal, ctx.scale = causal, scale
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_out):
+        q, k, v, row_ptr, col_ptr, out, lse = ctx.saved_tensors
+        dq, dk, dv = fused_attention.attention_backward(q, k, v, row_ptr, col_ptr, ctx.scale, ctx.causal, out, lse,
+                                                        grad_out)
+        return dq, dk, dv, None, None, None, None

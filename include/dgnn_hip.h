@@ -38,6 +38,11 @@ extern "C" {
 #define DGNN_ERR_ALIGNMENT (-4)     /* a pointer is not 4-byte aligned                    */
 #define DGNN_ERR_TOO_LARGE (-5)     /* beyond the static scratch of dgnn_gat_forward_noalloc */
 
+/* element types of the dense operators */
+#define DGNN_F32 0
+#define DGNN_BF16 1
+#define DGNN_F16 2
+
 int dgnn_abi_version(void);
 const char *dgnn_error_string(int code);
 
@@ -482,6 +487,58 @@ size_t dgnn_gat_epilogue_backward_workspace_bytes(int n, int hf);
 int dgnn_gat_epilogue_backward(int n, int hf, int activation, float act_param, const float *out,
                                const float *grad, float *grad_pre, float *grad_bias,
                                void *workspace, size_t workspace_bytes, void *stream);
+
+/* ------------------------------------------------------------------ sequence operators ----
+ * No counterpart in the reference.  Node-id embedding, attention of every node to every node of its
+ * own graph (or walk, or prompt), and a cross entropy over many classes: what a model on sequences of
+ * nodes trains with next to the sparse operators above.  Tensors are DGNN_F32, DGNN_BF16 or
+ * DGNN_F16 (all of one call alike); sums, softmax statistics and losses are float. */
+
+/* out[i,:] = scale * table[ids[i],:]; table [rows,dim], out [n,dim], contiguous, any dim.  ids int32
+ * (idx_bytes 4) or int64 (8); an id outside [0, rows) names no row: zeros out, no gradient. */
+int dgnn_embedding_forward(int dtype, int idx_bytes, int n, int rows, int dim, float scale, const void *ids,
+                           const void *table, void *out, void *stream);
+/* grad_table [rows,dim] = scale * sum of grad[i,:] over the i that name the row, in ascending i; fully
+ * written (rows nobody names: zeros).  Deterministic: a stable sort of the ids, no float atomics. */
+size_t dgnn_embedding_backward_workspace_bytes(int n, int rows, int dim);
+int dgnn_embedding_backward(int dtype, int idx_bytes, int n, int rows, int dim, float scale, const void *ids,
+                            const void *grad, void *grad_table, void *workspace, size_t workspace_bytes, void *stream);
+
+/* Packed attention.  q [tq,hq,d], k and v [tk,hk,d]; hk divides hq, query head i reads key head
+ * i / (hq / hk).  Sequence s holds the queries row_ptr[s] .. row_ptr[s+1] - 1 and the keys col_ptr[s] ..
+ * col_ptr[s+1] - 1 (int32 device arrays of nseq + 1 ascending offsets; pass the same array twice for self
+ * attention).  causal: query i of a sequence sees its keys j <= i + keys - queries, else all of them.
+ *   out [tq,hq,d] = softmax(scale q k^T) v;  lse [hq,tq] natural logarithm of the softmax's sum (may be NULL)
+ * A row that sees no key -- masked, an empty sequence, a row in front of the first or behind the
+ * last sequence -- gives out = 0, lse = -inf and has no gradient; rows no sequence holds are never read.
+ * strides: HOST array {q_token, q_head, k_token, k_head, v_token, v_head} in elements, the last
+ * dimension contiguous.  DGNN_ERR_UNSUPPORTED: d > 128, or rows that are not whole 16-byte chunks (d and
+ * every stride), or a token stride under d or of 16 MB and more.  The other tensors are contiguous. */
+int dgnn_attn_forward(int dtype, int nseq, int tq, int tk, int hq, int hk, int d, int causal, float scale,
+                      const void *q, const void *k, const void *v, const long long *strides, const int *row_ptr,
+                      const int *col_ptr, void *out, float *lse, void *stream);
+/* dq [tq,hq,d], dk and dv [tk,hk,d] from grad [tq,hq,d] and the forward's out and lse; fully written.
+ * No atomics: the same bits every time. */
+size_t dgnn_attn_backward_workspace_bytes(int tq, int hq);
+int dgnn_attn_backward(int dtype, int nseq, int tq, int tk, int hq, int hk, int d, int causal, float scale,
+                       const void *q, const void *k, const void *v, const long long *strides, const int *row_ptr,
+                       const int *col_ptr, const void *out, const float *lse, const void *grad, void *dq, void *dk,
+                       void *dv, void *workspace, size_t workspace_bytes, void *stream);
+
+/* Softmax cross entropy of a linear layer, z = x w^T, without the logits.  x [n,d], w [classes,d]
+ * contiguous; label int32 (label_bytes 4) or int64 (8).  A row whose label is ignore_index or outside
+ * [0, classes) has no label: loss 0, no gradient, never read.
+ *   reduction 0: loss [n]; 1: loss [1], the mean over the labelled rows (0 when there are none); 2: [1], the sum
+ *   lse [n]: log of the softmax's sum (0 for rows without a label), kept for the backward
+ * backward: grad is d / d loss, [n] for reduction 0, else [1]; dx [n,d] and dw [classes,d], either may be NULL.
+ * Limits: n <= 2^22, d <= 65536, classes <= 2^30 (DGNN_ERR_UNSUPPORTED). */
+size_t dgnn_linear_ce_workspace_bytes(int dtype, int n, int classes, int d, int backward);
+int dgnn_linear_ce_forward(int dtype, int label_bytes, int n, int classes, int d, long long ignore_index, int reduction,
+                           const void *x, const void *w, const void *label, float *loss, float *lse, void *workspace,
+                           size_t workspace_bytes, void *stream);
+int dgnn_linear_ce_backward(int dtype, int label_bytes, int n, int classes, int d, long long ignore_index, int reduction,
+                            const void *x, const void *w, const void *label, const float *lse, const float *grad,
+                            void *dx, void *dw, void *workspace, size_t workspace_bytes, void *stream);
 
 #ifdef __cplusplus
 }

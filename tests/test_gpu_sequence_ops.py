@@ -1,0 +1,405 @@
+"""GPU parity of the sequence operators (node embedding, packed attention, linear cross entropy)
+against plain float64 forms, at the sizes, layouts and masks where they can go wrong.  The
+tolerances are sums of rounding errors (tests/sequence_ref.py)."""
+import math
+
+import pytest
+import torch
+
+import sequence_ref as ref
+from dgnn_amd.operators import LinearCrossEntropyFuse, NodeEmbeddingFuse, PackedAttentionFuse
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = [torch.float32, torch.bfloat16, torch.float16]
+DEV = "cuda:0"
+
+
+def ids_of(x):
+    return str(x).replace("torch.", "")
+
+
+# ------------------------------------------------------------------------------------ embedding
+@pytest.mark.parametrize("dtype", DTYPES, ids=ids_of)
+@pytest.mark.parametrize("n,rows,dim", [(1, 1, 1), (1, 300, 64), (7, 5, 3), (63, 1000, 41), (4096, 41, 100),
+                                        (4097, 70000, 8), (5000, 257, 129), (20000, 3, 16), (300, 200000, 24),
+                                        (70001, 2708, 33)])
+def test_embedding(n, rows, dim, dtype):
+    gen = torch.Generator().manual_seed(n * 7 + dim)
+    ids = (torch.rand(n, generator=gen, dtype=torch.float64) ** 3 * (rows + 1)).long() - (torch.arange(n) % 5 == 3).long()
+    ids[0] = rows - 1
+    ids[n // 2:n // 2 + 1] = rows if n > 2 else rows - 1             # one behind the last row: names none
+    table = torch.randn(rows, dim, generator=gen).to(dtype)
+    grad = torch.randn(n, dim, generator=gen).to(dtype)
+    scale = 1.7
+    good = (ids >= 0) & (ids < rows)
+    at = ids.clamp(0, rows - 1)
+    want = (table[at].float() * torch.tensor(scale)) * good[:, None]
+    gsum = torch.zeros(rows, dim, dtype=torch.float64).index_add_(0, at[good], grad[good].double()) * scale
+    mass = torch.zeros(rows, dim, dtype=torch.float64).index_add_(0, at[good], grad[good].double().abs()) * scale
+    most = int(torch.bincount(at[good], minlength=1).max()) if bool(good.any()) else 0
+    bound = (most + 4) * ref.U * mass + ref.half_step(dtype) * gsum.abs() * (1 + 1e-6) + ref.tiny(dtype)
+    results = []
+    for wide in (torch.int64, torch.int32):
+        t = table.to(DEV).requires_grad_()
+        out = NodeEmbeddingFuse(ids.to(DEV, wide), t, scale)
+        assert torch.equal(out.detach().cpu(), want.to(dtype))
+        out.backward(grad.to(DEV))
+        ref.check(t.grad, (gsum, bound), f"grad_table {wide}")
+        results.append(t.grad.clone())
+    assert torch.equal(results[0], results[1])                       # the same bits, whatever the id type
+
+
+def test_embedding_shapes_empty_and_unaligned():
+    table = torch.randn(50, 12, device=DEV)
+    ids = torch.randint(0, 50, (3, 4, 5), device=DEV)
+    t = table.clone().requires_grad_()
+    out = NodeEmbeddingFuse(ids, t)
+    assert out.shape == (3, 4, 5, 12) and torch.equal(out, table[ids])
+    out.sum().backward()
+    assert torch.equal(t.grad, torch.bincount(ids.flatten(), minlength=50).float()[:, None].expand(50, 12))
+    for ids in (torch.empty(0, dtype=torch.int64, device=DEV), torch.full((9,), -1, device=DEV),
+                torch.full((9,), 1 << 40, device=DEV)):
+        t = table.clone().requires_grad_()
+        out = NodeEmbeddingFuse(ids, t)
+        assert out.shape == (ids.numel(), 12) and not out.any()
+        out.sum().backward()
+        assert not t.grad.any()
+    # rows that start off 16 bytes: a view behind one element
+    for dtype in DTYPES:
+        flat = torch.randn(50 * 16 + 1, device=DEV).to(dtype)
+        view = flat[1:].view(50, 16)
+        ids = torch.randint(0, 50, (77,), device=DEV)
+        assert torch.equal(NodeEmbeddingFuse(ids, view), view[ids])
+        # a transposed table and ids with a stride are taken as values
+        wide = torch.randn(16, 50, device=DEV).to(dtype)
+        assert torch.equal(NodeEmbeddingFuse(ids[::2], wide.t()), wide.t()[ids[::2]])
+
+
+# ------------------------------------------------------------------------------------ attention
+def offsets(lens, front=0):
+    off = [front]
+    for n in lens:
+        off.append(off[-1] + n)
+    return off
+
+
+def attention_case(lq, lk, hq, hk, d, causal, dtype, seed=0, front=0, back=0, scale=None, layout="split",
+                   poison=False, grads=True):
+    gen = torch.Generator().manual_seed(seed + 1000 * d + sum(lk))
+    q_off, k_off = offsets(lq, front), offsets(lk, front)
+    tq, tk = q_off[-1] + back, k_off[-1] + back
+    same = lq is lk
+
+    def make(t, h):
+        return torch.randn(t, h, d, generator=gen).to(dtype)
+
+    q, k, v, grad = make(tq, hq), make(tk, hk), make(tk, hk), make(tq, hq)
+    scale = d ** -0.5 if scale is None else scale
+    want = ref.attention(q, k, v, q_off, k_off, causal, scale, grad if grads else None)
+    if poison:                                            # rows of no sequence hold anything
+        for t, off in ((q, q_off), (k, k_off), (v, k_off), (grad, q_off)):
+            t[:off[0]] = float("nan")
+            t[off[-1]:] = float("inf")
+    if layout == "packed" and same:                       # slices of one projection
+        qkv = torch.cat([q, k, v], 1).to(DEV)
+        q, k, v = qkv[:, :hq], qkv[:, hq:hq + hk], qkv[:, hq + hk:]
+    elif layout == "heads":                               # head major
+        q, k, v = (t.transpose(0, 1).contiguous().to(DEV).transpose(0, 1) for t in (q, k, v))
+    elif layout == "last":                                # the last dimension has a stride
+        q, k, v = (t.permute(2, 0, 1).contiguous().to(DEV).permute(1, 2, 0) for t in (q, k, v))
+    elif layout == "offset":                              # rows off 16 bytes
+        q, k, v = (torch.cat([torch.zeros(1, dtype=dtype), t.flatten()]).to(DEV)[1:].view(t.shape) for t in (q, k, v))
+    else:
+        q, k, v = (t.to(DEV) for t in (q, k, v))
+    row_ptr = torch.tensor(q_off, dtype=torch.int32, device=DEV)
+    col_ptr = None if same else torch.tensor(k_off, dtype=torch.int32, device=DEV)
+    leaves = [t.detach().requires_grad_(grads) for t in (q, k, v)]
+    out = PackedAttentionFuse(*leaves, row_ptr, col_ptr, causal=causal, scale=scale)
+    assert out.dtype == dtype and out.is_contiguous()
+    ref.check(out, want["out"], "out")
+    if grads:
+        got = torch.autograd.grad(out, leaves, grad.to(DEV))
+        again = torch.autograd.grad(PackedAttentionFuse(*leaves, row_ptr, col_ptr, causal=causal, scale=scale), leaves,
+                                    grad.to(DEV))
+        for name, x, y in zip(("dq", "dk", "dv"), got, again):
+            ref.check(x, want[name], name)
+            assert torch.equal(x, y), f"{name} differs from run to run"
+
+
+SELF = [[1], [2], [31], [64, 1], [65, 0, 33], [0, 0, 1, 0], [5, 0, 128, 127, 129, 1], [300, 7]]
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=ids_of)
+@pytest.mark.parametrize("causal", [False, True], ids=["full", "causal"])
+@pytest.mark.parametrize("lens", SELF, ids=str)
+def test_attention_lengths(lens, causal, dtype):
+    attention_case(lens, lens, 4, 2, 64, causal, dtype)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=ids_of)
+@pytest.mark.parametrize("d", [1, 3, 8, 16, 24, 32, 33, 41, 63, 64, 72, 96, 100, 120, 127, 128])
+def test_attention_head_dims(d, dtype):
+    attention_case([70, 1, 33], [70, 1, 33], 2, 1, d, d % 2 == 0, dtype)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=ids_of)
+@pytest.mark.parametrize("hq,hk", [(1, 1), (3, 3), (3, 1), (6, 2), (8, 1), (40, 1), (10, 2), (16, 8)])
+def test_attention_heads(hq, hk, dtype):
+    lens = [45, 20, 131]
+    attention_case(lens, lens, hq, hk, 32, True, dtype)
+    attention_case(lens, lens, hq, hk, 32, False, dtype, seed=1)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=ids_of)
+@pytest.mark.parametrize("causal", [False, True], ids=["full", "causal"])
+def test_attention_queries_and_keys_of_different_lengths(causal, dtype):
+    """Single queries, rows that see nothing (more queries than keys), sequences without either."""
+    for lq, lk in (([1] * 6, [1, 2, 64, 65, 300, 1000]), ([9, 40, 0, 5, 1], [3, 1, 17, 0, 129]),
+                   ([150, 3], [20, 500]), ([1], [2500]), ([200], [1])):
+        attention_case(lq, lk, 8, 2, 64, causal, dtype)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=ids_of)
+@pytest.mark.parametrize("layout", ["packed", "heads", "last", "offset"])
+@pytest.mark.parametrize("d", [64, 41])
+def test_attention_layouts(layout, d, dtype):
+    lens = [70, 1, 200]
+    attention_case(lens, lens, 4, 2, d, True, dtype, layout=layout)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=ids_of)
+@pytest.mark.parametrize("causal", [False, True], ids=["full", "causal"])
+def test_attention_rows_of_no_sequence(causal, dtype):
+    """Padding in front and behind: never read (it holds NaN and infinities), zeros come back."""
+    lens = [33, 0, 90]
+    attention_case(lens, lens, 4, 4, 64, causal, dtype, front=37, back=150, poison=True)
+    attention_case([3, 1], [70, 5], 4, 1, 128, causal, dtype, front=2, back=3, poison=True)
+    attention_case([], [], 2, 1, 32, causal, dtype, back=5, poison=True)         # no sequence at all
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=ids_of)
+def test_attention_scales(dtype):
+    lens = [100, 29]
+    for scale in (0.0, -0.2, 0.5):
+        attention_case(lens, lens, 2, 2, 32, True, dtype, scale=scale)
+
+
+def test_attention_nan_stays_in_its_sequence():
+    for dtype in DTYPES:
+        q, k, v = (torch.randn(200, 2, 64, device=DEV).to(dtype) for _ in range(3))
+        ptr = torch.tensor([0, 70, 131, 200], dtype=torch.int32, device=DEV)
+        clean = PackedAttentionFuse(q, k, v, ptr)
+        for t in (q, k, v):
+            bad = [x.clone() for x in (q, k, v)]
+            bad[[x is t for x in (q, k, v)].index(True)][70:131] = float("nan")
+            leaves = [x.requires_grad_() for x in bad]
+            out = PackedAttentionFuse(*leaves, ptr)
+            assert torch.equal(out[:70], clean[:70]) and torch.equal(out[131:], clean[131:])
+            assert torch.isnan(out[70:131]).all()
+            for g in torch.autograd.grad(out, leaves, torch.ones_like(out)):
+                assert torch.isfinite(g[:70]).all() and torch.isfinite(g[131:]).all()
+    # a key or value far in the future of a causal row is not seen by it
+    q, k, v = (torch.randn(400, 2, 64, device=DEV) for _ in range(3))
+    ptr = torch.tensor([0, 400], dtype=torch.int32, device=DEV)
+    clean = PackedAttentionFuse(q, k, v, ptr, causal=True)
+    k[399], v[399] = float("inf"), float("nan")
+    assert torch.equal(PackedAttentionFuse(q, k, v, ptr, causal=True)[:256], clean[:256])
+
+
+def test_attention_large_scores_and_long_rows():
+    """Scores of +-300 (the running maximum moves), 5000 keys."""
+    for dtype in DTYPES:
+        gen = torch.Generator().manual_seed(3)
+        q, k, v = (torch.randn(600, 1, 64, generator=gen) for _ in range(3))
+        q, k, v = (t.to(dtype) for t in (q * 6, k * 6, v))
+        ptr = torch.tensor([0, 600], dtype=torch.int32, device=DEV)
+        want = ref.attention(q, k, v, [0, 600], [0, 600], True, 1.0)
+        ref.check(PackedAttentionFuse(q.to(DEV), k.to(DEV), v.to(DEV), ptr, causal=True, scale=1.0), want["out"], "out")
+    attention_case([40], [5000], 4, 1, 128, True, torch.bfloat16)
+
+
+def test_attention_many_small_graphs():
+    lens = [(i * 7) % 40 for i in range(700)]
+    attention_case(lens, lens, 1, 1, 32, False, torch.float32)
+    attention_case(lens, lens, 1, 1, 32, True, torch.bfloat16)
+
+
+# ------------------------------------------------------------------------------------ cross entropy
+def ce_case(n, classes, dim, dtype, reduction="mean", ignored=0.2, wide=True, seed=0, spread=2.0):
+    gen = torch.Generator().manual_seed(seed + n + classes)
+    feat = torch.randn(n, dim, generator=gen).to(dtype)
+    weight = (torch.randn(classes, dim, generator=gen) * spread / math.sqrt(dim)).to(dtype)
+    label = torch.randint(0, classes, (n,), generator=gen)
+    drop = torch.rand(n, generator=gen) < ignored
+    label[drop] = -100
+    if n > 3 and ignored:
+        label[1], label[2] = classes, -7                   # outside: no label either
+    label = label if wide else label.int()
+    grad = torch.rand(n, generator=gen) + 0.5 if reduction == "none" else torch.tensor(1.5)
+    want = ref.linear_ce(feat, weight, label, -100, reduction, grad)
+    clean = feat.clone()
+    feat[(label < 0) | (label >= classes)] = float("nan")  # rows without a label are never read
+    x, w = feat.to(DEV).requires_grad_(), weight.to(DEV).requires_grad_()
+    loss = LinearCrossEntropyFuse(x, w, label.to(DEV), reduction=reduction)
+    assert loss.dtype == torch.float32 and clean.shape == feat.shape
+    ref.check(loss, want["loss"], "loss")
+    got = torch.autograd.grad(loss, [x, w], grad.to(DEV))
+    again = torch.autograd.grad(LinearCrossEntropyFuse(x, w, label.to(DEV), reduction=reduction), [x, w], grad.to(DEV))
+    for name, a, b in zip(("dx", "dw"), got, again):
+        ref.check(a, want[name], name)
+        assert torch.equal(a, b), f"{name} differs from run to run"
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=ids_of)
+@pytest.mark.parametrize("n,classes,dim", [(1, 1, 1), (1, 1000, 64), (3, 2, 5), (64, 41, 64), (129, 127, 128),
+                                           (130, 129, 33), (257, 1000, 100), (500, 4099, 24), (33, 20011, 65),
+                                           (2500, 47, 16), (600, 130, 500)])
+def test_cross_entropy(n, classes, dim, dtype):
+    ce_case(n, classes, dim, dtype)
+    ce_case(n, classes, dim, dtype, reduction="none", wide=False, seed=1)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=ids_of)
+def test_cross_entropy_reductions_and_masks(dtype):
+    for reduction in ("none", "mean", "sum"):
+        for ignored in (0.0, 0.9, 1.0):
+            ce_case(300, 200, 40, dtype, reduction=reduction, ignored=ignored)
+    ce_case(200, 300, 64, dtype, spread=60.0)              # logits of some hundred
+
+
+def test_cross_entropy_only_one_gradient_and_no_rows():
+    feat, weight = torch.randn(40, 16, device=DEV), torch.randn(30, 16, device=DEV)
+    label = torch.randint(0, 30, (40,), device=DEV)
+    full = [t.clone().requires_grad_() for t in (feat, weight)]
+    LinearCrossEntropyFuse(*full, label).backward()
+    x = feat.clone().requires_grad_()
+    LinearCrossEntropyFuse(x, weight, label).backward()
+    w = weight.clone().requires_grad_()
+    LinearCrossEntropyFuse(feat, w, label).backward()
+    assert torch.equal(x.grad, full[0].grad) and torch.equal(w.grad, full[1].grad)
+    for reduction in ("none", "mean", "sum"):
+        x, w = feat[:0].clone().requires_grad_(), weight.clone().requires_grad_()
+        loss = LinearCrossEntropyFuse(x, w, label[:0], reduction=reduction)
+        assert loss.shape == ((0,) if reduction == "none" else ()) and not loss.any()
+        loss.sum().backward()
+        assert not w.grad.any() and x.grad.shape == (0, 16)
+
+
+# ------------------------------------------------------------------------------------ together
+def model(params, ids, ptr, label, heads, kv_heads, dim):
+    """Nodes -> embedding -> one attention layer with a residual -> scores against all nodes (tied table)."""
+    x = NodeEmbeddingFuse(ids, params["table"], math.sqrt(params["table"].size(1)))
+    qkv = (x @ params["qkv"]).view(-1, heads + 2 * kv_heads, dim)
+    o = PackedAttentionFuse(qkv[:, :heads], qkv[:, heads:heads + kv_heads], qkv[:, heads + kv_heads:], ptr, causal=True)
+    x = x + o.flatten(1) @ params["out"]
+    return LinearCrossEntropyFuse(x, params["table"], label)
+
+
+def model64(params, ids, off, label, heads, kv_heads, dim):
+    table = params["table"]
+    good = ids >= 0
+    x = table[ids.clamp(min=0)] * good[:, None] * math.sqrt(table.size(1))
+    qkv = (x @ params["qkv"]).view(-1, heads + 2 * kv_heads, dim)
+    outs = []
+    for a, b in zip(off[:-1], off[1:]):
+        q, k, v = (t.transpose(0, 1) for t in (qkv[a:b, :heads], qkv[a:b, heads:heads + kv_heads], qkv[a:b, heads + kv_heads:]))
+        k, v = (t.repeat_interleave(heads // kv_heads, 0) for t in (k, v))
+        z = q @ k.transpose(1, 2) * dim ** -0.5
+        z = z.masked_fill(torch.ones(b - a, b - a).triu(1).bool(), float("-inf"))
+        outs.append((torch.softmax(z, -1) @ v).transpose(0, 1))
+    x = x + torch.cat(outs + [torch.zeros(len(ids) - off[-1], heads, dim, dtype=x.dtype)]).flatten(1) @ params["out"]
+    kept = label >= 0
+    return torch.nn.functional.cross_entropy(x[kept] @ table.t(), label[kept])
+
+
+def test_a_training_step_of_the_three_together():
+    """Value and gradients of embedding + attention + loss on tied weights against float64 autograd:
+    float32 throughout, so a relative 1e-4 of each gradient's own norm covers sums of at most 400 terms
+    through four chained products (4 * 400 * 2^-24 = 1e-4)."""
+    heads, kv_heads, dim, width, nodes = 4, 2, 16, 48, 300
+    lens = [50, 1, 133, 0, 64]
+    off = offsets(lens)
+    n = off[-1] + 9
+    gen = torch.Generator().manual_seed(0)
+    p64 = dict(table=torch.randn(nodes, width, generator=gen).double() * 0.2,
+               qkv=torch.randn(width, (heads + 2 * kv_heads) * dim, generator=gen).double() / math.sqrt(width),
+               out=torch.randn(heads * dim, width, generator=gen).double() / 8)
+    p64 = {k: v.float().double().requires_grad_() for k, v in p64.items()}
+    ids = torch.randint(0, nodes, (n,), generator=gen)
+    label = torch.randint(0, nodes, (n,), generator=gen)
+    ids[off[-1]:], label[off[-1]:] = -1, -100
+    label[::7] = -100
+    want = model64(p64, ids, off, label, heads, kv_heads, dim)
+    want.backward()
+    params = {k: v.detach().float().to(DEV).requires_grad_() for k, v in p64.items()}
+    ptr = torch.tensor(off, dtype=torch.int32, device=DEV)
+    loss = model(params, ids.to(DEV), ptr, label.to(DEV), heads, kv_heads, dim)
+    loss.backward()
+    assert abs(loss.item() - want.item()) <= 1e-4 * abs(want.item())
+    for name in params:
+        a, b = params[name].grad.cpu().double(), p64[name].grad
+        assert (a - b).norm() <= 1e-4 * b.norm(), name
+
+
+def test_replayed_from_a_graph():
+    """Forward and backward of the three captured once and replayed with new inputs in between."""
+    heads, kv_heads, dim, width, nodes = 2, 1, 32, 64, 500
+    off = offsets([90, 3, 200])
+    gen = torch.Generator(device=DEV).manual_seed(5)
+    params = dict(table=torch.randn(nodes, width, device=DEV, generator=gen),
+                  qkv=torch.randn(width, (heads + 2 * kv_heads) * dim, device=DEV, generator=gen) / 8,
+                  out=torch.randn(heads * dim, width, device=DEV, generator=gen) / 8)
+    params = {k: v.to(torch.bfloat16).requires_grad_() for k, v in params.items()}
+    ids = torch.randint(0, nodes, (off[-1],), device=DEV, generator=gen)
+    label = torch.randint(0, nodes, (off[-1],), device=DEV, generator=gen)
+    ptr = torch.tensor(off, dtype=torch.int32, device=DEV)
+
+    def step():
+        loss = model(params, ids, ptr, label, heads, kv_heads, dim)
+        return [loss.detach()] + list(torch.autograd.grad(loss, list(params.values())))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        static = step()
+    for i in range(4):
+        ids.copy_(torch.randint(0, nodes, ids.shape, device=DEV, generator=gen))
+        label.copy_(torch.randint(-20, nodes, ids.shape, device=DEV, generator=gen))
+        ptr.copy_(torch.tensor(offsets([90 - 20 * i, 3 + i, 150]), dtype=torch.int32))
+        want = [t.clone() for t in step()]
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(static, want):
+            assert torch.equal(a, b)
+
+
+def test_on_a_side_stream():
+    """Calls run on the caller's current stream: inputs made there, with the default stream busy elsewhere."""
+    lens = [100, 50]
+    ptr = torch.tensor(offsets(lens), dtype=torch.int32, device=DEV)
+    q = torch.randn(150, 2, 64, device=DEV)
+    label = torch.randint(0, 77, (150,), device=DEV)
+    w = torch.randn(77, 128, device=DEV)
+    table = torch.randn(20, 64, device=DEV)
+    ids = torch.randint(0, 20, (150,), device=DEV)
+    torch.cuda.synchronize()
+
+    def work(x):
+        y = PackedAttentionFuse(x, x, x, ptr)
+        return y, LinearCrossEntropyFuse(y.flatten(1), w, label, reduction="none"), NodeEmbeddingFuse(ids, table * x[0, 0, 0])
+
+    want = work(q * 2)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        got = work(q * 2)
+    side.synchronize()
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
