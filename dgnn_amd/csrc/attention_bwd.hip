@@ -101,7 +101,6 @@ __global__ __launch_bounds__(64 * NW) void k_attn_bwd_kv(const AttnArgs a) {
       s = mma(TL::row_frag(qt, lane & 31, 16 * i + 8 * h), kf[i], s);
       dp = mma(TL::row_frag(gt, lane & 31, 16 * i + 8 * h), vf[i], dp);
     }
-    const bool masked = q0 < wave_all;
 #pragma unroll
     for (int r4 = 0; r4 < 4; ++r4) {
       const float4 lse = *(const float4 *)(stt + 8 * r4 + 4 * h);
@@ -110,10 +109,16 @@ __global__ __launch_bounds__(64 * NW) void k_attn_bwd_kv(const AttnArgs a) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int r = 4 * r4 + j;
-        const bool seen = !masked || q0 + acc_row(r, h) >= first;
-        const float p = seen ? exp2_fast(fmaf(s[r], c, -ls[j])) : 0.f;
-        s[r] = p;
-        dp[r] = seen ? p * (dp[r] - de[j]) : 0.f;
+        s[r] = exp2_fast(fmaf(s[r], c, -ls[j]));
+        dp[r] = s[r] * (dp[r] - de[j]);
+      }
+    }
+    if (q0 < wave_all) {                        // the diagonal crosses this block
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const bool seen = q0 + acc_row(r, h) >= first;
+        s[r] = seen ? s[r] : 0.f;
+        dp[r] = seen ? dp[r] : 0.f;
       }
     }
 #pragma unroll
@@ -204,12 +209,11 @@ __global__ __launch_bounds__(64 * NW) void k_attn_bwd_q(const AttnArgs a) {
       s = mma(TL::row_frag(kt, lane & 31, 16 * i + 8 * h), qf[i], s);
       dp = mma(TL::row_frag(vt, lane & 31, 16 * i + 8 * h), gf[i], dp);
     }
-    const bool masked = t * BN + BN - 1 > wave_all;
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      const bool on = !masked || t * BN + acc_row(r, h) <= limit;
-      const float p = exp2_fast(fmaf(s[r], c, -lse));
-      dp[r] = on ? p * (dp[r] - delta) : 0.f;
+    for (int r = 0; r < 16; ++r) dp[r] = exp2_fast(fmaf(s[r], c, -lse)) * (dp[r] - delta);
+    if (t * BN + BN - 1 > wave_all) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) dp[r] = t * BN + acc_row(r, h) <= limit ? dp[r] : 0.f;
     }
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
