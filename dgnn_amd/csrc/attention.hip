@@ -20,12 +20,14 @@ namespace dgnn {
 constexpr int ATTN_BN = 64;                    // keys of a tile
 
 template <class T, int DP, int NW>
-__global__ __launch_bounds__(64 * NW) void k_attn_fwd(const AttnArgs a) {
+__global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void k_attn_fwd(const AttnArgs a) {
   constexpr int BM = 32 * NW, BN = ATTN_BN, THREADS = 64 * NW;
   using TL = Tile<T, DP>;
-  __shared__ __align__(16) char lds_k[2][BN * TL::ROW_BYTES];
-  __shared__ __align__(16) char lds_v[2][BN * TL::ROW_BYTES];
+  using SG = Stager<T, DP, BN, THREADS>;
+  constexpr int TILE = BN * TL::ROW_BYTES, S = 2;
+  DGNN_RING2(lds, 2 * TILE);
   const int lane = lane_id(), h = lane >> 5, wave = uniform_i32(wave_in_block());
+  const int row_lane = TL::row_lane(lane), col_lane = TL::col_lane(lane);
   const int kvh = blockIdx.x % a.hk, slot = blockIdx.x / a.hk;
   const Segment seg = find_segment(a.row_ptr, a.nseq, a.tq, a.g, BM, slot, a.causal != 0);
   if (seg.tile < 0) return;
@@ -68,13 +70,13 @@ __global__ __launch_bounds__(64 * NW) void k_attn_fwd(const AttnArgs a) {
   const unsigned row_bytes = a.d * (unsigned)sizeof(T);
   const T *kbase = (const T *)a.k + (long long)ks * a.k_tok + (long long)kvh * a.k_head;
   const T *vbase = (const T *)a.v + (long long)ks * a.v_tok + (long long)kvh * a.v_head;
-  Stager<T, DP, BN, THREADS> st_k, st_v;
+  SG st_k, st_v;
   st_k.init(k_stride, a.d);
   st_v.init(v_stride, a.d);
-  auto stage = [&](int t, char *kt, char *vt) {
-    const int n = min(BN, lk - t * BN);
-    st_k.load(kt, buffer_over(kbase + (long long)t * BN * a.k_tok, span_bytes(n, k_stride, row_bytes)));
-    st_v.load(vt, buffer_over(vbase + (long long)t * BN * a.v_tok, span_bytes(n, v_stride, row_bytes)));
+  auto stage = [&](int t, auto i) {
+    const int n = t < tiles ? min(BN, lk - t * BN) : 0;
+    st_k.load(lds[i.value], buffer_over(kbase + (long long)t * BN * a.k_tok, span_bytes(n, k_stride, row_bytes)));
+    st_v.load(lds[i.value] + TILE, buffer_over(vbase + (long long)t * BN * a.v_tok, span_bytes(n, v_stride, row_bytes)));
   };
 
   acc16 acc[DP / 32];
@@ -82,15 +84,17 @@ __global__ __launch_bounds__(64 * NW) void k_attn_fwd(const AttnArgs a) {
   for (int b = 0; b < DP / 32; ++b) acc[b] = acc_zero();
   float m = -INFINITY, l = 0.f;                 // running maximum of z / scale, this half's share of the sum
 
-  auto work = [&](int t, const char *kt, const char *vt) {
+  auto work = [&](int t, auto i) {
+    const char *kt = lds[i.value], *vt = kt + TILE;
     if (t * BN > wave_any) return;
+    const int rl = opaque(row_lane), cl = opaque(col_lane);
     acc16 s[2];
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
       s[b] = acc_zero();
 #pragma unroll
       for (int i = 0; i < DP / 16; ++i)
-        s[b] = mma(TL::row_frag(kt, 32 * b + (lane & 31), 16 * i + 8 * h), qf[i], s[b]);
+        s[b] = mma(TL::row_frag(kt, rl, 32 * b, 16 * i), qf[i], s[b]);
     }
     if (t * BN + BN - 1 > wave_all) {
 #pragma unroll
@@ -127,21 +131,11 @@ __global__ __launch_bounds__(64 * NW) void k_attn_fwd(const AttnArgs a) {
     for (int i = 0; i < 4; ++i) {
       const frag8<T> p = frag_of<T>(s[i >> 1], 8 * (i & 1));
 #pragma unroll
-      for (int b = 0; b < DP / 32; ++b) acc[b] = mma(TL::col_frag(vt, 16 * i, 32 * b, lane), p, acc[b]);
+      for (int b = 0; b < DP / 32; ++b) acc[b] = mma(TL::col_frag(vt, cl, 16 * i, 32 * b), p, acc[b]);
     }
   };
 
-  if (tiles > 0) stage(0, lds_k[0], lds_v[0]);
-  for (int t = 0; t < tiles; t += 2) {
-    __syncthreads();                            // tile t has arrived; the other buffer is free
-    if (t + 1 < tiles) stage(t + 1, lds_k[1], lds_v[1]);
-    work(t, lds_k[0], lds_v[0]);
-    if (t + 1 < tiles) {
-      __syncthreads();
-      if (t + 2 < tiles) stage(t + 2, lds_k[0], lds_v[0]);
-      work(t + 1, lds_k[1], lds_v[1]);
-    }
-  }
+  ring<S, 2 * SG::LOADS>(tiles, stage, work);
 
   if (!valid) return;
   l += __shfl_xor(l, 32, 64);

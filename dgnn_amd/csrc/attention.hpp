@@ -10,7 +10,7 @@ struct AttnArgs {
   const void *q, *k, *v, *out, *grad;         // grad: of the output
   void *o, *dq, *dk, *dv;
   float *lse;                                 // [hq, tq], natural logarithm
-  float *stat;                                // backward: [2, hq, tq] = lse log2(e) (+inf for an empty row), <grad, out>
+  float *stat;                                // backward: [hq, tq] pairs {lse log2(e) (+inf for an empty row), <grad, out>}
   const int *row_ptr, *col_ptr;
   int nseq, tq, tk, hq, hk, g, d, causal;     // g = hq / hk
   long long q_tok, q_head, k_tok, k_head, v_tok, v_head;   // strides in elements; o, grad, dq, dk, dv are contiguous

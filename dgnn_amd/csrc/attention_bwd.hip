@@ -14,12 +14,12 @@ using namespace dgnn;
 
 namespace dgnn {
 
-// stat[0] = lse log2(e), +inf where the row saw no key (p = exp2(z - inf) = 0); stat[1] = <do, o>.
+// stat[head][row] = {lse log2(e), <do, o>}; the first is +inf where the row saw no key (p = exp2(z - inf) = 0).
 // One thread per 16-byte chunk, lanes of a row joined by shuffles.
 template <class T, int LPR>
 __global__ __launch_bounds__(DGNN_BLOCK) void k_attn_bwd_stat(long long rows, int d, int tq, int hq,
                                                               const T *__restrict__ out, const T *__restrict__ grad,
-                                                              const float *__restrict__ lse, float *__restrict__ stat) {
+                                                              const float *__restrict__ lse, float2 *__restrict__ stat) {
   constexpr int VEC = 16 / sizeof(T);
   const long long r = (blockIdx.x * (long long)DGNN_BLOCK + threadIdx.x) / LPR;
   const int c = (threadIdx.x % LPR) * VEC;
@@ -36,19 +36,25 @@ __global__ __launch_bounds__(DGNN_BLOCK) void k_attn_bwd_stat(long long rows, in
   if (r < rows && threadIdx.x % LPR == 0) {
     const long long tok = r / hq, head = r % hq, at = head * tq + tok;
     const float x = lse[at];
-    stat[at] = x == -INFINITY ? INFINITY : x * DGNN_LOG2E;
-    stat[rows + at] = sum;
+    stat[at] = make_float2(x == -INFINITY ? INFINITY : x * DGNN_LOG2E, sum);
   }
 }
 
+// Rows of a staged tile: 32, or 64 where 32 are too few bytes for one load of every wave.
 template <class T, int DP, int NW>
-__global__ __launch_bounds__(64 * NW) void k_attn_bwd_kv(const AttnArgs a) {
-  constexpr int BK = 32 * NW, BQ = 32, THREADS = 64 * NW;
+constexpr int bwd_rows() { return 32 * DP * (int)sizeof(T) >= 1024 * NW ? 32 : 64; }
+constexpr int BWD_STAGES = 4;
+
+template <class T, int DP, int NW>
+__global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void k_attn_bwd_kv(const AttnArgs a) {
+  constexpr int BK = 32 * NW, BQ = bwd_rows<T, DP, NW>(), THREADS = 64 * NW, S = BWD_STAGES;
   using TL = Tile<T, DP>;
-  __shared__ __align__(16) char lds_q[2][BQ * TL::ROW_BYTES];
-  __shared__ __align__(16) char lds_g[2][BQ * TL::ROW_BYTES];
-  __shared__ __align__(16) float lds_s[2][2 * BQ];
+  using SG = Stager<T, DP, BQ, THREADS>;
+  // a stage: q tile, do tile, and for every wave its own copy of the statistics (equal load counts)
+  constexpr int TILE = BQ * TL::ROW_BYTES, STAT = 2 * BQ * 4;
+  DGNN_RING4(lds, 2 * TILE + NW * STAT);
   const int lane = lane_id(), h = lane >> 5, wave = uniform_i32(wave_in_block());
+  const int row_lane = TL::row_lane(lane), col_lane = TL::col_lane(lane);
   const int kvh = blockIdx.x % a.hk, slot = blockIdx.x / a.hk;
   const Segment seg = find_segment(a.col_ptr, a.nseq, a.tk, 1, BK, slot, false);
   if (seg.tile < 0) return;
@@ -72,77 +78,76 @@ __global__ __launch_bounds__(64 * NW) void k_attn_bwd_kv(const AttnArgs a) {
 
   const unsigned q_stride = (unsigned)(a.q_tok * sizeof(T)), g_stride = (unsigned)((long long)a.hq * a.d * sizeof(T));
   const unsigned row_bytes = a.d * (unsigned)sizeof(T);
-  Stager<T, DP, BQ, THREADS> st_q, st_g;
+  SG st_q, st_g;
   st_q.init(q_stride, a.d);
   st_g.init(g_stride, a.d);
-  auto stage = [&](int u, char *qt, char *gt, float *stt) {
-    const int head = kvh * a.g + u / per_head, t = t0 + u % per_head;
-    const int n = min(BQ, lq - t * BQ);
-    const long long tq0 = qs + (long long)t * BQ;
-    st_q.load(qt, buffer_over((const T *)a.q + tq0 * a.q_tok + (long long)head * a.q_head, span_bytes(n, q_stride, row_bytes)));
-    st_g.load(gt, buffer_over((const T *)a.grad + (tq0 * a.hq + head) * a.d, span_bytes(n, g_stride, row_bytes)));
-    if (threadIdx.x < 2 * BQ) {
-      const int i = threadIdx.x % BQ;
-      const float *src = a.stat + (threadIdx.x < BQ ? 0 : (long long)a.hq * a.tq) + (long long)head * a.tq + tq0;
-      stt[threadIdx.x] = i < n ? src[i] : (threadIdx.x < BQ ? INFINITY : 0.f);     // rows behind the end: p = 0
-    }
+  int s_head = kvh * a.g, s_tile = t0, s_left = total;       // next tile to stage
+  auto stage = [&](int, auto i) {
+    // rows behind the end arrive as zeros: p = exp2(0 - 0) = 1 there, on do = 0 and delta = 0
+    const int n = s_left > 0 ? min(BQ, lq - s_tile * BQ) : 0;
+    const long long tq0 = qs + (long long)s_tile * BQ;
+    const auto stat = buffer_over(a.stat + ((long long)s_head * a.tq + tq0) * 2, n * 8u);
+#pragma unroll
+    for (int w = 0; w < BQ / 32; ++w) load_words(lds[i.value] + 2 * TILE + wave * STAT + 256 * w, stat, (64 * w + lane) * 4u);
+    st_q.load(lds[i.value], buffer_over((const T *)a.q + tq0 * a.q_tok + (long long)s_head * a.q_head, span_bytes(n, q_stride, row_bytes)));
+    st_g.load(lds[i.value] + TILE, buffer_over((const T *)a.grad + (tq0 * a.hq + s_head) * a.d, span_bytes(n, g_stride, row_bytes)));
+    --s_left;
+    if (++s_tile == tiles) s_tile = t0, ++s_head;
   };
 
   acc16 dk[DP / 32], dv[DP / 32];
 #pragma unroll
   for (int b = 0; b < DP / 32; ++b) dk[b] = acc_zero(), dv[b] = acc_zero();
 
-  auto work = [&](int u, const char *qt, const char *gt, const float *stt) {
-    const int q0 = (t0 + u % per_head) * BQ;
-    if (q0 + BQ - 1 < wave_first || key0 >= lk) return;
-    acc16 s = acc_zero(), dp = acc_zero();
+  int w_tile = t0;                                           // tile worked on
+  auto work = [&](int, auto i) {
+    const char *qt = lds[i.value], *gt = qt + TILE;
+    const float *stt = (const float *)(gt + TILE + wave * STAT);
+    const int q00 = w_tile * BQ;
+    if (++w_tile == tiles) w_tile = t0;
 #pragma unroll
-    for (int i = 0; i < DP / 16; ++i) {
-      s = mma(TL::row_frag(qt, lane & 31, 16 * i + 8 * h), kf[i], s);
-      dp = mma(TL::row_frag(gt, lane & 31, 16 * i + 8 * h), vf[i], dp);
-    }
+    for (int qb = 0; qb < BQ / 32; ++qb) {
+      const int q0 = q00 + 32 * qb;
+      if (q0 + 31 < wave_first || key0 >= lk) continue;
+      const int rl = opaque(row_lane), cl = opaque(col_lane);
+      acc16 s = acc_zero(), dp = acc_zero();
 #pragma unroll
-    for (int r4 = 0; r4 < 4; ++r4) {
-      const float4 lse = *(const float4 *)(stt + 8 * r4 + 4 * h);
-      const float4 dl = *(const float4 *)(stt + BQ + 8 * r4 + 4 * h);
-      const float ls[4] = {lse.x, lse.y, lse.z, lse.w}, de[4] = {dl.x, dl.y, dl.z, dl.w};
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int r = 4 * r4 + j;
-        s[r] = exp2_fast(fmaf(s[r], c, -ls[j]));
-        dp[r] = s[r] * (dp[r] - de[j]);
+      for (int k = 0; k < DP / 16; ++k) {
+        s = mma(TL::row_frag(qt, rl, 32 * qb, 16 * k), kf[k], s);
+        dp = mma(TL::row_frag(gt, rl, 32 * qb, 16 * k), vf[k], dp);
       }
-    }
-    if (q0 < wave_all) {                        // the diagonal crosses this block
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const bool seen = q0 + acc_row(r, h) >= first;
-        s[r] = seen ? s[r] : 0.f;
-        dp[r] = seen ? dp[r] : 0.f;
+      for (int r4 = 0; r4 < 4; ++r4) {
+        const float4 *st = (const float4 *)(stt + 2 * (32 * qb + 8 * r4 + 4 * h));
+        const float4 x = st[0], y = st[1];
+        const float ls[4] = {x.x, x.z, y.x, y.z}, de[4] = {x.y, x.w, y.y, y.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int r = 4 * r4 + j;
+          s[r] = exp2_fast(fmaf(s[r], c, -ls[j]));
+          dp[r] = s[r] * (dp[r] - de[j]);
+        }
       }
-    }
+      if (q0 < wave_all) {                      // the diagonal crosses this block
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const frag8<T> p = frag_of<T>(s, 8 * i), ds = frag_of<T>(dp, 8 * i);
+        for (int r = 0; r < 16; ++r) {
+          const bool seen = q0 + acc_row(r, h) >= first;
+          s[r] = seen ? s[r] : 0.f;
+          dp[r] = seen ? dp[r] : 0.f;
+        }
+      }
 #pragma unroll
-      for (int b = 0; b < DP / 32; ++b) {
-        dv[b] = mma(TL::col_frag(gt, 16 * i, 32 * b, lane), p, dv[b]);
-        dk[b] = mma(TL::col_frag(qt, 16 * i, 32 * b, lane), ds, dk[b]);
+      for (int k = 0; k < 2; ++k) {
+        const frag8<T> p = frag_of<T>(s, 8 * k), ds = frag_of<T>(dp, 8 * k);
+#pragma unroll
+        for (int b = 0; b < DP / 32; ++b) {
+          dv[b] = mma(TL::col_frag(gt, cl, 32 * qb + 16 * k, 32 * b), p, dv[b]);
+          dk[b] = mma(TL::col_frag(qt, cl, 32 * qb + 16 * k, 32 * b), ds, dk[b]);
+        }
       }
     }
   };
-
-  if (total > 0) stage(0, lds_q[0], lds_g[0], lds_s[0]);
-  for (int u = 0; u < total; u += 2) {
-    __syncthreads();
-    if (u + 1 < total) stage(u + 1, lds_q[1], lds_g[1], lds_s[1]);
-    work(u, lds_q[0], lds_g[0], lds_s[0]);
-    if (u + 1 < total) {
-      __syncthreads();
-      if (u + 2 < total) stage(u + 2, lds_q[0], lds_g[0], lds_s[0]);
-      work(u + 1, lds_q[1], lds_g[1], lds_s[1]);
-    }
-  }
+  ring<S, 2 * SG::LOADS + BQ / 32>(total, stage, work);
 
   if (!valid) return;
   const long long at = (tok * a.hk + kvh) * a.d;
@@ -151,12 +156,14 @@ __global__ __launch_bounds__(64 * NW) void k_attn_bwd_kv(const AttnArgs a) {
 }
 
 template <class T, int DP, int NW>
-__global__ __launch_bounds__(64 * NW) void k_attn_bwd_q(const AttnArgs a) {
-  constexpr int BM = 32 * NW, BN = 32, THREADS = 64 * NW;
+__global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void k_attn_bwd_q(const AttnArgs a) {
+  constexpr int BM = 32 * NW, BN = bwd_rows<T, DP, NW>(), THREADS = 64 * NW, S = BWD_STAGES;
   using TL = Tile<T, DP>;
-  __shared__ __align__(16) char lds_k[2][BN * TL::ROW_BYTES];
-  __shared__ __align__(16) char lds_v[2][BN * TL::ROW_BYTES];
+  using SG = Stager<T, DP, BN, THREADS>;
+  constexpr int TILE = BN * TL::ROW_BYTES;
+  DGNN_RING4(lds, 2 * TILE);
   const int lane = lane_id(), h = lane >> 5, wave = uniform_i32(wave_in_block());
+  const int row_lane = TL::row_lane(lane), col_lane = TL::col_lane(lane);
   const int kvh = blockIdx.x % a.hk, slot = blockIdx.x / a.hk;
   const Segment seg = find_segment(a.row_ptr, a.nseq, a.tq, a.g, BM, slot, a.causal != 0);
   if (seg.tile < 0) return;
@@ -180,60 +187,55 @@ __global__ __launch_bounds__(64 * NW) void k_attn_bwd_q(const AttnArgs a) {
   frag8<T> qf[DP / 16], gf[DP / 16];
   load_row_frags<T, DP>(qf, (const T *)a.q + tok * a.q_tok + (long long)head * a.q_head, a.d, h, valid);
   load_row_frags<T, DP>(gf, (const T *)a.grad + (tok * a.hq + head) * a.d, a.d, h, valid);
-  const long long at = (long long)head * a.tq + tok;
-  const float lse = valid ? a.stat[at] : INFINITY, delta = valid ? a.stat[(long long)a.hq * a.tq + at] : 0.f;
+  const float2 stat = valid ? ((const float2 *)a.stat)[(long long)head * a.tq + tok] : make_float2(INFINITY, 0.f);
+  const float lse = stat.x, delta = stat.y;
   const float c = a.scale * DGNN_LOG2E;
 
   const unsigned k_stride = (unsigned)(a.k_tok * sizeof(T)), v_stride = (unsigned)(a.v_tok * sizeof(T));
   const unsigned row_bytes = a.d * (unsigned)sizeof(T);
   const T *kbase = (const T *)a.k + (long long)ks * a.k_tok + (long long)kvh * a.k_head;
   const T *vbase = (const T *)a.v + (long long)ks * a.v_tok + (long long)kvh * a.v_head;
-  Stager<T, DP, BN, THREADS> st_k, st_v;
+  SG st_k, st_v;
   st_k.init(k_stride, a.d);
   st_v.init(v_stride, a.d);
-  auto stage = [&](int t, char *kt, char *vt) {
-    const int n = min(BN, lk - t * BN);
-    st_k.load(kt, buffer_over(kbase + (long long)t * BN * a.k_tok, span_bytes(n, k_stride, row_bytes)));
-    st_v.load(vt, buffer_over(vbase + (long long)t * BN * a.v_tok, span_bytes(n, v_stride, row_bytes)));
+  auto stage = [&](int t, auto i) {
+    const int n = t < tiles ? min(BN, lk - t * BN) : 0;
+    st_k.load(lds[i.value], buffer_over(kbase + (long long)t * BN * a.k_tok, span_bytes(n, k_stride, row_bytes)));
+    st_v.load(lds[i.value] + TILE, buffer_over(vbase + (long long)t * BN * a.v_tok, span_bytes(n, v_stride, row_bytes)));
   };
 
   acc16 dq[DP / 32];
 #pragma unroll
   for (int b = 0; b < DP / 32; ++b) dq[b] = acc_zero();
 
-  auto work = [&](int t, const char *kt, const char *vt) {
-    if (t * BN > wave_any) return;
-    acc16 s = acc_zero(), dp = acc_zero();
+  auto work = [&](int t, auto i) {
+    const char *kt = lds[i.value], *vt = kt + TILE;
 #pragma unroll
-    for (int i = 0; i < DP / 16; ++i) {
-      s = mma(TL::row_frag(kt, lane & 31, 16 * i + 8 * h), qf[i], s);
-      dp = mma(TL::row_frag(vt, lane & 31, 16 * i + 8 * h), gf[i], dp);
-    }
+    for (int kb = 0; kb < BN / 32; ++kb) {
+      const int k0 = t * BN + 32 * kb;
+      if (k0 > wave_any) continue;
+      const int rl = opaque(row_lane), cl = opaque(col_lane);
+      acc16 s = acc_zero(), dp = acc_zero();
 #pragma unroll
-    for (int r = 0; r < 16; ++r) dp[r] = exp2_fast(fmaf(s[r], c, -lse)) * (dp[r] - delta);
-    if (t * BN + BN - 1 > wave_all) {
+      for (int k = 0; k < DP / 16; ++k) {
+        s = mma(TL::row_frag(kt, rl, 32 * kb, 16 * k), qf[k], s);
+        dp = mma(TL::row_frag(vt, rl, 32 * kb, 16 * k), gf[k], dp);
+      }
 #pragma unroll
-      for (int r = 0; r < 16; ++r) dp[r] = t * BN + acc_row(r, h) <= limit ? dp[r] : 0.f;
-    }
+      for (int r = 0; r < 16; ++r) dp[r] = exp2_fast(fmaf(s[r], c, -lse)) * (dp[r] - delta);
+      if (k0 + 31 > wave_all) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const frag8<T> ds = frag_of<T>(dp, 8 * i);
+        for (int r = 0; r < 16; ++r) dp[r] = k0 + acc_row(r, h) <= limit ? dp[r] : 0.f;
+      }
 #pragma unroll
-      for (int b = 0; b < DP / 32; ++b) dq[b] = mma(TL::col_frag(kt, 16 * i, 32 * b, lane), ds, dq[b]);
+      for (int k = 0; k < 2; ++k) {
+        const frag8<T> ds = frag_of<T>(dp, 8 * k);
+#pragma unroll
+        for (int b = 0; b < DP / 32; ++b) dq[b] = mma(TL::col_frag(kt, cl, 32 * kb + 16 * k, 32 * b), ds, dq[b]);
+      }
     }
   };
-
-  if (tiles > 0) stage(0, lds_k[0], lds_v[0]);
-  for (int t = 0; t < tiles; t += 2) {
-    __syncthreads();
-    if (t + 1 < tiles) stage(t + 1, lds_k[1], lds_v[1]);
-    work(t, lds_k[0], lds_v[0]);
-    if (t + 1 < tiles) {
-      __syncthreads();
-      if (t + 2 < tiles) stage(t + 2, lds_k[0], lds_v[0]);
-      work(t + 1, lds_k[1], lds_v[1]);
-    }
-  }
+  ring<S, 2 * SG::LOADS>(tiles, stage, work);
 
   if (valid) store_row<T, DP>((T *)a.dq + (tok * a.hq + head) * a.d, dq, a.scale, a.d, h);
 }
@@ -245,7 +247,8 @@ static int launch_bwd(const AttnArgs &a, const float *lse, hipStream_t st) {
   if (rows > 0) {
     constexpr int LPR = DP * (int)sizeof(T) / 16;
     hipLaunchKernelGGL((k_attn_bwd_stat<T, LPR>), dim3((unsigned)((rows * LPR + DGNN_BLOCK - 1) / DGNN_BLOCK)),
-                       dim3(DGNN_BLOCK), 0, st, rows, a.d, a.tq, a.hq, (const T *)a.out, (const T *)a.grad, lse, a.stat);
+                       dim3(DGNN_BLOCK), 0, st, rows, a.d, a.tq, a.hq, (const T *)a.out, (const T *)a.grad, lse,
+                       (float2 *)a.stat);
     DGNN_LAUNCH_CHECK();
   }
   if (a.tk > 0) {
@@ -290,7 +293,7 @@ int dgnn_attn_backward(int dtype, int nseq, int tq, int tk, int hq, int hk, int 
   for (const void *p : {out, grad, (const void *)dq, (const void *)dk, (const void *)dv})
     if ((uintptr_t)p & 15) return DGNN_ERR_ALIGNMENT;
   if (workspace_bytes < dgnn_attn_backward_workspace_bytes(tq, hq) || (tq > 0 && !workspace)) return DGNN_ERR_WORKSPACE;
-  if ((((uintptr_t)workspace) | ((uintptr_t)lse)) & 3) return DGNN_ERR_ALIGNMENT;
+  if (((uintptr_t)workspace & 15) || ((uintptr_t)lse & 3)) return DGNN_ERR_ALIGNMENT;
   if ((long long)hq * d * (dtype == DGNN_F32 ? 4 : 2) >= (1LL << 31) / 128) return DGNN_ERR_UNSUPPORTED;
   a.out = out, a.grad = grad, a.dq = dq, a.dk = dk, a.dv = dv;
   a.stat = (float *)workspace;

@@ -29,7 +29,8 @@ struct Gemm {
   static constexpr int THREADS = 256, MB = BM / 64, NB = BN / 64;      // 32 x 32 blocks of a wave
   using TA = Tile<T, AROW ? BK : BM>;
   using TB = Tile<T, BROW ? BK : BN>;
-  static constexpr int A_BYTES = BM * BK * (int)sizeof(T), B_BYTES = BN * BK * (int)sizeof(T);
+  static constexpr int A_BYTES = BM * BK * (int)sizeof(T), B_BYTES = BN * BK * (int)sizeof(T), S = 2;
+  static constexpr int BYTES = A_BYTES + B_BYTES;      // of a stage
 
   // an operand: first element of the tile's rows (or columns), how many of them exist, row stride
   struct Operand {
@@ -39,45 +40,50 @@ struct Gemm {
   };
 
   // acc[m][n] += over k in [0, kn)
-  __device__ static __forceinline__ void run(const Operand &a, const Operand &b, int kn, char (&la)[2][A_BYTES],
-                                             char (&lb)[2][B_BYTES], acc16 (&acc)[MB][NB]) {
-    const int lane = lane_id(), h = lane >> 5, wave = uniform_i32(wave_in_block());
+  __device__ static __forceinline__ void run(const Operand &a, const Operand &b, int kn, char *const (&lds)[S],
+                                             acc16 (&acc)[MB][NB]) {
+    const int lane = lane_id(), wave = uniform_i32(wave_in_block());
     const int m0 = (wave >> 1) * (BM / 2), n0 = (wave & 1) * (BN / 2);
+    // two row operands: consecutive k; against a column operand the order is its transposing read's
+    const int ra = AROW ? (BROW ? TA::row_lane(lane) : TA::row_lane_split(lane)) : TA::col_lane(lane);
+    const int rb = BROW ? (AROW ? TB::row_lane(lane) : TB::row_lane_split(lane)) : TB::col_lane(lane);
     Stager<T, AROW ? BK : BM, AROW ? BM : BK, THREADS> sa;
     Stager<T, BROW ? BK : BN, BROW ? BN : BK, THREADS> sb;
     sa.init(a.stride, AROW ? min(BK, kn) : a.count);
     sb.init(b.stride, BROW ? min(BK, kn) : b.count);
-    auto stage = [&](int k0, char *ta, char *tb) {
-      const int left = min(BK, kn - k0);
+    auto stage = [&](int t, auto i) {
+      char *const ta = lds[i.value], *const tb = ta + A_BYTES;
+      const int k0 = t * BK, left = max(0, min(BK, kn - k0));
       // rows end with a whole chunk (rows of dz are padded with zeros): a descriptor that ended inside one would
       // drop the dword the end falls into
       const unsigned row_bytes = (left * (unsigned)sizeof(T) + 15u) & ~15u;
-      if (left < BK && k0 > 0) {                       // the last, shorter step
+      if (left < BK && left > 0 && k0 > 0) {                       // the last, shorter step
         if (AROW) sa.init(a.stride, left);
         if (BROW) sb.init(b.stride, left);
       }
       if (AROW)
-        sa.load(ta, buffer_over(a.p + k0, span_bytes(min(a.count, BM), a.stride, row_bytes)));
+        sa.load(ta, buffer_over(a.p + k0, span_bytes(left > 0 ? min(a.count, BM) : 0, a.stride, row_bytes)));
       else
         sa.load(ta, buffer_over((const char *)a.p + (long long)k0 * a.stride, span_bytes(left, a.stride, min(a.count, BM) * (unsigned)sizeof(T))));
       if (BROW)
-        sb.load(tb, buffer_over(b.p + k0, span_bytes(min(b.count, BN), b.stride, row_bytes)));
+        sb.load(tb, buffer_over(b.p + k0, span_bytes(left > 0 ? min(b.count, BN) : 0, b.stride, row_bytes)));
       else
         sb.load(tb, buffer_over((const char *)b.p + (long long)k0 * b.stride, span_bytes(left, b.stride, min(b.count, BN) * (unsigned)sizeof(T))));
     };
-    auto work = [&](const char *ta, const char *tb) {
+    auto work = [&](int, auto i) {
+      const char *const ta = lds[i.value], *const tb = ta + A_BYTES;
 #pragma unroll
       for (int k = 0; k < BK; k += 16) {
         frag8<T> fa[MB], fb[NB];
 #pragma unroll
         for (int i = 0; i < MB; ++i) {
-          if constexpr (AROW) fa[i] = row_k(TA::row_frag, ta, m0 + 32 * i + (lane & 31), k, h);
-          else fa[i] = TA::col_frag(ta, k, m0 + 32 * i, lane);
+          if constexpr (AROW) fa[i] = BROW ? TA::row_frag(ta, ra, m0 + 32 * i, k) : TA::row_frag_split(ta, ra, m0 + 32 * i, k);
+          else fa[i] = TA::col_frag(ta, ra, k, m0 + 32 * i);
         }
 #pragma unroll
         for (int i = 0; i < NB; ++i) {
-          if constexpr (BROW) fb[i] = row_k(TB::row_frag, tb, n0 + 32 * i + (lane & 31), k, h);
-          else fb[i] = TB::col_frag(tb, k, n0 + 32 * i, lane);
+          if constexpr (BROW) fb[i] = AROW ? TB::row_frag(tb, rb, n0 + 32 * i, k) : TB::row_frag_split(tb, rb, n0 + 32 * i, k);
+          else fb[i] = TB::col_frag(tb, rb, k, n0 + 32 * i);
         }
 #pragma unroll
         for (int i = 0; i < MB; ++i)
@@ -85,34 +91,7 @@ struct Gemm {
           for (int j = 0; j < NB; ++j) acc[i][j] = mma(fa[i], fb[j], acc[i][j]);
       }
     };
-    if (kn > 0) stage(0, la[0], lb[0]);
-    for (int k0 = 0; k0 < kn; k0 += 2 * BK) {
-      __syncthreads();
-      if (k0 + BK < kn) stage(k0 + BK, la[1], lb[1]);
-      work(la[0], lb[0]);
-      if (k0 + BK < kn) {
-        __syncthreads();
-        if (k0 + 2 * BK < kn) stage(k0 + 2 * BK, la[0], lb[0]);
-        work(la[1], lb[1]);
-      }
-    }
-  }
-  // eight k elements of a row.  Two row operands: consecutive ones.  Against a column operand the order is
-  // the transposing read's (mma.hpp): 8 (j / 4) + 4 h + j % 4, two half chunks.
-  template <class F>
-  __device__ static __forceinline__ frag8<T> row_k(F row_frag, const char *t, int row, int k, int h) {
-    if constexpr (AROW && BROW) {
-      return row_frag(t, row, k + 8 * h);
-    } else {
-      using TL = typename std::conditional<AROW, TA, TB>::type;
-      union { vec4<T> v[2]; frag8<T> f; } u;
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int col = k + 8 * i + 4 * h;
-        u.v[i] = *(const vec4<T> *)(t + TL::chunk_addr(row, col / TL::CHUNK) + (col % TL::CHUNK) * (int)sizeof(T));
-      }
-      return u.f;
-    }
+    ring<S, decltype(sa)::LOADS + decltype(sb)::LOADS>((kn + BK - 1) / BK, stage, work);
   }
 };
 
@@ -240,7 +219,7 @@ constexpr int CE_BM = 128, CE_BN = 128;
 template <class T>
 __global__ __launch_bounds__(256) void k_ce_fwd(const CeArgs a) {
   using G = Gemm<T, CE_BM, CE_BN, ce_bk<T>(), true, true>;
-  __shared__ __align__(16) char la[2][G::A_BYTES], lb[2][G::B_BYTES];
+  DGNN_RING2(lds, G::BYTES);
   __shared__ float sm[2][CE_BN], ss[2][CE_BN];
   const int vt = blockIdx.x, v0 = vt * CE_BM, r0 = blockIdx.y * CE_BN;
   const int rows = min(a.n, *a.count);
@@ -251,7 +230,7 @@ __global__ __launch_bounds__(256) void k_ce_fwd(const CeArgs a) {
 #pragma unroll
     for (int j = 0; j < G::NB; ++j) acc[i][j] = acc_zero();
   G::run({(const T *)a.w + (long long)v0 * a.ldw, a.classes - v0, (unsigned)(a.ldw * sizeof(T))},
-         {(const T *)a.x + (long long)r0 * a.dk, rows - r0, (unsigned)(a.dk * sizeof(T))}, a.dk, la, lb, acc);
+         {(const T *)a.x + (long long)r0 * a.dk, rows - r0, (unsigned)(a.dk * sizeof(T))}, a.dk, lds, acc);
   const int lane = lane_id(), h = lane >> 5, wave = uniform_i32(wave_in_block());
   const int m0 = v0 + (wave >> 1) * (CE_BM / 2), n0 = (wave & 1) * (CE_BN / 2);
 #pragma unroll
@@ -346,7 +325,7 @@ __global__ __launch_bounds__(1024) void k_ce_reduce(int n, int mean, const int *
 template <class T>
 __global__ __launch_bounds__(256) void k_ce_dz(const CeArgs a) {
   using G = Gemm<T, CE_BM, CE_BN, ce_bk<T>(), true, true>;
-  __shared__ __align__(16) char la[2][G::A_BYTES], lb[2][G::B_BYTES];
+  DGNN_RING2(lds, G::BYTES);
   const int p0 = blockIdx.x * CE_BM, v0 = a.v0 + p0, r0 = blockIdx.y * CE_BN;
   const int rows = min(a.n, *a.count);
   if (r0 >= rows) return;
@@ -356,7 +335,7 @@ __global__ __launch_bounds__(256) void k_ce_dz(const CeArgs a) {
 #pragma unroll
     for (int j = 0; j < G::NB; ++j) acc[i][j] = acc_zero();
   G::run({(const T *)a.w + (long long)v0 * a.ldw, a.classes - v0, (unsigned)(a.ldw * sizeof(T))},
-         {(const T *)a.x + (long long)r0 * a.dk, rows - r0, (unsigned)(a.dk * sizeof(T))}, a.dk, la, lb, acc);
+         {(const T *)a.x + (long long)r0 * a.dk, rows - r0, (unsigned)(a.dk * sizeof(T))}, a.dk, lds, acc);
   const int lane = lane_id(), h = lane >> 5, wave = uniform_i32(wave_in_block());
   const int m0 = p0 + (wave >> 1) * (CE_BM / 2), n0 = (wave & 1) * (CE_BN / 2);
   const CeScale scale = ce_scale<T>(a, rows);
@@ -412,7 +391,7 @@ template <class T>
 __global__ __launch_bounds__(256) void k_ce_dx(const CeArgs a) {
   constexpr int BK = ce_bk<T>();
   using G = Gemm<T, CE_BM, CE_BN, BK, false, true>;
-  __shared__ __align__(16) char la[2][G::A_BYTES], lb[2][G::B_BYTES];
+  DGNN_RING2(lds, G::BYTES);
   const int c0 = blockIdx.x * CE_BM, r0 = blockIdx.y * CE_BN, split = blockIdx.z;
   const int rows = min(a.n, *a.count);
   if (r0 >= rows) return;
@@ -434,7 +413,7 @@ __global__ __launch_bounds__(256) void k_ce_dx(const CeArgs a) {
   const int steps = (a.vn + BK - 1) / BK, per = (steps + a.splits - 1) / a.splits;
   const int ka = min(a.vn, split * per * BK), kb = min(a.vn, (split + 1) * per * BK);
   G::run({(const T *)a.w + (long long)(a.v0 + ka) * a.ldw + c0, a.dk - c0, (unsigned)(a.ldw * sizeof(T))},
-         {(const T *)a.dz + (long long)r0 * a.ldz + ka, rows - r0, (unsigned)(a.ldz * sizeof(T))}, kb - ka, la, lb, acc);
+         {(const T *)a.dz + (long long)r0 * a.ldz + ka, rows - r0, (unsigned)(a.ldz * sizeof(T))}, kb - ka, lds, acc);
 #pragma unroll
   for (int j = 0; j < G::NB; ++j) {
     const int r = r0 + n0 + 32 * j + (lane & 31);
@@ -478,7 +457,7 @@ template <class T>
 __global__ __launch_bounds__(256) void k_ce_dw(const CeArgs a, int wide) {
   constexpr int BK = ce_bk<T>();
   using G = Gemm<T, CE_BM, CE_BN, BK, false, false>;
-  __shared__ __align__(16) char la[2][G::A_BYTES], lb[2][G::B_BYTES];
+  DGNN_RING2(lds, G::BYTES);
   const int c0 = blockIdx.x * CE_BM, p0 = blockIdx.y * CE_BN, split = blockIdx.z;
   const int rows = min(a.n, *a.count);
   acc16 acc[G::MB][G::NB];
@@ -489,7 +468,7 @@ __global__ __launch_bounds__(256) void k_ce_dw(const CeArgs a, int wide) {
   const int steps = (rows + BK - 1) / BK, per = (steps + a.splits - 1) / a.splits;
   const int ka = min(rows, split * per * BK), kb = min(rows, (split + 1) * per * BK);
   G::run({(const T *)a.x + (long long)ka * a.dk + c0, a.dk - c0, (unsigned)(a.dk * sizeof(T))},
-         {(const T *)a.dz + (long long)ka * a.ldz + p0, a.ldz - p0, (unsigned)(a.ldz * sizeof(T))}, kb - ka, la, lb, acc);
+         {(const T *)a.dz + (long long)ka * a.ldz + p0, a.ldz - p0, (unsigned)(a.ldz * sizeof(T))}, kb - ka, lds, acc);
   const int lane = lane_id(), h = lane >> 5, wave = uniform_i32(wave_in_block());
   const int m0 = c0 + (wave >> 1) * (CE_BM / 2), n0 = (wave & 1) * (CE_BN / 2);
   const float unit = ce_scale<T>(a, rows).unit;

@@ -8,9 +8,20 @@
 // as long as A and B agree, so the rows a lane holds of one product are, unmoved, the k elements of
 // its column in the next: element j of half h stands for k = 8 (j / 4) + 4 h + j % 4 there.
 #pragma once
+#include <type_traits>
+
 #include "common.hpp"
 
 namespace dgnn {
+
+// f(integral_constant I) for I = A .. B - 1
+template <int A, int B, class F>
+__device__ __forceinline__ void unrolled(const F &f) {
+  if constexpr (A < B) {
+    f(std::integral_constant<int, A>());
+    unrolled<A + 1, B>(f);
+  }
+}
 
 typedef _Float16 half_t;
 typedef __bf16 bf16_t;
@@ -77,40 +88,73 @@ struct Tile {
   __device__ static __forceinline__ int chunk_addr(int row, int chunk) {
     return row * ROW_BYTES + ((chunk ^ swizzle(row)) << 4);
   }
-  // eight consecutive elements (a lane's k elements of a product that sums over the columns)
-  __device__ static __forceinline__ frag8<T> row_frag(const char *tile, int row, int k0) {
+  // Addresses are a lane's part, computed once, and a constant part.  The permutation is linear in the
+  // bits of row and chunk, so where a row is the sum of a lane's and a constant row with no bit in common
+  //   addr = (lane's row bytes | lane's chunk ^ swizzle) ^ (constant chunk ^ swizzle) + constant row bytes,
+  // one exclusive or a read.
+  __device__ static __forceinline__ int lane_addr(int row, int chunk) { return chunk_addr(row, chunk); }
+  __device__ static constexpr __forceinline__ int const_swizzle(int row) {
+    return CPR >= 16 ? ((row & 7) << 1) | ((row >> 3) & 1)
+           : CPR == 8 ? (((row >> 1) & 3) << 1) | ((row >> 3) & 1) : (((row >> 2) & 1) << 1) | ((row >> 3) & 1);
+  }
+  __device__ static __forceinline__ const char *at(const char *tile, int lane_part, int row, int chunk) {
+    return tile + (lane_part ^ ((const_swizzle(row) ^ chunk) << 4)) + row * ROW_BYTES;
+  }
+  // A lane's k elements of a product that sums over the columns: eight consecutive ones, of row
+  // row0 + lane % 32 (row0 a multiple of 32) from column k0 + 8 (lane / 32).
+  __device__ static __forceinline__ int row_lane(int lane) {
+    return lane_addr(lane & 31, (lane >> 5) * (8 / CHUNK));
+  }
+  __device__ static __forceinline__ frag8<T> row_frag(const char *tile, int part, int row0, int k0) {
     if constexpr (sizeof(T) == 2) {
-      return *(const frag8<T> *)(tile + chunk_addr(row, k0 / 8));
+      return *(const frag8<T> *)at(tile, part, row0, k0 / CHUNK);
     } else {
-      const vec4<T> a = *(const vec4<T> *)(tile + chunk_addr(row, k0 / 4));
-      const vec4<T> b = *(const vec4<T> *)(tile + chunk_addr(row, k0 / 4 + 1));
+      const vec4<T> a = *(const vec4<T> *)at(tile, part, row0, k0 / CHUNK);
+      const vec4<T> b = *(const vec4<T> *)at(tile, part, row0, k0 / CHUNK + 1);
       return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
     }
   }
-  // a lane's k elements of a product that sums over the rows, for column col0 + lane % 32: rows
-  // row0 + 8 (j / 4) + 4 (lane / 32) + j % 4.  16-bit: ds_read_b64_tr_b16 hands each lane of a group of
-  // sixteen one column of a 4 x 16 block, lane i supplying the address of row i / 4, columns 4 (i % 4) ..
-  __device__ static __forceinline__ frag8<T> col_frag(const char *tile, int row0, int col0, int lane) {
-    const int h = lane >> 5;
+  // The same in the order of the column reads below, columns k0 + 8 (j / 4) + 4 (lane / 32) + j % 4: the other
+  // operand of a product with one of those.
+  __device__ static __forceinline__ int row_lane_split(int lane) {
+    return sizeof(T) == 2 ? lane_addr(lane & 31, 0) + (lane >> 5) * 8 : lane_addr(lane & 31, lane >> 5);
+  }
+  __device__ static __forceinline__ frag8<T> row_frag_split(const char *tile, int part, int row0, int k0) {
+    const vec4<T> a = *(const vec4<T> *)at(tile, part, row0, k0 / CHUNK);
+    const vec4<T> b = *(const vec4<T> *)at(tile, part, row0, (k0 + 8) / CHUNK);
+    return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+  }
+  // A lane's k elements of a product that sums over the rows, for column col0 + lane % 32 (col0 a multiple of
+  // 32): rows row0 + 8 (j / 4) + 4 (lane / 32) + j % 4 (row0 a multiple of 16).  16-bit: ds_read_b64_tr_b16
+  // hands each lane of a group of sixteen one column of a 4 x 16 block, lane i supplying the address
+  // of row i / 4, columns 4 (i % 4) ...
+  __device__ static __forceinline__ int col_lane(int lane) {
+    if (sizeof(T) == 2)
+      return lane_addr(4 * (lane >> 5) + ((lane & 15) >> 2), 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) + (lane & 1) * 8;
+    return lane_addr(4 * (lane >> 5), (lane & 31) >> 2) + (lane & 3) * 4;
+  }
+  __device__ static __forceinline__ frag8<T> col_frag(const char *tile, int part, int row0, int col0) {
     if constexpr (sizeof(T) == 2) {
       typedef __attribute__((address_space(3))) s16x4 *lds_p;
-      const int row = row0 + 4 * h + ((lane & 15) >> 2), chunk = col0 / 8 + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
-      const char *p0 = tile + chunk_addr(row, chunk) + (lane & 1) * 8;
-      const char *p1 = tile + chunk_addr(row + 8, chunk) + (lane & 1) * 8;
       union { s16x4 s[2]; frag8<T> f; } u;
-      u.s[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p)p0);
-      u.s[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p)p1);
+      u.s[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p)at(tile, part, row0, col0 / CHUNK));
+      u.s[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p)at(tile, part, row0 + 8, col0 / CHUNK));
       return u.f;
     } else {
-      const int col = col0 + (lane & 31);
       frag8<T> f;
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        f[j] = *(const T *)(tile + chunk_addr(row0 + acc_row(j, h), col / 4) + (col & 3) * 4);
+      for (int j = 0; j < 8; ++j) f[j] = *(const T *)at(tile, part, row0 + 8 * (j >> 2) + (j & 3), col0 / CHUNK);
       return f;
     }
   }
 };
+
+// Keeps the compiler from computing what depends on x once for all iterations and holding every
+// result in a register of its own.
+__device__ __forceinline__ int opaque(int x) {
+  asm("" : "+v"(x));
+  return x;
+}
 
 // 128-bit buffer descriptor over `bytes` bytes at p: reads behind them give zeros.
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_over(const void *p, unsigned bytes) {
@@ -145,6 +189,53 @@ struct Stager {
         __builtin_amdgcn_raw_ptr_buffer_load_lds(src, (lds_p)(tile + (i * THREADS + wave * 64) * 16), 16, (int)off[i], 0, 0, 0);
   }
 };
+
+// Waits until at most N of this wave's loads are in flight.  Loads return in order, so the oldest have
+// arrived; the memory clobber keeps the compiler from moving LDS reads over it.
+template <int N>
+__device__ __forceinline__ void wait_loads() {
+  static_assert(N >= 0 && N < 64, "six bits");
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+// Workgroup barrier that leaves loads to LDS in flight (__syncthreads waits for all of them).
+__device__ __forceinline__ void barrier_in_flight() {
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+// Ring of S tile buffers over `tiles` steps: while a step works on its buffer, the loads of the next
+// S - 1 are in flight.  stage(t, i) issues exactly LOADS loads of this wave into buffer i (also behind
+// the last tile, where they read nothing), work(t, i) uses buffer i.  Every buffer is a __shared__
+// variable of its own and the indices are constants after unrolling: the compiler, which waits for
+// all loads to LDS that a read may touch, then knows which those are.
+#define DGNN_RING2(name, bytes)                                     \
+  __shared__ __align__(16) char name##_0[bytes], name##_1[bytes];   \
+  char *const name[2] = {name##_0, name##_1}
+#define DGNN_RING4(name, bytes)                                                                     \
+  __shared__ __align__(16) char name##_0[bytes], name##_1[bytes], name##_2[bytes], name##_3[bytes]; \
+  char *const name[4] = {name##_0, name##_1, name##_2, name##_3}
+template <int S, int LOADS, class Stage, class Work>
+__device__ __forceinline__ void ring(int tiles, const Stage &stage, const Work &work) {
+  if (tiles <= 0) return;
+  unrolled<0, S - 1>([&](auto i) { stage(i.value, i); });
+  for (int t = 0; t < tiles; t += S)
+    unrolled<0, S>([&](auto i) {
+      if (t + i.value < tiles) {
+        wait_loads<LOADS * (S - 2)>();
+        barrier_in_flight();
+        stage(t + i.value + S - 1, std::integral_constant<int, (i.value + S - 1) % S>());
+        work(t + i.value, i);
+      }
+    });
+  wait_loads<0>();                             // the loads behind the last tile still write LDS
+}
+
+// One load of 4 bytes a lane to 64 consecutive words of LDS.
+__device__ __forceinline__ void load_words(void *to, __amdgpu_buffer_rsrc_t src, unsigned off) {
+  typedef __attribute__((address_space(3))) void *lds_p;
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(src, (lds_p)to, 4, (int)off, 0, 0, 0);
+}
 
 // bytes a descriptor over `rows` rows spans (0 rows: nothing is readable)
 __device__ __forceinline__ unsigned span_bytes(int rows, unsigned row_stride_bytes, unsigned row_bytes) {
