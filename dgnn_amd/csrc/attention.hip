@@ -25,7 +25,7 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void k_attn_fwd(co
   using TL = Tile<T, DP>;
   using SG = Stager<T, DP, BN, THREADS>;
   constexpr int TILE = BN * TL::ROW_BYTES, S = 2;
-  DGNN_RING2(lds, 2 * TILE);
+  DGNN_RING(lds, 2 * TILE);
   const int lane = lane_id(), h = lane >> 5, wave = uniform_i32(wave_in_block());
   const int row_lane = TL::row_lane(lane), col_lane = TL::col_lane(lane);
   const int kvh = blockIdx.x % a.hk, slot = blockIdx.x / a.hk;

@@ -52,7 +52,7 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void k_attn_bwd_kv
   using SG = Stager<T, DP, BQ, THREADS>;
   // a stage: q tile, do tile, and for every wave its own copy of the statistics (equal load counts)
   constexpr int TILE = BQ * TL::ROW_BYTES, STAT = 2 * BQ * 4;
-  DGNN_RING4(lds, 2 * TILE + NW * STAT);
+  DGNN_RING(lds, 2 * TILE + NW * STAT);
   const int lane = lane_id(), h = lane >> 5, wave = uniform_i32(wave_in_block());
   const int row_lane = TL::row_lane(lane), col_lane = TL::col_lane(lane);
   const int kvh = blockIdx.x % a.hk, slot = blockIdx.x / a.hk;
@@ -161,7 +161,7 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void k_attn_bwd_q(
   using TL = Tile<T, DP>;
   using SG = Stager<T, DP, BN, THREADS>;
   constexpr int TILE = BN * TL::ROW_BYTES;
-  DGNN_RING4(lds, 2 * TILE);
+  DGNN_RING(lds, 2 * TILE);
   const int lane = lane_id(), h = lane >> 5, wave = uniform_i32(wave_in_block());
   const int row_lane = TL::row_lane(lane), col_lane = TL::col_lane(lane);
   const int kvh = blockIdx.x % a.hk, slot = blockIdx.x / a.hk;

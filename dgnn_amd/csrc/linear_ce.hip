@@ -21,15 +21,21 @@ namespace dgnn {
 #define DGNN_LOG2E 1.44269504088896340736f
 
 // ------------------------------------------------------------------ one tile of C^T = A B^T
-// Block of 4 waves, 2 x 2, each BM / 2 x BN / 2; operands are staged BK k elements at a time,
-// double buffered.  An operand lies either with k along its rows (ROW: tile [BM][BK], read by row
-// fragments) or with k down its columns (tile [BK][BM], read by transposing column fragments).
-template <class T, int BM, int BN, int BK, bool AROW, bool BROW>
+// WM x WN waves, each BM / WM x BN / WN of the tile; operands are staged BK k elements at a time through
+// a ring of STAGES buffers.  An operand lies either with k along its rows (ROW: tile [BM][BK], read
+// by row fragments) or with k down its columns (tile [BK][BM], read by transposing column fragments).
+template <int BM_, int BN_, int BK_, int WM_, int WN_, int STAGES_>
+struct Shape {
+  static constexpr int BM = BM_, BN = BN_, BK = BK_, WM = WM_, WN = WN_, STAGES = STAGES_, THREADS = 64 * WM_ * WN_;
+  static constexpr int MB = BM / WM / 32, NB = BN / WN / 32;           // 32 x 32 blocks of a wave
+};
+
+template <class T, class C, bool AROW, bool BROW>
 struct Gemm {
-  static constexpr int THREADS = 256, MB = BM / 64, NB = BN / 64;      // 32 x 32 blocks of a wave
+  static constexpr int BM = C::BM, BN = C::BN, BK = C::BK, MB = C::MB, NB = C::NB, S = C::STAGES;
   using TA = Tile<T, AROW ? BK : BM>;
   using TB = Tile<T, BROW ? BK : BN>;
-  static constexpr int A_BYTES = BM * BK * (int)sizeof(T), B_BYTES = BN * BK * (int)sizeof(T), S = 2;
+  static constexpr int A_BYTES = BM * BK * (int)sizeof(T), B_BYTES = BN * BK * (int)sizeof(T);
   static constexpr int BYTES = A_BYTES + B_BYTES;      // of a stage
 
   // an operand: first element of the tile's rows (or columns), how many of them exist, row stride
@@ -37,20 +43,26 @@ struct Gemm {
     const T *p;
     int count;                    // rows (ROW) or columns that exist from p on
     unsigned stride;              // bytes between rows
+    const int *list = nullptr;    // ROW: the tile's rows are rows list[0 .. count) from p on
+    unsigned bytes = 0;           // with a list: what the matrix spans from p on
   };
 
   // acc[m][n] += over k in [0, kn)
-  __device__ static __forceinline__ void run(const Operand &a, const Operand &b, int kn, char *const (&lds)[S],
+  __device__ static __forceinline__ void run(const Operand &a, const Operand &b, int kn, char *const (&lds)[4],
                                              acc16 (&acc)[MB][NB]) {
     const int lane = lane_id(), wave = uniform_i32(wave_in_block());
-    const int m0 = (wave >> 1) * (BM / 2), n0 = (wave & 1) * (BN / 2);
-    // two row operands: consecutive k; against a column operand the order is its transposing read's
-    const int ra = AROW ? (BROW ? TA::row_lane(lane) : TA::row_lane_split(lane)) : TA::col_lane(lane);
-    const int rb = BROW ? (AROW ? TB::row_lane(lane) : TB::row_lane_split(lane)) : TB::col_lane(lane);
-    Stager<T, AROW ? BK : BM, AROW ? BM : BK, THREADS> sa;
-    Stager<T, BROW ? BK : BN, BROW ? BN : BK, THREADS> sb;
+    const int m0 = wave / C::WN * (BM / C::WM), n0 = wave % C::WN * (BN / C::WN);
+    // two row operands: consecutive k; against a column operand the order is its transposing read's.  The
+    // wave's first row or column is part of the lane's address.
+    const int ra = AROW ? (BROW ? TA::row_lane(lane) : TA::row_lane_split(lane)) + m0 * TA::ROW_BYTES
+                        : TA::col_lane(lane) ^ (m0 / TA::CHUNK << 4);
+    const int rb = BROW ? (AROW ? TB::row_lane(lane) : TB::row_lane_split(lane)) + n0 * TB::ROW_BYTES
+                        : TB::col_lane(lane) ^ (n0 / TB::CHUNK << 4);
+    Stager<T, AROW ? BK : BM, AROW ? BM : BK, C::THREADS> sa;
+    Stager<T, BROW ? BK : BN, BROW ? BN : BK, C::THREADS> sb;
     sa.init(a.stride, AROW ? min(BK, kn) : a.count);
-    sb.init(b.stride, BROW ? min(BK, kn) : b.count);
+    if (BROW && b.list) sb.init_list(b.list, b.count, b.stride, min(BK, kn));
+    else sb.init(b.stride, BROW ? min(BK, kn) : b.count);
     auto stage = [&](int t, auto i) {
       char *const ta = lds[i.value], *const tb = ta + A_BYTES;
       const int k0 = t * BK, left = max(0, min(BK, kn - k0));
@@ -58,14 +70,16 @@ struct Gemm {
       // drop the dword the end falls into
       const unsigned row_bytes = (left * (unsigned)sizeof(T) + 15u) & ~15u;
       if (left < BK && left > 0 && k0 > 0) {                       // the last, shorter step
-        if (AROW) sa.init(a.stride, left);
-        if (BROW) sb.init(b.stride, left);
+        if (AROW) sa.narrow(left);
+        if (BROW) sb.narrow(left);
       }
       if (AROW)
         sa.load(ta, buffer_over(a.p + k0, span_bytes(left > 0 ? min(a.count, BM) : 0, a.stride, row_bytes)));
       else
         sa.load(ta, buffer_over((const char *)a.p + (long long)k0 * a.stride, span_bytes(left, a.stride, min(a.count, BM) * (unsigned)sizeof(T))));
-      if (BROW)
+      if (BROW && b.list)
+        sb.load(tb, buffer_over(b.p + k0, left > 0 ? b.bytes - k0 * (unsigned)sizeof(T) : 0u));
+      else if (BROW)
         sb.load(tb, buffer_over(b.p + k0, span_bytes(left > 0 ? min(b.count, BN) : 0, b.stride, row_bytes)));
       else
         sb.load(tb, buffer_over((const char *)b.p + (long long)k0 * b.stride, span_bytes(left, b.stride, min(b.count, BN) * (unsigned)sizeof(T))));
@@ -76,24 +90,46 @@ struct Gemm {
       for (int k = 0; k < BK; k += 16) {
         frag8<T> fa[MB], fb[NB];
 #pragma unroll
-        for (int i = 0; i < MB; ++i) {
-          if constexpr (AROW) fa[i] = BROW ? TA::row_frag(ta, ra, m0 + 32 * i, k) : TA::row_frag_split(ta, ra, m0 + 32 * i, k);
-          else fa[i] = TA::col_frag(ta, ra, k, m0 + 32 * i);
+        for (int x = 0; x < MB; ++x) {
+          if constexpr (AROW) fa[x] = BROW ? TA::row_frag(ta, ra, 32 * x, k) : TA::row_frag_split(ta, ra, 32 * x, k);
+          else fa[x] = TA::col_frag(ta, ra, k, 32 * x);
         }
 #pragma unroll
-        for (int i = 0; i < NB; ++i) {
-          if constexpr (BROW) fb[i] = AROW ? TB::row_frag(tb, rb, n0 + 32 * i, k) : TB::row_frag_split(tb, rb, n0 + 32 * i, k);
-          else fb[i] = TB::col_frag(tb, rb, k, n0 + 32 * i);
+        for (int x = 0; x < NB; ++x) {
+          if constexpr (BROW) fb[x] = AROW ? TB::row_frag(tb, rb, 32 * x, k) : TB::row_frag_split(tb, rb, 32 * x, k);
+          else fb[x] = TB::col_frag(tb, rb, k, 32 * x);
         }
-#pragma unroll
-        for (int i = 0; i < MB; ++i)
-#pragma unroll
-          for (int j = 0; j < NB; ++j) acc[i][j] = mma(fa[i], fb[j], acc[i][j]);
+        mma_block<MB, NB, T>(fa, fb, acc, T());
       }
     };
     ring<S, decltype(sa)::LOADS + decltype(sb)::LOADS>((kn + BK - 1) / BK, stage, work);
   }
+  __device__ static __forceinline__ void clear(acc16 (&acc)[MB][NB]) {
+#pragma unroll
+    for (int i = 0; i < MB; ++i)
+#pragma unroll
+      for (int j = 0; j < NB; ++j) acc[i][j] = acc_zero();
+  }
 };
+
+// Which tile a workgroup takes.  Consecutive workgroups go to the eight XCDs in turn, so every XCD gets a
+// contiguous range of an order that runs over `m` tiles first inside bands of eight `n` tiles: the 32
+// workgroups of an XCD then read about 4 + 8 strips of the operands through its L2, not 1 + 32.
+struct TileAt {
+  int m, n;
+};
+__device__ __forceinline__ TileAt tile_at(unsigned id, int ms, int ns) {
+  const int u = (int)xcd_contiguous_id(id, (unsigned)ms * (unsigned)ns);
+  const int band = u / (ms * 8), width = min(8, ns - band * 8), r = u - band * ms * 8;
+  return {r / width, band * 8 + r % width};
+}
+
+// Tile shapes.  Wide: 16-bit types with enough tiles for every compute unit; two waves a SIMD, 128 KB of
+// LDS.  Thin: at most 32 rows, bound by reading the weight.  Plain: the rest, and float, whose matrix
+// instructions are sixteen times slower and bound every shape.
+using Wide = Shape<256, 256, 32, 2, 4, 4>;
+template <class T> using Plain = Shape<128, 128, sizeof(T) == 2 ? 64 : 16, 2, 2, sizeof(T) == 2 ? 2 : 3>;
+template <class T> using Thin = Shape<256, 32, sizeof(T) == 2 ? 64 : 32, 4, 1, 2>;
 
 // ------------------------------------------------------------------ labelled rows
 template <class I>
@@ -102,27 +138,45 @@ __device__ __forceinline__ int class_of(const I *label, int i, int classes, long
   return x != ignore && x >= 0 && x < classes ? (int)x : -1;
 }
 
-// list[j] = j-th labelled row, count[0] = how many; one workgroup, in order
+// list[j] = j-th labelled row, count[0] = how many; one workgroup, in order.  The rows without a label get
+// their loss and lse, 0, here.
 template <class I>
 __global__ __launch_bounds__(1024) void k_ce_rows(int n, int classes, long long ignore, const I *__restrict__ label,
-                                                  int *__restrict__ list, int *__restrict__ count) {
+                                                  int *__restrict__ list, int *__restrict__ count,
+                                                  float *__restrict__ loss, float *__restrict__ lse) {
+  constexpr int PER = 8;                        // labels a thread takes at a time
   __shared__ int part[16];
-  __shared__ int carry;
-  if (threadIdx.x == 0) carry = 0;
-  __syncthreads();
   const int lane = lane_id(), wave = wave_in_block();
-  for (int base = 0; base < n; base += 1024) {
-    const int i = base + threadIdx.x;
-    const bool on = i < n && class_of(label, i, classes, ignore) >= 0;
-    const unsigned long long b = __ballot(on);
-    if (lane == 0) part[wave] = __popcll(b);
+  int carry = 0;
+  for (int base = 0; base < n; base += 1024 * PER) {
+    const int i = base + threadIdx.x * PER;
+    unsigned on = 0;
+#pragma unroll
+    for (int k = 0; k < PER; ++k)
+      if (i + k < n) {
+        if (class_of(label, i + k, classes, ignore) >= 0) on |= 1u << k;
+        else if (lse) {
+          lse[i + k] = 0.f;
+          if (loss) loss[i + k] = 0.f;
+        }
+      }
+    const int own = __popc(on);
+    int incl = own;
+#pragma unroll
+    for (int w = 1; w < 64; w <<= 1) {
+      const int up = __shfl_up(incl, w, 64);
+      if (lane >= w) incl += up;
+    }
+    if (lane == 63) part[wave] = incl;
     __syncthreads();
-    int at = carry;
-    for (int w = 0; w < wave; ++w) at += part[w];
-    if (on) list[at + __popcll(b & ((1ULL << lane) - 1))] = i;
-    __syncthreads();
-    if (threadIdx.x == 0)
-      for (int w = 0; w < 16; ++w) carry += part[w];
+    int at = carry + incl - own;
+    for (int w = 0; w < 16; ++w) {
+      if (w < wave) at += part[w];
+      carry += part[w];
+    }
+#pragma unroll
+    for (int k = 0; k < PER; ++k)
+      if (on >> k & 1) list[at++] = i + k;
     __syncthreads();
   }
   if (threadIdx.x == 0) count[0] = carry;
@@ -151,11 +205,11 @@ __global__ __launch_bounds__(DGNN_BLOCK) void k_ce_gather(int n, int d, int ldt,
 }
 
 struct CeArgs {
-  const void *x, *w;              // gathered rows [n, ldx], weight [classes, ldw]
+  const void *x, *w;              // rows [n, dk] (gathered: only those with a label), weight [classes, dk]
+  int gathered;
   const void *label;
   const int *list, *count;
   int n, classes, d, dk;          // dk = d rounded up to whole chunks
-  long long ldw;                  // elements
   int label_bytes;
   float *part_m, *part_s;         // [class tiles, n]
   float *z_label;                 // [n], by gathered row
@@ -166,7 +220,7 @@ struct CeArgs {
   void *dz;                       // [n, ldz]
   int v0, vn, ldz;                // piece of the classes
   float *acc;                     // split sums [splits][rows][d]
-  int splits, first;
+  int splits, first, direct;      // direct: one split of one piece, results go where they belong
   void *dx, *dw;
 };
 
@@ -211,97 +265,105 @@ __global__ __launch_bounds__(1024) void k_ce_grad_top(int n, const int *__restri
   }
 }
 
-template <class T> constexpr int ce_bk() { return sizeof(T) == 2 ? 64 : 32; }
-constexpr int CE_BM = 128, CE_BN = 128;
+// the rows' operand of z
+template <class T, class G>
+__device__ __forceinline__ typename G::Operand rows_operand(const CeArgs &a, int r0, int rows) {
+  const unsigned stride = (unsigned)(a.dk * sizeof(T));
+  if (a.gathered) return {(const T *)a.x + (long long)r0 * a.dk, rows - r0, stride};
+  return {(const T *)a.x, rows - r0, stride, a.list + r0, a.n * stride};
+}
 
 // Forward: classes along m, rows along n.  Leaves the tile's maximum and sum of exp for every row and
 // the logit of its label.
-template <class T>
-__global__ __launch_bounds__(256) void k_ce_fwd(const CeArgs a) {
-  using G = Gemm<T, CE_BM, CE_BN, ce_bk<T>(), true, true>;
-  DGNN_RING2(lds, G::BYTES);
-  __shared__ float sm[2][CE_BN], ss[2][CE_BN];
-  const int vt = blockIdx.x, v0 = vt * CE_BM, r0 = blockIdx.y * CE_BN;
+template <class T, class C>
+__global__ __launch_bounds__(C::THREADS, C::THREADS == 512 ? 2 : 1) void k_ce_fwd(const CeArgs a) {
+  using G = Gemm<T, C, true, true>;
+  DGNN_RING(lds, G::BYTES);
+  __shared__ float sm[C::WM][C::BN], ss[C::WM][C::BN];
+  const TileAt tile = tile_at(blockIdx.x, (a.classes + C::BM - 1) / C::BM, (a.n + C::BN - 1) / C::BN);
+  const int v0 = tile.m * C::BM, r0 = tile.n * C::BN;
   const int rows = min(a.n, *a.count);
   if (r0 >= rows) return;
-  acc16 acc[G::MB][G::NB];
-#pragma unroll
-  for (int i = 0; i < G::MB; ++i)
-#pragma unroll
-    for (int j = 0; j < G::NB; ++j) acc[i][j] = acc_zero();
-  G::run({(const T *)a.w + (long long)v0 * a.ldw, a.classes - v0, (unsigned)(a.ldw * sizeof(T))},
-         {(const T *)a.x + (long long)r0 * a.dk, rows - r0, (unsigned)(a.dk * sizeof(T))}, a.dk, lds, acc);
+  acc16 acc[C::MB][C::NB];
+  G::clear(acc);
+  G::run({(const T *)a.w + (long long)v0 * a.dk, a.classes - v0, (unsigned)(a.dk * sizeof(T))},
+         rows_operand<T, G>(a, r0, rows), a.dk, lds, acc);
   const int lane = lane_id(), h = lane >> 5, wave = uniform_i32(wave_in_block());
-  const int m0 = v0 + (wave >> 1) * (CE_BM / 2), n0 = (wave & 1) * (CE_BN / 2);
+  const int wm = wave / C::WN, m0 = v0 + wm * (C::BM / C::WM), n0 = wave % C::WN * (C::BN / C::WN);
+  const bool whole = v0 + C::BM <= a.classes;
 #pragma unroll
-  for (int j = 0; j < G::NB; ++j) {
+  for (int j = 0; j < C::NB; ++j) {
     const int col = n0 + 32 * j + (lane & 31), r = r0 + col;
-    const long long want = r < rows ? label_at(a, a.list[r]) : -1;
+    const long long want = r < rows ? label_at(a, a.list[r]) - m0 : -1;
     float top = -INFINITY;
+    if (want >= 0 && want < C::BM / C::WM) {
 #pragma unroll
-    for (int i = 0; i < G::MB; ++i)
+      for (int i = 0; i < C::MB; ++i)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const int v = m0 + 32 * i + acc_row(e, h);
-        if (v == want) a.z_label[r] = acc[i][j][e];
-        if (v >= a.classes) acc[i][j][e] = -INFINITY;
-        top = fmaxf(top, acc[i][j][e]);
-      }
+        for (int e = 0; e < 16; ++e)
+          if (32 * i + acc_row(e, h) == (int)want) a.z_label[r] = acc[i][j][e];
+    }
+    if (!whole) {
+#pragma unroll
+      for (int i = 0; i < C::MB; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if (m0 + 32 * i + acc_row(e, h) >= a.classes) acc[i][j][e] = -INFINITY;
+    }
+#pragma unroll
+    for (int i = 0; i < C::MB; ++i)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) top = fmaxf(top, acc[i][j][e]);
     top = fmaxf(top, __shfl_xor(top, 32, 64));
     const float base = top == -INFINITY ? 0.f : top * DGNN_LOG2E;
     float sum = 0.f;
 #pragma unroll
-    for (int i = 0; i < G::MB; ++i)
+    for (int i = 0; i < C::MB; ++i)
 #pragma unroll
       for (int e = 0; e < 16; ++e) sum += __builtin_amdgcn_exp2f(fmaf(acc[i][j][e], DGNN_LOG2E, -base));
     sum += __shfl_xor(sum, 32, 64);
-    if (h == 0) sm[wave >> 1][col] = top, ss[wave >> 1][col] = sum;
+    if (h == 0) sm[wm][col] = top, ss[wm][col] = sum;
   }
   __syncthreads();
-  if (threadIdx.x < CE_BN && r0 + (int)threadIdx.x < rows) {
-    const float m_a = sm[0][threadIdx.x], m_b = sm[1][threadIdx.x], top = fmaxf(m_a, m_b);
+  if (threadIdx.x < C::BN && r0 + (int)threadIdx.x < rows) {
+    float top = sm[0][threadIdx.x], s = 0.f;
+#pragma unroll
+    for (int w = 1; w < C::WM; ++w) top = fmaxf(top, sm[w][threadIdx.x]);
     const float base = top == -INFINITY ? 0.f : top;
-    const float s = ss[0][threadIdx.x] * __builtin_amdgcn_exp2f((m_a - base) * DGNN_LOG2E) +
-                    ss[1][threadIdx.x] * __builtin_amdgcn_exp2f((m_b - base) * DGNN_LOG2E);
-    const long long at = (long long)vt * a.n + r0 + threadIdx.x;
+#pragma unroll
+    for (int w = 0; w < C::WM; ++w) s += ss[w][threadIdx.x] * __builtin_amdgcn_exp2f((sm[w][threadIdx.x] - base) * DGNN_LOG2E);
+    const long long at = (long long)tile.m * a.n + r0 + threadIdx.x;
     a.part_m[at] = top;
     a.part_s[at] = s;
   }
 }
 
-// lse and loss of every row from its tiles' pairs, one wave a gathered row; rows without a label get 0
-// (they are not in the list, so the fill comes first)
-__global__ __launch_bounds__(DGNN_BLOCK) void k_ce_fill(int n, float *__restrict__ loss, float *__restrict__ lse) {
-  const int i = blockIdx.x * DGNN_BLOCK + threadIdx.x;
-  if (i < n) {
-    if (loss) loss[i] = 0.f;
-    lse[i] = 0.f;
-  }
-}
+// lse and loss of every labelled row from its tiles' pairs: eight rows a workgroup, 32 threads a row
 __global__ __launch_bounds__(DGNN_BLOCK) void k_ce_join(int n, int tiles, const int *__restrict__ list,
                                                         const int *__restrict__ count, const float *__restrict__ pm,
                                                         const float *__restrict__ ps, const float *__restrict__ z_label,
                                                         float *__restrict__ loss, float *__restrict__ lse) {
-  // 64 rows a workgroup, the tiles dealt to its four waves
-  __shared__ float sm[DGNN_WAVES_PER_BLOCK][DGNN_WAVE], ss[DGNN_WAVES_PER_BLOCK][DGNN_WAVE];
-  const int lane = lane_id(), wave = wave_in_block(), r = blockIdx.x * DGNN_WAVE + lane, rows = min(n, *count);
-  if ((int)blockIdx.x * DGNN_WAVE >= rows) return;
+  __shared__ float sm[32][8], ss[32][8];
+  const int c = threadIdx.x & 7, lane = threadIdx.x >> 3, r = blockIdx.x * 8 + c, rows = min(n, *count);
+  if ((int)blockIdx.x * 8 >= rows) return;
   float m = -INFINITY, s = 0.f;
-  if (r < rows)
-    for (int t = wave; t < tiles; t += DGNN_WAVES_PER_BLOCK) {
+  if (r < rows) {
+#pragma unroll 4
+    for (int t = lane; t < tiles; t += 32) {
       const float tm = pm[(long long)t * n + r], ts = ps[(long long)t * n + r], top = fmaxf(m, tm);
       const float base = top == -INFINITY ? 0.f : top;
       s = s * expf(m - base) + ts * expf(tm - base);
       m = top;
     }
-  sm[wave][lane] = m, ss[wave][lane] = s;
+  }
+  sm[lane][c] = m, ss[lane][c] = s;
   __syncthreads();
-  if (wave != 0 || r >= rows) return;
-  float top = sm[0][lane];
-  for (int w = 1; w < DGNN_WAVES_PER_BLOCK; ++w) top = fmaxf(top, sm[w][lane]);
+  if (lane != 0 || r >= rows) return;
+  float top = sm[0][c];
+  for (int w = 1; w < 32; ++w) top = fmaxf(top, sm[w][c]);
   const float base = top == -INFINITY ? 0.f : top;
   float sum = 0.f;
-  for (int w = 0; w < DGNN_WAVES_PER_BLOCK; ++w) sum += ss[w][lane] * expf(sm[w][lane] - base);
+  for (int w = 0; w < 32; ++w) sum += ss[w][c] * expf(sm[w][c] - base);
   const float v = base + logf(sum);
   lse[list[r]] = v;
   loss[list[r]] = v - z_label[r];
@@ -321,106 +383,159 @@ __global__ __launch_bounds__(1024) void k_ce_reduce(int n, int mean, const int *
   }
 }
 
-// dz of a piece of the classes, [rows, ldz]; columns behind the piece's last class are zeros
-template <class T>
-__global__ __launch_bounds__(256) void k_ce_dz(const CeArgs a) {
-  using G = Gemm<T, CE_BM, CE_BN, ce_bk<T>(), true, true>;
-  DGNN_RING2(lds, G::BYTES);
-  const int p0 = blockIdx.x * CE_BM, v0 = a.v0 + p0, r0 = blockIdx.y * CE_BN;
-  const int rows = min(a.n, *a.count);
-  if (r0 >= rows) return;
-  acc16 acc[G::MB][G::NB];
-#pragma unroll
-  for (int i = 0; i < G::MB; ++i)
-#pragma unroll
-    for (int j = 0; j < G::NB; ++j) acc[i][j] = acc_zero();
-  G::run({(const T *)a.w + (long long)v0 * a.ldw, a.classes - v0, (unsigned)(a.ldw * sizeof(T))},
-         {(const T *)a.x + (long long)r0 * a.dk, rows - r0, (unsigned)(a.dk * sizeof(T))}, a.dk, lds, acc);
+// Turns a workgroup's C^T tile into rows of T through LDS, 32 rows of every wave column at a time in a ring
+// buffer of its own, and hands 16-byte pieces to sink(row, column, piece): a lane holds four elements of
+// one row, and stored from there every instruction would touch 32 rows.  The ring is drained by then.
+template <class T, class C, class Value, class Sink>
+__device__ __forceinline__ void rows_of_tile(char *const (&lds)[4], const Value &value, const Sink &sink) {
+  using TL = Tile<T, C::BM>;
+  constexpr int PIECES = 32 * TL::CPR;
   const int lane = lane_id(), h = lane >> 5, wave = uniform_i32(wave_in_block());
-  const int m0 = p0 + (wave >> 1) * (CE_BM / 2), n0 = (wave & 1) * (CE_BN / 2);
-  const CeScale scale = ce_scale<T>(a, rows);
+  const int wm = wave / C::WN, wn = wave % C::WN, m0 = wm * (C::BM / C::WM);
 #pragma unroll
-  for (int j = 0; j < G::NB; ++j) {
-    const int r = r0 + n0 + 32 * j + (lane & 31);
-    if (r >= rows) continue;
-    const int row = a.list[r];
-    const int want = (int)label_at(a, row) - a.v0;
-    const float lse = a.lse[row] * DGNN_LOG2E;
-    const float g = a.grad[a.grad_rows ? row : 0] * scale.by;
+  for (int j = 0; j < C::NB; ++j) {
+    __syncthreads();
+    unrolled<0, C::WN>([&](auto b) {
+      if (wn != b.value) return;
+      char *const buf = lds[b.value];
 #pragma unroll
-    for (int i = 0; i < G::MB; ++i)
+      for (int i = 0; i < C::MB; ++i)
 #pragma unroll
-      for (int e4 = 0; e4 < 4; ++e4) {
-        const int p = m0 + 32 * i + 8 * e4 + 4 * h;
-        vec4<T> v;
+        for (int e4 = 0; e4 < 4; ++e4) {
+          const int m = m0 + 32 * i + 8 * e4 + 4 * h;
+          vec4<T> v;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          float y = __builtin_amdgcn_exp2f(fmaf(acc[i][j][4 * e4 + e], DGNN_LOG2E, -lse));
-          if (p + e == want) y -= 1.f;
-          v[e] = p + e < a.vn ? (T)(y * g) : (T)0.f;
+          for (int e = 0; e < 4; ++e) v[e] = value(i, j, 4 * e4 + e, m + e);
+          *(vec4<T> *)(buf + TL::chunk_addr(lane & 31, m / TL::CHUNK) + m % TL::CHUNK * (int)sizeof(T)) = v;
         }
-        if (p < a.ldz) *(vec4<T> *)((T *)a.dz + (long long)r * a.ldz + p) = v;
+    });
+    __syncthreads();
+    unrolled<0, C::WN>([&](auto b) {
+      if (wn != b.value) return;
+      const char *const buf = lds[b.value];
+      for (int u = wm * 64 + lane; u < PIECES; u += C::WM * 64) {
+        const int row = u / TL::CPR, chunk = u % TL::CPR;
+        sink(wn * (C::BN / C::WN) + 32 * j + row, chunk * TL::CHUNK, *(const u32x4 *)(buf + TL::chunk_addr(row, chunk)));
       }
+    });
+  }
+}
+// A piece of a row: as one store, or the elements of it that exist.
+template <class T>
+__device__ __forceinline__ void store_piece(T *row, int col, int cols, u32x4 piece, bool whole) {
+  constexpr int VEC = 16 / sizeof(T);
+  if (whole) {
+    if (col < cols) *(u32x4 *)(row + col) = piece;
+  } else {
+    T v[VEC];
+    *(u32x4 *)v = piece;
+#pragma unroll
+    for (int k = 0; k < VEC; ++k)
+      if (col + k < cols) row[col + k] = v[k];
   }
 }
 
-// Stores a lane's column of C^T (four consecutive m a group) to row `to`, columns m0 .. < d.
-template <class T, int MB>
-__device__ __forceinline__ void store_col(T *to, const acc16 (&c)[MB], float by, int m0, int d, int h, bool wide) {
+// dz of a piece of the classes, [rows, ldz]; columns behind the piece's last class are zeros
+template <class T, class C>
+__global__ __launch_bounds__(C::THREADS, C::THREADS == 512 ? 2 : 1) void k_ce_dz(const CeArgs a) {
+  using G = Gemm<T, C, true, true>;
+  static_assert(32 * C::BM * sizeof(T) <= G::BYTES && C::WN <= 4, "the tile as rows fits the ring");
+  DGNN_RING(lds, G::BYTES);
+  const TileAt tile = tile_at(blockIdx.x, a.ldz / C::BM, (a.n + C::BN - 1) / C::BN);
+  const int p0 = tile.m * C::BM, v0 = a.v0 + p0, r0 = tile.n * C::BN;
+  const int rows = min(a.n, *a.count);
+  if (r0 >= rows) return;
+  acc16 acc[C::MB][C::NB];
+  G::clear(acc);
+  G::run({(const T *)a.w + (long long)v0 * a.dk, a.classes - v0, (unsigned)(a.dk * sizeof(T))},
+         rows_operand<T, G>(a, r0, rows), a.dk, lds, acc);
+  const int lane = lane_id(), wave = uniform_i32(wave_in_block()), n0 = wave % C::WN * (C::BN / C::WN);
+  const CeScale scale = ce_scale<T>(a, rows);
+  float lse[C::NB], g[C::NB];
+  int want[C::NB];
 #pragma unroll
-  for (int i = 0; i < MB; ++i)
+  for (int j = 0; j < C::NB; ++j) {
+    const int r = r0 + n0 + 32 * j + (lane & 31), row = r < rows ? a.list[r] : a.list[0];
+    want[j] = (int)(label_at(a, row) - v0);
+    lse[j] = a.lse[row] * DGNN_LOG2E;
+    g[j] = a.grad[a.grad_rows ? row : 0] * scale.by;
+  }
+  const int left = a.vn - p0;                   // classes of this tile
+  rows_of_tile<T, C>(
+      lds,
+      [&](int i, int j, int e, int m) {
+        float y = __builtin_amdgcn_exp2f(fmaf(acc[i][j][e], DGNN_LOG2E, -lse[j]));
+        y = m == want[j] ? y - 1.f : y;
+        return (T)(m < left ? y * g[j] : 0.f);
+      },
+      [&](int row, int col, u32x4 piece) {
+        if (r0 + row < rows) *(u32x4 *)((T *)a.dz + (long long)(r0 + row) * a.ldz + p0 + col) = piece;
+      });
+}
+
+// A lane's columns of C^T as rows of partial sums: row r at acc + r * ld, columns m0 .. < d.
+template <class C>
+__device__ __forceinline__ void store_sums(float *to, const acc16 (&acc)[C::MB][C::NB], int j, int m0, int d, int h) {
+#pragma unroll
+  for (int i = 0; i < C::MB; ++i)
 #pragma unroll
     for (int e4 = 0; e4 < 4; ++e4) {
       const int at = m0 + 32 * i + 8 * e4 + 4 * h;
-      if (wide) {
-        vec4<T> v;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = (T)(c[i][4 * e4 + e] * by);
-        if (at < d) *(vec4<T> *)(to + at) = v;
-      } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (at + e < d) to[at + e] = (T)(c[i][4 * e4 + e] * by);
-      }
+      const acc16 &c = acc[i][j];
+      if (at < d) *(float4 *)(to + at) = make_float4(c[4 * e4], c[4 * e4 + 1], c[4 * e4 + 2], c[4 * e4 + 3]);
     }
 }
 
-// dx of a piece: C^T[d, rows] += W_piece^T dz^T.  splits == 1 and one piece: straight to dx; else into
-// acc[split], continued over the pieces, joined by k_ce_join_acc.
-template <class T>
-__global__ __launch_bounds__(256) void k_ce_dx(const CeArgs a) {
-  constexpr int BK = ce_bk<T>();
-  using G = Gemm<T, CE_BM, CE_BN, BK, false, true>;
-  DGNN_RING2(lds, G::BYTES);
-  const int c0 = blockIdx.x * CE_BM, r0 = blockIdx.y * CE_BN, split = blockIdx.z;
+// dx of a piece: C^T[d, rows] += W_piece^T dz^T.  One split of a single piece: straight to dx; else into
+// acc[split], continued over the pieces, joined by k_ce_dx_join.
+template <class T, class C>
+__global__ __launch_bounds__(C::THREADS, C::THREADS == 512 ? 2 : 1) void k_ce_dx(const CeArgs a, int whole) {
+  using G = Gemm<T, C, false, true>;
+  DGNN_RING(lds, G::BYTES);
+  const int ms = (a.dk + C::BM - 1) / C::BM, ns = (a.n + C::BN - 1) / C::BN;
+  const int split = blockIdx.x / (ms * ns);
+  const TileAt tile = tile_at(blockIdx.x % (ms * ns), ms, ns);
+  const int c0 = tile.m * C::BM, r0 = tile.n * C::BN;
   const int rows = min(a.n, *a.count);
   if (r0 >= rows) return;
   const int lane = lane_id(), h = lane >> 5, wave = uniform_i32(wave_in_block());
-  const int m0 = c0 + (wave >> 1) * (CE_BM / 2), n0 = (wave & 1) * (CE_BN / 2);
-  acc16 acc[G::MB][G::NB];
+  const int m0 = c0 + wave / C::WN * (C::BM / C::WM), n0 = wave % C::WN * (C::BN / C::WN);
+  acc16 acc[C::MB][C::NB];
+  G::clear(acc);
+  if (!a.first) {
 #pragma unroll
-  for (int j = 0; j < G::NB; ++j) {
-    const int r = r0 + n0 + 32 * j + (lane & 31);
-    const float *old = a.acc + ((long long)split * a.n + r) * a.dk;
+    for (int j = 0; j < C::NB; ++j) {
+      const int r = r0 + n0 + 32 * j + (lane & 31);
+      const float *old = a.acc + ((long long)split * a.n + r) * a.dk;
 #pragma unroll
-    for (int i = 0; i < G::MB; ++i)
+      for (int i = 0; i < C::MB; ++i)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const int c = m0 + 32 * i + acc_row(e, h);
-        acc[i][j][e] = !a.first && r < rows && c < a.dk ? old[c] : 0.f;
-      }
+        for (int e4 = 0; e4 < 4; ++e4) {
+          const int c = m0 + 32 * i + 8 * e4 + 4 * h;
+          if (r < rows && c < a.dk) {
+            const float4 v = *(const float4 *)(old + c);
+            acc[i][j][4 * e4] = v.x, acc[i][j][4 * e4 + 1] = v.y, acc[i][j][4 * e4 + 2] = v.z, acc[i][j][4 * e4 + 3] = v.w;
+          }
+        }
+    }
   }
-  const int steps = (a.vn + BK - 1) / BK, per = (steps + a.splits - 1) / a.splits;
-  const int ka = min(a.vn, split * per * BK), kb = min(a.vn, (split + 1) * per * BK);
-  G::run({(const T *)a.w + (long long)(a.v0 + ka) * a.ldw + c0, a.dk - c0, (unsigned)(a.ldw * sizeof(T))},
+  const int steps = (a.vn + C::BK - 1) / C::BK, per = (steps + a.splits - 1) / a.splits;
+  const int ka = min(a.vn, split * per * C::BK), kb = min(a.vn, (split + 1) * per * C::BK);
+  G::run({(const T *)a.w + (long long)(a.v0 + ka) * a.dk + c0, a.dk - c0, (unsigned)(a.dk * sizeof(T))},
          {(const T *)a.dz + (long long)r0 * a.ldz + ka, rows - r0, (unsigned)(a.ldz * sizeof(T))}, kb - ka, lds, acc);
+  if (a.direct) {
+    const float unit = ce_scale<T>(a, rows).unit;
+    rows_of_tile<T, C>(
+        lds, [&](int i, int j, int e, int) { return (T)(acc[i][j][e] * unit); },
+        [&](int row, int col, u32x4 piece) {
+          if (r0 + row < rows) store_piece<T>((T *)a.dx + (long long)a.list[r0 + row] * a.d, c0 + col, a.d, piece, whole != 0);
+        });
+    return;
+  }
 #pragma unroll
-  for (int j = 0; j < G::NB; ++j) {
+  for (int j = 0; j < C::NB; ++j) {
     const int r = r0 + n0 + 32 * j + (lane & 31);
-    acc16 col[G::MB];
-#pragma unroll
-    for (int i = 0; i < G::MB; ++i) col[i] = acc[i][j];
-    if (r < rows) store_col<float, G::MB>(a.acc + ((long long)split * a.n + r) * a.dk, col, 1.f, m0, a.dk, h, true);
+    if (r < rows) store_sums<C>(a.acc + ((long long)split * a.n + r) * a.dk, acc, j, m0, a.dk, h);
   }
 }
 // dx[list[r]] = sum over the splits, in order
@@ -453,34 +568,36 @@ __global__ __launch_bounds__(DGNN_BLOCK) void k_ce_dx_zero(const CeArgs a, long 
 }
 
 // dW of a piece: C^T[d, classes of the piece] = x^T dz.  splits > 1: partial sums over shares of the rows.
-template <class T>
-__global__ __launch_bounds__(256) void k_ce_dw(const CeArgs a, int wide) {
-  constexpr int BK = ce_bk<T>();
-  using G = Gemm<T, CE_BM, CE_BN, BK, false, false>;
-  DGNN_RING2(lds, G::BYTES);
-  const int c0 = blockIdx.x * CE_BM, p0 = blockIdx.y * CE_BN, split = blockIdx.z;
+template <class T, class C>
+__global__ __launch_bounds__(C::THREADS, C::THREADS == 512 ? 2 : 1) void k_ce_dw(const CeArgs a, int whole) {
+  using G = Gemm<T, C, false, false>;
+  DGNN_RING(lds, G::BYTES);
+  const int ms = (a.dk + C::BM - 1) / C::BM, ns = (a.vn + C::BN - 1) / C::BN;
+  const int split = blockIdx.x / (ms * ns);
+  const TileAt tile = tile_at(blockIdx.x % (ms * ns), ms, ns);
+  const int c0 = tile.m * C::BM, p0 = tile.n * C::BN;
   const int rows = min(a.n, *a.count);
-  acc16 acc[G::MB][G::NB];
-#pragma unroll
-  for (int i = 0; i < G::MB; ++i)
-#pragma unroll
-    for (int j = 0; j < G::NB; ++j) acc[i][j] = acc_zero();
-  const int steps = (rows + BK - 1) / BK, per = (steps + a.splits - 1) / a.splits;
-  const int ka = min(rows, split * per * BK), kb = min(rows, (split + 1) * per * BK);
+  acc16 acc[C::MB][C::NB];
+  G::clear(acc);
+  const int steps = (rows + C::BK - 1) / C::BK, per = (steps + a.splits - 1) / a.splits;
+  const int ka = min(rows, split * per * C::BK), kb = min(rows, (split + 1) * per * C::BK);
   G::run({(const T *)a.x + (long long)ka * a.dk + c0, a.dk - c0, (unsigned)(a.dk * sizeof(T))},
          {(const T *)a.dz + (long long)ka * a.ldz + p0, a.ldz - p0, (unsigned)(a.ldz * sizeof(T))}, kb - ka, lds, acc);
+  if (a.splits == 1) {
+    const float unit = ce_scale<T>(a, rows).unit;
+    rows_of_tile<T, C>(
+        lds, [&](int i, int j, int e, int) { return (T)(acc[i][j][e] * unit); },
+        [&](int row, int col, u32x4 piece) {
+          if (p0 + row < a.vn) store_piece<T>((T *)a.dw + (long long)(a.v0 + p0 + row) * a.d, c0 + col, a.d, piece, whole != 0);
+        });
+    return;
+  }
   const int lane = lane_id(), h = lane >> 5, wave = uniform_i32(wave_in_block());
-  const int m0 = c0 + (wave >> 1) * (CE_BM / 2), n0 = (wave & 1) * (CE_BN / 2);
-  const float unit = ce_scale<T>(a, rows).unit;
+  const int m0 = c0 + wave / C::WN * (C::BM / C::WM), n0 = wave % C::WN * (C::BN / C::WN);
 #pragma unroll
-  for (int j = 0; j < G::NB; ++j) {
+  for (int j = 0; j < C::NB; ++j) {
     const int p = p0 + n0 + 32 * j + (lane & 31);
-    acc16 col[G::MB];
-#pragma unroll
-    for (int i = 0; i < G::MB; ++i) col[i] = acc[i][j];
-    if (p >= a.vn) continue;
-    if (a.splits == 1) store_col<T, G::MB>((T *)a.dw + (long long)(a.v0 + p) * a.d, col, unit, m0, a.d, h, wide != 0);
-    else store_col<float, G::MB>(a.acc + ((long long)split * a.ldz + p) * a.dk, col, 1.f, m0, a.dk, h, true);
+    if (p < a.vn) store_sums<C>(a.acc + ((long long)split * a.ldz + p) * a.dk, acc, j, m0, a.dk, h);
   }
 }
 template <class T>
@@ -510,47 +627,64 @@ static inline unsigned grid_for(long long units) {
   return (unsigned)(b < 1 ? 1 : b > 8192 ? 8192 : b);
 }
 
+enum CeShape { CE_PLAIN, CE_WIDE, CE_THIN };
 struct CePlan {
-  int dk, tiles, copy_w;                              // class tiles of the forward
-  size_t list, x, w, part, zl, lossrow, fwd_total;    // bytes
-  int piece, ldz, dx_splits, dw_splits;
+  int dk, tiles, copy_w, gather;                      // class tiles of the forward
+  CeShape z, dx_shape, dw_shape;
+  size_t list, x, w, part, zl, fwd_total;             // bytes
+  int piece, pieces, dx_splits, dw_splits;
   size_t dz, dxacc, dwacc, bwd_total;
 };
-static CePlan ce_plan(int dtype, int n, int classes, int d, int aligned_w) {
+// Wide tiles halve what every product reads from LDS, but there have to be enough of them for 256 compute
+// units; `tiles` counts 256 x 256 ones.  Measured at 8192 x 50000 x 1024 bfloat16: see k_ce_fwd.
+static CeShape ce_shape(int dtype, long long m, long long n, long long splits) {
+  const long long wide = ((m + 255) / 256) * ((n + 255) / 256) * splits;
+  return dtype != DGNN_F32 && wide >= 256 ? CE_WIDE : CE_PLAIN;
+}
+static CePlan ce_plan(int dtype, int n, int classes, int d, const void *x, const void *w) {
   CePlan p;
   memset(&p, 0, sizeof(p));
   const int size = dtype == DGNN_F32 ? 4 : 2, vec = 16 / size;
   p.dk = (d + vec - 1) / vec * vec;
-  p.copy_w = !aligned_w || p.dk != d;
-  p.tiles = ceil_div(classes, CE_BM);
+  // rows are read where they are if they are whole, aligned chunks within 32-bit offsets
+  p.copy_w = p.dk != d || ((uintptr_t)w & 15) != 0;
+  p.gather = p.dk != d || ((uintptr_t)x & 15) != 0 || (long long)n * p.dk * size >= 0x7fffffffLL;
+  p.z = n <= 32 ? CE_THIN : ce_shape(dtype, classes, n, 1);
+  p.tiles = ceil_div(classes, p.z == CE_PLAIN ? 128 : 256);
   p.list = align256(sizeof(int) * ((size_t)n + 1));
   p.x = align256((size_t)n * p.dk * size);
   p.w = p.copy_w ? align256((size_t)classes * p.dk * size) : 0;
   p.part = align256(sizeof(float) * (size_t)p.tiles * n);
   p.zl = align256(sizeof(float) * (size_t)n);
-  p.lossrow = p.zl;
-  p.fwd_total = p.list + p.x + p.w + 2 * p.part + 2 * p.zl;
-  // pieces: dz of about 256 MB, whole tiles
-  long long cols = (256LL << 20) / ((long long)size * (n > 0 ? n : 1));
-  cols = cols < 1024 ? 1024 : cols;
-  if (cols > (1 << 20)) cols = 1 << 20;        // 128 rows of a piece stay inside 32-bit offsets
+  p.fwd_total = p.list + (p.gather ? p.x : 0) + p.w + 2 * p.part + 2 * p.zl;
+  // pieces: dz of about 384 MB, whole tiles; at most 2^20 columns: 256 rows of a piece stay in 32-bit offsets
+  long long cols = (384LL << 20) / ((long long)size * n);
+  cols = cols < 1024 ? 1024 : cols > (1 << 20) ? 1 << 20 : cols;
   if (cols > classes) cols = classes;
-  const int pieces = ceil_div(classes, cols);
-  p.piece = ceil_div(ceil_div(classes, pieces), CE_BM) * CE_BM;
-  p.ldz = p.piece;
-  // enough workgroups for 256 compute units: split the long axis while tiles are few
-  const long long dx_tiles = (long long)ceil_div(p.dk, CE_BM) * ceil_div(n, CE_BN);
-  const long long dw_tiles = (long long)ceil_div(p.dk, CE_BM) * ceil_div(p.piece, CE_BN);
+  p.piece = ceil_div(ceil_div(classes, ceil_div(classes, cols)), 256) * 256;
+  p.pieces = ceil_div(classes, p.piece);
+  // enough workgroups for every compute unit: split the long axis while tiles are few
   auto splits = [](long long tiles, int steps) {
     long long s = tiles > 0 ? 512 / tiles : 1;
     if (s > steps / 4) s = steps / 4;
     return (int)(s < 1 ? 1 : s > 64 ? 64 : s);
   };
-  p.dx_splits = splits(dx_tiles, p.piece / 64);
-  p.dw_splits = splits(dw_tiles, n / 64);
-  p.dz = align256((size_t)n * p.ldz * size);
-  p.dxacc = align256(sizeof(float) * (size_t)p.dx_splits * n * p.dk);
-  p.dwacc = p.dw_splits > 1 ? align256(sizeof(float) * (size_t)p.dw_splits * p.ldz * p.dk) : 0;
+  auto choose = [&](long long cols_of, int steps, CeShape *shape, int *split) {
+    const long long wide = (long long)ceil_div(p.dk, 256) * ceil_div(cols_of, 256);
+    // a wide tile is worth having if splitting the long axis still gives every compute unit one
+    const int s = wide >= 256 ? 1 : (int)((256 + wide - 1) / wide);
+    if (dtype != DGNN_F32 && s <= 4 && steps / s >= 16 && p.dk > 128) {
+      *shape = CE_WIDE, *split = s;
+    } else {
+      *shape = CE_PLAIN;
+      *split = splits((long long)ceil_div(p.dk, 128) * ceil_div(cols_of, 128), steps);
+    }
+  };
+  choose(n, p.piece / 64, &p.dx_shape, &p.dx_splits);
+  choose(p.piece, n / 64, &p.dw_shape, &p.dw_splits);
+  p.dz = align256((size_t)n * p.piece * size);
+  p.dxacc = p.dx_splits > 1 || p.pieces > 1 ? align256(sizeof(float) * (size_t)p.dx_splits * n * p.dk) : 0;
+  p.dwacc = p.dw_splits > 1 ? align256(sizeof(float) * (size_t)p.dw_splits * p.piece * p.dk) : 0;
   p.bwd_total = p.list + p.x + p.w + p.dz + p.dxacc + p.dwacc + 256;
   return p;
 }
@@ -561,49 +695,62 @@ static int ce_check(int dtype, int label_bytes, int n, int classes, int d) {
   return DGNN_OK;
 }
 
-// labelled rows -> list, count, gathered x; padded weight where its rows are not whole chunks
+// labelled rows -> list, count; gathered x where asked; padded weight where its rows are not whole chunks
 template <class T>
-static int ce_prepare(const CePlan &p, int n, int classes, int d, const void *x, const void *w, const void *label,
-                      int label_bytes, long long ignore, char *ws, CeArgs *a, hipStream_t st) {
+static int ce_prepare(const CePlan &p, int n, int classes, int d, bool gather, const void *x, const void *w, const void *label,
+                      int label_bytes, long long ignore, float *loss, float *lse, char *ws, CeArgs *a, hipStream_t st) {
   int *list = (int *)ws, *count = list + n;
-  T *xc = (T *)(ws + p.list), *wc = (T *)(ws + p.list + p.x);
+  T *xc = (T *)(ws + p.list), *wc = (T *)(ws + p.list + (gather ? p.x : 0));
   if (label_bytes == 8)
-    hipLaunchKernelGGL(k_ce_rows<long long>, dim3(1), dim3(1024), 0, st, n, classes, ignore, (const long long *)label, list, count);
+    hipLaunchKernelGGL(k_ce_rows<long long>, dim3(1), dim3(1024), 0, st, n, classes, ignore, (const long long *)label, list, count, loss, lse);
   else
-    hipLaunchKernelGGL(k_ce_rows<int>, dim3(1), dim3(1024), 0, st, n, classes, ignore, (const int *)label, list, count);
+    hipLaunchKernelGGL(k_ce_rows<int>, dim3(1), dim3(1024), 0, st, n, classes, ignore, (const int *)label, list, count, loss, lse);
   DGNN_LAUNCH_CHECK();
   const int per = p.dk / (16 / (int)sizeof(T));
-  hipLaunchKernelGGL(k_ce_gather<T>, dim3(grid_for((long long)n * per)), dim3(DGNN_BLOCK), 0, st, n, d, p.dk,
-                     (const int *)list, (const int *)count, (const T *)x, (long long)d,
-                     (int)(p.dk == d && ((uintptr_t)x & 15) == 0), xc);
-  DGNN_LAUNCH_CHECK();
+  if (gather) {
+    hipLaunchKernelGGL(k_ce_gather<T>, dim3(grid_for((long long)n * per)), dim3(DGNN_BLOCK), 0, st, n, d, p.dk,
+                       (const int *)list, (const int *)count, (const T *)x, (long long)d,
+                       (int)(p.dk == d && ((uintptr_t)x & 15) == 0), xc);
+    DGNN_LAUNCH_CHECK();
+  }
   if (p.copy_w) {
     hipLaunchKernelGGL(k_ce_gather<T>, dim3(grid_for((long long)classes * per)), dim3(DGNN_BLOCK), 0, st, classes, d, p.dk,
                        (const int *)nullptr, (const int *)nullptr, (const T *)w, (long long)d, 0, wc);
     DGNN_LAUNCH_CHECK();
   }
   memset(a, 0, sizeof(*a));
-  a->x = xc, a->w = p.copy_w ? (const void *)wc : w;
-  a->ldw = p.dk;
+  a->x = gather ? (const void *)xc : x, a->gathered = gather, a->w = p.copy_w ? (const void *)wc : w;
   a->label = label, a->label_bytes = label_bytes, a->list = list, a->count = count;
   a->n = n, a->classes = classes, a->d = d, a->dk = p.dk;
   return DGNN_OK;
 }
 
+// LAUNCH(kernel, shape's columns along m, along n, splits, args...) for the shape chosen at run time
+#define DGNN_CE_LAUNCH(KERNEL, C, ms, ns, splits, ...)                                                          \
+  do {                                                                                                         \
+    const long long grid_ = (long long)ceil_div(ms, C::BM) * ceil_div(ns, C::BN) * (splits);                    \
+    if (grid_ > 0x7fffffffLL) return DGNN_ERR_UNSUPPORTED;                                                     \
+    hipLaunchKernelGGL((KERNEL<T, C>), dim3((unsigned)grid_), dim3(C::THREADS), 0, st, __VA_ARGS__);           \
+    DGNN_LAUNCH_CHECK();                                                                                       \
+  } while (0)
+
 template <class T>
 static int ce_forward(const CePlan &p, int n, int classes, int d, const void *x, const void *w, const void *label,
                       int label_bytes, long long ignore, int reduction, float *loss, float *lse, char *ws, hipStream_t st) {
   CeArgs a;
-  const int rc = ce_prepare<T>(p, n, classes, d, x, w, label, label_bytes, ignore, ws, &a, st);
-  if (rc != DGNN_OK) return rc;
-  char *at = ws + p.list + p.x + p.w;
-  a.part_m = (float *)at, a.part_s = (float *)(at + p.part), a.z_label = (float *)(at + 2 * p.part);
+  char *at = ws + p.list + (p.gather ? p.x : 0) + p.w;
   float *row = reduction == 0 ? loss : (float *)(at + 2 * p.part + p.zl);
-  hipLaunchKernelGGL(k_ce_fill, dim3(ceil_div(n, DGNN_BLOCK)), dim3(DGNN_BLOCK), 0, st, n, row, lse);
-  DGNN_LAUNCH_CHECK();
-  hipLaunchKernelGGL(k_ce_fwd<T>, dim3(p.tiles, ceil_div(n, CE_BN)), dim3(256), 0, st, a);
-  DGNN_LAUNCH_CHECK();
-  hipLaunchKernelGGL(k_ce_join, dim3(ceil_div(n, DGNN_WAVE)), dim3(DGNN_BLOCK), 0, st, n, p.tiles, a.list, a.count,
+  const int rc = ce_prepare<T>(p, n, classes, d, p.gather != 0, x, w, label, label_bytes, ignore, row, lse, ws, &a, st);
+  if (rc != DGNN_OK) return rc;
+  a.part_m = (float *)at, a.part_s = (float *)(at + p.part), a.z_label = (float *)(at + 2 * p.part);
+  if (p.z == CE_THIN) {
+    DGNN_CE_LAUNCH(k_ce_fwd, Thin<T>, classes, n, 1, a);
+  } else if (p.z == CE_PLAIN) {
+    DGNN_CE_LAUNCH(k_ce_fwd, Plain<T>, classes, n, 1, a);
+  } else if constexpr (sizeof(T) == 2) {
+    DGNN_CE_LAUNCH(k_ce_fwd, Wide, classes, n, 1, a);
+  }
+  hipLaunchKernelGGL(k_ce_join, dim3(ceil_div(n, 8)), dim3(DGNN_BLOCK), 0, st, n, p.tiles, a.list, a.count,
                      (const float *)a.part_m, (const float *)a.part_s, (const float *)a.z_label, row, lse);
   DGNN_LAUNCH_CHECK();
   if (reduction != 0) {
@@ -618,10 +765,10 @@ static int ce_backward(const CePlan &p, int n, int classes, int d, const void *x
                        int label_bytes, long long ignore, int reduction, const float *lse, const float *grad, void *dx,
                        void *dw, char *ws, hipStream_t st) {
   CeArgs a;
-  const int rc = ce_prepare<T>(p, n, classes, d, x, w, label, label_bytes, ignore, ws, &a, st);
+  const int rc = ce_prepare<T>(p, n, classes, d, true, x, w, label, label_bytes, ignore, nullptr, nullptr, ws, &a, st);
   if (rc != DGNN_OK) return rc;
   char *at = ws + p.list + p.x + p.w;
-  a.dz = at, a.ldz = p.ldz;
+  a.dz = at, a.ldz = p.piece;
   float *dxacc = (float *)(at + p.dz), *dwacc = (float *)(at + p.dz + p.dxacc);
   a.lse = (float *)lse, a.grad = grad, a.grad_rows = reduction == 0, a.mean = reduction == 1;
   a.dx = dx, a.dw = dw;
@@ -631,30 +778,44 @@ static int ce_backward(const CePlan &p, int n, int classes, int d, const void *x
     DGNN_LAUNCH_CHECK();
     a.grad_top = top;
   }
-  const int wide = d % 4 == 0 && ((uintptr_t)dw & (4 * sizeof(T) - 1)) == 0;
+  a.direct = p.dx_splits == 1 && p.pieces == 1;
+  const int whole_x = p.dk == d && ((uintptr_t)dx & 15) == 0, whole_w = p.dk == d && ((uintptr_t)dw & 15) == 0;
+  if (dx) {
+    hipLaunchKernelGGL(k_ce_dx_zero<T>, dim3(n < 4096 ? n : 4096), dim3(DGNN_BLOCK), 0, st, a, ignore);
+    DGNN_LAUNCH_CHECK();
+  }
   for (int v0 = 0; v0 < classes; v0 += p.piece) {
     a.v0 = v0, a.vn = classes - v0 < p.piece ? classes - v0 : p.piece, a.first = v0 == 0;
-    hipLaunchKernelGGL(k_ce_dz<T>, dim3(p.piece / CE_BM, ceil_div(n, CE_BN)), dim3(256), 0, st, a);
-    DGNN_LAUNCH_CHECK();
+    if (p.z == CE_THIN) {
+      DGNN_CE_LAUNCH(k_ce_dz, Thin<T>, p.piece, n, 1, a);
+    } else if (p.z == CE_PLAIN) {
+      DGNN_CE_LAUNCH(k_ce_dz, Plain<T>, p.piece, n, 1, a);
+    } else if constexpr (sizeof(T) == 2) {
+      DGNN_CE_LAUNCH(k_ce_dz, Wide, p.piece, n, 1, a);
+    }
     if (dx) {
       a.acc = dxacc, a.splits = p.dx_splits;
-      hipLaunchKernelGGL(k_ce_dx<T>, dim3(ceil_div(p.dk, CE_BM), ceil_div(n, CE_BN), p.dx_splits), dim3(256), 0, st, a);
-      DGNN_LAUNCH_CHECK();
+      if (p.dx_shape == CE_PLAIN) {
+        DGNN_CE_LAUNCH(k_ce_dx, Plain<T>, p.dk, n, p.dx_splits, a, whole_x);
+      } else if constexpr (sizeof(T) == 2) {
+        DGNN_CE_LAUNCH(k_ce_dx, Wide, p.dk, n, p.dx_splits, a, whole_x);
+      }
     }
     if (dw) {
       a.acc = dwacc, a.splits = p.dw_splits;
-      hipLaunchKernelGGL(k_ce_dw<T>, dim3(ceil_div(p.dk, CE_BM), ceil_div(a.vn, CE_BN), p.dw_splits), dim3(256), 0, st, a, wide);
-      DGNN_LAUNCH_CHECK();
+      if (p.dw_shape == CE_PLAIN) {
+        DGNN_CE_LAUNCH(k_ce_dw, Plain<T>, p.dk, a.vn, p.dw_splits, a, whole_w);
+      } else if constexpr (sizeof(T) == 2) {
+        DGNN_CE_LAUNCH(k_ce_dw, Wide, p.dk, a.vn, p.dw_splits, a, whole_w);
+      }
       if (p.dw_splits > 1) {
         hipLaunchKernelGGL(k_ce_dw_join<T>, dim3(grid_for((long long)a.vn * p.dk / 4)), dim3(DGNN_BLOCK), 0, st, a);
         DGNN_LAUNCH_CHECK();
       }
     }
   }
-  if (dx) {
+  if (dx && !a.direct) {
     a.acc = dxacc, a.splits = p.dx_splits;
-    hipLaunchKernelGGL(k_ce_dx_zero<T>, dim3(n < 4096 ? n : 4096), dim3(DGNN_BLOCK), 0, st, a, ignore);
-    DGNN_LAUNCH_CHECK();
     hipLaunchKernelGGL(k_ce_dx_join<T>, dim3(grid_for((long long)n * p.dk / 4)), dim3(DGNN_BLOCK), 0, st, a);
     DGNN_LAUNCH_CHECK();
   }
@@ -667,7 +828,7 @@ extern "C" {
 
 size_t dgnn_linear_ce_workspace_bytes(int dtype, int n, int classes, int d, int backward) {
   if (ce_check(dtype, 4, n, classes, d) != DGNN_OK || n == 0) return 0;
-  const CePlan p = ce_plan(dtype, n, classes, d, 0);
+  const CePlan p = ce_plan(dtype, n, classes, d, (const void *)1, (const void *)1);    // the larger case: copies of both
   return backward ? p.bwd_total : p.fwd_total;
 }
 
@@ -689,7 +850,7 @@ int dgnn_linear_ce_forward(int dtype, int label_bytes, int n, int classes, int d
   const int size = dtype == DGNN_F32 ? 4 : 2;
   if ((uintptr_t)x % size || (uintptr_t)w % size || (uintptr_t)label % label_bytes || ((uintptr_t)loss & 3) || ((uintptr_t)lse & 3))
     return DGNN_ERR_ALIGNMENT;
-  const CePlan p = ce_plan(dtype, n, classes, d, ((uintptr_t)w & 15) == 0);
+  const CePlan p = ce_plan(dtype, n, classes, d, x, w);
   if (!workspace || workspace_bytes < p.fwd_total) return DGNN_ERR_WORKSPACE;
   if ((uintptr_t)workspace & 15) return DGNN_ERR_ALIGNMENT;
   if (dtype == DGNN_F32) return ce_forward<float>(p, n, classes, d, x, w, label, label_bytes, ignore_index, reduction, loss, lse, (char *)workspace, st);
@@ -710,7 +871,7 @@ int dgnn_linear_ce_backward(int dtype, int label_bytes, int n, int classes, int 
   if ((uintptr_t)x % size || (uintptr_t)w % size || (uintptr_t)dx % size || (uintptr_t)dw % size ||
       (uintptr_t)label % label_bytes || ((uintptr_t)lse & 3) || ((uintptr_t)grad & 3))
     return DGNN_ERR_ALIGNMENT;
-  const CePlan p = ce_plan(dtype, n, classes, d, ((uintptr_t)w & 15) == 0);
+  const CePlan p = ce_plan(dtype, n, classes, d, x, w);
   if (!workspace || workspace_bytes < p.bwd_total) return DGNN_ERR_WORKSPACE;
   if ((uintptr_t)workspace & 15) return DGNN_ERR_ALIGNMENT;
   hipStream_t st = (hipStream_t)stream;

@@ -52,6 +52,24 @@ __device__ __forceinline__ acc16 mma(frag8<float> a, frag8<float> b, acc16 c) {
   for (int j = 0; j < 8; ++j) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[j], b[j], c, 0, 0, 0);
   return c;
 }
+// acc[i][j] += a[i] b[j].  float: the eight products of one accumulator depend on each other, so they
+// are interleaved over all of them.
+template <int MB, int NB, class T>
+__device__ __forceinline__ void mma_block(const frag8<T> (&a)[MB], const frag8<T> (&b)[NB], acc16 (&acc)[MB][NB], T) {
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+#pragma unroll
+      for (int i = 0; i < MB; ++i)
+#pragma unroll
+        for (int j = 0; j < NB; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x2f32(a[i][e], b[j][e], acc[i][j], 0, 0, 0);
+  } else {
+#pragma unroll
+    for (int i = 0; i < MB; ++i)
+#pragma unroll
+      for (int j = 0; j < NB; ++j) acc[i][j] = mma(a[i], b[j], acc[i][j]);
+  }
+}
 __device__ __forceinline__ acc16 acc_zero() {
   acc16 c;
 #pragma unroll
@@ -180,6 +198,22 @@ struct Stager {
       off[i] = chunk * TL::CHUNK < cols ? row * row_stride_bytes + chunk * 16u : DGNN_OOB;
     }
   }
+  // the tile's rows are rows list[0], list[1], ... of the matrix; there are `rows` of them
+  __device__ __forceinline__ void init_list(const int *__restrict__ list, int rows, unsigned row_stride_bytes, int cols) {
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      const int c = i * THREADS + threadIdx.x, row = c / TL::CPR, chunk = (c % TL::CPR) ^ TL::swizzle(row);
+      off[i] = chunk * TL::CHUNK < cols && row < rows ? (unsigned)list[row] * row_stride_bytes + chunk * 16u : DGNN_OOB;
+    }
+  }
+  // from now on only `cols` columns exist
+  __device__ __forceinline__ void narrow(int cols) {
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      const int c = i * THREADS + threadIdx.x, row = c / TL::CPR, chunk = (c % TL::CPR) ^ TL::swizzle(row);
+      if (chunk * TL::CHUNK >= cols) off[i] = DGNN_OOB;
+    }
+  }
   __device__ __forceinline__ void load(char *tile, __amdgpu_buffer_rsrc_t src) const {
     typedef __attribute__((address_space(3))) void *lds_p;
     const int wave = uniform_i32(threadIdx.x >> 6);
@@ -209,10 +243,8 @@ __device__ __forceinline__ void barrier_in_flight() {
 // the last tile, where they read nothing), work(t, i) uses buffer i.  Every buffer is a __shared__
 // variable of its own and the indices are constants after unrolling: the compiler, which waits for
 // all loads to LDS that a read may touch, then knows which those are.
-#define DGNN_RING2(name, bytes)                                     \
-  __shared__ __align__(16) char name##_0[bytes], name##_1[bytes];   \
-  char *const name[2] = {name##_0, name##_1}
-#define DGNN_RING4(name, bytes)                                                                     \
+// DGNN_RING declares four; a ring of fewer leaves the others out of the kernel.
+#define DGNN_RING(name, bytes)                                                                      \
   __shared__ __align__(16) char name##_0[bytes], name##_1[bytes], name##_2[bytes], name##_3[bytes]; \
   char *const name[4] = {name##_0, name##_1, name##_2, name##_3}
 template <int S, int LOADS, class Stage, class Work>

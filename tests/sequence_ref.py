@@ -134,7 +134,7 @@ def linear_ce(feat, weight, label, ignore, reduction, grad=None):
 
 def check(got, want, what):
     """|got - value| <= bound everywhere; infinities equal."""
-    value, bound = want
+    value, bound = (t.detach().cpu() for t in want)
     got = got.detach().cpu().double()
     assert got.shape == value.shape, (what, got.shape, value.shape)
     inf = torch.isinf(value)

@@ -268,6 +268,25 @@ def test_cross_entropy_reductions_and_masks(dtype):
     ce_case(200, 300, 64, dtype, spread=60.0)              # logits of some hundred
 
 
+@pytest.mark.parametrize("dtype", DTYPES, ids=ids_of)
+@pytest.mark.parametrize("n,classes,dim", [(4100, 4300, 72), (8200, 8210, 520), (5000, 20000, 264), (900, 70000, 136)])
+def test_cross_entropy_large_tiles_and_pieces(n, classes, dim, dtype):
+    """Enough tiles for the wide shapes, several pieces of the classes, split sums (reference in
+    float64 on the GPU)."""
+    gen = torch.Generator(device=DEV).manual_seed(n)
+    feat = torch.randn(n, dim, generator=gen, device=DEV).to(dtype)
+    weight = (torch.randn(classes, dim, generator=gen, device=DEV) * 2 / math.sqrt(dim)).to(dtype)
+    label = torch.randint(-classes // 20, classes, (n,), generator=gen, device=DEV)
+    grad = torch.tensor(1.5, device=DEV)
+    with torch.device(DEV):
+        want = ref.linear_ce(feat, weight, label, -100, "mean", grad)
+    x, w = feat.requires_grad_(), weight.requires_grad_()
+    loss = LinearCrossEntropyFuse(x, w, label)
+    ref.check(loss, want["loss"], "loss")
+    for name, got in zip(("dx", "dw"), torch.autograd.grad(loss, [x, w], grad)):
+        ref.check(got, want[name], name)
+
+
 def test_cross_entropy_only_one_gradient_and_no_rows():
     feat, weight = torch.randn(40, 16, device=DEV), torch.randn(30, 16, device=DEV)
     label = torch.randint(0, 30, (40,), device=DEV)
