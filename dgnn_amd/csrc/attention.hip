@@ -17,148 +17,267 @@ using namespace dgnn;
 
 namespace dgnn {
 
-constexpr int ATTN_BN = 64;                    // keys of a tile
-
-template <class T, int DP, int NW>
-__global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void k_attn_fwd(const AttnArgs a) {
-  constexpr int BM = 32 * NW, BN = ATTN_BN, THREADS = 64 * NW;
+// One tile: 32 NW packed rows row0 .. of a sequence (`rows` of them exist) against its keys key0 .. key1 - 1.
+// Leaves the lane's unnormalised output row in acc, the running maximum (of z / scale) in m and this
+// lane half's share of the sum in l.
+template <class T, int DP, int NW, int BN, int S>
+struct AttnTile {
   using TL = Tile<T, DP>;
-  using SG = Stager<T, DP, BN, THREADS>;
-  constexpr int TILE = BN * TL::ROW_BYTES, S = 2;
-  DGNN_RING(lds, 2 * TILE);
-  const int lane = lane_id(), h = lane >> 5, wave = uniform_i32(wave_in_block());
-  const int row_lane = TL::row_lane(lane), col_lane = TL::col_lane(lane);
-  const int kvh = blockIdx.x % a.hk, slot = blockIdx.x / a.hk;
-  const Segment seg = find_segment(a.row_ptr, a.nseq, a.tq, a.g, BM, slot, a.causal != 0);
-  if (seg.tile < 0) return;
-  int ks, lk;
-  other_side(a.col_ptr, a.nseq, a.tk, seg.seq, &ks, &lk);
-
-  // this lane's row
-  const long long rows = (long long)seg.len * a.g;
-  const long long row = (long long)seg.tile * BM + wave * 32 + (lane & 31);
-  const bool valid = row < rows;
-  const int qi = (int)(row / a.g), head = kvh * a.g + (int)(row % a.g);
-  const long long tok = seg.start + (long long)qi;
-  // last key it sees; a.causal: queries and keys end together
-  const int limit = !valid ? -1 : a.causal ? qi + (lk - seg.len) : lk - 1;
-  const long long last_row = min(rows, (long long)(seg.tile + 1) * BM) - 1;
-  const int seen = a.causal ? max(0, min(lk, (int)(last_row / a.g) + (lk - seg.len) + 1)) : lk;
-  const int tiles = (seen + BN - 1) / BN;
-  // every row of the wave sees keys 0 .. wave_all, none sees a key behind wave_any
-  const long long wrow = (long long)seg.tile * BM + wave * 32;
-  const int wave_all = a.causal ? (int)(min(wrow, last_row) / a.g) + (lk - seg.len) : lk - 1;
-  const int wave_any = wrow > last_row ? -1
-                       : a.causal ? (int)(min(wrow + 31, last_row) / a.g) + (lk - seg.len) : lk - 1;
-
-  frag8<T> qf[DP / 16];
-  const T *qrow = (const T *)a.q + tok * a.q_tok + (long long)head * a.q_head;
-  load_row_frags<T, DP>(qf, qrow, a.d, h, valid);
-  float c = a.scale * DGNN_LOG2E;
-  // the running maximum is taken before the scale, which must be positive there: the sign goes into
-  // q, and a scale of zero becomes q = 0 (a masked score, -inf, stays -inf)
-  if (!(c > 0.f)) {
-    const bool zero = c == 0.f;
-    c = zero ? 1.f : -c;
-#pragma unroll
-    for (int s = 0; s < DP / 16; ++s)
-#pragma unroll
-      for (int j = 0; j < 8; ++j) qf[s][j] = zero ? (T)0.f : (T)-qf[s][j];
-  }
-
-  const unsigned k_stride = (unsigned)(a.k_tok * sizeof(T)), v_stride = (unsigned)(a.v_tok * sizeof(T));
-  const unsigned row_bytes = a.d * (unsigned)sizeof(T);
-  const T *kbase = (const T *)a.k + (long long)ks * a.k_tok + (long long)kvh * a.k_head;
-  const T *vbase = (const T *)a.v + (long long)ks * a.v_tok + (long long)kvh * a.v_head;
-  SG st_k, st_v;
-  st_k.init(k_stride, a.d);
-  st_v.init(v_stride, a.d);
-  auto stage = [&](int t, auto i) {
-    const int n = t < tiles ? min(BN, lk - t * BN) : 0;
-    st_k.load(lds[i.value], buffer_over(kbase + (long long)t * BN * a.k_tok, span_bytes(n, k_stride, row_bytes)));
-    st_v.load(lds[i.value] + TILE, buffer_over(vbase + (long long)t * BN * a.v_tok, span_bytes(n, v_stride, row_bytes)));
-  };
+  using SG = Stager<T, DP, BN, 64 * NW>;
+  static constexpr int TILE = BN * TL::ROW_BYTES, BYTES = 2 * TILE;
+  static_assert(2 * SG::LOADS * (S - 2) < 64, "loads in flight are counted in six bits");
 
   acc16 acc[DP / 32];
-#pragma unroll
-  for (int b = 0; b < DP / 32; ++b) acc[b] = acc_zero();
-  float m = -INFINITY, l = 0.f;                 // running maximum of z / scale, this half's share of the sum
+  float m, l, c;
+  bool valid;
+  int head, limit;
+  long long tok;
 
-  auto work = [&](int t, auto i) {
-    const char *kt = lds[i.value], *vt = kt + TILE;
-    if (t * BN > wave_any) return;
-    const int rl = opaque(row_lane), cl = opaque(col_lane);
-    acc16 s[2];
+  __device__ __forceinline__ void run(const AttnArgs &a, char *const (&lds)[4], int qs, int lq, int ks, int lk, int kvh,
+                                      long long row0, long long rows, int key0, int key1) {
+    const int lane = lane_id(), h = lane >> 5, wave = NW == 1 ? 0 : uniform_i32(wave_in_block());
+    const int row_lane = TL::row_lane(lane), col_lane = TL::col_lane(lane);
+    // this lane's row
+    const long long wrow = row0 + wave * 32, row = wrow + (lane & 31);
+    valid = row < rows;
+    const int qi = (int)((unsigned)row / (unsigned)a.g);
+    head = kvh * a.g + (int)((unsigned)row % (unsigned)a.g);
+    tok = qs + (long long)qi;
+    // last key it sees; causal: queries and keys end together
+    const int shift = lk - lq;
+    limit = !valid ? -1 : a.causal ? qi + shift : lk - 1;
+    const int last_row = (int)(min(rows, row0 + 32 * NW) - 1);
+    const int seen = a.causal ? max(0, min(key1, last_row / a.g + shift + 1)) : key1;
+    const int tiles = (max(seen - key0, 0) + BN - 1) / BN;
+    // every row of the wave sees the keys up to wave_all, none sees a key behind wave_any
+    const int wave_all = a.causal ? min((int)wrow, last_row) / a.g + shift : lk - 1;
+    const int wave_any = wrow > last_row ? -1 : a.causal ? min((int)wrow + 31, last_row) / a.g + shift : lk - 1;
+
+    frag8<T> qf[DP / 16];
+    load_row_frags<T, DP>(qf, (const T *)a.q + tok * a.q_tok + (long long)head * a.q_head, a.d, h, valid);
+    c = a.scale * DGNN_LOG2E;
+    // the running maximum is taken before the scale, which must be positive there: the sign goes into
+    // q, and a scale of zero becomes q = 0 (a masked score, -inf, stays -inf)
+    if (!(c > 0.f)) {
+      const bool zero = c == 0.f;
+      c = zero ? 1.f : -c;
 #pragma unroll
-    for (int b = 0; b < 2; ++b) {
-      s[b] = acc_zero();
+      for (int s = 0; s < DP / 16; ++s)
 #pragma unroll
-      for (int i = 0; i < DP / 16; ++i)
-        s[b] = mma(TL::row_frag(kt, rl, 32 * b, 16 * i), qf[i], s[b]);
+        for (int j = 0; j < 8; ++j) qf[s][j] = zero ? (T)0.f : (T)-qf[s][j];
     }
-    if (t * BN + BN - 1 > wave_all) {
+
+    const unsigned k_stride = (unsigned)(a.k_tok * sizeof(T)), v_stride = (unsigned)(a.v_tok * sizeof(T));
+    const unsigned row_bytes = a.d * (unsigned)sizeof(T);
+    const T *kbase = (const T *)a.k + (long long)(ks + (long long)key0) * a.k_tok + (long long)kvh * a.k_head;
+    const T *vbase = (const T *)a.v + (long long)(ks + (long long)key0) * a.v_tok + (long long)kvh * a.v_head;
+    SG st_k, st_v;
+    st_k.init(k_stride, a.d);
+    st_v.init(v_stride, a.d);
+    auto stage = [&](int t, auto i) {
+      const int n = t < tiles ? min(BN, key1 - key0 - t * BN) : 0;
+      st_k.load(lds[i.value], buffer_over(kbase + (long long)t * BN * a.k_tok, span_bytes(n, k_stride, row_bytes)));
+      st_v.load(lds[i.value] + TILE, buffer_over(vbase + (long long)t * BN * a.v_tok, span_bytes(n, v_stride, row_bytes)));
+    };
+
 #pragma unroll
-      for (int b = 0; b < 2; ++b)
+    for (int b = 0; b < DP / 32; ++b) acc[b] = acc_zero();
+    m = -INFINITY, l = 0.f;
+
+    auto work = [&](int t, auto i) {
+      const char *kt = lds[i.value], *vt = kt + TILE;
+      const int k0 = key0 + t * BN;
+      if (k0 > wave_any) return;
+      const int rl = opaque(row_lane), cl = opaque(col_lane);
+      acc16 s[BN / 32];
 #pragma unroll
-        for (int r = 0; r < 16; ++r)
-          if (t * BN + 32 * b + acc_row(r, h) > limit) s[b][r] = -INFINITY;
-    }
-    float top = m;
+      for (int b = 0; b < BN / 32; ++b) {
+        s[b] = acc_zero();
 #pragma unroll
-    for (int b = 0; b < 2; ++b)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) top = fmaxf(top, s[b][r]);
-    top = fmaxf(top, __shfl_xor(top, 32, 64));
-    if (__any(top > m)) {
-      const float by = top == m ? 1.f : exp2_fast((m - top) * c);     // m = -inf: 0
-      m = top;
-      l *= by;
-#pragma unroll
-      for (int b = 0; b < DP / 32; ++b)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) acc[b][r] *= by;
-    }
-    const float mc = m == -INFINITY ? 0.f : m * c;
-#pragma unroll
-    for (int b = 0; b < 2; ++b) {
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        s[b][r] = exp2_fast(fmaf(s[b][r], c, -mc));
-        l += s[b][r];
+        for (int k = 0; k < DP / 16; ++k) s[b] = mma(TL::row_frag(kt, rl, 32 * b, 16 * k), qf[k], s[b]);
       }
-    }
+      if (k0 + BN - 1 > min(wave_all, key1 - 1)) {
+        const int last = min(limit, key1 - 1) - k0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const frag8<T> p = frag_of<T>(s[i >> 1], 8 * (i & 1));
+        for (int b = 0; b < BN / 32; ++b)
 #pragma unroll
-      for (int b = 0; b < DP / 32; ++b) acc[b] = mma(TL::col_frag(vt, cl, 16 * i, 32 * b), p, acc[b]);
-    }
-  };
+          for (int r = 0; r < 16; ++r)
+            if (32 * b + acc_row(r, h) > last) s[b][r] = -INFINITY;
+      }
+      float top = m;
+#pragma unroll
+      for (int b = 0; b < BN / 32; ++b)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) top = fmaxf(top, s[b][r]);
+      top = fmaxf(top, __shfl_xor(top, 32, 64));
+      if (__any(top > m)) {
+        const float by = top == m ? 1.f : exp2_fast((m - top) * c);     // m = -inf: 0
+        m = top;
+        l *= by;
+#pragma unroll
+        for (int b = 0; b < DP / 32; ++b)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) acc[b][r] *= by;
+      }
+      const float mc = m == -INFINITY ? 0.f : m * c;
+#pragma unroll
+      for (int b = 0; b < BN / 32; ++b)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          s[b][r] = exp2_fast(fmaf(s[b][r], c, -mc));
+          l += s[b][r];
+        }
+#pragma unroll
+      for (int k = 0; k < BN / 16; ++k) {
+        const frag8<T> p = frag_of<T>(s[k >> 1], 8 * (k & 1));
+#pragma unroll
+        for (int b = 0; b < DP / 32; ++b) acc[b] = mma(TL::col_frag(vt, cl, 16 * k, 32 * b), p, acc[b]);
+      }
+    };
+    ring<S, 2 * SG::LOADS>(tiles, stage, work);
+    l += __shfl_xor(l, 32, 64);
+  }
 
-  ring<S, 2 * SG::LOADS>(tiles, stage, work);
+  __device__ __forceinline__ void finish(const AttnArgs &a, int lk) const {
+    if (!valid) return;
+    const int h = lane_id() >> 5;
+    const bool none = limit < 0 || lk == 0;
+    store_row<T, DP>((T *)a.o + (tok * a.hq + head) * a.d, acc, none ? 0.f : 1.f / l, a.d, h);
+    if (a.lse != nullptr && h == 0)
+      a.lse[(long long)head * a.tq + tok] = none ? -INFINITY : (m * c + __builtin_amdgcn_logf(l)) * DGNN_LN2;
+  }
+};
 
-  if (!valid) return;
-  l += __shfl_xor(l, 32, 64);
-  const bool none = limit < 0 || lk == 0;
-  store_row<T, DP>((T *)a.o + (tok * a.hq + head) * a.d, acc, none ? 0.f : 1.f / l, a.d, h);
-  if (a.lse != nullptr && h == 0)
-    a.lse[(long long)head * a.tq + tok] = none ? -INFINITY : (m * c + __builtin_amdgcn_logf(l)) * DGNN_LN2;
+template <class T, int DP, int NW, int BN, int S>
+__global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void k_attn_fwd(const AttnArgs a) {
+  using AT = AttnTile<T, DP, NW, BN, S>;
+  DGNN_RING(lds, AT::BYTES);
+  const int kvh = blockIdx.x % a.hk, slot = blockIdx.x / a.hk;
+  const Segment seg = find_segment(a.row_ptr, a.nseq, a.tq, a.g, 32 * NW, slot, a.causal != 0);
+  if (seg.tile < 0) return;
+  int ks, lk;
+  other_side(a.col_ptr, a.row_ptr, a.nseq, a.tk, seg, &ks, &lk);
+  AT t;
+  t.run(a, lds, seg.start, seg.len, ks, lk, kvh, (long long)seg.tile * 32 * NW, (long long)seg.len * a.g, 0, lk);
+  t.finish(a, lk);
 }
 
+// ------------------------------------------------------------------ few rows, long keys
+// Single queries and poolings: a sequence's first a.few packed rows of a key head are split over chunks of
+// a.chunk keys, one wave a chunk, which reads its keys and values once for all query heads of the key
+// head; k_attn_join puts the parts together.  Part (slot, key head) holds {output row, maximum, sum} of
+// each of the rows.  What rows a sequence has beyond those are dealt to its chunks' workgroups in
+// tiles of 32, unsplit.
 template <class T, int DP>
-static int launch_fwd(const AttnArgs &a, hipStream_t st) {
-  constexpr int NW = 4;
+__global__ __launch_bounds__(64, sizeof(T) == 2 ? 2 : 1) void k_attn_split(const AttnArgs a) {
+  using AT = AttnTile<T, DP, 1, 32, DP * sizeof(T) >= 512 ? 3 : 4>;
+  DGNN_RING(lds, AT::BYTES);
+  const int kvh = blockIdx.x % a.hk, slot = blockIdx.x / a.hk, lane = lane_id(), h = lane >> 5;
+  const Segment seg = find_segment(a.col_ptr, a.nseq, a.tk, 1, a.chunk, slot, false);
+  if (seg.tile < 0) return;
+  int qs, lq;
+  other_side(a.row_ptr, a.col_ptr, a.nseq, a.tq, seg, &qs, &lq);
+  const long long rows = (long long)lq * a.g;
+  const int chunks = (seg.len + a.chunk - 1) / a.chunk;
+  AT t;
+  if (rows > 0) {
+    t.run(a, lds, qs, lq, seg.start, seg.len, kvh, 0, min(rows, (long long)a.few), seg.tile * a.chunk,
+          min(seg.len, (seg.tile + 1) * a.chunk));
+    if (t.valid) {
+      float *part = a.part + (((long long)slot * a.hk + kvh) * a.few + (lane & 31)) * (a.d + 4);
+      store_row<float, DP>(part + 4, t.acc, 1.f, a.d, h);
+      if (h == 0) part[0] = t.m == -INFINITY ? -INFINITY : t.m * t.c, part[1] = t.l;
+    }
+  }
+  for (long long row0 = a.few + 32LL * seg.tile; row0 < rows; row0 += 32LL * chunks) {
+    __syncthreads();
+    t.run(a, lds, qs, lq, seg.start, seg.len, kvh, row0, rows, 0, seg.len);
+    t.finish(a, seg.len);
+  }
+}
+
+// out and lse of the rows k_attn_split left in parts; rows that see no key at all.  One wave a row.
+template <class T>
+__global__ __launch_bounds__(DGNN_BLOCK) void k_attn_join(const AttnArgs a) {
+  const int lane = lane_id();
+  const long long r = (long long)blockIdx.x * DGNN_WAVES_PER_BLOCK + uniform_i32(wave_in_block());
+  if (r >= (long long)a.tq * a.hq) return;
+  const int tok = (int)(r / a.hq), head = (int)(r % a.hq);
+  const Segment seg = find_segment(a.row_ptr, a.nseq, a.tq, 1, 1, tok, false, true);   // the row's sequence
+  const int seq = seg.seq, qs = seg.start, lq = seg.len;
+  int ks, lk;
+  other_side(a.col_ptr, a.row_ptr, a.nseq, a.tk, seg, &ks, &lk);
+  const int qi = tok - qs, packed = qi * a.g + head % a.g;
+  const int seen = seq < 0 || seq >= a.nseq ? 0 : a.causal ? max(0, min(lk, qi + lk - lq + 1)) : lk;
+  if (seen > 0 && packed >= a.few) return;                          // written unsplit
+  T *out = (T *)a.o + r * a.d;
+  float *lse = a.lse != nullptr ? a.lse + (long long)head * a.tq + tok : nullptr;
+  const int chunks = (seen + a.chunk - 1) / a.chunk;
+  const long long slot = (long long)ks / a.chunk + seq + 1, stride = (long long)a.hk * a.few * (a.d + 4);
+  const float *part = a.part + ((slot * a.hk + head / a.g) * a.few + packed) * (a.d + 4);
+  float top = -INFINITY;
+  for (int j = lane; j < chunks; j += 64) top = fmaxf(top, part[j * stride]);
+  top = wave_max(top);
+  const float base = top == -INFINITY ? 0.f : top;
+  float sum = 0.f;
+  for (int j = lane; j < chunks; j += 64) sum += part[j * stride + 1] * exp2_fast(part[j * stride] - base);
+  sum = wave_sum(sum);
+  for (int c = lane; c < a.d; c += 64) {
+    float x = 0.f;
+#pragma unroll 4
+    for (int j = 0; j < chunks; ++j) x = fmaf(part[j * stride + 4 + c], exp2_fast(part[j * stride] - base), x);
+    out[c] = (T)(seen > 0 ? x / sum : 0.f);
+  }
+  if (lse && lane == 0) *lse = seen > 0 ? (base + __builtin_amdgcn_logf(sum)) * DGNN_LN2 : -INFINITY;
+}
+
+// ------------------------------------------------------------------ which kernel
+struct AttnPlan {
+  int few, chunk;                       // split: rows kept in parts, keys of a chunk (few = 0: not split)
+  long long slots;
+  size_t bytes;
+};
+static AttnPlan attn_plan(int nseq, int tq, int tk, int hq, int hk, int d) {
+  AttnPlan p = {0, 0, 0, 0};
+  const long long g = hq / hk, rows = nseq > 0 ? ((long long)tq * g + nseq - 1) / nseq : 0;     // of a sequence, on average
+  const long long keys = nseq > 0 ? tk / nseq : 0;
+  if (rows == 0 || rows > 32 || keys < 256) return p;
+  p.few = rows <= 4 ? 4 : rows <= 8 ? 8 : rows <= 16 ? 16 : 32;
+  long long c = ((long long)tk * hk / 2048 + 63) / 64 * 64;
+  p.chunk = (int)(c < 256 ? 256 : c > 2048 ? 2048 : c);
+  p.slots = tile_slots(tk, nseq, 1, p.chunk);
+  p.bytes = sizeof(float) * (size_t)p.slots * hk * p.few * (d + 4);
+  return p;
+}
+
+template <class T, int DP, int NW, int BN, int S>
+static int launch_rows(const AttnArgs &a, hipStream_t st) {
   const long long slots = tile_slots(a.tq, a.nseq, a.g, 32 * NW);
   if (slots * a.hk > 0x7fffffffLL) return DGNN_ERR_UNSUPPORTED;
-  hipLaunchKernelGGL((k_attn_fwd<T, DP, NW>), dim3((unsigned)(slots * a.hk)), dim3(64 * NW), 0, st, a);
+  hipLaunchKernelGGL((k_attn_fwd<T, DP, NW, BN, S>), dim3((unsigned)(slots * a.hk)), dim3(64 * NW), 0, st, a);
   DGNN_LAUNCH_CHECK();
   return DGNN_OK;
 }
+template <class T, int DP>
+static int launch_fwd(const AttnArgs &a, const AttnPlan &p, hipStream_t st) {
+  if (p.few > 0) {
+    if (p.slots * a.hk > 0x7fffffffLL) return DGNN_ERR_UNSUPPORTED;
+    hipLaunchKernelGGL((k_attn_split<T, DP>), dim3((unsigned)(p.slots * a.hk)), dim3(64), 0, st, a);
+    DGNN_LAUNCH_CHECK();
+    const long long rows = (long long)a.tq * a.hq;
+    hipLaunchKernelGGL(k_attn_join<T>, dim3((unsigned)((rows + DGNN_WAVES_PER_BLOCK - 1) / DGNN_WAVES_PER_BLOCK)),
+                       dim3(DGNN_BLOCK), 0, st, a);
+    DGNN_LAUNCH_CHECK();
+    return DGNN_OK;
+  }
+  if (short_rows(a.tq, a.nseq, a.g, a.hk)) return launch_rows<T, DP, 1, 32, 2>(a, st);
+  return launch_rows<T, DP, 4, 64, 2>(a, st);
+}
 template <class T>
-static int launch_fwd_d(const AttnArgs &a, hipStream_t st) {
-  if (a.d <= 32) return launch_fwd<T, 32>(a, st);
-  if (a.d <= 64) return launch_fwd<T, 64>(a, st);
-  return launch_fwd<T, 128>(a, st);
+static int launch_fwd_d(const AttnArgs &a, const AttnPlan &p, hipStream_t st) {
+  if (a.d <= 32) return launch_fwd<T, 32>(a, p, st);
+  if (a.d <= 64) return launch_fwd<T, 64>(a, p, st);
+  return launch_fwd<T, 128>(a, p, st);
 }
 
 static bool stride_ok(long long s, int size) {
@@ -199,21 +318,30 @@ int attn_args(int dtype, int nseq, int tq, int tk, int hq, int hk, int d, int ca
 
 extern "C" {
 
+size_t dgnn_attn_forward_workspace_bytes(int nseq, int tq, int tk, int hq, int hk, int d) {
+  if (nseq <= 0 || tq <= 0 || tk <= 0 || hq <= 0 || hk <= 0 || d <= 0 || hq % hk != 0) return 0;
+  return attn_plan(nseq, tq, tk, hq, hk, d).bytes;
+}
+
 int dgnn_attn_forward(int dtype, int nseq, int tq, int tk, int hq, int hk, int d, int causal, float scale,
                       const void *q, const void *k, const void *v, const long long *strides, const int *row_ptr,
-                      const int *col_ptr, void *out, float *lse, void *stream) {
+                      const int *col_ptr, void *out, float *lse, void *workspace, size_t workspace_bytes, void *stream) {
   AttnArgs a;
   const int rc = attn_args(dtype, nseq, tq, tk, hq, hk, d, causal, scale, q, k, v, row_ptr, col_ptr, strides, &a);
   if (rc != DGNN_OK) return rc;
   if (tq == 0) return DGNN_OK;
   if (!out) return DGNN_ERR_BAD_ARG;
   if (((uintptr_t)out & 15) || ((uintptr_t)lse & 3)) return DGNN_ERR_ALIGNMENT;
+  const AttnPlan p = attn_plan(nseq, tq, tk, hq, hk, d);
+  if (p.bytes > 0 && (!workspace || workspace_bytes < p.bytes)) return DGNN_ERR_WORKSPACE;
+  if (p.bytes > 0 && ((uintptr_t)workspace & 15)) return DGNN_ERR_ALIGNMENT;
   a.o = out;
   a.lse = lse;
+  a.part = (float *)workspace, a.few = p.few, a.chunk = p.chunk;
   hipStream_t st = (hipStream_t)stream;
-  if (dtype == DGNN_F32) return launch_fwd_d<float>(a, st);
-  if (dtype == DGNN_BF16) return launch_fwd_d<bf16_t>(a, st);
-  return launch_fwd_d<half_t>(a, st);
+  if (dtype == DGNN_F32) return launch_fwd_d<float>(a, p, st);
+  if (dtype == DGNN_BF16) return launch_fwd_d<bf16_t>(a, p, st);
+  return launch_fwd_d<half_t>(a, p, st);
 }
 
 }  // extern "C"

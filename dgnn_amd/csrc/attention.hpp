@@ -11,6 +11,8 @@ struct AttnArgs {
   void *o, *dq, *dk, *dv;
   float *lse;                                 // [hq, tq], natural logarithm
   float *stat;                                // backward: [hq, tq] pairs {lse log2(e) (+inf for an empty row), <grad, out>}
+  float *part;                                // split forward: partial rows
+  int few, chunk;
   const int *row_ptr, *col_ptr;
   int nseq, tq, tk, hq, hk, g, d, causal;     // g = hq / hk
   long long q_tok, q_head, k_tok, k_head, v_tok, v_head;   // strides in elements; o, grad, dq, dk, dv are contiguous
@@ -33,25 +35,29 @@ struct Segment {
 
 // Workgroup -> tile without a list of tiles: segment s owns the tile slots from
 // floor(bound(s) g / rows) + s up to the next segment's, at least as many as it has tiles (the spare
-// ones find nothing to do).  The segment of a slot is searched with 64 probes a step.
+// ones find nothing to do).  by_row: the segment that holds row `slot` itself.  The segment of a slot is searched with 63 probes a step; the last step's
+// probes are neighbours, so both of its bounds are in two lanes already.
 __device__ __forceinline__ Segment find_segment(const int *__restrict__ ptr, int nseq, int total, int g, int rows,
-                                                int slot, bool last_first) {
-  int lo = 0, hi = nseq + 2;
+                                                int slot, bool last_first, bool by_row = false) {
+  int lo = 0, hi = nseq + 2, bound, n, step;
   const int lane = lane_id();
-  while (hi - lo > 1) {
-    const int step = (hi - lo + 63) >> 6, s = lo + lane * step;
-    const bool below = s < hi && seg_bound(ptr, nseq, total, s) * (long long)g / rows + s <= slot;
-    const int n = __popcll(__ballot(below));
-    lo += max(n - 1, 0) * step;
-    hi = min(hi, lo + step);
-  }
-  lo = uniform_i32(lo);
+  do {
+    step = (hi - lo + 62) / 63;
+    const int s = min(lo + lane * step, hi);
+    bound = seg_bound(ptr, nseq, total, s);
+    n = __popcll(__ballot(s < hi && (unsigned)bound * (unsigned)g / (unsigned)rows + (by_row ? 0 : s) <= (unsigned)slot));
+    n = max(n - 1, 0);
+    if (step > 1) {
+      lo += n * step;
+      hi = min(hi, lo + step);
+    }
+  } while (step > 1);
+  lo = uniform_i32(lo + n);
   Segment r;
   r.seq = lo - 1;
-  r.start = uniform_i32(seg_bound(ptr, nseq, total, lo));
-  const int end = uniform_i32(seg_bound(ptr, nseq, total, lo + 1));
-  r.len = max(end - r.start, 0);
-  r.tile = slot - (int)(r.start * (long long)g / rows + lo);
+  r.start = __builtin_amdgcn_readlane(bound, n);
+  r.len = max(__builtin_amdgcn_readlane(bound, n + 1) - r.start, 0);
+  r.tile = slot - (int)((unsigned)r.start * (unsigned)g / (unsigned)rows + lo);
   const int tiles = (int)((r.len * (long long)g + rows - 1) / rows);
   if (r.tile < 0 || r.tile >= tiles) r.tile = -1;
   else if (last_first) r.tile = tiles - 1 - r.tile;
@@ -60,12 +66,22 @@ __device__ __forceinline__ Segment find_segment(const int *__restrict__ ptr, int
 static inline long long tile_slots(int total, int nseq, int g, int rows) {
   return (long long)total * g / rows + nseq + 2;
 }
-// rows of a sequence in the other index (keys of a query's sequence and the other way round)
-__device__ __forceinline__ void other_side(const int *__restrict__ ptr, int nseq, int total, int seq, int *start, int *len) {
+// Sequences of few rows, or few workgroups in all: one wave a workgroup instead of four.
+static inline bool short_rows(long long total, int nseq, int g, int hk) {
+  static const int limit = [] { const char *e = getenv("DGNN_SHORT"); return e ? atoi(e) : 96; }();
+  return total * g <= (long long)limit * nseq || tile_slots((int)total, nseq, g, 128) * hk < 256;
+}
+// Rows of a segment's sequence in the other index: keys of its queries and the other way round.
+__device__ __forceinline__ void other_side(const int *__restrict__ ptr, const int *__restrict__ own, int nseq, int total,
+                                           const Segment &seg, int *start, int *len) {
   *start = 0;
   *len = 0;
-  if (seq < 0 || seq >= nseq) return;
-  const int s = uniform_i32(seg_bound(ptr, nseq, total, seq + 1)), e = uniform_i32(seg_bound(ptr, nseq, total, seq + 2));
+  if (seg.seq < 0 || seg.seq >= nseq) return;
+  if (ptr == own) {                            // self attention
+    *start = min(seg.start, total), *len = min(seg.len, total - *start);
+    return;
+  }
+  const int s = uniform_i32(seg_bound(ptr, nseq, total, seg.seq + 1)), e = uniform_i32(seg_bound(ptr, nseq, total, seg.seq + 2));
   *start = s;
   *len = max(e - s, 0);
 }

@@ -43,23 +43,24 @@ __global__ __launch_bounds__(DGNN_BLOCK) void k_attn_bwd_stat(long long rows, in
 // Rows of a staged tile: 32, or 64 where 32 are too few bytes for one load of every wave.
 template <class T, int DP, int NW>
 constexpr int bwd_rows() { return 32 * DP * (int)sizeof(T) >= 1024 * NW ? 32 : 64; }
-constexpr int BWD_STAGES = 4;
+// one wave a workgroup: more workgroups a compute unit hide latency, not more buffers
+template <int NW> constexpr int bwd_stages() { return NW == 1 ? 2 : 4; }
 
 template <class T, int DP, int NW>
-__global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void k_attn_bwd_kv(const AttnArgs a) {
-  constexpr int BK = 32 * NW, BQ = bwd_rows<T, DP, NW>(), THREADS = 64 * NW, S = BWD_STAGES;
+__global__ __launch_bounds__(64 * NW, sizeof(T) == 2 && NW > 1 ? 2 : 1) void k_attn_bwd_kv(const AttnArgs a) {
+  constexpr int BK = 32 * NW, BQ = bwd_rows<T, DP, NW>(), THREADS = 64 * NW, S = bwd_stages<NW>();
   using TL = Tile<T, DP>;
   using SG = Stager<T, DP, BQ, THREADS>;
   // a stage: q tile, do tile, and for every wave its own copy of the statistics (equal load counts)
   constexpr int TILE = BQ * TL::ROW_BYTES, STAT = 2 * BQ * 4;
   DGNN_RING(lds, 2 * TILE + NW * STAT);
-  const int lane = lane_id(), h = lane >> 5, wave = uniform_i32(wave_in_block());
+  const int lane = lane_id(), h = lane >> 5, wave = NW == 1 ? 0 : uniform_i32(wave_in_block());
   const int row_lane = TL::row_lane(lane), col_lane = TL::col_lane(lane);
   const int kvh = blockIdx.x % a.hk, slot = blockIdx.x / a.hk;
   const Segment seg = find_segment(a.col_ptr, a.nseq, a.tk, 1, BK, slot, false);
   if (seg.tile < 0) return;
   int qs, lq;
-  other_side(a.row_ptr, a.nseq, a.tq, seg.seq, &qs, &lq);
+  other_side(a.row_ptr, a.col_ptr, a.nseq, a.tq, seg, &qs, &lq);
   const int lk = seg.len;
 
   const int key0 = seg.tile * BK + wave * 32, key = key0 + (lane & 31);
@@ -156,19 +157,19 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void k_attn_bwd_kv
 }
 
 template <class T, int DP, int NW>
-__global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void k_attn_bwd_q(const AttnArgs a) {
-  constexpr int BM = 32 * NW, BN = bwd_rows<T, DP, NW>(), THREADS = 64 * NW, S = BWD_STAGES;
+__global__ __launch_bounds__(64 * NW, sizeof(T) == 2 && NW > 1 ? 2 : 1) void k_attn_bwd_q(const AttnArgs a) {
+  constexpr int BM = 32 * NW, BN = bwd_rows<T, DP, NW>(), THREADS = 64 * NW, S = bwd_stages<NW>();
   using TL = Tile<T, DP>;
   using SG = Stager<T, DP, BN, THREADS>;
   constexpr int TILE = BN * TL::ROW_BYTES;
   DGNN_RING(lds, 2 * TILE);
-  const int lane = lane_id(), h = lane >> 5, wave = uniform_i32(wave_in_block());
+  const int lane = lane_id(), h = lane >> 5, wave = NW == 1 ? 0 : uniform_i32(wave_in_block());
   const int row_lane = TL::row_lane(lane), col_lane = TL::col_lane(lane);
   const int kvh = blockIdx.x % a.hk, slot = blockIdx.x / a.hk;
   const Segment seg = find_segment(a.row_ptr, a.nseq, a.tq, a.g, BM, slot, a.causal != 0);
   if (seg.tile < 0) return;
   int ks, lk;
-  other_side(a.col_ptr, a.nseq, a.tk, seg.seq, &ks, &lk);
+  other_side(a.col_ptr, a.row_ptr, a.nseq, a.tk, seg, &ks, &lk);
 
   const long long rows = (long long)seg.len * a.g;
   const long long row = (long long)seg.tile * BM + wave * 32 + (lane & 31);
@@ -240,30 +241,39 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void k_attn_bwd_q(
   if (valid) store_row<T, DP>((T *)a.dq + (tok * a.hq + head) * a.d, dq, a.scale, a.d, h);
 }
 
+template <class T, int DP, int NW>
+static int launch_bwd_kv(const AttnArgs &a, hipStream_t st) {
+  const long long slots = tile_slots(a.tk, a.nseq, 1, 32 * NW) * a.hk;
+  if (slots > 0x7fffffffLL) return DGNN_ERR_UNSUPPORTED;
+  hipLaunchKernelGGL((k_attn_bwd_kv<T, DP, NW>), dim3((unsigned)slots), dim3(64 * NW), 0, st, a);
+  DGNN_LAUNCH_CHECK();
+  return DGNN_OK;
+}
+template <class T, int DP, int NW>
+static int launch_bwd_q(const AttnArgs &a, hipStream_t st) {
+  const long long slots = tile_slots(a.tq, a.nseq, a.g, 32 * NW) * a.hk;
+  if (slots > 0x7fffffffLL) return DGNN_ERR_UNSUPPORTED;
+  hipLaunchKernelGGL((k_attn_bwd_q<T, DP, NW>), dim3((unsigned)slots), dim3(64 * NW), 0, st, a);
+  DGNN_LAUNCH_CHECK();
+  return DGNN_OK;
+}
 template <class T, int DP>
 static int launch_bwd(const AttnArgs &a, const float *lse, hipStream_t st) {
-  constexpr int NW = 4;
   const long long rows = (long long)a.tq * a.hq;
+  int rc = DGNN_OK;
   if (rows > 0) {
     constexpr int LPR = DP * (int)sizeof(T) / 16;
-    hipLaunchKernelGGL((k_attn_bwd_stat<T, LPR>), dim3((unsigned)((rows * LPR + DGNN_BLOCK - 1) / DGNN_BLOCK)),
-                       dim3(DGNN_BLOCK), 0, st, rows, a.d, a.tq, a.hq, (const T *)a.out, (const T *)a.grad, lse,
-                       (float2 *)a.stat);
+    const long long blocks = (rows * LPR + DGNN_BLOCK - 1) / DGNN_BLOCK;
+    if (blocks > 0x7fffffffLL) return DGNN_ERR_UNSUPPORTED;
+    hipLaunchKernelGGL((k_attn_bwd_stat<T, LPR>), dim3((unsigned)blocks), dim3(DGNN_BLOCK), 0, st, rows, a.d, a.tq, a.hq,
+                       (const T *)a.out, (const T *)a.grad, lse, (float2 *)a.stat);
     DGNN_LAUNCH_CHECK();
   }
-  if (a.tk > 0) {
-    const long long slots = tile_slots(a.tk, a.nseq, 1, 32 * NW) * a.hk;
-    if (slots > 0x7fffffffLL) return DGNN_ERR_UNSUPPORTED;
-    hipLaunchKernelGGL((k_attn_bwd_kv<T, DP, NW>), dim3((unsigned)slots), dim3(64 * NW), 0, st, a);
-    DGNN_LAUNCH_CHECK();
-  }
-  if (a.tq > 0) {
-    const long long slots = tile_slots(a.tq, a.nseq, a.g, 32 * NW) * a.hk;
-    if (slots > 0x7fffffffLL) return DGNN_ERR_UNSUPPORTED;
-    hipLaunchKernelGGL((k_attn_bwd_q<T, DP, NW>), dim3((unsigned)slots), dim3(64 * NW), 0, st, a);
-    DGNN_LAUNCH_CHECK();
-  }
-  return DGNN_OK;
+  if (a.tk > 0)
+    rc = short_rows(a.tk, a.nseq, 1, a.hk) ? launch_bwd_kv<T, DP, 1>(a, st) : launch_bwd_kv<T, DP, 4>(a, st);
+  if (rc == DGNN_OK && a.tq > 0)
+    rc = short_rows(a.tq, a.nseq, a.g, a.hk) ? launch_bwd_q<T, DP, 1>(a, st) : launch_bwd_q<T, DP, 4>(a, st);
+  return rc;
 }
 template <class T>
 static int launch_bwd_d(const AttnArgs &a, const float *lse, hipStream_t st) {

@@ -58,7 +58,7 @@ __global__ __launch_bounds__(DGNN_BLOCK) void k_embed_fwd(int n, int rows, int d
 }
 
 // ------------------------------------------------------------------ stable radix sort of (row, i)
-constexpr int SORT_TILE = 4096, SORT_BINS = 256;
+constexpr int SORT_TILE = 1024, SORT_BINS = 256, SORT_SMALL = 4096;
 static inline int sort_tiles(int n) { return (n + SORT_TILE - 1) / SORT_TILE; }
 
 template <class I>
@@ -82,35 +82,104 @@ __global__ __launch_bounds__(DGNN_BLOCK) void k_sort_count(int n, int shift, Sor
   counts[(long long)threadIdx.x * gridDim.x + blockIdx.x] = bins[threadIdx.x];
 }
 
-// exclusive sums in place, one workgroup
+// exclusive prefix over the 1024 threads of a workgroup; *total gets the sum
+__device__ __forceinline__ int block_prefix(int x, int (&part)[16], int *total) {
+  const int lane = lane_id(), wave = wave_in_block();
+  int incl = x;
+#pragma unroll
+  for (int w = 1; w < 64; w <<= 1) {
+    const int up = __shfl_up(incl, w, 64);
+    if (lane >= w) incl += up;
+  }
+  if (lane == 63) part[wave] = incl;
+  __syncthreads();
+  int before = 0, all = 0;
+#pragma unroll
+  for (int w = 0; w < 16; ++w) {
+    if (w < wave) before += part[w];
+    all += part[w];
+  }
+  __syncthreads();
+  *total = all;
+  return before + incl - x;
+}
+
+// exclusive sums in place, one workgroup, 16 numbers a thread at a time (total is a multiple of 4)
 __global__ __launch_bounds__(1024) void k_sort_scan(int total, int *__restrict__ x) {
-  __shared__ int part[1024];
+  __shared__ int part[16];
   int carry = 0;
-  for (int base = 0; base < total; base += 4096) {
-    const int i = base + threadIdx.x * 4;
-    int v[4], s = 0;
+  for (int base = 0; base < total; base += 16384) {
+    const int i = base + threadIdx.x * 16;
+    int4 v[4];
+    int s = 0, all;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      v[j] = i + j < total ? x[i + j] : 0;
-      s += v[j];
+      v[j] = i + 4 * j < total ? *(const int4 *)(x + i + 4 * j) : make_int4(0, 0, 0, 0);
+      s += v[j].x + v[j].y + v[j].z + v[j].w;
     }
-    part[threadIdx.x] = s;
+    int run = carry + block_prefix(s, part, &all);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int4 w = make_int4(run, run + v[j].x, run + v[j].x + v[j].y, run + v[j].x + v[j].y + v[j].z);
+      run = w.w + v[j].w;
+      if (i + 4 * j < total) *(int4 *)(x + i + 4 * j) = w;
+    }
+    carry += all;
+  }
+}
+
+// Lanes of the wave whose digit equals this lane's (of the lanes that take part).
+__device__ __forceinline__ unsigned long long same_digit(int digit, bool on) {
+  unsigned long long same = __ballot(on);
+#pragma unroll
+  for (int b = 0; b < 8; ++b) {
+    const unsigned long long set = __ballot((digit >> b) & 1);
+    same &= (digit >> b) & 1 ? set : ~set;
+  }
+  return same;
+}
+
+// The whole sort of up to SORT_SMALL ids in one workgroup: every wave owns 256 consecutive positions; a
+// pass counts the wave's digits, turns the counts into first positions (digit, then wave) and moves
+// the pairs within LDS in order.
+template <class I>
+__global__ __launch_bounds__(1024) void k_sort_small(int n, int rows, int passes, const I *__restrict__ ids,
+                                                     int *__restrict__ key, int *__restrict__ val) {
+  constexpr int WAVES = 16, PART = SORT_SMALL / WAVES;
+  __shared__ int at[WAVES][SORT_BINS], ks[2][SORT_SMALL], vs[2][SORT_SMALL], part[16];
+  const int lane = lane_id(), wave = wave_in_block();
+  for (int i = threadIdx.x; i < n; i += 1024) ks[0][i] = row_of_id(ids, i, rows), vs[0][i] = i;
+  for (int p = 0; p < passes; ++p) {
+    const int *ki = ks[p & 1], *vi = vs[p & 1];
+    int *ko = ks[(p + 1) & 1], *vo = vs[(p + 1) & 1];
+    const int shift = 8 * p, lo = wave * PART, hi = min(n, lo + PART);
+    for (int i = threadIdx.x; i < WAVES * SORT_BINS; i += 1024) ((int *)at)[i] = 0;
     __syncthreads();
-    for (int w = 1; w < 1024; w <<= 1) {
-      const int add = threadIdx.x >= (unsigned)w ? part[threadIdx.x - w] : 0;
-      __syncthreads();
-      part[threadIdx.x] += add;
-      __syncthreads();
-    }
-    int run = carry + part[threadIdx.x] - s;
+    for (int i = lo + lane; i < hi; i += DGNN_WAVE) atomicAdd(&at[wave][(ki[i] >> shift) & (SORT_BINS - 1)], 1);
+    __syncthreads();
+    int c[4], s = 0, all;                       // thread t: digit t / 4, waves 4 (t % 4) ..
+    const int digit = threadIdx.x >> 2, w0 = 4 * (threadIdx.x & 3);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if (i + j < total) x[i + j] = run;
-      run += v[j];
+    for (int j = 0; j < 4; ++j) c[j] = at[w0 + j][digit], s += c[j];
+    int run = block_prefix(s, part, &all);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) at[w0 + j][digit] = run, run += c[j];
+    __syncthreads();
+    for (int base = lo; base < hi; base += DGNN_WAVE) {
+      const int i = base + lane;
+      const bool on = i < hi;
+      const int k = on ? ki[i] : 0, d = (k >> shift) & (SORT_BINS - 1);
+      const unsigned long long same = same_digit(d, on);
+      const int rank = __popcll(same & ((1ULL << lane) - 1));
+      const int to = on ? at[wave][d] + rank : 0;
+      wave_lds_sync();
+      if (on && rank == 0) at[wave][d] += __popcll(same);
+      wave_lds_sync();
+      if (on) ko[to] = k, vo[to] = vi[i];
     }
-    carry += part[1023];
     __syncthreads();
   }
+  for (int i = threadIdx.x; i < n; i += 1024) key[i] = ks[passes & 1][i], val[i] = vs[passes & 1][i];
 }
 
 // Every wave owns a quarter of the tile; it counts its digits, then walks it again in order: the rank
@@ -138,12 +207,7 @@ __global__ __launch_bounds__(DGNN_BLOCK) void k_sort_scatter(int n, int shift, S
     const int i = base + lane;
     const bool on = i < hi;
     const int k = on ? src.k(i) : 0, digit = (k >> shift) & (SORT_BINS - 1);
-    unsigned long long same = __ballot(on);
-#pragma unroll
-    for (int b = 0; b < 8; ++b) {
-      const unsigned long long set = __ballot((digit >> b) & 1);
-      same &= (digit >> b) & 1 ? set : ~set;
-    }
+    const unsigned long long same = same_digit(digit, on);
     const int rank = __popcll(same & ((1ULL << lane) - 1)), count = __popcll(same);
     const int to = on ? at[wave][digit] + rank : 0;
     wave_lds_sync();
@@ -157,11 +221,23 @@ __global__ __launch_bounds__(DGNN_BLOCK) void k_sort_scatter(int n, int shift, S
 }
 
 // ------------------------------------------------------------------ sums of the runs
-__device__ __forceinline__ int first_not_below(const int *__restrict__ key, int n, int k) {
-  int lo = 0, hi = n;
+__device__ __forceinline__ int first_not_below(const int *__restrict__ key, int lo, int hi, int k) {
   while (lo < hi) {
     const int mid = (lo + hi) >> 1;
     if (key[mid] < k) lo = mid + 1; else hi = mid;
+  }
+  return lo;
+}
+// the same by a whole wave, 64 probes a step
+__device__ __forceinline__ int first_not_below_wave(const int *__restrict__ key, int n, int k) {
+  int lo = 0, hi = n;                           // the answer lies in [lo, hi]
+  const int lane = lane_id();
+  while (lo < hi) {
+    const int step = (hi - lo + 63) >> 6, i = lo + lane * step;
+    const int below = __popcll(__ballot(i < hi && key[i] < k));
+    if (below == 0) return lo;
+    lo += (below - 1) * step + 1;
+    hi = min(hi, lo + step - 1);
   }
   return lo;
 }
@@ -181,14 +257,14 @@ __global__ __launch_bounds__(DGNN_BLOCK) void k_embed_long(int n, int rows, int 
   for (int which = 0; which < 2; ++which) {
     const int k = ends[which];
     if (k >= rows || (which == 1 && k == ends[0])) continue;
-    const int s = first_not_below(key, n, k), e = first_not_below(key, n, k + 1);
+    const int s = first_not_below_wave(key, n, k), e = first_not_below_wave(key, n, k + 1);
     if (e - s <= run) continue;
     const int a = max(s, lo), b = min(e, hi);
     float acc[N];
 #pragma unroll
     for (int j = 0; j < N; ++j) acc[j] = 0.f;
     if (c < dim) {
-#pragma unroll 4
+#pragma unroll 8
       for (int i = a + wave; i < b; i += DGNN_WAVES_PER_BLOCK) {
         const Pack<T, N> p = *(const Pack<T, N> *)(grad + (long long)val[i] * dim + c);
 #pragma unroll
@@ -209,37 +285,78 @@ __global__ __launch_bounds__(DGNN_BLOCK) void k_embed_long(int n, int rows, int 
   }
 }
 
-constexpr int EMBED_ROWS = 64;       // rows of the table a workgroup writes
+constexpr int EMBED_ROWS = 256;      // most rows of the table a workgroup writes
 
+// A workgroup writes `per_block` consecutive rows.  It finds the sorted positions that name them, marks
+// where each row's run begins and ends, stores zeros to the rows without one as one stream of pieces, and
+// gives every other row to `lanes` threads.
 template <class T, int N>
-__global__ __launch_bounds__(DGNN_BLOCK) void k_embed_rows(int n, int rows, int dim, int lanes, int run, float scale,
+__global__ __launch_bounds__(DGNN_BLOCK) void k_embed_rows(int n, int rows, int dim, int lanes, int per_block, int run, float scale,
                                                            const int *__restrict__ key, const int *__restrict__ val,
                                                            const T *__restrict__ grad, const float *__restrict__ part,
                                                            T *__restrict__ out) {
-  __shared__ int start[EMBED_ROWS + 1];
-  const int row0 = blockIdx.x * EMBED_ROWS;
-  if (threadIdx.x <= EMBED_ROWS) start[threadIdx.x] = first_not_below(key, n, (int)min((long long)rows, row0 + (long long)threadIdx.x));
+  __shared__ int begin[EMBED_ROWS], end[EMBED_ROWS], list[EMBED_ROWS], bounds[2], count;
+  const int row0 = blockIdx.x * per_block, mine = min(per_block, rows - row0), wave = wave_in_block();
+  if (wave < 2) {
+    const int at = first_not_below_wave(key, n, wave == 0 ? row0 : row0 + mine);
+    if (lane_id() == 0) bounds[wave] = at;
+  }
+  if ((int)threadIdx.x < EMBED_ROWS) begin[threadIdx.x] = 0, end[threadIdx.x] = 0;
+  if (threadIdx.x == 0) count = 0;
   __syncthreads();
-  const int per = DGNN_BLOCK / lanes, group = threadIdx.x / lanes, lane = threadIdx.x & (lanes - 1);
-  for (int rr = group; rr < EMBED_ROWS && row0 + rr < rows; rr += per) {
-    const int s = start[rr], e = start[rr + 1];
-    T *to = out + (long long)(row0 + rr) * dim;
+  const int p0 = bounds[0], p1 = bounds[1];
+  if (p1 - p0 <= 4 * DGNN_BLOCK) {              // few: read them all, a run begins and ends where the key changes
+    for (int i = p0 + threadIdx.x; i < p1; i += DGNN_BLOCK) {
+      const int k = key[i];
+      if (i == p0 || key[i - 1] != k) begin[k - row0] = i;
+      if (i == p1 - 1 || key[i + 1] != k) end[k - row0] = i + 1;
+    }
+  } else if ((int)threadIdx.x < mine) {         // long runs among them: search
+    const int a = first_not_below(key, p0, p1, row0 + threadIdx.x);
+    const int b = first_not_below(key, a, p1, row0 + threadIdx.x + 1);
+    if (b > a) begin[threadIdx.x] = a, end[threadIdx.x] = b;
+  }
+  __syncthreads();
+  if (wave == 0)                                // the rows that have a run, in order
+    for (int b = 0; b < mine; b += DGNN_WAVE) {
+      const int r = b + lane_id();
+      const bool on = r < mine && end[r] > begin[r];
+      const unsigned long long set = __ballot(on);
+      if (on) list[count + __popcll(set & ((1ULL << lane_id()) - 1))] = r;
+      wave_lds_sync();
+      if (lane_id() == 0) count += __popcll(set);
+      wave_lds_sync();
+    }
+  const int pieces = dim / N;
+  for (int u = threadIdx.x; u < mine * pieces; u += DGNN_BLOCK) {
+    const int r = u / pieces;
+    if (end[r] > begin[r]) continue;
+    Pack<T, N> p;
+#pragma unroll
+    for (int j = 0; j < N; ++j) p.v[j] = (T)0.f;
+    *(Pack<T, N> *)(out + (long long)row0 * dim + (long long)u * N) = p;
+  }
+  __syncthreads();
+  const int groups = DGNN_BLOCK / lanes, group = threadIdx.x / lanes, lane = threadIdx.x & (lanes - 1);
+  for (int x = group; x < count; x += groups) {
+    const int r = list[x], s = begin[r], e = end[r];
+    T *to = out + (long long)(row0 + r) * dim;
     for (int c = lane * N; c < dim; c += lanes * N) {
       float acc[N];
 #pragma unroll
       for (int j = 0; j < N; ++j) acc[j] = 0.f;
       if (e - s <= run) {
-#pragma unroll 4
+#pragma unroll 8
         for (int i = s; i < e; ++i) {
           const Pack<T, N> p = *(const Pack<T, N> *)(grad + (long long)val[i] * dim + c);
 #pragma unroll
           for (int j = 0; j < N; ++j) acc[j] += (float)p.v[j];
         }
       } else {
-        const int p0 = s / run, p1 = (e - 1) / run;
-#pragma unroll 4
-        for (int p = p0; p <= p1; ++p) {
-          const float *src = part + (long long)(2 * p + (p == p0 && s != p * run ? 1 : 0)) * dim + c;
+        const int q0 = s / run, q1 = (e - 1) / run;
+#pragma unroll 8
+        for (int q = q0; q <= q1; ++q) {
+          const float *src = part + (long long)(2 * q + (q == q0 && s != q * run ? 1 : 0)) * dim + c;
 #pragma unroll
           for (int j = 0; j < N; ++j) acc[j] += src[j];
         }
@@ -252,10 +369,10 @@ __global__ __launch_bounds__(DGNN_BLOCK) void k_embed_rows(int n, int rows, int 
   }
 }
 
-// pieces of about sqrt(n): a run of all n ids is summed in two balanced steps
+// pieces of about sqrt(n) / 4: the longest run possible is summed in two steps of some hundred terms
 static inline int embed_run(int n) {
   int r = 64;
-  while ((long long)r * r < n) r <<= 1;
+  while (16LL * r * r < n) r <<= 1;
   return r;
 }
 static inline size_t align256(size_t x) { return (x + 255) / 256 * 256; }
@@ -307,8 +424,10 @@ static int launch_embed_sums(int n, int rows, int dim, float scale, const EmbedP
                        dim3(DGNN_BLOCK), 0, st, n, rows, dim, p.run, key, val, (const T *)grad, part);
     DGNN_LAUNCH_CHECK();
   }
-  hipLaunchKernelGGL((k_embed_rows<T, N>), dim3((unsigned)((rows + (long long)EMBED_ROWS - 1) / EMBED_ROWS)), dim3(DGNN_BLOCK), 0, st, n,
-                     rows, dim, row_lanes(dim, N), p.run, scale, key, val, (const T *)grad, part, (T *)out);
+  const int lanes = row_lanes(dim, N), groups = DGNN_BLOCK / lanes;
+  const int per_block = groups * 16 < 16 ? 16 : groups * 16 > EMBED_ROWS ? EMBED_ROWS : groups * 16;
+  hipLaunchKernelGGL((k_embed_rows<T, N>), dim3((unsigned)((rows + (long long)per_block - 1) / per_block)), dim3(DGNN_BLOCK), 0, st, n,
+                     rows, dim, lanes, per_block, p.run, scale, key, val, (const T *)grad, part, (T *)out);
   DGNN_LAUNCH_CHECK();
   return DGNN_OK;
 }
@@ -318,6 +437,12 @@ static int sort_ids(int n, int rows, const void *ids, const EmbedPlan &p, char *
   int *k[2] = {(int *)ws, (int *)(ws + p.pairs)}, *v[2] = {(int *)(ws + 2 * p.pairs), (int *)(ws + 3 * p.pairs)};
   int *counts = (int *)(ws + 4 * p.pairs);
   const int tiles = sort_tiles(n);
+  if (n <= SORT_SMALL) {
+    hipLaunchKernelGGL(k_sort_small<I>, dim3(1), dim3(1024), 0, st, n, rows, p.passes, (const I *)ids, k[0], v[0]);
+    DGNN_LAUNCH_CHECK();
+    *key = k[0], *val = v[0];
+    return DGNN_OK;
+  }
   for (int i = 0; i < p.passes; ++i) {
     const SortSrc<I> src = {i == 0 ? (const I *)ids : nullptr, k[(i + 1) & 1], v[(i + 1) & 1], rows};
     hipLaunchKernelGGL(k_sort_count<I>, dim3(tiles), dim3(DGNN_BLOCK), 0, st, n, 8 * i, src, counts);

@@ -1066,8 +1066,10 @@ std::tuple<Tensor, Tensor> attention_forward(const Tensor &q, const Tensor &k, c
   c10::DeviceGuard guard(q.device());
   const AttnCall c = attn_call(q, k, v, row_ptr, col_ptr);
   Tensor out = at::empty({c.tq, c.hq, c.width}, q.options()), lse = new_f32({c.hq, c.tq}, q);
+  const size_t nb = API(dgnn_attn_forward_workspace_bytes)(c.nseq, c.tq, c.tk, c.hq, c.hk, c.d);
+  Tensor ws = workspace(nb, q);
   check_rc(API(dgnn_attn_forward)(c.dtype, c.nseq, c.tq, c.tk, c.hq, c.hk, c.d, causal, (float)scale, cv(c.q), cv(c.k),
-                                  cv(c.v), c.strides, ip(row_ptr), ip(col_ptr), vo(out), fo(lse), stream_of(q)),
+                                  cv(c.v), c.strides, ip(row_ptr), ip(col_ptr), vo(out), fo(lse), vo(ws), nb, stream_of(q)),
            "dgnn_attn_forward");
   return std::make_tuple(cut(out, q.size(2)), lse);
 }

@@ -514,9 +514,10 @@ int dgnn_embedding_backward(int dtype, int idx_bytes, int n, int rows, int dim, 
  * strides: HOST array {q_token, q_head, k_token, k_head, v_token, v_head} in elements, the last
  * dimension contiguous.  DGNN_ERR_UNSUPPORTED: d > 128, or rows that are not whole 16-byte chunks (d and
  * every stride), or a token stride under d or of 16 MB and more.  The other tensors are contiguous. */
+size_t dgnn_attn_forward_workspace_bytes(int nseq, int tq, int tk, int hq, int hk, int d);
 int dgnn_attn_forward(int dtype, int nseq, int tq, int tk, int hq, int hk, int d, int causal, float scale,
                       const void *q, const void *k, const void *v, const long long *strides, const int *row_ptr,
-                      const int *col_ptr, void *out, float *lse, void *stream);
+                      const int *col_ptr, void *out, float *lse, void *workspace, size_t workspace_bytes, void *stream);
 /* dq [tq,hq,d], dk and dv [tk,hk,d] from grad [tq,hq,d] and the forward's out and lse; fully written.
  * No atomics: the same bits every time. */
 size_t dgnn_attn_backward_workspace_bytes(int tq, int hq);

@@ -219,6 +219,17 @@ def test_attention_large_scores_and_long_rows():
     attention_case([40], [5000], 4, 1, 128, True, torch.bfloat16)
 
 
+@pytest.mark.parametrize("dtype", DTYPES, ids=ids_of)
+@pytest.mark.parametrize("causal", [False, True], ids=["full", "causal"])
+@pytest.mark.parametrize("hq,hk,d", [(1, 1, 32), (8, 2, 64), (16, 1, 128), (6, 2, 41)])
+def test_attention_few_rows_long_keys(hq, hk, d, causal, dtype):
+    """Rows split over chunks of the keys: ragged keys, some sequences with many rows, with none, without
+    keys, padding in front and behind."""
+    attention_case([1] * 7, [300, 1, 700, 0, 257, 256, 1500], hq, hk, d, causal, dtype, front=3, back=2, poison=True)
+    attention_case([2, 0, 70, 1, 3], [1000, 600, 900, 0, 513], hq, hk, d, causal, dtype)
+    attention_case([1], [4000], hq, hk, d, causal, dtype)
+
+
 def test_attention_many_small_graphs():
     lens = [(i * 7) % 40 for i in range(700)]
     attention_case(lens, lens, 1, 1, 32, False, torch.float32)

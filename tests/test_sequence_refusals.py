@@ -14,10 +14,11 @@ P = 0x10000                      # an aligned address that is never read
 
 
 def attn(dtype=1, nseq=1, tq=8, tk=8, hq=4, hk=2, d=64, q=P, k=P, v=P, strides=None, row_ptr=P, col_ptr=P, out=P,
-         lse=P, null_strides=False):
+         lse=P, ws=P, wsb=1 << 30, null_strides=False):
     size = (hq * d, d, hk * d, d, hk * d, d) if strides is None else strides
     arr = None if null_strides else (ctypes.c_longlong * 6)(*size)
-    return _lib.lib().dgnn_attn_forward(dtype, nseq, tq, tk, hq, hk, d, 0, 1.0, q, k, v, arr, row_ptr, col_ptr, out, lse, None)
+    return _lib.lib().dgnn_attn_forward(dtype, nseq, tq, tk, hq, hk, d, 0, 1.0, q, k, v, arr, row_ptr, col_ptr, out, lse, ws, wsb,
+                                        None)
 
 
 @pytest.mark.parametrize("change,code", [
@@ -34,6 +35,8 @@ def attn(dtype=1, nseq=1, tq=8, tk=8, hq=4, hk=2, d=64, q=P, k=P, v=P, strides=N
     (dict(strides=(1 << 23, 64, 128, 64, 128, 64)), UNSUPPORTED),
     (dict(q=P + 8), ALIGNMENT), (dict(v=P + 2), ALIGNMENT), (dict(out=P + 4), ALIGNMENT), (dict(row_ptr=P + 2), ALIGNMENT),
     (dict(lse=P + 1), ALIGNMENT),
+    (dict(tk=4096, tq=2, ws=None), WORKSPACE), (dict(tk=4096, tq=2, wsb=4096), WORKSPACE),
+    (dict(tk=4096, tq=2, ws=P + 4), ALIGNMENT),                           # single queries: split over the keys
 ])
 def test_attention_forward_refuses(change, code):
     assert attn(**change) == code
