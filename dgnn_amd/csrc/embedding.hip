@@ -82,7 +82,8 @@ __global__ __launch_bounds__(DGNN_BLOCK) void k_sort_count(int n, int shift, Sor
   counts[(long long)threadIdx.x * gridDim.x + blockIdx.x] = bins[threadIdx.x];
 }
 
-// exclusive prefix over the 1024 threads of a workgroup; *total gets the sum
+// exclusive prefix over the threads of a workgroup of WAVES waves; *total gets the sum
+template <int WAVES>
 __device__ __forceinline__ int block_prefix(int x, int (&part)[16], int *total) {
   const int lane = lane_id(), wave = wave_in_block();
   int incl = x;
@@ -95,7 +96,7 @@ __device__ __forceinline__ int block_prefix(int x, int (&part)[16], int *total) 
   __syncthreads();
   int before = 0, all = 0;
 #pragma unroll
-  for (int w = 0; w < 16; ++w) {
+  for (int w = 0; w < WAVES; ++w) {
     if (w < wave) before += part[w];
     all += part[w];
   }
@@ -104,28 +105,35 @@ __device__ __forceinline__ int block_prefix(int x, int (&part)[16], int *total) 
   return before + incl - x;
 }
 
-// exclusive sums in place, one workgroup, 16 numbers a thread at a time (total is a multiple of 4)
-__global__ __launch_bounds__(1024) void k_sort_scan(int total, int *__restrict__ x) {
-  __shared__ int part[16];
+// counts[bin][.] becomes its exclusive prefix over the tiles, totals[bin] the bin's sum; one wave a bin
+__global__ __launch_bounds__(DGNN_WAVE) void k_sort_scan(int tiles, int *__restrict__ counts, int *__restrict__ totals) {
+  int *x = counts + (long long)blockIdx.x * tiles;
+  const int lane = lane_id();
   int carry = 0;
-  for (int base = 0; base < total; base += 16384) {
-    const int i = base + threadIdx.x * 16;
-    int4 v[4];
-    int s = 0, all;
+  for (int base = 0; base < tiles; base += 4 * DGNN_WAVE) {
+    int v[4], s = 0;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      v[j] = i + 4 * j < total ? *(const int4 *)(x + i + 4 * j) : make_int4(0, 0, 0, 0);
-      s += v[j].x + v[j].y + v[j].z + v[j].w;
+      const int i = base + lane * 4 + j;
+      v[j] = i < tiles ? x[i] : 0;
+      s += v[j];
     }
-    int run = carry + block_prefix(s, part, &all);
+    int incl = s;
+#pragma unroll
+    for (int w = 1; w < 64; w <<= 1) {
+      const int up = __shfl_up(incl, w, 64);
+      if (lane >= w) incl += up;
+    }
+    int run = carry + incl - s;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const int4 w = make_int4(run, run + v[j].x, run + v[j].x + v[j].y, run + v[j].x + v[j].y + v[j].z);
-      run = w.w + v[j].w;
-      if (i + 4 * j < total) *(int4 *)(x + i + 4 * j) = w;
+      const int i = base + lane * 4 + j;
+      if (i < tiles) x[i] = run;
+      run += v[j];
     }
-    carry += all;
+    carry += __shfl(incl, 63, 64);
   }
+  if (lane == 0) totals[blockIdx.x] = carry;
 }
 
 // Lanes of the wave whose digit equals this lane's (of the lanes that take part).
@@ -161,7 +169,7 @@ __global__ __launch_bounds__(1024) void k_sort_small(int n, int rows, int passes
     const int digit = threadIdx.x >> 2, w0 = 4 * (threadIdx.x & 3);
 #pragma unroll
     for (int j = 0; j < 4; ++j) c[j] = at[w0 + j][digit], s += c[j];
-    int run = block_prefix(s, part, &all);
+    int run = block_prefix<WAVES>(s, part, &all);
 #pragma unroll
     for (int j = 0; j < 4; ++j) at[w0 + j][digit] = run, run += c[j];
     __syncthreads();
@@ -186,9 +194,9 @@ __global__ __launch_bounds__(1024) void k_sort_small(int n, int rows, int passes
 // of a key among the 64 of a step is the number of lower lanes with its digit.
 template <class I>
 __global__ __launch_bounds__(DGNN_BLOCK) void k_sort_scatter(int n, int shift, SortSrc<I> src,
-                                                             const int *__restrict__ offs, int *__restrict__ key,
-                                                             int *__restrict__ val) {
-  __shared__ int at[DGNN_WAVES_PER_BLOCK][SORT_BINS];
+                                                             const int *__restrict__ offs, const int *__restrict__ totals,
+                                                             int *__restrict__ key, int *__restrict__ val) {
+  __shared__ int at[DGNN_WAVES_PER_BLOCK][SORT_BINS], part[16];
   const int lane = lane_id(), wave = wave_in_block();
   for (int w = 0; w < DGNN_WAVES_PER_BLOCK; ++w) at[w][threadIdx.x] = 0;
   __syncthreads();
@@ -196,7 +204,8 @@ __global__ __launch_bounds__(DGNN_BLOCK) void k_sort_scatter(int n, int shift, S
   const int lo = blockIdx.x * SORT_TILE + wave * PART, hi = min(n, lo + PART);
   for (int i = lo + lane; i < hi; i += DGNN_WAVE) atomicAdd(&at[wave][(src.k(i) >> shift) & (SORT_BINS - 1)], 1);
   __syncthreads();
-  int run = offs[(long long)threadIdx.x * gridDim.x + blockIdx.x];
+  int all, run = offs[(long long)threadIdx.x * gridDim.x + blockIdx.x];
+  run += block_prefix<DGNN_WAVES_PER_BLOCK>(totals[threadIdx.x], part, &all);      // the smaller digits
   for (int w = 0; w < DGNN_WAVES_PER_BLOCK; ++w) {
     const int c = at[w][threadIdx.x];
     at[w][threadIdx.x] = run;
@@ -327,15 +336,6 @@ __global__ __launch_bounds__(DGNN_BLOCK) void k_embed_rows(int n, int rows, int 
       if (lane_id() == 0) count += __popcll(set);
       wave_lds_sync();
     }
-  const int pieces = dim / N;
-  for (int u = threadIdx.x; u < mine * pieces; u += DGNN_BLOCK) {
-    const int r = u / pieces;
-    if (end[r] > begin[r]) continue;
-    Pack<T, N> p;
-#pragma unroll
-    for (int j = 0; j < N; ++j) p.v[j] = (T)0.f;
-    *(Pack<T, N> *)(out + (long long)row0 * dim + (long long)u * N) = p;
-  }
   __syncthreads();
   const int groups = DGNN_BLOCK / lanes, group = threadIdx.x / lanes, lane = threadIdx.x & (lanes - 1);
   for (int x = group; x < count; x += groups) {
@@ -367,6 +367,16 @@ __global__ __launch_bounds__(DGNN_BLOCK) void k_embed_rows(int n, int rows, int 
       *(Pack<T, N> *)(to + c) = p;
     }
   }
+  // last, so that the stores drain while the next workgroup searches
+  const int pieces = dim / N;
+  for (int u = threadIdx.x; u < mine * pieces; u += DGNN_BLOCK) {
+    const int r = u / pieces;
+    if (end[r] > begin[r]) continue;
+    Pack<T, N> p;
+#pragma unroll
+    for (int j = 0; j < N; ++j) p.v[j] = (T)0.f;
+    *(Pack<T, N> *)(out + (long long)row0 * dim + (long long)u * N) = p;
+  }
 }
 
 // pieces of about sqrt(n) / 4: the longest run possible is summed in two steps of some hundred terms
@@ -388,7 +398,7 @@ static EmbedPlan embed_plan(int n, int rows, int dim) {
   p.run = embed_run(n);
   p.pieces = (n + p.run - 1) / p.run;
   p.pairs = align256(sizeof(int) * (size_t)n);
-  p.counts = align256(sizeof(int) * (size_t)SORT_BINS * sort_tiles(n));
+  p.counts = align256(sizeof(int) * (size_t)SORT_BINS * (sort_tiles(n) + 1));
   p.part = align256(sizeof(float) * 2 * (size_t)p.pieces * dim);
   p.total = 4 * p.pairs + p.counts + p.part;
   return p;
@@ -425,7 +435,7 @@ static int launch_embed_sums(int n, int rows, int dim, float scale, const EmbedP
     DGNN_LAUNCH_CHECK();
   }
   const int lanes = row_lanes(dim, N), groups = DGNN_BLOCK / lanes;
-  const int per_block = groups * 16 < 16 ? 16 : groups * 16 > EMBED_ROWS ? EMBED_ROWS : groups * 16;
+  const int per_block = groups * 16 > EMBED_ROWS / 2 ? EMBED_ROWS : groups * 16;
   hipLaunchKernelGGL((k_embed_rows<T, N>), dim3((unsigned)((rows + (long long)per_block - 1) / per_block)), dim3(DGNN_BLOCK), 0, st, n,
                      rows, dim, lanes, per_block, p.run, scale, key, val, (const T *)grad, part, (T *)out);
   DGNN_LAUNCH_CHECK();
@@ -435,7 +445,7 @@ template <class I>
 static int sort_ids(int n, int rows, const void *ids, const EmbedPlan &p, char *ws, const int **key, const int **val,
                     hipStream_t st) {
   int *k[2] = {(int *)ws, (int *)(ws + p.pairs)}, *v[2] = {(int *)(ws + 2 * p.pairs), (int *)(ws + 3 * p.pairs)};
-  int *counts = (int *)(ws + 4 * p.pairs);
+  int *counts = (int *)(ws + 4 * p.pairs), *totals = counts + (size_t)SORT_BINS * sort_tiles(n);
   const int tiles = sort_tiles(n);
   if (n <= SORT_SMALL) {
     hipLaunchKernelGGL(k_sort_small<I>, dim3(1), dim3(1024), 0, st, n, rows, p.passes, (const I *)ids, k[0], v[0]);
@@ -447,10 +457,10 @@ static int sort_ids(int n, int rows, const void *ids, const EmbedPlan &p, char *
     const SortSrc<I> src = {i == 0 ? (const I *)ids : nullptr, k[(i + 1) & 1], v[(i + 1) & 1], rows};
     hipLaunchKernelGGL(k_sort_count<I>, dim3(tiles), dim3(DGNN_BLOCK), 0, st, n, 8 * i, src, counts);
     DGNN_LAUNCH_CHECK();
-    hipLaunchKernelGGL(k_sort_scan, dim3(1), dim3(1024), 0, st, SORT_BINS * tiles, counts);
+    hipLaunchKernelGGL(k_sort_scan, dim3(SORT_BINS), dim3(DGNN_WAVE), 0, st, tiles, counts, totals);
     DGNN_LAUNCH_CHECK();
     hipLaunchKernelGGL(k_sort_scatter<I>, dim3(tiles), dim3(DGNN_BLOCK), 0, st, n, 8 * i, src, (const int *)counts,
-                       k[i & 1], v[i & 1]);
+                       (const int *)totals, k[i & 1], v[i & 1]);
     DGNN_LAUNCH_CHECK();
   }
   *key = k[(p.passes - 1) & 1];
