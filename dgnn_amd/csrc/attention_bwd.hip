@@ -54,6 +54,10 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 && NW > 1 ? 2 : 1) void k_a
   // a stage: q tile, do tile, and for every wave its own copy of the statistics (equal load counts)
   constexpr int TILE = BQ * TL::ROW_BYTES, STAT = 2 * BQ * 4;
   DGNN_RING(lds, 2 * TILE + NW * STAT);
+  // Two waves a SIMD leave 256 registers; at DP = 128 the accumulators and both operands take 192, and the
+  // last fragments of k did not fit (a spill to memory whose wait drains the ring).  They live in LDS.
+  constexpr int PARK = DP == 128 && sizeof(T) == 2 && NW > 1 ? 2 : 0, KEPT = DP / 16 - PARK;
+  __shared__ __align__(16) char parked[PARK ? PARK * THREADS * 16 : 16];
   const int lane = lane_id(), h = lane >> 5, wave = NW == 1 ? 0 : uniform_i32(wave_in_block());
   const int row_lane = TL::row_lane(lane), col_lane = TL::col_lane(lane);
   const int kvh = blockIdx.x % a.hk, slot = blockIdx.x / a.hk;
@@ -75,6 +79,8 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 && NW > 1 ? 2 : 1) void k_a
   frag8<T> kf[DP / 16], vf[DP / 16];
   load_row_frags<T, DP>(kf, (const T *)a.k + tok * a.k_tok + (long long)kvh * a.k_head, a.d, h, valid);
   load_row_frags<T, DP>(vf, (const T *)a.v + tok * a.v_tok + (long long)kvh * a.v_head, a.d, h, valid);
+#pragma unroll
+  for (int k = KEPT; k < DP / 16; ++k) *(frag8<T> *)(parked + ((k - KEPT) * THREADS + threadIdx.x) * 16) = kf[k];
   const float c = a.scale * DGNN_LOG2E;
 
   const unsigned q_stride = (unsigned)(a.q_tok * sizeof(T)), g_stride = (unsigned)((long long)a.hq * a.d * sizeof(T));
@@ -114,7 +120,8 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 && NW > 1 ? 2 : 1) void k_a
       acc16 s = acc_zero(), dp = acc_zero();
 #pragma unroll
       for (int k = 0; k < DP / 16; ++k) {
-        s = mma(TL::row_frag(qt, rl, 32 * qb, 16 * k), kf[k], s);
+        const frag8<T> kk = k < KEPT ? kf[k] : *(const frag8<T> *)(parked + ((k - KEPT) * THREADS + threadIdx.x) * 16);
+        s = mma(TL::row_frag(qt, rl, 32 * qb, 16 * k), kk, s);
         dp = mma(TL::row_frag(gt, rl, 32 * qb, 16 * k), vf[k], dp);
       }
 #pragma unroll
@@ -150,10 +157,12 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 && NW > 1 ? 2 : 1) void k_a
   };
   ring<S, 2 * SG::LOADS + BQ / 32>(total, stage, work);
 
-  if (!valid) return;
-  const long long at = (tok * a.hk + kvh) * a.d;
-  store_row<T, DP>((T *)a.dk + at, dk, a.scale, a.d, h);
-  store_row<T, DP>((T *)a.dv + at, dv, 1.f, a.d, h);
+  // the lane's key once more, rather than in registers throughout the loop
+  const int lane2 = opaque(lane), key2 = key0 + (lane2 & 31);
+  if (key2 >= lk) return;
+  const long long at = ((seg.start + (long long)key2) * a.hk + kvh) * a.d;
+  store_row<T, DP>((T *)a.dk + at, dk, a.scale, a.d, lane2 >> 5);
+  store_row<T, DP>((T *)a.dv + at, dv, 1.f, a.d, lane2 >> 5);
 }
 
 template <class T, int DP, int NW>

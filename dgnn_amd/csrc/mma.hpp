@@ -251,15 +251,19 @@ template <int S, int LOADS, class Stage, class Work>
 __device__ __forceinline__ void ring(int tiles, const Stage &stage, const Work &work) {
   if (tiles <= 0) return;
   unrolled<0, S - 1>([&](auto i) { stage(i.value, i); });
-  for (int t = 0; t < tiles; t += S)
-    unrolled<0, S>([&](auto i) {
-      if (t + i.value < tiles) {
-        wait_loads<LOADS * (S - 2)>();
-        barrier_in_flight();
-        stage(t + i.value + S - 1, std::integral_constant<int, (i.value + S - 1) % S>());
-        work(t + i.value, i);
-      }
-    });
+  auto step = [&](int t, auto i) {
+    wait_loads<LOADS * (S - 2)>();
+    barrier_in_flight();
+    stage(t + S - 1, std::integral_constant<int, (i.value + S - 1) % S>());
+    work(t, i);
+  };
+  // whole rounds without a branch, then the rest: joining paths, the compiler would wait for loads of
+  // the path that issued fewer
+  int t = 0;
+  for (; t + S <= tiles; t += S) unrolled<0, S>([&](auto i) { step(t + i.value, i); });
+  unrolled<0, S - 1>([&](auto i) {
+    if (t + i.value < tiles) step(t + i.value, i);
+  });
   wait_loads<0>();                             // the loads behind the last tile still write LDS
 }
 
