@@ -74,16 +74,20 @@ static inline bool short_rows(long long total, int nseq, int g, int hk) {
 // Rows of a segment's sequence in the other index: keys of its queries and the other way round.
 __device__ __forceinline__ void other_side(const int *__restrict__ ptr, const int *__restrict__ own, int nseq, int total,
                                            const Segment &seg, int *start, int *len) {
-  *start = 0;
-  *len = 0;
-  if (seg.seq < 0 || seg.seq >= nseq) return;
-  if (ptr == own) {                            // self attention
-    *start = min(seg.start, total), *len = min(seg.len, total - *start);
-    return;
+  int s = 0, e = 0;
+  if (seg.seq >= 0 && seg.seq < nseq) {
+    if (ptr == own) {                          // self attention
+      s = min(seg.start, total);
+      e = min(seg.start + seg.len, total);
+    } else {
+      s = seg_bound(ptr, nseq, total, seg.seq + 1);
+      e = seg_bound(ptr, nseq, total, seg.seq + 2);
+    }
   }
-  const int s = uniform_i32(seg_bound(ptr, nseq, total, seg.seq + 1)), e = uniform_i32(seg_bound(ptr, nseq, total, seg.seq + 2));
-  *start = s;
-  *len = max(e - s, 0);
+  // into scalar registers whatever the compiler makes of the branches: a buffer descriptor in vector
+  // registers costs a loop per load
+  *start = uniform_i32(s);
+  *len = uniform_i32(max(e - s, 0));
 }
 
 // A query row's (or key row's) DP / 16 fragments straight from global memory; columns behind d are zeros.

@@ -174,9 +174,13 @@ __device__ __forceinline__ int opaque(int x) {
   return x;
 }
 
-// 128-bit buffer descriptor over `bytes` bytes at p: reads behind them give zeros.
+// 128-bit buffer descriptor over `bytes` bytes at p: reads behind them give zeros.  Both are the same in
+// all lanes and are made scalars here: where the compiler cannot prove it, every load through the
+// descriptor becomes a loop over the lanes' values.
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_over(const void *p, unsigned bytes) {
-  return __builtin_amdgcn_make_buffer_rsrc((void *)p, 0, (int)bytes, 0x00020000);
+  const unsigned long long at = (unsigned long long)p;
+  const unsigned long long lo = (unsigned)uniform_i32((int)at), hi = (unsigned)uniform_i32((int)(at >> 32));
+  return __builtin_amdgcn_make_buffer_rsrc((void *)(lo | hi << 32), 0, uniform_i32((int)bytes), 0x00020000);
 }
 #define DGNN_OOB 0x80000000u                       // an offset behind every descriptor used here
 
