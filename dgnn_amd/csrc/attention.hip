@@ -25,7 +25,7 @@ struct AttnTile {
   using TL = Tile<T, DP>;
   using SG = Stager<T, DP, BN, 64 * NW>;
   static constexpr int TILE = BN * TL::ROW_BYTES, BYTES = 2 * TILE;
-  static_assert(2 * SG::LOADS * (S - 2) < 64, "loads in flight are counted in six bits");
+  static_assert(S == 1 || 2 * SG::LOADS * (S - 2) < 64, "loads in flight are counted in six bits");
 
   acc16 acc[DP / 32];
   float m, l, c;
@@ -33,7 +33,7 @@ struct AttnTile {
   int head, limit;
   long long tok;
 
-  __device__ __forceinline__ void run(const AttnArgs &a, char *const (&lds)[4], int qs, int lq, int ks, int lk, int kvh,
+  __device__ __forceinline__ void run(const AttnArgs &a, const lds_ptr (&lds)[4], int qs, int lq, int ks, int lk, int kvh,
                                       long long row0, long long rows, int key0, int key1) {
     const int lane = lane_id(), h = lane >> 5, wave = NW == 1 ? 0 : uniform_i32(wave_in_block());
     const int row_lane = TL::row_lane(lane), col_lane = TL::col_lane(lane);
@@ -85,7 +85,7 @@ struct AttnTile {
     m = -INFINITY, l = 0.f;
 
     auto work = [&](int t, auto i) {
-      const char *kt = lds[i.value], *vt = kt + TILE;
+      const lds_ptr kt = lds[i.value], vt = kt + TILE;
       const int k0 = key0 + t * BN;
       if (k0 > wave_any) return;
       const int rl = opaque(row_lane), cl = opaque(col_lane);
@@ -134,7 +134,7 @@ struct AttnTile {
         for (int b = 0; b < DP / 32; ++b) acc[b] = mma(TL::col_frag(vt, cl, 16 * k, 32 * b), p, acc[b]);
       }
     };
-    ring<S, 2 * SG::LOADS>(tiles, stage, work);
+    ring<S, 2 * SG::LOADS, NW == 1>(tiles, stage, work);
     l += __shfl_xor(l, 32, 64);
   }
 
@@ -148,12 +148,15 @@ struct AttnTile {
   }
 };
 
-template <class T, int DP, int NW, int BN, int S>
-__global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void k_attn_fwd(const AttnArgs a) {
+template <class T, int DP, int NW, int HW, int BN, int S>
+__global__ __launch_bounds__(64 * NW * HW, sizeof(T) == 2 ? 2 : 1) void k_attn_fwd(const AttnArgs a) {
   using AT = AttnTile<T, DP, NW, BN, S>;
-  DGNN_RING(lds, AT::BYTES);
-  const int kvh = blockIdx.x % a.hk, slot = blockIdx.x / a.hk;
-  const Segment seg = find_segment(a.row_ptr, a.nseq, a.tq, a.g, 32 * NW, slot, a.causal != 0);
+  DGNN_RING(all, HW * AT::BYTES);
+  const HeadSlot at = head_slot<HW>(a.hk, 1);
+  if (at.head >= a.hk) return;
+  const int kvh = at.head;
+  const lds_ptr lds[4] = {all[0] + at.wave * AT::BYTES, all[1] + at.wave * AT::BYTES, all[2] + at.wave * AT::BYTES, all[3] + at.wave * AT::BYTES};
+  const Segment seg = find_segment(a.row_ptr, a.nseq, a.tq, a.g, 32 * NW, at.slot, a.causal != 0);
   if (seg.tile < 0) return;
   int ks, lk;
   other_side(a.col_ptr, a.row_ptr, a.nseq, a.tk, seg, &ks, &lk);
@@ -250,11 +253,11 @@ static AttnPlan attn_plan(int nseq, int tq, int tk, int hq, int hk, int d) {
   return p;
 }
 
-template <class T, int DP, int NW, int BN, int S>
+template <class T, int DP, int NW, int HW, int BN, int S>
 static int launch_rows(const AttnArgs &a, hipStream_t st) {
-  const long long slots = tile_slots(a.tq, a.nseq, a.g, 32 * NW);
-  if (slots * a.hk > 0x7fffffffLL) return DGNN_ERR_UNSUPPORTED;
-  hipLaunchKernelGGL((k_attn_fwd<T, DP, NW, BN, S>), dim3((unsigned)(slots * a.hk)), dim3(64 * NW), 0, st, a);
+  const long long groups = tile_slots(a.tq, a.nseq, a.g, 32 * NW) * ((a.hk + HW - 1) / HW);
+  if (groups > 0x7fffffffLL) return DGNN_ERR_UNSUPPORTED;
+  hipLaunchKernelGGL((k_attn_fwd<T, DP, NW, HW, BN, S>), dim3((unsigned)groups), dim3(64 * NW * HW), 0, st, a);
   DGNN_LAUNCH_CHECK();
   return DGNN_OK;
 }
@@ -270,8 +273,11 @@ static int launch_fwd(const AttnArgs &a, const AttnPlan &p, hipStream_t st) {
     DGNN_LAUNCH_CHECK();
     return DGNN_OK;
   }
-  if (short_rows(a.tq, a.nseq, a.g, a.hk)) return launch_rows<T, DP, 1, 32, 2>(a, st);
-  return launch_rows<T, DP, 4, 64, 2>(a, st);
+  switch (rows_kind(a.tq, a.nseq, a.g, a.hk)) {
+    case ROWS_SHORT: return a.hk >= 4 ? launch_rows<T, DP, 1, 4, 32, 1>(a, st) : launch_rows<T, DP, 1, 1, 32, 1>(a, st);
+    case ROWS_FEW: return launch_rows<T, DP, 1, 1, 32, 2>(a, st);
+    default: return launch_rows<T, DP, 4, 1, 64, 2>(a, st);
+  }
 }
 template <class T>
 static int launch_fwd_d(const AttnArgs &a, const AttnPlan &p, hipStream_t st) {

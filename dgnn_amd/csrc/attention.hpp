@@ -11,8 +11,8 @@ struct AttnArgs {
   void *o, *dq, *dk, *dv;
   float *lse;                                 // [hq, tq], natural logarithm
   float *stat;                                // backward: [hq, tq] pairs {lse log2(e) (+inf for an empty row), <grad, out>}
-  float *part;                                // split forward: partial rows
-  int few, chunk;
+  float *part;                                // partial rows (split forward) or gradients (split backward)
+  int few, chunk, splits;
   const int *row_ptr, *col_ptr;
   int nseq, tq, tk, hq, hk, g, d, causal;     // g = hq / hk
   long long q_tok, q_head, k_tok, k_head, v_tok, v_head;   // strides in elements; o, grad, dq, dk, dv are contiguous
@@ -66,10 +66,27 @@ __device__ __forceinline__ Segment find_segment(const int *__restrict__ ptr, int
 static inline long long tile_slots(int total, int nseq, int g, int rows) {
   return (long long)total * g / rows + nseq + 2;
 }
-// Sequences of few rows, or few workgroups in all: one wave a workgroup instead of four.
-static inline bool short_rows(long long total, int nseq, int g, int hk) {
-  static const int limit = [] { const char *e = getenv("DGNN_SHORT"); return e ? atoi(e) : 96; }();
-  return total * g <= (long long)limit * nseq || tile_slots((int)total, nseq, g, 128) * hk < 256;
+// How the rows of an index are dealt out.  Long: four waves share a tile of 128 packed rows and the tiles
+// staged for it.  Short sequences (96 packed rows on average or less): a wave alone has 32 rows, and four
+// waves of a workgroup take four heads, since workgroups are then so many and so brief that starting
+// them counts; one buffer, because more waves on a compute unit hide more than a second buffer (1024
+// graphs of 1 .. 63 nodes, 8 heads of 32, float: forward 38 us with two buffers and 33 with one).  Few: long
+// sequences, but not a workgroup for every compute unit: a wave a workgroup.
+enum RowsKind { ROWS_LONG, ROWS_SHORT, ROWS_FEW };
+static inline RowsKind rows_kind(int total, int nseq, int g, int hk) {
+  if ((long long)total * g <= 96LL * nseq) return ROWS_SHORT;
+  return tile_slots(total, nseq, g, 128) * hk < 256 ? ROWS_FEW : ROWS_LONG;
+}
+// Workgroup -> key head and tile slot (and split).  Neighbouring workgroups take neighbouring heads: they go to
+// the eight XCDs in turn, so the tiles of one head meet in few of them.  HW > 1: wave w has the group's w-th head.
+struct HeadSlot {
+  int head, slot, split, wave;
+};
+template <int HW>
+__device__ __forceinline__ HeadSlot head_slot(int hk, int splits) {
+  const int groups = (hk + HW - 1) / HW, wave = HW == 1 ? 0 : uniform_i32(wave_in_block());
+  const int rest = blockIdx.x / groups;
+  return {(int)(blockIdx.x % groups) * HW + wave, rest / splits, rest % splits, wave};
 }
 // Rows of a segment's sequence in the other index: keys of its queries and the other way round.
 __device__ __forceinline__ void other_side(const int *__restrict__ ptr, const int *__restrict__ own, int nseq, int total,

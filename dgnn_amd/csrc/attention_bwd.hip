@@ -43,25 +43,27 @@ __global__ __launch_bounds__(DGNN_BLOCK) void k_attn_bwd_stat(long long rows, in
 // Rows of a staged tile: 32, or 64 where 32 are too few bytes for one load of every wave.
 template <class T, int DP, int NW>
 constexpr int bwd_rows() { return 32 * DP * (int)sizeof(T) >= 1024 * NW ? 32 : 64; }
-// one wave a workgroup: more workgroups a compute unit hide latency, not more buffers
-template <int NW> constexpr int bwd_stages() { return NW == 1 ? 2 : 4; }
 
-template <class T, int DP, int NW>
-__global__ __launch_bounds__(64 * NW, sizeof(T) == 2 && NW > 1 ? 2 : 1) void k_attn_bwd_kv(const AttnArgs a) {
-  constexpr int BK = 32 * NW, BQ = bwd_rows<T, DP, NW>(), THREADS = 64 * NW, S = bwd_stages<NW>();
+template <class T, int DP, int NW, int HW, int S>
+__global__ __launch_bounds__(64 * NW * HW, sizeof(T) == 2 && (NW > 1 || DP < 128) ? 2 : 1) void k_attn_bwd_kv(const AttnArgs a) {
+  constexpr int BK = 32 * NW, BQ = bwd_rows<T, DP, NW>(), THREADS = 64 * NW;
   using TL = Tile<T, DP>;
   using SG = Stager<T, DP, BQ, THREADS>;
   // a stage: q tile, do tile, and for every wave its own copy of the statistics (equal load counts)
   constexpr int TILE = BQ * TL::ROW_BYTES, STAT = 2 * BQ * 4;
-  DGNN_RING(lds, 2 * TILE + NW * STAT);
+  constexpr int BYTES = 2 * TILE + NW * STAT;
+  DGNN_RING(all, HW * BYTES);
+  const HeadSlot at = head_slot<HW>(a.hk, a.splits);
+  if (at.head >= a.hk) return;
+  const lds_ptr lds[4] = {all[0] + at.wave * BYTES, all[1] + at.wave * BYTES, all[2] + at.wave * BYTES, all[3] + at.wave * BYTES};
   // Two waves a SIMD leave 256 registers; at DP = 128 the accumulators and both operands take 192, and the
   // last fragments of k did not fit (a spill to memory whose wait drains the ring).  They live in LDS.
   constexpr int PARK = DP == 128 && sizeof(T) == 2 && NW > 1 ? 2 : 0, KEPT = DP / 16 - PARK;
   __shared__ __align__(16) char parked[PARK ? PARK * THREADS * 16 : 16];
   const int lane = lane_id(), h = lane >> 5, wave = NW == 1 ? 0 : uniform_i32(wave_in_block());
   const int row_lane = TL::row_lane(lane), col_lane = TL::col_lane(lane);
-  const int kvh = blockIdx.x % a.hk, slot = blockIdx.x / a.hk;
-  const Segment seg = find_segment(a.col_ptr, a.nseq, a.tk, 1, BK, slot, false);
+  const int kvh = at.head, split = at.split;
+  const Segment seg = find_segment(a.col_ptr, a.nseq, a.tk, 1, BK, at.slot, false);
   if (seg.tile < 0) return;
   int qs, lq;
   other_side(a.row_ptr, a.col_ptr, a.nseq, a.tq, seg, &qs, &lq);
@@ -74,7 +76,10 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 && NW > 1 ? 2 : 1) void k_a
   const int first = a.causal ? key - (lk - lq) : 0;
   const int wave_first = a.causal ? key0 - (lk - lq) : 0, wave_all = a.causal ? key0 + 31 - (lk - lq) : 0;
   const int t0 = a.causal ? max(0, seg.tile * BK - (lk - lq)) / BQ : 0;
-  const int tiles = (lq + BQ - 1) / BQ, per_head = max(0, tiles - t0), total = per_head * a.g;
+  const int tiles = (lq + BQ - 1) / BQ, per_head = max(0, tiles - t0);
+  // this workgroup's share of the query tiles of all heads
+  const int share = (per_head * a.g + a.splits - 1) / a.splits, from = min(split * share, per_head * a.g);
+  const int total = min(share, per_head * a.g - from);
 
   frag8<T> kf[DP / 16], vf[DP / 16];
   load_row_frags<T, DP>(kf, (const T *)a.k + tok * a.k_tok + (long long)kvh * a.k_head, a.d, h, valid);
@@ -88,7 +93,8 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 && NW > 1 ? 2 : 1) void k_a
   SG st_q, st_g;
   st_q.init(q_stride, a.d);
   st_g.init(g_stride, a.d);
-  int s_head = kvh * a.g, s_tile = t0, s_left = total;       // next tile to stage
+  // next tile to stage
+  int s_head = kvh * a.g + from / max(per_head, 1), s_tile = t0 + from % max(per_head, 1), s_left = total;
   auto stage = [&](int, auto i) {
     // rows behind the end arrive as zeros: p = exp2(0 - 0) = 1 there, on do = 0 and delta = 0
     const int n = s_left > 0 ? min(BQ, lq - s_tile * BQ) : 0;
@@ -106,10 +112,10 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 && NW > 1 ? 2 : 1) void k_a
 #pragma unroll
   for (int b = 0; b < DP / 32; ++b) dk[b] = acc_zero(), dv[b] = acc_zero();
 
-  int w_tile = t0;                                           // tile worked on
+  int w_tile = s_tile;                                       // tile worked on
   auto work = [&](int, auto i) {
-    const char *qt = lds[i.value], *gt = qt + TILE;
-    const float *stt = (const float *)(gt + TILE + wave * STAT);
+    const lds_ptr qt = lds[i.value], gt = qt + TILE;
+    const DGNN_LDS float *stt = (const DGNN_LDS float *)(gt + TILE + wave * STAT);
     const int q00 = w_tile * BQ;
     if (++w_tile == tiles) w_tile = t0;
 #pragma unroll
@@ -126,9 +132,9 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 && NW > 1 ? 2 : 1) void k_a
       }
 #pragma unroll
       for (int r4 = 0; r4 < 4; ++r4) {
-        const float4 *st = (const float4 *)(stt + 2 * (32 * qb + 8 * r4 + 4 * h));
-        const float4 x = st[0], y = st[1];
-        const float ls[4] = {x.x, x.z, y.x, y.z}, de[4] = {x.y, x.w, y.y, y.w};
+        const DGNN_LDS vec4<float> *st = (const DGNN_LDS vec4<float> *)(stt + 2 * (32 * qb + 8 * r4 + 4 * h));
+        const vec4<float> x = st[0], y = st[1];
+        const float ls[4] = {x[0], x[2], y[0], y[2]}, de[4] = {x[1], x[3], y[1], y[3]};
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const int r = 4 * r4 + j;
@@ -155,27 +161,54 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 && NW > 1 ? 2 : 1) void k_a
       }
     }
   };
-  ring<S, 2 * SG::LOADS + BQ / 32>(total, stage, work);
+  ring<S, 2 * SG::LOADS + BQ / 32, NW == 1>(total, stage, work);
 
   // the lane's key once more, rather than in registers throughout the loop
   const int lane2 = opaque(lane), key2 = key0 + (lane2 & 31);
   if (key2 >= lk) return;
-  const long long at = ((seg.start + (long long)key2) * a.hk + kvh) * a.d;
-  store_row<T, DP>((T *)a.dk + at, dk, a.scale, a.d, lane2 >> 5);
-  store_row<T, DP>((T *)a.dv + at, dv, 1.f, a.d, lane2 >> 5);
+  const long long to = ((seg.start + (long long)key2) * a.hk + kvh) * a.d;
+  if (a.splits > 1) {
+    float *part = a.part + 2 * ((long long)split * a.tk * a.hk * a.d + to);
+    store_row<float, DP>(part, dk, a.scale, a.d, lane2 >> 5);
+    store_row<float, DP>(part + a.d, dv, 1.f, a.d, lane2 >> 5);
+    return;
+  }
+  store_row<T, DP>((T *)a.dk + to, dk, a.scale, a.d, lane2 >> 5);
+  store_row<T, DP>((T *)a.dv + to, dv, 1.f, a.d, lane2 >> 5);
 }
 
-template <class T, int DP, int NW>
-__global__ __launch_bounds__(64 * NW, sizeof(T) == 2 && NW > 1 ? 2 : 1) void k_attn_bwd_q(const AttnArgs a) {
-  constexpr int BM = 32 * NW, BN = bwd_rows<T, DP, NW>(), THREADS = 64 * NW, S = bwd_stages<NW>();
+// dk and dv of every (key, key head): the sum of the splits' {dk row, dv row}, in order
+template <class T>
+__global__ __launch_bounds__(DGNN_BLOCK) void k_attn_bwd_join(const AttnArgs a) {
+  const long long rows = (long long)a.tk * a.hk, per = a.d / 4, u = blockIdx.x * (long long)DGNN_BLOCK + threadIdx.x;
+  if (u >= rows * per * 2) return;
+  const long long row = u / (per * 2);
+  const int c = (int)(u % (per * 2)) * 4;
+  const float *part = a.part + row * 2 * a.d + c;
+  float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int i = 0; i < a.splits; ++i) {
+    const float4 v = *(const float4 *)(part + i * rows * 2 * a.d);
+    s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
+  }
+  vec4<T> o;
+  o[0] = (T)s.x, o[1] = (T)s.y, o[2] = (T)s.z, o[3] = (T)s.w;
+  *(vec4<T> *)((T *)(c < a.d ? a.dk : a.dv) + row * a.d + (c < a.d ? c : c - a.d)) = o;
+}
+
+template <class T, int DP, int NW, int HW, int S>
+__global__ __launch_bounds__(64 * NW * HW, sizeof(T) == 2 ? 2 : 1) void k_attn_bwd_q(const AttnArgs a) {
+  constexpr int BM = 32 * NW, BN = bwd_rows<T, DP, NW>(), THREADS = 64 * NW;
   using TL = Tile<T, DP>;
   using SG = Stager<T, DP, BN, THREADS>;
   constexpr int TILE = BN * TL::ROW_BYTES;
-  DGNN_RING(lds, 2 * TILE);
+  DGNN_RING(all, HW * 2 * TILE);
+  const HeadSlot at = head_slot<HW>(a.hk, 1);
+  if (at.head >= a.hk) return;
+  const lds_ptr lds[4] = {all[0] + at.wave * 2 * TILE, all[1] + at.wave * 2 * TILE, all[2] + at.wave * 2 * TILE, all[3] + at.wave * 2 * TILE};
   const int lane = lane_id(), h = lane >> 5, wave = NW == 1 ? 0 : uniform_i32(wave_in_block());
   const int row_lane = TL::row_lane(lane), col_lane = TL::col_lane(lane);
-  const int kvh = blockIdx.x % a.hk, slot = blockIdx.x / a.hk;
-  const Segment seg = find_segment(a.row_ptr, a.nseq, a.tq, a.g, BM, slot, a.causal != 0);
+  const int kvh = at.head;
+  const Segment seg = find_segment(a.row_ptr, a.nseq, a.tq, a.g, BM, at.slot, a.causal != 0);
   if (seg.tile < 0) return;
   int ks, lk;
   other_side(a.col_ptr, a.row_ptr, a.nseq, a.tk, seg, &ks, &lk);
@@ -219,7 +252,7 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 && NW > 1 ? 2 : 1) void k_a
   for (int b = 0; b < DP / 32; ++b) dq[b] = acc_zero();
 
   auto work = [&](int t, auto i) {
-    const char *kt = lds[i.value], *vt = kt + TILE;
+    const lds_ptr kt = lds[i.value], vt = kt + TILE;
 #pragma unroll
     for (int kb = 0; kb < BN / 32; ++kb) {
       const int k0 = t * BN + 32 * kb;
@@ -245,24 +278,44 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 && NW > 1 ? 2 : 1) void k_a
       }
     }
   };
-  ring<S, 2 * SG::LOADS>(tiles, stage, work);
+  ring<S, 2 * SG::LOADS, NW == 1>(tiles, stage, work);
 
   if (valid) store_row<T, DP>((T *)a.dq + (tok * a.hq + head) * a.d, dq, a.scale, a.d, h);
 }
 
-template <class T, int DP, int NW>
+// Into how many parts the query tiles of a key tile are split.  A key tile's workgroup walks the queries of
+// every head that shares the key head, the first ones of a causal sequence all of them: with fewer
+// workgroups than four rounds of the card, the longest of them are most of the time.  The parts cost
+// writing and reading dk and dv once each in float: 20 k tokens, 16 / 4 heads of 128, causal, lengths up to
+// 8000: 1.59 ms unsplit.
+static int bwd_splits(int nseq, int tq, int tk, int hq, int hk) {
+  if (nseq <= 0 || tk <= 0 || tq <= 0 || rows_kind(tk, nseq, 1, 1 << 20) == ROWS_SHORT) return 1;
+  const long long groups = tile_slots(tk, nseq, 1, 128) * hk, steps = (long long)tq / nseq / 32 * (hq / hk);
+  long long s = (2047 + groups) / groups;
+  if (s > steps / 16) s = steps / 16;
+  return (int)(s < 1 ? 1 : s > 8 ? 8 : s);
+}
+static size_t align256(size_t x) { return (x + 255) / 256 * 256; }
+
+template <class T, int DP, int NW, int HW, int S>
 static int launch_bwd_kv(const AttnArgs &a, hipStream_t st) {
-  const long long slots = tile_slots(a.tk, a.nseq, 1, 32 * NW) * a.hk;
-  if (slots > 0x7fffffffLL) return DGNN_ERR_UNSUPPORTED;
-  hipLaunchKernelGGL((k_attn_bwd_kv<T, DP, NW>), dim3((unsigned)slots), dim3(64 * NW), 0, st, a);
+  const long long groups = tile_slots(a.tk, a.nseq, 1, 32 * NW) * ((a.hk + HW - 1) / HW) * a.splits;
+  if (groups > 0x7fffffffLL) return DGNN_ERR_UNSUPPORTED;
+  hipLaunchKernelGGL((k_attn_bwd_kv<T, DP, NW, HW, S>), dim3((unsigned)groups), dim3(64 * NW * HW), 0, st, a);
   DGNN_LAUNCH_CHECK();
+  if (a.splits > 1) {
+    const long long blocks = ((long long)a.tk * a.hk * (a.d / 2) + DGNN_BLOCK - 1) / DGNN_BLOCK;
+    if (blocks > 0x7fffffffLL) return DGNN_ERR_UNSUPPORTED;
+    hipLaunchKernelGGL(k_attn_bwd_join<T>, dim3((unsigned)blocks), dim3(DGNN_BLOCK), 0, st, a);
+    DGNN_LAUNCH_CHECK();
+  }
   return DGNN_OK;
 }
-template <class T, int DP, int NW>
+template <class T, int DP, int NW, int HW, int S>
 static int launch_bwd_q(const AttnArgs &a, hipStream_t st) {
-  const long long slots = tile_slots(a.tq, a.nseq, a.g, 32 * NW) * a.hk;
-  if (slots > 0x7fffffffLL) return DGNN_ERR_UNSUPPORTED;
-  hipLaunchKernelGGL((k_attn_bwd_q<T, DP, NW>), dim3((unsigned)slots), dim3(64 * NW), 0, st, a);
+  const long long groups = tile_slots(a.tq, a.nseq, a.g, 32 * NW) * ((a.hk + HW - 1) / HW);
+  if (groups > 0x7fffffffLL) return DGNN_ERR_UNSUPPORTED;
+  hipLaunchKernelGGL((k_attn_bwd_q<T, DP, NW, HW, S>), dim3((unsigned)groups), dim3(64 * NW * HW), 0, st, a);
   DGNN_LAUNCH_CHECK();
   return DGNN_OK;
 }
@@ -278,10 +331,16 @@ static int launch_bwd(const AttnArgs &a, const float *lse, hipStream_t st) {
                        (const T *)a.out, (const T *)a.grad, lse, (float2 *)a.stat);
     DGNN_LAUNCH_CHECK();
   }
-  if (a.tk > 0)
-    rc = short_rows(a.tk, a.nseq, 1, a.hk) ? launch_bwd_kv<T, DP, 1>(a, st) : launch_bwd_kv<T, DP, 4>(a, st);
-  if (rc == DGNN_OK && a.tq > 0)
-    rc = short_rows(a.tq, a.nseq, a.g, a.hk) ? launch_bwd_q<T, DP, 1>(a, st) : launch_bwd_q<T, DP, 4>(a, st);
+  if (a.tk > 0) switch (a.splits > 1 ? ROWS_LONG : rows_kind(a.tk, a.nseq, 1, a.hk)) {
+      case ROWS_SHORT: rc = a.hk >= 4 ? launch_bwd_kv<T, DP, 1, 4, 1>(a, st) : launch_bwd_kv<T, DP, 1, 1, 1>(a, st); break;
+      case ROWS_FEW: rc = launch_bwd_kv<T, DP, 1, 1, 2>(a, st); break;
+      default: rc = launch_bwd_kv<T, DP, 4, 1, 4>(a, st);
+    }
+  if (rc == DGNN_OK && a.tq > 0) switch (rows_kind(a.tq, a.nseq, a.g, a.hk)) {
+      case ROWS_SHORT: rc = a.hk >= 4 ? launch_bwd_q<T, DP, 1, 4, 1>(a, st) : launch_bwd_q<T, DP, 1, 1, 1>(a, st); break;
+      case ROWS_FEW: rc = launch_bwd_q<T, DP, 1, 1, 2>(a, st); break;
+      default: rc = launch_bwd_q<T, DP, 4, 1, 4>(a, st);
+    }
   return rc;
 }
 template <class T>
@@ -295,9 +354,11 @@ static int launch_bwd_d(const AttnArgs &a, const float *lse, hipStream_t st) {
 
 extern "C" {
 
-size_t dgnn_attn_backward_workspace_bytes(int tq, int hq) {
-  if (tq <= 0 || hq <= 0) return 0;
-  return 2 * sizeof(float) * (size_t)tq * (size_t)hq;
+size_t dgnn_attn_backward_workspace_bytes(int nseq, int tq, int tk, int hq, int hk, int d) {
+  if (nseq < 0 || tq < 0 || tk < 0 || hq <= 0 || hk <= 0 || d <= 0 || hq % hk != 0) return 0;
+  const int splits = bwd_splits(nseq, tq, tk, hq, hk);
+  return align256(2 * sizeof(float) * (size_t)tq * (size_t)hq) +
+         (splits > 1 ? 2 * sizeof(float) * (size_t)splits * (size_t)tk * (size_t)hk * (size_t)d : 0);
 }
 
 int dgnn_attn_backward(int dtype, int nseq, int tq, int tk, int hq, int hk, int d, int causal, float scale,
@@ -311,11 +372,13 @@ int dgnn_attn_backward(int dtype, int nseq, int tq, int tk, int hq, int hk, int 
   if (tk > 0 && (!dk || !dv)) return DGNN_ERR_BAD_ARG;
   for (const void *p : {out, grad, (const void *)dq, (const void *)dk, (const void *)dv})
     if ((uintptr_t)p & 15) return DGNN_ERR_ALIGNMENT;
-  if (workspace_bytes < dgnn_attn_backward_workspace_bytes(tq, hq) || (tq > 0 && !workspace)) return DGNN_ERR_WORKSPACE;
+  if (workspace_bytes < dgnn_attn_backward_workspace_bytes(nseq, tq, tk, hq, hk, d) || (tq > 0 && !workspace)) return DGNN_ERR_WORKSPACE;
   if (((uintptr_t)workspace & 15) || ((uintptr_t)lse & 3)) return DGNN_ERR_ALIGNMENT;
   if ((long long)hq * d * (dtype == DGNN_F32 ? 4 : 2) >= (1LL << 31) / 128) return DGNN_ERR_UNSUPPORTED;
   a.out = out, a.grad = grad, a.dq = dq, a.dk = dk, a.dv = dv;
   a.stat = (float *)workspace;
+  a.splits = bwd_splits(nseq, tq, tk, hq, hk);
+  a.part = (float *)((char *)workspace + align256(2 * sizeof(float) * (size_t)tq * (size_t)hq));
   hipStream_t st = (hipStream_t)stream;
   if (dtype == DGNN_F32) return launch_bwd_d<float>(a, lse, st);
   if (dtype == DGNN_BF16) return launch_bwd_d<bf16_t>(a, lse, st);

@@ -48,7 +48,7 @@ struct Gemm {
   };
 
   // acc[m][n] += over k in [0, kn)
-  __device__ static __forceinline__ void run(const Operand &a, const Operand &b, int kn, char *const (&lds)[4],
+  __device__ static __forceinline__ void run(const Operand &a, const Operand &b, int kn, const lds_ptr (&lds)[4],
                                              acc16 (&acc)[MB][NB]) {
     const int lane = lane_id(), wave = uniform_i32(wave_in_block());
     const int m0 = wave / C::WN * (BM / C::WM), n0 = wave % C::WN * (BN / C::WN);
@@ -64,7 +64,7 @@ struct Gemm {
     if (BROW && b.list) sb.init_list(b.list, b.count, b.stride, min(BK, kn));
     else sb.init(b.stride, BROW ? min(BK, kn) : b.count);
     auto stage = [&](int t, auto i) {
-      char *const ta = lds[i.value], *const tb = ta + A_BYTES;
+      const lds_ptr ta = lds[i.value], tb = ta + A_BYTES;
       const int k0 = t * BK, left = max(0, min(BK, kn - k0));
       // rows end with a whole chunk (rows of dz are padded with zeros): a descriptor that ended inside one would
       // drop the dword the end falls into
@@ -85,7 +85,7 @@ struct Gemm {
         sb.load(tb, buffer_over((const char *)b.p + (long long)k0 * b.stride, span_bytes(left, b.stride, min(b.count, BN) * (unsigned)sizeof(T))));
     };
     auto work = [&](int, auto i) {
-      const char *const ta = lds[i.value], *const tb = ta + A_BYTES;
+      const lds_ptr ta = lds[i.value], tb = ta + A_BYTES;
 #pragma unroll
       for (int k = 0; k < BK; k += 16) {
         frag8<T> fa[MB], fb[NB];
@@ -102,7 +102,7 @@ struct Gemm {
         mma_block<MB, NB, T>(fa, fb, acc, T());
       }
     };
-    ring<S, decltype(sa)::LOADS + decltype(sb)::LOADS>((kn + BK - 1) / BK, stage, work);
+    ring<S, decltype(sa)::LOADS + decltype(sb)::LOADS, false>((kn + BK - 1) / BK, stage, work);
   }
   __device__ static __forceinline__ void clear(acc16 (&acc)[MB][NB]) {
 #pragma unroll
@@ -387,7 +387,7 @@ __global__ __launch_bounds__(1024) void k_ce_reduce(int n, int mean, const int *
 // buffer of its own, and hands 16-byte pieces to sink(row, column, piece): a lane holds four elements of
 // one row, and stored from there every instruction would touch 32 rows.  The ring is drained by then.
 template <class T, class C, class Value, class Sink>
-__device__ __forceinline__ void rows_of_tile(char *const (&lds)[4], const Value &value, const Sink &sink) {
+__device__ __forceinline__ void rows_of_tile(const lds_ptr (&lds)[4], const Value &value, const Sink &sink) {
   using TL = Tile<T, C::BM>;
   constexpr int PIECES = 32 * TL::CPR;
   const int lane = lane_id(), h = lane >> 5, wave = uniform_i32(wave_in_block());
@@ -397,7 +397,7 @@ __device__ __forceinline__ void rows_of_tile(char *const (&lds)[4], const Value 
     __syncthreads();
     unrolled<0, C::WN>([&](auto b) {
       if (wn != b.value) return;
-      char *const buf = lds[b.value];
+      const lds_ptr buf = lds[b.value];
 #pragma unroll
       for (int i = 0; i < C::MB; ++i)
 #pragma unroll
@@ -406,16 +406,16 @@ __device__ __forceinline__ void rows_of_tile(char *const (&lds)[4], const Value 
           vec4<T> v;
 #pragma unroll
           for (int e = 0; e < 4; ++e) v[e] = value(i, j, 4 * e4 + e, m + e);
-          *(vec4<T> *)(buf + TL::chunk_addr(lane & 31, m / TL::CHUNK) + m % TL::CHUNK * (int)sizeof(T)) = v;
+          *(DGNN_LDS vec4<T> *)(buf + TL::chunk_addr(lane & 31, m / TL::CHUNK) + m % TL::CHUNK * (int)sizeof(T)) = v;
         }
     });
     __syncthreads();
     unrolled<0, C::WN>([&](auto b) {
       if (wn != b.value) return;
-      const char *const buf = lds[b.value];
+      const lds_ptr buf = lds[b.value];
       for (int u = wm * 64 + lane; u < PIECES; u += C::WM * 64) {
         const int row = u / TL::CPR, chunk = u % TL::CPR;
-        sink(wn * (C::BN / C::WN) + 32 * j + row, chunk * TL::CHUNK, *(const u32x4 *)(buf + TL::chunk_addr(row, chunk)));
+        sink(wn * (C::BN / C::WN) + 32 * j + row, chunk * TL::CHUNK, *(const DGNN_LDS u32x4 *)(buf + TL::chunk_addr(row, chunk)));
       }
     });
   }

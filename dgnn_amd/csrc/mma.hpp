@@ -30,6 +30,11 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 
+// Pointers into LDS carry their address space: a generic pointer is only proven to be one where the
+// compiler can see the variable it came from.
+#define DGNN_LDS __attribute__((address_space(3)))
+typedef DGNN_LDS char *lds_ptr;
+
 template <class T> struct frag8_of;
 template <> struct frag8_of<bf16_t> { typedef bf16_t type __attribute__((ext_vector_type(8))); };
 template <> struct frag8_of<half_t> { typedef half_t type __attribute__((ext_vector_type(8))); };
@@ -115,7 +120,7 @@ struct Tile {
     return CPR >= 16 ? ((row & 7) << 1) | ((row >> 3) & 1)
            : CPR == 8 ? (((row >> 1) & 3) << 1) | ((row >> 3) & 1) : (((row >> 2) & 1) << 1) | ((row >> 3) & 1);
   }
-  __device__ static __forceinline__ const char *at(const char *tile, int lane_part, int row, int chunk) {
+  __device__ static __forceinline__ lds_ptr at(lds_ptr tile, int lane_part, int row, int chunk) {
     return tile + (lane_part ^ ((const_swizzle(row) ^ chunk) << 4)) + row * ROW_BYTES;
   }
   // A lane's k elements of a product that sums over the columns: eight consecutive ones, of row
@@ -123,12 +128,12 @@ struct Tile {
   __device__ static __forceinline__ int row_lane(int lane) {
     return lane_addr(lane & 31, (lane >> 5) * (8 / CHUNK));
   }
-  __device__ static __forceinline__ frag8<T> row_frag(const char *tile, int part, int row0, int k0) {
+  __device__ static __forceinline__ frag8<T> row_frag(lds_ptr tile, int part, int row0, int k0) {
     if constexpr (sizeof(T) == 2) {
-      return *(const frag8<T> *)at(tile, part, row0, k0 / CHUNK);
+      return *(const DGNN_LDS frag8<T> *)at(tile, part, row0, k0 / CHUNK);
     } else {
-      const vec4<T> a = *(const vec4<T> *)at(tile, part, row0, k0 / CHUNK);
-      const vec4<T> b = *(const vec4<T> *)at(tile, part, row0, k0 / CHUNK + 1);
+      const vec4<T> a = *(const DGNN_LDS vec4<T> *)at(tile, part, row0, k0 / CHUNK);
+      const vec4<T> b = *(const DGNN_LDS vec4<T> *)at(tile, part, row0, k0 / CHUNK + 1);
       return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
     }
   }
@@ -137,9 +142,9 @@ struct Tile {
   __device__ static __forceinline__ int row_lane_split(int lane) {
     return sizeof(T) == 2 ? lane_addr(lane & 31, 0) + (lane >> 5) * 8 : lane_addr(lane & 31, lane >> 5);
   }
-  __device__ static __forceinline__ frag8<T> row_frag_split(const char *tile, int part, int row0, int k0) {
-    const vec4<T> a = *(const vec4<T> *)at(tile, part, row0, k0 / CHUNK);
-    const vec4<T> b = *(const vec4<T> *)at(tile, part, row0, (k0 + 8) / CHUNK);
+  __device__ static __forceinline__ frag8<T> row_frag_split(lds_ptr tile, int part, int row0, int k0) {
+    const vec4<T> a = *(const DGNN_LDS vec4<T> *)at(tile, part, row0, k0 / CHUNK);
+    const vec4<T> b = *(const DGNN_LDS vec4<T> *)at(tile, part, row0, (k0 + 8) / CHUNK);
     return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
   }
   // A lane's k elements of a product that sums over the rows, for column col0 + lane % 32 (col0 a multiple of
@@ -151,9 +156,9 @@ struct Tile {
       return lane_addr(4 * (lane >> 5) + ((lane & 15) >> 2), 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) + (lane & 1) * 8;
     return lane_addr(4 * (lane >> 5), (lane & 31) >> 2) + (lane & 3) * 4;
   }
-  __device__ static __forceinline__ frag8<T> col_frag(const char *tile, int part, int row0, int col0) {
+  __device__ static __forceinline__ frag8<T> col_frag(lds_ptr tile, int part, int row0, int col0) {
     if constexpr (sizeof(T) == 2) {
-      typedef __attribute__((address_space(3))) s16x4 *lds_p;
+      typedef DGNN_LDS s16x4 *lds_p;
       union { s16x4 s[2]; frag8<T> f; } u;
       u.s[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p)at(tile, part, row0, col0 / CHUNK));
       u.s[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p)at(tile, part, row0 + 8, col0 / CHUNK));
@@ -161,7 +166,7 @@ struct Tile {
     } else {
       frag8<T> f;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) f[j] = *(const T *)at(tile, part, row0 + 8 * (j >> 2) + (j & 3), col0 / CHUNK);
+      for (int j = 0; j < 8; ++j) f[j] = *(const DGNN_LDS T *)at(tile, part, row0 + 8 * (j >> 2) + (j & 3), col0 / CHUNK);
       return f;
     }
   }
@@ -194,11 +199,13 @@ struct Stager {
   using TL = Tile<T, COLS>;
   static constexpr int LOADS = (ROWS * TL::CPR + THREADS - 1) / THREADS;
   static_assert(ROWS * TL::CPR % 64 == 0, "whole waves");
+  // 64 threads: every wave of the workgroup stages tiles of its own
+  __device__ static __forceinline__ int thread() { return THREADS == 64 ? lane_id() : (int)threadIdx.x; }
   unsigned off[LOADS];
   __device__ __forceinline__ void init(unsigned row_stride_bytes, int cols) {
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
-      const int c = i * THREADS + threadIdx.x, row = c / TL::CPR, chunk = (c % TL::CPR) ^ TL::swizzle(row);
+      const int c = i * THREADS + thread(), row = c / TL::CPR, chunk = (c % TL::CPR) ^ TL::swizzle(row);
       off[i] = chunk * TL::CHUNK < cols ? row * row_stride_bytes + chunk * 16u : DGNN_OOB;
     }
   }
@@ -206,7 +213,7 @@ struct Stager {
   __device__ __forceinline__ void init_list(const int *__restrict__ list, int rows, unsigned row_stride_bytes, int cols) {
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
-      const int c = i * THREADS + threadIdx.x, row = c / TL::CPR, chunk = (c % TL::CPR) ^ TL::swizzle(row);
+      const int c = i * THREADS + thread(), row = c / TL::CPR, chunk = (c % TL::CPR) ^ TL::swizzle(row);
       off[i] = chunk * TL::CHUNK < cols && row < rows ? (unsigned)list[row] * row_stride_bytes + chunk * 16u : DGNN_OOB;
     }
   }
@@ -214,17 +221,16 @@ struct Stager {
   __device__ __forceinline__ void narrow(int cols) {
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
-      const int c = i * THREADS + threadIdx.x, row = c / TL::CPR, chunk = (c % TL::CPR) ^ TL::swizzle(row);
+      const int c = i * THREADS + thread(), row = c / TL::CPR, chunk = (c % TL::CPR) ^ TL::swizzle(row);
       if (chunk * TL::CHUNK >= cols) off[i] = DGNN_OOB;
     }
   }
-  __device__ __forceinline__ void load(char *tile, __amdgpu_buffer_rsrc_t src) const {
-    typedef __attribute__((address_space(3))) void *lds_p;
-    const int wave = uniform_i32(threadIdx.x >> 6);
+  __device__ __forceinline__ void load(lds_ptr tile, __amdgpu_buffer_rsrc_t src) const {
+    const int wave = THREADS == 64 ? 0 : uniform_i32(threadIdx.x >> 6);
 #pragma unroll
     for (int i = 0; i < LOADS; ++i)
       if (ROWS * TL::CPR % THREADS == 0 || i * THREADS + wave * 64 < ROWS * TL::CPR)
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(src, (lds_p)(tile + (i * THREADS + wave * 64) * 16), 16, (int)off[i], 0, 0, 0);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(src, tile + (i * THREADS + wave * 64) * 16, 16, (int)off[i], 0, 0, 0);
   }
 };
 
@@ -235,10 +241,12 @@ __device__ __forceinline__ void wait_loads() {
   static_assert(N >= 0 && N < 64, "six bits");
   asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
-// Workgroup barrier that leaves loads to LDS in flight (__syncthreads waits for all of them).
+// Workgroup barrier that leaves loads to LDS in flight (__syncthreads waits for all of them).  OWN: only
+// this wave's LDS reads are waited for, before loads that overwrite what they read.
+template <bool OWN>
 __device__ __forceinline__ void barrier_in_flight() {
   asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-  __builtin_amdgcn_s_barrier();
+  if (!OWN) __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
 }
 
@@ -250,14 +258,26 @@ __device__ __forceinline__ void barrier_in_flight() {
 // DGNN_RING declares four; a ring of fewer leaves the others out of the kernel.
 #define DGNN_RING(name, bytes)                                                                      \
   __shared__ __align__(16) char name##_0[bytes], name##_1[bytes], name##_2[bytes], name##_3[bytes]; \
-  char *const name[4] = {name##_0, name##_1, name##_2, name##_3}
-template <int S, int LOADS, class Stage, class Work>
+  const lds_ptr name[4] = {(lds_ptr)name##_0, (lds_ptr)name##_1, (lds_ptr)name##_2, (lds_ptr)name##_3}
+// OWN: the buffers belong to one wave, no barrier is needed.
+template <int S, int LOADS, bool OWN, class Stage, class Work>
 __device__ __forceinline__ void ring(int tiles, const Stage &stage, const Work &work) {
   if (tiles <= 0) return;
+  if constexpr (S == 1) {
+    constexpr std::integral_constant<int, 0> i;
+    for (int t = 0; t < tiles; ++t) {
+      stage(t, i);
+      wait_loads<0>();
+      barrier_in_flight<OWN>();
+      work(t, i);
+      barrier_in_flight<OWN>();
+    }
+    return;
+  }
   unrolled<0, S - 1>([&](auto i) { stage(i.value, i); });
   auto step = [&](int t, auto i) {
-    wait_loads<LOADS * (S - 2)>();
-    barrier_in_flight();
+    wait_loads<S == 1 ? 0 : LOADS * (S - 2)>();
+    barrier_in_flight<OWN>();
     stage(t + S - 1, std::integral_constant<int, (i.value + S - 1) % S>());
     work(t, i);
   };
@@ -272,9 +292,8 @@ __device__ __forceinline__ void ring(int tiles, const Stage &stage, const Work &
 }
 
 // One load of 4 bytes a lane to 64 consecutive words of LDS.
-__device__ __forceinline__ void load_words(void *to, __amdgpu_buffer_rsrc_t src, unsigned off) {
-  typedef __attribute__((address_space(3))) void *lds_p;
-  __builtin_amdgcn_raw_ptr_buffer_load_lds(src, (lds_p)to, 4, (int)off, 0, 0, 0);
+__device__ __forceinline__ void load_words(lds_ptr to, __amdgpu_buffer_rsrc_t src, unsigned off) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(src, to, 4, (int)off, 0, 0, 0);
 }
 
 // bytes a descriptor over `rows` rows spans (0 rows: nothing is readable)

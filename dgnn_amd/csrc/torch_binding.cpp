@@ -1091,7 +1091,7 @@ std::tuple<Tensor, Tensor, Tensor> attention_backward(const Tensor &q, const Ten
   const Tensor o = dense(out), g = dense(grad);
   Tensor dq = at::empty({c.tq, c.hq, c.width}, q.options()), dk = at::empty({c.tk, c.hk, c.width}, q.options()),
          dv = at::empty({c.tk, c.hk, c.width}, q.options());
-  const size_t nb = API(dgnn_attn_backward_workspace_bytes)(c.tq, c.hq);
+  const size_t nb = API(dgnn_attn_backward_workspace_bytes)(c.nseq, c.tq, c.tk, c.hq, c.hk, c.d);
   Tensor ws = workspace(nb, q);
   check_rc(API(dgnn_attn_backward)(c.dtype, c.nseq, c.tq, c.tk, c.hq, c.hk, c.d, causal, (float)scale, cv(c.q), cv(c.k),
                                    cv(c.v), c.strides, ip(row_ptr), ip(col_ptr), cv(o), fp(lse), cv(g), vo(dq), vo(dk),

@@ -520,7 +520,7 @@ int dgnn_attn_forward(int dtype, int nseq, int tq, int tk, int hq, int hk, int d
                       const int *col_ptr, void *out, float *lse, void *workspace, size_t workspace_bytes, void *stream);
 /* dq [tq,hq,d], dk and dv [tk,hk,d] from grad [tq,hq,d] and the forward's out and lse; fully written.
  * No atomics: the same bits every time. */
-size_t dgnn_attn_backward_workspace_bytes(int tq, int hq);
+size_t dgnn_attn_backward_workspace_bytes(int nseq, int tq, int tk, int hq, int hk, int d);
 int dgnn_attn_backward(int dtype, int nseq, int tq, int tk, int hq, int hk, int d, int causal, float scale,
                        const void *q, const void *k, const void *v, const long long *strides, const int *row_ptr,
                        const int *col_ptr, const void *out, const float *lse, const void *grad, void *dq, void *dk,

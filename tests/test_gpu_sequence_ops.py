@@ -221,6 +221,15 @@ def test_attention_large_scores_and_long_rows():
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=ids_of)
 @pytest.mark.parametrize("causal", [False, True], ids=["full", "causal"])
+@pytest.mark.parametrize("hq,hk,d", [(1, 1, 32), (6, 2, 64), (4, 1, 128)])
+def test_attention_long_rows_split_backward(hq, hk, d, causal, dtype):
+    """Long sequences, few key tiles: the queries of a key tile are split and joined."""
+    attention_case([1100, 0, 901], [1100, 0, 901], hq, hk, d, causal, dtype, back=5, poison=True)
+    attention_case([1500], [333], hq, hk, d, causal, dtype)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=ids_of)
+@pytest.mark.parametrize("causal", [False, True], ids=["full", "causal"])
 @pytest.mark.parametrize("hq,hk,d", [(1, 1, 32), (8, 2, 64), (16, 1, 128), (6, 2, 41)])
 def test_attention_few_rows_long_keys(hq, hk, d, causal, dtype):
     """Rows split over chunks of the keys: ragged keys, some sequences with many rows, with none, without

@@ -100,8 +100,8 @@ def test_cross_entropy_refuses(call, change, code):
 
 def test_workspace_sizes_are_host_functions():
     lib = _lib.lib()
-    assert lib.dgnn_attn_backward_workspace_bytes(100, 4) >= 2 * 4 * 400
-    assert lib.dgnn_attn_backward_workspace_bytes(-1, 4) == 0
+    assert lib.dgnn_attn_backward_workspace_bytes(2, 100, 100, 4, 4, 64) >= 2 * 4 * 400
+    assert lib.dgnn_attn_backward_workspace_bytes(2, -1, 100, 4, 4, 64) == 0
     assert lib.dgnn_embedding_backward_workspace_bytes(1000, 50, 64) >= 4 * 4000
     assert lib.dgnn_embedding_backward_workspace_bytes(0, 50, 64) == 0
     assert lib.dgnn_linear_ce_workspace_bytes(1, 100, 50, 64, 0) > 0
