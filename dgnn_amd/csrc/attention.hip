@@ -18,8 +18,8 @@ using namespace dgnn;
 namespace dgnn {
 
 // One tile: 32 NW packed rows row0 .. of a sequence (`rows` of them exist) against its keys key0 .. key1 - 1.
-// Leaves the lane's unnormalised output row in acc, the running maximum (of z / scale) in m and this
-// lane half's share of the sum in l.
+// Leaves the lane's unnormalised output row in acc, the reference its weights are relative to (near the maximum
+// of z / scale) in m and their sum in l.
 template <class T, int DP, int NW, int BN, int S>
 struct AttnTile {
   using TL = Tile<T, DP>;
@@ -110,7 +110,10 @@ struct AttnTile {
 #pragma unroll
         for (int r = 0; r < 16; ++r) top = fmaxf(top, s[b][r]);
       top = fmaxf(top, __shfl_xor(top, 32, 64));
-      if (__any(top > m)) {
+      // m is a reference near the maximum, not the maximum itself: it moves only when a score exceeds it by more
+      // than 8 (in log2), so weights run up to 256, far from any type's end, and most tiles rescale nothing.
+      // With 32 rows a wave one of them has a new maximum in nearly every tile of some thousand keys.
+      if (__any((top - m) * c > 8.f)) {
         const float by = top == m ? 1.f : exp2_fast((m - top) * c);     // m = -inf: 0
         m = top;
         l *= by;
