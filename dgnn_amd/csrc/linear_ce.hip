@@ -208,12 +208,13 @@ struct CeArgs {
   const void *x, *w;              // rows [n, dk] (gathered: only those with a label), weight [classes, dk]
   int gathered;
   const void *label;
-  const int *list, *count;
+  const int *list, *count;        // labelled rows in order and how many (NULL: row r is row r, all n take part)
+  long long ignore;
   int n, classes, d, dk;          // dk = d rounded up to whole chunks
   int label_bytes;
   float *part_m, *part_s;         // [class tiles, n]
   float *z_label;                 // [n], by gathered row
-  float *lse;                     // [n], by gathered row (backward: by original row)
+  float *lse, *loss;              // [n], by original row
   const float *grad;              // of the loss: n values or one
   int grad_rows, mean;
   const float *grad_top;          // one gradient a row: the largest magnitude
@@ -224,6 +225,8 @@ struct CeArgs {
   void *dx, *dw;
 };
 
+__device__ __forceinline__ int rows_of(const CeArgs &a) { return a.count ? min(a.n, *a.count) : a.n; }
+__device__ __forceinline__ int row_at(const CeArgs &a, int r) { return a.list ? a.list[r] : r; }
 __device__ __forceinline__ long long label_at(const CeArgs &a, int row) {
   return a.label_bytes == 8 ? ((const long long *)a.label)[row] : (long long)((const int *)a.label)[row];
 }
@@ -269,7 +272,7 @@ __global__ __launch_bounds__(1024) void k_ce_grad_top(int n, const int *__restri
 template <class T, class G>
 __device__ __forceinline__ typename G::Operand rows_operand(const CeArgs &a, int r0, int rows) {
   const unsigned stride = (unsigned)(a.dk * sizeof(T));
-  if (a.gathered) return {(const T *)a.x + (long long)r0 * a.dk, rows - r0, stride};
+  if (a.gathered || !a.list) return {(const T *)a.x + (long long)r0 * a.dk, rows - r0, stride};
   return {(const T *)a.x, rows - r0, stride, a.list + r0, a.n * stride};
 }
 
@@ -279,10 +282,10 @@ template <class T, class C>
 __global__ __launch_bounds__(C::THREADS, C::THREADS == 512 ? 2 : 1) void k_ce_fwd(const CeArgs a) {
   using G = Gemm<T, C, true, true>;
   DGNN_RING(lds, G::BYTES);
-  __shared__ float sm[C::WM][C::BN], ss[C::WM][C::BN];
+  __shared__ float sm[C::WM][C::BN], ss[C::WM][C::BN], zl[C::BN];
   const TileAt tile = tile_at(blockIdx.x, (a.classes + C::BM - 1) / C::BM, (a.n + C::BN - 1) / C::BN);
   const int v0 = tile.m * C::BM, r0 = tile.n * C::BN;
-  const int rows = min(a.n, *a.count);
+  const int rows = rows_of(a);
   if (r0 >= rows) return;
   acc16 acc[C::MB][C::NB];
   G::clear(acc);
@@ -294,14 +297,17 @@ __global__ __launch_bounds__(C::THREADS, C::THREADS == 512 ? 2 : 1) void k_ce_fw
 #pragma unroll
   for (int j = 0; j < C::NB; ++j) {
     const int col = n0 + 32 * j + (lane & 31), r = r0 + col;
-    const long long want = r < rows ? label_at(a, a.list[r]) - m0 : -1;
+    const long long label = r < rows ? label_at(a, row_at(a, r)) : -1, want = label == a.ignore ? -1 : label - m0;
     float top = -INFINITY;
     if (want >= 0 && want < C::BM / C::WM) {
 #pragma unroll
       for (int i = 0; i < C::MB; ++i)
 #pragma unroll
         for (int e = 0; e < 16; ++e)
-          if (32 * i + acc_row(e, h) == (int)want) a.z_label[r] = acc[i][j][e];
+          if (32 * i + acc_row(e, h) == (int)want) {
+            if (a.part_m == nullptr) zl[col] = acc[i][j][e];
+            else a.z_label[r] = acc[i][j][e];
+          }
     }
     if (!whole) {
 #pragma unroll
@@ -332,6 +338,15 @@ __global__ __launch_bounds__(C::THREADS, C::THREADS == 512 ? 2 : 1) void k_ce_fw
     const float base = top == -INFINITY ? 0.f : top;
 #pragma unroll
     for (int w = 0; w < C::WM; ++w) s += ss[w][threadIdx.x] * __builtin_amdgcn_exp2f((sm[w][threadIdx.x] - base) * DGNN_LOG2E);
+    if (a.part_m == nullptr) {                  // one tile of classes: this is all there is
+      const int row = r0 + threadIdx.x;
+      const long long label = label_at(a, row);
+      const bool on = label != a.ignore && label >= 0 && label < a.classes;
+      const float lse = base + logf(s);
+      a.lse[row] = on ? lse : 0.f;
+      a.loss[row] = on ? lse - zl[threadIdx.x] : 0.f;
+      return;
+    }
     const long long at = (long long)tile.m * a.n + r0 + threadIdx.x;
     a.part_m[at] = top;
     a.part_s[at] = s;
@@ -339,12 +354,11 @@ __global__ __launch_bounds__(C::THREADS, C::THREADS == 512 ? 2 : 1) void k_ce_fw
 }
 
 // lse and loss of every labelled row from its tiles' pairs: eight rows a workgroup, 32 threads a row
-__global__ __launch_bounds__(DGNN_BLOCK) void k_ce_join(int n, int tiles, const int *__restrict__ list,
-                                                        const int *__restrict__ count, const float *__restrict__ pm,
-                                                        const float *__restrict__ ps, const float *__restrict__ z_label,
-                                                        float *__restrict__ loss, float *__restrict__ lse) {
+__global__ __launch_bounds__(DGNN_BLOCK) void k_ce_join(const CeArgs a, int tiles) {
+  const float *__restrict__ pm = a.part_m, *__restrict__ ps = a.part_s;
+  const int n = a.n;
   __shared__ float sm[32][8], ss[32][8];
-  const int c = threadIdx.x & 7, lane = threadIdx.x >> 3, r = blockIdx.x * 8 + c, rows = min(n, *count);
+  const int c = threadIdx.x & 7, lane = threadIdx.x >> 3, r = blockIdx.x * 8 + c, rows = rows_of(a);
   if ((int)blockIdx.x * 8 >= rows) return;
   float m = -INFINITY, s = 0.f;
   if (r < rows) {
@@ -365,21 +379,32 @@ __global__ __launch_bounds__(DGNN_BLOCK) void k_ce_join(int n, int tiles, const 
   float sum = 0.f;
   for (int w = 0; w < 32; ++w) sum += ss[w][c] * expf(sm[w][c] - base);
   const float v = base + logf(sum);
-  lse[list[r]] = v;
-  loss[list[r]] = v - z_label[r];
+  const int row = row_at(a, r);
+  const long long label = label_at(a, row);
+  const bool on = label != a.ignore && label >= 0 && label < a.classes;
+  a.lse[row] = on ? v : 0.f;
+  a.loss[row] = on ? v - a.z_label[r] : 0.f;
 }
 // out[0] = sum of the losses (/ labelled rows), in a fixed order; no labelled row: 0
-__global__ __launch_bounds__(1024) void k_ce_reduce(int n, int mean, const int *__restrict__ count,
-                                                    const float *__restrict__ loss, float *__restrict__ out) {
+__global__ __launch_bounds__(1024) void k_ce_reduce(const CeArgs a, int mean, const float *__restrict__ loss, float *__restrict__ out) {
   __shared__ double part[16];
+  __shared__ int counts[16];
   double s = 0.;
-  for (int i = threadIdx.x; i < n; i += 1024) s += (double)loss[i];
-  for (int w = 32; w > 0; w >>= 1) s += __shfl_xor(s, w, 64);
-  if (lane_id() == 0) part[wave_in_block()] = s;
+  int c = 0;
+  for (int i = threadIdx.x; i < a.n; i += 1024) {
+    s += (double)loss[i];
+    if (mean && !a.count) {
+      const long long label = label_at(a, i);
+      c += label != a.ignore && label >= 0 && label < a.classes;
+    }
+  }
+  for (int w = 32; w > 0; w >>= 1) s += __shfl_xor(s, w, 64), c += __shfl_xor(c, w, 64);
+  if (lane_id() == 0) part[wave_in_block()] = s, counts[wave_in_block()] = c;
   __syncthreads();
   if (threadIdx.x == 0) {
-    for (int w = 1; w < 16; ++w) s += part[w];
-    out[0] = (float)(mean ? s / (double)max(1, *count) : s);
+    for (int w = 1; w < 16; ++w) s += part[w], c += counts[w];
+    if (a.count) c = *a.count;
+    out[0] = (float)(mean ? s / (double)max(1, c) : s);
   }
 }
 
@@ -629,7 +654,7 @@ static inline unsigned grid_for(long long units) {
 
 enum CeShape { CE_PLAIN, CE_WIDE, CE_THIN };
 struct CePlan {
-  int dk, tiles, copy_w, gather;                      // class tiles of the forward
+  int dk, tiles, copy_w, gather, all;                 // class tiles of the forward; all: no list of labelled rows
   CeShape z, dx_shape, dw_shape;
   size_t list, x, w, part, zl, fwd_total;             // bytes
   int piece, pieces, dx_splits, dw_splits;
@@ -649,6 +674,8 @@ static CePlan ce_plan(int dtype, int n, int classes, int d, const void *x, const
   // rows are read where they are if they are whole, aligned chunks within 32-bit offsets
   p.copy_w = p.dk != d || ((uintptr_t)w & 15) != 0;
   p.gather = p.dk != d || ((uintptr_t)x & 15) != 0 || (long long)n * p.dk * size >= 0x7fffffffLL;
+  // up to about 1e9 operations finding the labelled rows (5 us) costs more than scoring all
+  p.all = !p.gather && 2.0 * n * classes * d <= 1e9;
   p.z = n <= 32 ? CE_THIN : ce_shape(dtype, classes, n, 1);
   p.tiles = ceil_div(classes, p.z == CE_PLAIN ? 128 : 256);
   p.list = align256(sizeof(int) * ((size_t)n + 1));
@@ -698,15 +725,17 @@ static int ce_check(int dtype, int label_bytes, int n, int classes, int d) {
 
 // labelled rows -> list, count; gathered x where asked; padded weight where its rows are not whole chunks
 template <class T>
-static int ce_prepare(const CePlan &p, int n, int classes, int d, bool gather, const void *x, const void *w, const void *label,
+static int ce_prepare(const CePlan &p, int n, int classes, int d, bool all, bool gather, const void *x, const void *w, const void *label,
                       int label_bytes, long long ignore, float *loss, float *lse, char *ws, CeArgs *a, hipStream_t st) {
   int *list = (int *)ws, *count = list + n;
   T *xc = (T *)(ws + p.list), *wc = (T *)(ws + p.list + (gather ? p.x : 0));
-  if (label_bytes == 8)
-    hipLaunchKernelGGL(k_ce_rows<long long>, dim3(1), dim3(1024), 0, st, n, classes, ignore, (const long long *)label, list, count, loss, lse);
-  else
-    hipLaunchKernelGGL(k_ce_rows<int>, dim3(1), dim3(1024), 0, st, n, classes, ignore, (const int *)label, list, count, loss, lse);
-  DGNN_LAUNCH_CHECK();
+  if (!all) {
+    if (label_bytes == 8)
+      hipLaunchKernelGGL(k_ce_rows<long long>, dim3(1), dim3(1024), 0, st, n, classes, ignore, (const long long *)label, list, count, loss, lse);
+    else
+      hipLaunchKernelGGL(k_ce_rows<int>, dim3(1), dim3(1024), 0, st, n, classes, ignore, (const int *)label, list, count, loss, lse);
+    DGNN_LAUNCH_CHECK();
+  }
   const int per = p.dk / (16 / (int)sizeof(T));
   if (gather) {
     hipLaunchKernelGGL(k_ce_gather<T>, dim3(grid_for((long long)n * per)), dim3(DGNN_BLOCK), 0, st, n, d, p.dk,
@@ -721,7 +750,8 @@ static int ce_prepare(const CePlan &p, int n, int classes, int d, bool gather, c
   }
   memset(a, 0, sizeof(*a));
   a->x = gather ? (const void *)xc : x, a->gathered = gather, a->w = p.copy_w ? (const void *)wc : w;
-  a->label = label, a->label_bytes = label_bytes, a->list = list, a->count = count;
+  a->label = label, a->label_bytes = label_bytes, a->ignore = ignore;
+  if (!all) a->list = list, a->count = count;
   a->n = n, a->classes = classes, a->d = d, a->dk = p.dk;
   return DGNN_OK;
 }
@@ -741,9 +771,10 @@ static int ce_forward(const CePlan &p, int n, int classes, int d, const void *x,
   CeArgs a;
   char *at = ws + p.list + (p.gather ? p.x : 0) + p.w;
   float *row = reduction == 0 ? loss : (float *)(at + 2 * p.part + p.zl);
-  const int rc = ce_prepare<T>(p, n, classes, d, p.gather != 0, x, w, label, label_bytes, ignore, row, lse, ws, &a, st);
+  const int rc = ce_prepare<T>(p, n, classes, d, p.all != 0, p.gather != 0, x, w, label, label_bytes, ignore, row, lse, ws, &a, st);
   if (rc != DGNN_OK) return rc;
-  a.part_m = (float *)at, a.part_s = (float *)(at + p.part), a.z_label = (float *)(at + 2 * p.part);
+  a.lse = lse, a.loss = row;
+  if (!p.all || p.tiles > 1) a.part_m = (float *)at, a.part_s = (float *)(at + p.part), a.z_label = (float *)(at + 2 * p.part);
   if (p.z == CE_THIN) {
     DGNN_CE_LAUNCH(k_ce_fwd, Thin<T>, classes, n, 1, a);
   } else if (p.z == CE_PLAIN) {
@@ -751,11 +782,12 @@ static int ce_forward(const CePlan &p, int n, int classes, int d, const void *x,
   } else if constexpr (sizeof(T) == 2) {
     DGNN_CE_LAUNCH(k_ce_fwd, Wide, classes, n, 1, a);
   }
-  hipLaunchKernelGGL(k_ce_join, dim3(ceil_div(n, 8)), dim3(DGNN_BLOCK), 0, st, n, p.tiles, a.list, a.count,
-                     (const float *)a.part_m, (const float *)a.part_s, (const float *)a.z_label, row, lse);
-  DGNN_LAUNCH_CHECK();
+  if (a.part_m) {
+    hipLaunchKernelGGL(k_ce_join, dim3(ceil_div(n, 8)), dim3(DGNN_BLOCK), 0, st, a, p.tiles);
+    DGNN_LAUNCH_CHECK();
+  }
   if (reduction != 0) {
-    hipLaunchKernelGGL(k_ce_reduce, dim3(1), dim3(1024), 0, st, n, (int)(reduction == 1), a.count, (const float *)row, loss);
+    hipLaunchKernelGGL(k_ce_reduce, dim3(1), dim3(1024), 0, st, a, (int)(reduction == 1), (const float *)row, loss);
     DGNN_LAUNCH_CHECK();
   }
   return DGNN_OK;
@@ -766,7 +798,7 @@ static int ce_backward(const CePlan &p, int n, int classes, int d, const void *x
                        int label_bytes, long long ignore, int reduction, const float *lse, const float *grad, void *dx,
                        void *dw, char *ws, hipStream_t st) {
   CeArgs a;
-  const int rc = ce_prepare<T>(p, n, classes, d, true, x, w, label, label_bytes, ignore, nullptr, nullptr, ws, &a, st);
+  const int rc = ce_prepare<T>(p, n, classes, d, false, true, x, w, label, label_bytes, ignore, nullptr, nullptr, ws, &a, st);
   if (rc != DGNN_OK) return rc;
   char *at = ws + p.list + p.x + p.w;
   a.dz = at, a.ldz = p.piece;
@@ -842,7 +874,9 @@ int dgnn_linear_ce_forward(int dtype, int label_bytes, int n, int classes, int d
   hipStream_t st = (hipStream_t)stream;
   if (n == 0) {
     if (reduction != 0 && loss) {
-      hipLaunchKernelGGL(k_ce_reduce, dim3(1), dim3(1024), 0, st, 0, 0, (const int *)nullptr, (const float *)nullptr, loss);
+      CeArgs a;
+      memset(&a, 0, sizeof(a));
+      hipLaunchKernelGGL(k_ce_reduce, dim3(1), dim3(1024), 0, st, a, 0, (const float *)nullptr, loss);
       DGNN_LAUNCH_CHECK();
     }
     return DGNN_OK;

@@ -22,7 +22,11 @@ def PackedAttentionFuse(q, k, v, row_ptr, col_ptr=None, causal=False, scale=None
     value may reach rows that the causal mask keeps from it, as a weight of zero times it does."""
     if scale is None:
         scale = q.size(-1) ** -0.5
-    return PackedAttentionFunction.apply(q, k, v, row_ptr, row_ptr if col_ptr is None else col_ptr, causal, scale)
+    if col_ptr is None:
+        col_ptr = row_ptr
+    if not (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)):
+        return fused_attention.attention_forward(q, k, v, row_ptr, col_ptr, scale, causal)[0]
+    return PackedAttentionFunction.apply(q, k, v, row_ptr, col_ptr, causal, scale)
 
 
 class PackedAttentionFunction(torch.autograd.Function):

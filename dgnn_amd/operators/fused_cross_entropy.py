@@ -13,13 +13,16 @@ def LinearCrossEntropyFuse(feat, weight, label, ignore_index=-100, reduction="me
 
     feat [rows, dim] and weight [classes, dim] of one type (float32, bfloat16 or float16), label int32 or
     int64.  Rows labelled ignore_index, or with a label outside [0, classes), have no loss and no
-    gradient, and nothing of them is read.  reduction: "mean" over the labelled rows (0 if there are
+    gradient, whatever they hold.  reduction: "mean" over the labelled rows (0 if there are
     none), "sum", or "none" (one loss a row, 0 without a label).
 
     The gradient of the logits, rounded to feat's type, is rebuilt a piece of the classes at a
     time; both gradients are summed in float32 in a fixed order."""
     if reduction not in _REDUCTION:
         raise DgnnError(f"reduction must be 'none', 'mean' or 'sum', got {reduction!r}")
+    if not (torch.is_grad_enabled() and (feat.requires_grad or weight.requires_grad)):
+        return fused_cross_entropy.linear_ce_forward(feat.contiguous(), weight.contiguous(), label.contiguous(),
+                                                     ignore_index, _REDUCTION[reduction])[0]
     return LinearCrossEntropyFunction.apply(feat, weight, label, ignore_index, _REDUCTION[reduction])
 
 
