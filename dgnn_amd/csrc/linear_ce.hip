@@ -118,17 +118,21 @@ struct Gemm {
 struct TileAt {
   int m, n;
 };
+// ns counts the tiles that have rows, known on the device alone: the workgroups behind them, which find
+// nothing to do, are then the last ones and not an XCD's whole share.  n = -1: none left.
 __device__ __forceinline__ TileAt tile_at(unsigned id, int ms, int ns) {
+  if (id >= (unsigned)ms * (unsigned)ns) return {0, -1};
   const int u = (int)xcd_contiguous_id(id, (unsigned)ms * (unsigned)ns);
   const int band = u / (ms * 8), width = min(8, ns - band * 8), r = u - band * ms * 8;
   return {r / width, band * 8 + r % width};
 }
 
 // Tile shapes.  Wide: 16-bit types with enough tiles for every compute unit; two waves a SIMD, 128 KB of
-// LDS.  Thin: at most 32 rows, bound by reading the weight.  Plain: the rest, and float, whose matrix
-// instructions are sixteen times slower and bound every shape.
+// LDS.  Thin: at most 32 rows, bound by reading the weight.  Narrow: at most 64 classes.  Plain: the rest,
+// and float, whose matrix instructions are sixteen times slower and bound every shape.
 using Wide = Shape<256, 256, 32, 2, 4, 4>;
 template <class T> using Plain = Shape<128, 128, sizeof(T) == 2 ? 64 : 16, 2, 2, sizeof(T) == 2 ? 2 : 3>;
+template <class T> using Narrow = Shape<64, 64, sizeof(T) == 2 ? 64 : 32, 2, 2, 2>;
 template <class T> using Thin = Shape<256, 32, sizeof(T) == 2 ? 64 : 32, 4, 1, 2>;
 
 // ------------------------------------------------------------------ labelled rows
@@ -182,12 +186,31 @@ __global__ __launch_bounds__(1024) void k_ce_rows(int n, int classes, long long 
   if (threadIdx.x == 0) count[0] = carry;
 }
 
+struct Labels {
+  const void *label;
+  int bytes, classes;
+  long long ignore;
+  __device__ __forceinline__ long long at(int row) const {
+    return bytes == 8 ? ((const long long *)label)[row] : (long long)((const int *)label)[row];
+  }
+  __device__ __forceinline__ bool valid(int row) const {
+    const long long x = at(row);
+    return x != ignore && x >= 0 && x < classes;
+  }
+};
+
 // to[j, 0 .. ldt) = from[list[j], 0 .. d), zeros behind d; list == NULL: j itself.  j < count (count == NULL: n)
 template <class T>
 __global__ __launch_bounds__(DGNN_BLOCK) void k_ce_gather(int n, int d, int ldt, const int *__restrict__ list,
                                                           const int *__restrict__ count, const T *__restrict__ from,
-                                                          long long ldf, int wide, T *__restrict__ to) {
+                                                          long long ldf, int wide, T *__restrict__ to, const Labels labels,
+                                                          T *__restrict__ zero) {
   constexpr int VEC = 16 / sizeof(T);
+  // the rows of dx that have no label
+  if (zero != nullptr)
+    for (int r = blockIdx.x; r < n; r += gridDim.x)
+      if (!labels.valid(r))
+        for (int c = threadIdx.x; c < d; c += DGNN_BLOCK) zero[(long long)r * d + c] = (T)0.f;
   const int per = ldt / VEC, rows = count ? min(n, *count) : n;
   for (long long u = blockIdx.x * (long long)DGNN_BLOCK + threadIdx.x; u < (long long)rows * per; u += (long long)gridDim.x * DGNN_BLOCK) {
     const int j = (int)(u / per), c = (int)(u % per) * VEC;
@@ -207,11 +230,9 @@ __global__ __launch_bounds__(DGNN_BLOCK) void k_ce_gather(int n, int d, int ldt,
 struct CeArgs {
   const void *x, *w;              // rows [n, dk] (gathered: only those with a label), weight [classes, dk]
   int gathered;
-  const void *label;
+  Labels labels;
   const int *list, *count;        // labelled rows in order and how many (NULL: row r is row r, all n take part)
-  long long ignore;
   int n, classes, d, dk;          // dk = d rounded up to whole chunks
-  int label_bytes;
   float *part_m, *part_s;         // [class tiles, n]
   float *z_label;                 // [n], by gathered row
   float *lse, *loss;              // [n], by original row
@@ -227,10 +248,6 @@ struct CeArgs {
 
 __device__ __forceinline__ int rows_of(const CeArgs &a) { return a.count ? min(a.n, *a.count) : a.n; }
 __device__ __forceinline__ int row_at(const CeArgs &a, int r) { return a.list ? a.list[r] : r; }
-__device__ __forceinline__ long long label_at(const CeArgs &a, int row) {
-  return a.label_bytes == 8 ? ((const long long *)a.label)[row] : (long long)((const int *)a.label)[row];
-}
-
 // dz is kept in T as (softmax - onehot) g_i / unit and the products carry the factor unit, the largest |g|
 // (with the mean's division).  A common factor kept out of dz costs no rounding: rounded into it, one
 // g for all rows would put the same error, up to half a step of T, on every gradient.  float16 also has too
@@ -283,10 +300,10 @@ __global__ __launch_bounds__(C::THREADS, C::THREADS == 512 ? 2 : 1) void k_ce_fw
   using G = Gemm<T, C, true, true>;
   DGNN_RING(lds, G::BYTES);
   __shared__ float sm[C::WM][C::BN], ss[C::WM][C::BN], zl[C::BN];
-  const TileAt tile = tile_at(blockIdx.x, (a.classes + C::BM - 1) / C::BM, (a.n + C::BN - 1) / C::BN);
-  const int v0 = tile.m * C::BM, r0 = tile.n * C::BN;
   const int rows = rows_of(a);
-  if (r0 >= rows) return;
+  const TileAt tile = tile_at(blockIdx.x, (a.classes + C::BM - 1) / C::BM, (rows + C::BN - 1) / C::BN);
+  if (tile.n < 0) return;
+  const int v0 = tile.m * C::BM, r0 = tile.n * C::BN;
   acc16 acc[C::MB][C::NB];
   G::clear(acc);
   G::run({(const T *)a.w + (long long)v0 * a.dk, a.classes - v0, (unsigned)(a.dk * sizeof(T))},
@@ -297,7 +314,7 @@ __global__ __launch_bounds__(C::THREADS, C::THREADS == 512 ? 2 : 1) void k_ce_fw
 #pragma unroll
   for (int j = 0; j < C::NB; ++j) {
     const int col = n0 + 32 * j + (lane & 31), r = r0 + col;
-    const long long label = r < rows ? label_at(a, row_at(a, r)) : -1, want = label == a.ignore ? -1 : label - m0;
+    const long long label = r < rows ? a.labels.at(row_at(a, r)) : -1, want = label == a.labels.ignore ? -1 : label - m0;
     float top = -INFINITY;
     if (want >= 0 && want < C::BM / C::WM) {
 #pragma unroll
@@ -340,8 +357,7 @@ __global__ __launch_bounds__(C::THREADS, C::THREADS == 512 ? 2 : 1) void k_ce_fw
     for (int w = 0; w < C::WM; ++w) s += ss[w][threadIdx.x] * __builtin_amdgcn_exp2f((sm[w][threadIdx.x] - base) * DGNN_LOG2E);
     if (a.part_m == nullptr) {                  // one tile of classes: this is all there is
       const int row = r0 + threadIdx.x;
-      const long long label = label_at(a, row);
-      const bool on = label != a.ignore && label >= 0 && label < a.classes;
+      const bool on = a.labels.valid(row);
       const float lse = base + logf(s);
       a.lse[row] = on ? lse : 0.f;
       a.loss[row] = on ? lse - zl[threadIdx.x] : 0.f;
@@ -380,8 +396,7 @@ __global__ __launch_bounds__(DGNN_BLOCK) void k_ce_join(const CeArgs a, int tile
   for (int w = 0; w < 32; ++w) sum += ss[w][c] * expf(sm[w][c] - base);
   const float v = base + logf(sum);
   const int row = row_at(a, r);
-  const long long label = label_at(a, row);
-  const bool on = label != a.ignore && label >= 0 && label < a.classes;
+  const bool on = a.labels.valid(row);
   a.lse[row] = on ? v : 0.f;
   a.loss[row] = on ? v - a.z_label[r] : 0.f;
 }
@@ -393,10 +408,7 @@ __global__ __launch_bounds__(1024) void k_ce_reduce(const CeArgs a, int mean, co
   int c = 0;
   for (int i = threadIdx.x; i < a.n; i += 1024) {
     s += (double)loss[i];
-    if (mean && !a.count) {
-      const long long label = label_at(a, i);
-      c += label != a.ignore && label >= 0 && label < a.classes;
-    }
+    if (mean && !a.count) c += a.labels.valid(i);
   }
   for (int w = 32; w > 0; w >>= 1) s += __shfl_xor(s, w, 64), c += __shfl_xor(c, w, 64);
   if (lane_id() == 0) part[wave_in_block()] = s, counts[wave_in_block()] = c;
@@ -466,10 +478,10 @@ __global__ __launch_bounds__(C::THREADS, C::THREADS == 512 ? 2 : 1) void k_ce_dz
   using G = Gemm<T, C, true, true>;
   static_assert(32 * C::BM * sizeof(T) <= G::BYTES && C::WN <= 4, "the tile as rows fits the ring");
   DGNN_RING(lds, G::BYTES);
-  const TileAt tile = tile_at(blockIdx.x, a.ldz / C::BM, (a.n + C::BN - 1) / C::BN);
+  const int rows = rows_of(a);
+  const TileAt tile = tile_at(blockIdx.x, a.ldz / C::BM, (rows + C::BN - 1) / C::BN);
+  if (tile.n < 0) return;
   const int p0 = tile.m * C::BM, v0 = a.v0 + p0, r0 = tile.n * C::BN;
-  const int rows = min(a.n, *a.count);
-  if (r0 >= rows) return;
   acc16 acc[C::MB][C::NB];
   G::clear(acc);
   G::run({(const T *)a.w + (long long)v0 * a.dk, a.classes - v0, (unsigned)(a.dk * sizeof(T))},
@@ -481,7 +493,7 @@ __global__ __launch_bounds__(C::THREADS, C::THREADS == 512 ? 2 : 1) void k_ce_dz
 #pragma unroll
   for (int j = 0; j < C::NB; ++j) {
     const int r = r0 + n0 + 32 * j + (lane & 31), row = r < rows ? a.list[r] : a.list[0];
-    want[j] = (int)(label_at(a, row) - v0);
+    want[j] = (int)(a.labels.at(row) - v0);
     lse[j] = a.lse[row] * DGNN_LOG2E;
     g[j] = a.grad[a.grad_rows ? row : 0] * scale.by;
   }
@@ -517,12 +529,11 @@ template <class T, class C>
 __global__ __launch_bounds__(C::THREADS, C::THREADS == 512 ? 2 : 1) void k_ce_dx(const CeArgs a, int whole) {
   using G = Gemm<T, C, false, true>;
   DGNN_RING(lds, G::BYTES);
-  const int ms = (a.dk + C::BM - 1) / C::BM, ns = (a.n + C::BN - 1) / C::BN;
-  const int split = blockIdx.x / (ms * ns);
+  const int rows = rows_of(a), ms = (a.dk + C::BM - 1) / C::BM, ns = (rows + C::BN - 1) / C::BN;
+  const int split = ns > 0 ? blockIdx.x / (ms * ns) : a.splits;
+  if (split >= a.splits) return;
   const TileAt tile = tile_at(blockIdx.x % (ms * ns), ms, ns);
   const int c0 = tile.m * C::BM, r0 = tile.n * C::BN;
-  const int rows = min(a.n, *a.count);
-  if (r0 >= rows) return;
   const int lane = lane_id(), h = lane >> 5, wave = uniform_i32(wave_in_block());
   const int m0 = c0 + wave / C::WN * (C::BM / C::WM), n0 = wave % C::WN * (C::BN / C::WN);
   acc16 acc[C::MB][C::NB];
@@ -566,7 +577,7 @@ __global__ __launch_bounds__(C::THREADS, C::THREADS == 512 ? 2 : 1) void k_ce_dx
 // dx[list[r]] = sum over the splits, in order
 template <class T>
 __global__ __launch_bounds__(DGNN_BLOCK) void k_ce_dx_join(const CeArgs a) {
-  const int rows = min(a.n, *a.count), per = a.dk / 4;
+  const int rows = rows_of(a), per = a.dk / 4;
   const float unit = ce_scale<T>(a, rows).unit;
   for (long long u = blockIdx.x * (long long)DGNN_BLOCK + threadIdx.x; u < (long long)rows * per; u += (long long)gridDim.x * DGNN_BLOCK) {
     const int r = (int)(u / per), c = (int)(u % per) * 4;
@@ -582,16 +593,6 @@ __global__ __launch_bounds__(DGNN_BLOCK) void k_ce_dx_join(const CeArgs a) {
       if (c + j < a.d) to[j] = (T)f[j];
   }
 }
-// rows without a label: dx = 0
-template <class T>
-__global__ __launch_bounds__(DGNN_BLOCK) void k_ce_dx_zero(const CeArgs a, long long ignore) {
-  for (int r = blockIdx.x; r < a.n; r += gridDim.x) {
-    const long long x = label_at(a, r);
-    if (x != ignore && x >= 0 && x < a.classes) continue;
-    for (int c = threadIdx.x; c < a.d; c += DGNN_BLOCK) ((T *)a.dx)[(long long)r * a.d + c] = (T)0.f;
-  }
-}
-
 // dW of a piece: C^T[d, classes of the piece] = x^T dz.  splits > 1: partial sums over shares of the rows.
 template <class T, class C>
 __global__ __launch_bounds__(C::THREADS, C::THREADS == 512 ? 2 : 1) void k_ce_dw(const CeArgs a, int whole) {
@@ -601,7 +602,7 @@ __global__ __launch_bounds__(C::THREADS, C::THREADS == 512 ? 2 : 1) void k_ce_dw
   const int split = blockIdx.x / (ms * ns);
   const TileAt tile = tile_at(blockIdx.x % (ms * ns), ms, ns);
   const int c0 = tile.m * C::BM, p0 = tile.n * C::BN;
-  const int rows = min(a.n, *a.count);
+  const int rows = rows_of(a);
   acc16 acc[C::MB][C::NB];
   G::clear(acc);
   const int steps = (rows + C::BK - 1) / C::BK, per = (steps + a.splits - 1) / a.splits;
@@ -652,7 +653,7 @@ static inline unsigned grid_for(long long units) {
   return (unsigned)(b < 1 ? 1 : b > 8192 ? 8192 : b);
 }
 
-enum CeShape { CE_PLAIN, CE_WIDE, CE_THIN };
+enum CeShape { CE_PLAIN, CE_WIDE, CE_THIN, CE_NARROW };
 struct CePlan {
   int dk, tiles, copy_w, gather, all;                 // class tiles of the forward; all: no list of labelled rows
   CeShape z, dx_shape, dw_shape;
@@ -676,8 +677,9 @@ static CePlan ce_plan(int dtype, int n, int classes, int d, const void *x, const
   p.gather = p.dk != d || ((uintptr_t)x & 15) != 0 || (long long)n * p.dk * size >= 0x7fffffffLL;
   // up to about 1e9 operations finding the labelled rows (5 us) costs more than scoring all
   p.all = !p.gather && 2.0 * n * classes * d <= 1e9;
-  p.z = n <= 32 ? CE_THIN : ce_shape(dtype, classes, n, 1);
-  p.tiles = ceil_div(classes, p.z == CE_PLAIN ? 128 : 256);
+  p.z = classes <= 64 ? CE_NARROW : n <= 32 ? CE_THIN : ce_shape(dtype, classes, n, 1);
+  const int class_tile = p.z == CE_NARROW ? 64 : p.z == CE_PLAIN ? 128 : 256;
+  p.tiles = ceil_div(classes, class_tile);
   p.list = align256(sizeof(int) * ((size_t)n + 1));
   p.x = align256((size_t)n * p.dk * size);
   p.w = p.copy_w ? align256((size_t)classes * p.dk * size) : 0;
@@ -689,7 +691,7 @@ static CePlan ce_plan(int dtype, int n, int classes, int d, const void *x, const
   long long cols = (1LL << 27) / n;
   cols = cols < 1024 ? 1024 : cols > (1 << 20) ? 1 << 20 : cols;
   if (cols > classes) cols = classes;
-  p.piece = ceil_div(ceil_div(classes, ceil_div(classes, cols)), 256) * 256;
+  p.piece = ceil_div(ceil_div(classes, ceil_div(classes, cols)), class_tile) * class_tile;
   p.pieces = ceil_div(classes, p.piece);
   // enough workgroups for every compute unit: split the long axis while tiles are few
   auto splits = [](long long tiles, int steps) {
@@ -726,7 +728,7 @@ static int ce_check(int dtype, int label_bytes, int n, int classes, int d) {
 // labelled rows -> list, count; gathered x where asked; padded weight where its rows are not whole chunks
 template <class T>
 static int ce_prepare(const CePlan &p, int n, int classes, int d, bool all, bool gather, const void *x, const void *w, const void *label,
-                      int label_bytes, long long ignore, float *loss, float *lse, char *ws, CeArgs *a, hipStream_t st) {
+                      int label_bytes, long long ignore, float *loss, float *lse, void *dx, char *ws, CeArgs *a, hipStream_t st) {
   int *list = (int *)ws, *count = list + n;
   T *xc = (T *)(ws + p.list), *wc = (T *)(ws + p.list + (gather ? p.x : 0));
   if (!all) {
@@ -740,17 +742,17 @@ static int ce_prepare(const CePlan &p, int n, int classes, int d, bool all, bool
   if (gather) {
     hipLaunchKernelGGL(k_ce_gather<T>, dim3(grid_for((long long)n * per)), dim3(DGNN_BLOCK), 0, st, n, d, p.dk,
                        (const int *)list, (const int *)count, (const T *)x, (long long)d,
-                       (int)(p.dk == d && ((uintptr_t)x & 15) == 0), xc);
+                       (int)(p.dk == d && ((uintptr_t)x & 15) == 0), xc, Labels{label, label_bytes, classes, ignore}, (T *)dx);
     DGNN_LAUNCH_CHECK();
   }
   if (p.copy_w) {
     hipLaunchKernelGGL(k_ce_gather<T>, dim3(grid_for((long long)classes * per)), dim3(DGNN_BLOCK), 0, st, classes, d, p.dk,
-                       (const int *)nullptr, (const int *)nullptr, (const T *)w, (long long)d, 0, wc);
+                       (const int *)nullptr, (const int *)nullptr, (const T *)w, (long long)d, 0, wc, Labels{nullptr, 4, 0, 0}, (T *)nullptr);
     DGNN_LAUNCH_CHECK();
   }
   memset(a, 0, sizeof(*a));
   a->x = gather ? (const void *)xc : x, a->gathered = gather, a->w = p.copy_w ? (const void *)wc : w;
-  a->label = label, a->label_bytes = label_bytes, a->ignore = ignore;
+  a->labels = Labels{label, label_bytes, classes, ignore};
   if (!all) a->list = list, a->count = count;
   a->n = n, a->classes = classes, a->d = d, a->dk = p.dk;
   return DGNN_OK;
@@ -771,12 +773,14 @@ static int ce_forward(const CePlan &p, int n, int classes, int d, const void *x,
   CeArgs a;
   char *at = ws + p.list + (p.gather ? p.x : 0) + p.w;
   float *row = reduction == 0 ? loss : (float *)(at + 2 * p.part + p.zl);
-  const int rc = ce_prepare<T>(p, n, classes, d, p.all != 0, p.gather != 0, x, w, label, label_bytes, ignore, row, lse, ws, &a, st);
+  const int rc = ce_prepare<T>(p, n, classes, d, p.all != 0, p.gather != 0, x, w, label, label_bytes, ignore, row, lse, nullptr, ws, &a, st);
   if (rc != DGNN_OK) return rc;
   a.lse = lse, a.loss = row;
   if (!p.all || p.tiles > 1) a.part_m = (float *)at, a.part_s = (float *)(at + p.part), a.z_label = (float *)(at + 2 * p.part);
   if (p.z == CE_THIN) {
     DGNN_CE_LAUNCH(k_ce_fwd, Thin<T>, classes, n, 1, a);
+  } else if (p.z == CE_NARROW) {
+    DGNN_CE_LAUNCH(k_ce_fwd, Narrow<T>, classes, n, 1, a);
   } else if (p.z == CE_PLAIN) {
     DGNN_CE_LAUNCH(k_ce_fwd, Plain<T>, classes, n, 1, a);
   } else if constexpr (sizeof(T) == 2) {
@@ -798,7 +802,7 @@ static int ce_backward(const CePlan &p, int n, int classes, int d, const void *x
                        int label_bytes, long long ignore, int reduction, const float *lse, const float *grad, void *dx,
                        void *dw, char *ws, hipStream_t st) {
   CeArgs a;
-  const int rc = ce_prepare<T>(p, n, classes, d, false, true, x, w, label, label_bytes, ignore, nullptr, nullptr, ws, &a, st);
+  const int rc = ce_prepare<T>(p, n, classes, d, false, true, x, w, label, label_bytes, ignore, nullptr, nullptr, dx, ws, &a, st);
   if (rc != DGNN_OK) return rc;
   char *at = ws + p.list + p.x + p.w;
   a.dz = at, a.ldz = p.piece;
@@ -813,14 +817,12 @@ static int ce_backward(const CePlan &p, int n, int classes, int d, const void *x
   }
   a.direct = p.dx_splits == 1 && p.pieces == 1;
   const int whole_x = p.dk == d && ((uintptr_t)dx & 15) == 0, whole_w = p.dk == d && ((uintptr_t)dw & 15) == 0;
-  if (dx) {
-    hipLaunchKernelGGL(k_ce_dx_zero<T>, dim3(n < 4096 ? n : 4096), dim3(DGNN_BLOCK), 0, st, a, ignore);
-    DGNN_LAUNCH_CHECK();
-  }
   for (int v0 = 0; v0 < classes; v0 += p.piece) {
     a.v0 = v0, a.vn = classes - v0 < p.piece ? classes - v0 : p.piece, a.first = v0 == 0;
     if (p.z == CE_THIN) {
       DGNN_CE_LAUNCH(k_ce_dz, Thin<T>, p.piece, n, 1, a);
+    } else if (p.z == CE_NARROW) {
+      DGNN_CE_LAUNCH(k_ce_dz, Narrow<T>, p.piece, n, 1, a);
     } else if (p.z == CE_PLAIN) {
       DGNN_CE_LAUNCH(k_ce_dz, Plain<T>, p.piece, n, 1, a);
     } else if constexpr (sizeof(T) == 2) {
