@@ -83,9 +83,9 @@ SIGNATURES = {
     "dgnn_embedding_backward_workspace_bytes": (_sz, [_i, _i, _i]),
     "dgnn_embedding_backward": (_i, [_i] * 5 + [_f] + [_vp] * 3 + [_vp, _sz, _vp]),
     "dgnn_attn_forward_workspace_bytes": (_sz, [_i] * 6),
-    "dgnn_attn_forward": (_i, [_i] * 8 + [_f] + [_vp] * 8 + [_vp, _sz, _vp]),
+    "dgnn_attn_forward": (_i, [_i] * 8 + [_f] + [_vp] * 9 + [_vp, _sz, _vp]),
     "dgnn_attn_backward_workspace_bytes": (_sz, [_i] * 6),
-    "dgnn_attn_backward": (_i, [_i] * 8 + [_f] + [_vp] * 12 + [_vp, _sz, _vp]),
+    "dgnn_attn_backward": (_i, [_i] * 8 + [_f] + [_vp] * 13 + [_vp, _sz, _vp]),
     "dgnn_linear_ce_workspace_bytes": (_sz, [_i] * 5),
     "dgnn_linear_ce_forward": (_i, [_i] * 5 + [_ll, _i] + [_vp] * 5 + [_vp, _sz, _vp]),
     "dgnn_linear_ce_backward": (_i, [_i] * 5 + [_ll, _i] + [_vp] * 7 + [_vp, _sz, _vp]),

@@ -145,7 +145,8 @@ struct AttnTile {
     if (!valid) return;
     const int h = lane_id() >> 5;
     const bool none = limit < 0 || lk == 0;
-    store_row<T, DP>((T *)a.o + (tok * a.hq + head) * a.d, acc, none ? 0.f : 1.f / l, a.d, h);
+    const long long to = (tok * a.hq + head) * a.d;
+    store_row<T, DP>((T *)a.o + to, acc, none ? 0.f : 1.f / l, a.d, h, a.rest != nullptr ? (T *)a.rest + to : nullptr);
     if (a.lse != nullptr && h == 0)
       a.lse[(long long)head * a.tq + tok] = none ? -INFINITY : (m * c + __builtin_amdgcn_logf(l)) * DGNN_LN2;
   }
@@ -232,7 +233,9 @@ __global__ __launch_bounds__(DGNN_BLOCK) void k_attn_join(const AttnArgs a) {
     float x = 0.f;
 #pragma unroll 4
     for (int j = 0; j < chunks; ++j) x = fmaf(part[j * stride + 4 + c], exp2_fast(part[j * stride] - base), x);
-    out[c] = (T)(seen > 0 ? x / sum : 0.f);
+    x = seen > 0 ? x / sum : 0.f;
+    out[c] = (T)x;
+    if (a.rest != nullptr) ((T *)a.rest)[r * a.d + c] = (T)(x - (float)(T)x);
   }
   if (lse && lane == 0) *lse = seen > 0 ? (base + __builtin_amdgcn_logf(sum)) * DGNN_LN2 : -INFINITY;
 }
@@ -334,17 +337,18 @@ size_t dgnn_attn_forward_workspace_bytes(int nseq, int tq, int tk, int hq, int h
 
 int dgnn_attn_forward(int dtype, int nseq, int tq, int tk, int hq, int hk, int d, int causal, float scale,
                       const void *q, const void *k, const void *v, const long long *strides, const int *row_ptr,
-                      const int *col_ptr, void *out, float *lse, void *workspace, size_t workspace_bytes, void *stream) {
+                      const int *col_ptr, void *out, void *out_rest, float *lse, void *workspace, size_t workspace_bytes, void *stream) {
   AttnArgs a;
   const int rc = attn_args(dtype, nseq, tq, tk, hq, hk, d, causal, scale, q, k, v, row_ptr, col_ptr, strides, &a);
   if (rc != DGNN_OK) return rc;
   if (tq == 0) return DGNN_OK;
   if (!out) return DGNN_ERR_BAD_ARG;
-  if (((uintptr_t)out & 15) || ((uintptr_t)lse & 3)) return DGNN_ERR_ALIGNMENT;
+  if (((uintptr_t)out & 15) || ((uintptr_t)out_rest & 15) || ((uintptr_t)lse & 3)) return DGNN_ERR_ALIGNMENT;
   const AttnPlan p = attn_plan(nseq, tq, tk, hq, hk, d);
   if (p.bytes > 0 && (!workspace || workspace_bytes < p.bytes)) return DGNN_ERR_WORKSPACE;
   if (p.bytes > 0 && ((uintptr_t)workspace & 15)) return DGNN_ERR_ALIGNMENT;
   a.o = out;
+  a.rest = out_rest;
   a.lse = lse;
   a.part = (float *)workspace, a.few = p.few, a.chunk = p.chunk;
   hipStream_t st = (hipStream_t)stream;

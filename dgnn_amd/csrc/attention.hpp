@@ -9,6 +9,7 @@ namespace dgnn {
 struct AttnArgs {
   const void *q, *k, *v, *out, *grad;         // grad: of the output
   void *o, *dq, *dk, *dv;
+  void *rest;                                 // [tq, hq, d], what rounding took from the output (may be NULL)
   float *lse;                                 // [hq, tq], natural logarithm
   float *stat;                                // backward: [hq, tq] pairs {lse log2(e) (+inf for an empty row), <grad, out>}
   float *part;                                // partial rows (split forward) or gradients (split backward)
@@ -131,9 +132,10 @@ __device__ __forceinline__ void load_row_frags(frag8<T> (&f)[DP / 16], const T *
     }
   }
 }
-// The transposed result blocks of a lane's row, times `by`, to global memory (d is a multiple of four).
+// The transposed result blocks of a lane's row, times `by`, to global memory (d is a multiple of four); what
+// the rounding to T took, rounded itself, to `rest`.
 template <class T, int DP>
-__device__ __forceinline__ void store_row(T *row, const acc16 (&c)[DP / 32], float by, int d, int h) {
+__device__ __forceinline__ void store_row(T *row, const acc16 (&c)[DP / 32], float by, int d, int h, T *rest = nullptr) {
 #pragma unroll
   for (int b = 0; b < DP / 32; ++b)
 #pragma unroll
@@ -143,6 +145,12 @@ __device__ __forceinline__ void store_row(T *row, const acc16 (&c)[DP / 32], flo
 #pragma unroll
       for (int j = 0; j < 4; ++j) v[j] = (T)(c[b][4 * i + j] * by);
       if (at < d) *(vec4<T> *)(row + at) = v;
+      if (rest != nullptr && at < d) {
+        vec4<T> lo;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) lo[j] = (T)(c[b][4 * i + j] * by - (float)v[j]);
+        *(vec4<T> *)(rest + at) = lo;
+      }
     }
 }
 

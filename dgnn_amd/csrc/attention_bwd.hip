@@ -14,11 +14,13 @@ using namespace dgnn;
 
 namespace dgnn {
 
-// stat[head][row] = {lse log2(e), <do, o>}; the first is +inf where the row saw no key (p = exp2(z - inf) = 0).
+// stat[head][row] = {lse log2(e), <do, o>}, o with what its rounding took (`rest`): <do, v_j> - <do, o> cancels
+// in rows that see few keys, and half a step of a 16-bit o is all that was left of it; the first is +inf where the row saw no key (p = exp2(z - inf) = 0).
 // One thread per 16-byte chunk, lanes of a row joined by shuffles.
 template <class T, int LPR>
 __global__ __launch_bounds__(DGNN_BLOCK) void k_attn_bwd_stat(long long rows, int d, int tq, int hq,
-                                                              const T *__restrict__ out, const T *__restrict__ grad,
+                                                              const T *__restrict__ out, const T *__restrict__ rest,
+                                                              const T *__restrict__ grad,
                                                               const float *__restrict__ lse, float2 *__restrict__ stat) {
   constexpr int VEC = 16 / sizeof(T);
   const long long r = (blockIdx.x * (long long)DGNN_BLOCK + threadIdx.x) / LPR;
@@ -30,6 +32,11 @@ __global__ __launch_bounds__(DGNN_BLOCK) void k_attn_bwd_stat(long long rows, in
     *(u32x4 *)g = *(const u32x4 *)(grad + r * d + c);
 #pragma unroll
     for (int j = 0; j < VEC; ++j) sum = fmaf((float)o[j], (float)g[j], sum);
+    if (rest != nullptr) {
+      *(u32x4 *)o = *(const u32x4 *)(rest + r * d + c);
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) sum = fmaf((float)o[j], (float)g[j], sum);
+    }
   }
 #pragma unroll
   for (int w = LPR / 2; w > 0; w >>= 1) sum += __shfl_xor(sum, w, 64);
@@ -328,7 +335,7 @@ static int launch_bwd(const AttnArgs &a, const float *lse, hipStream_t st) {
     const long long blocks = (rows * LPR + DGNN_BLOCK - 1) / DGNN_BLOCK;
     if (blocks > 0x7fffffffLL) return DGNN_ERR_UNSUPPORTED;
     hipLaunchKernelGGL((k_attn_bwd_stat<T, LPR>), dim3((unsigned)blocks), dim3(DGNN_BLOCK), 0, st, rows, a.d, a.tq, a.hq,
-                       (const T *)a.out, (const T *)a.grad, lse, (float2 *)a.stat);
+                       (const T *)a.out, (const T *)a.rest, (const T *)a.grad, lse, (float2 *)a.stat);
     DGNN_LAUNCH_CHECK();
   }
   if (a.tk > 0) switch (a.splits > 1 ? ROWS_LONG : rows_kind(a.tk, a.nseq, 1, a.hk)) {
@@ -363,19 +370,19 @@ size_t dgnn_attn_backward_workspace_bytes(int nseq, int tq, int tk, int hq, int 
 
 int dgnn_attn_backward(int dtype, int nseq, int tq, int tk, int hq, int hk, int d, int causal, float scale,
                        const void *q, const void *k, const void *v, const long long *strides, const int *row_ptr,
-                       const int *col_ptr, const void *out, const float *lse, const void *grad, void *dq, void *dk,
+                       const int *col_ptr, const void *out, const void *out_rest, const float *lse, const void *grad, void *dq, void *dk,
                        void *dv, void *workspace, size_t workspace_bytes, void *stream) {
   AttnArgs a;
   const int rc = attn_args(dtype, nseq, tq, tk, hq, hk, d, causal, scale, q, k, v, row_ptr, col_ptr, strides, &a);
   if (rc != DGNN_OK) return rc;
   if (tq > 0 && (!out || !lse || !grad || !dq)) return DGNN_ERR_BAD_ARG;
   if (tk > 0 && (!dk || !dv)) return DGNN_ERR_BAD_ARG;
-  for (const void *p : {out, grad, (const void *)dq, (const void *)dk, (const void *)dv})
+  for (const void *p : {out, out_rest, grad, (const void *)dq, (const void *)dk, (const void *)dv})
     if ((uintptr_t)p & 15) return DGNN_ERR_ALIGNMENT;
   if (workspace_bytes < dgnn_attn_backward_workspace_bytes(nseq, tq, tk, hq, hk, d) || (tq > 0 && !workspace)) return DGNN_ERR_WORKSPACE;
   if (((uintptr_t)workspace & 15) || ((uintptr_t)lse & 3)) return DGNN_ERR_ALIGNMENT;
   if ((long long)hq * d * (dtype == DGNN_F32 ? 4 : 2) >= (1LL << 31) / 128) return DGNN_ERR_UNSUPPORTED;
-  a.out = out, a.grad = grad, a.dq = dq, a.dk = dk, a.dv = dv;
+  a.out = out, a.rest = (void *)out_rest, a.grad = grad, a.dq = dq, a.dk = dk, a.dv = dv;
   a.stat = (float *)workspace;
   a.splits = bwd_splits(nseq, tq, tk, hq, hk);
   a.part = (float *)((char *)workspace + align256(2 * sizeof(float) * (size_t)tq * (size_t)hq));

@@ -510,21 +510,27 @@ __global__ __launch_bounds__(C::THREADS, C::THREADS == 512 ? 2 : 1) void k_ce_dz
       });
 }
 
-// A lane's columns of C^T as rows of partial sums: row r at acc + r * ld, columns m0 .. < d.
+// A lane's columns of C^T as a row of partial sums, columns m0 .. < d; add: to what an earlier piece left there.
 template <class C>
-__device__ __forceinline__ void store_sums(float *to, const acc16 (&acc)[C::MB][C::NB], int j, int m0, int d, int h) {
+__device__ __forceinline__ void store_sums(float *to, const acc16 (&acc)[C::MB][C::NB], int j, int m0, int d, int h, bool add) {
 #pragma unroll
   for (int i = 0; i < C::MB; ++i)
 #pragma unroll
     for (int e4 = 0; e4 < 4; ++e4) {
       const int at = m0 + 32 * i + 8 * e4 + 4 * h;
       const acc16 &c = acc[i][j];
-      if (at < d) *(float4 *)(to + at) = make_float4(c[4 * e4], c[4 * e4 + 1], c[4 * e4 + 2], c[4 * e4 + 3]);
+      if (at >= d) continue;
+      float4 v = make_float4(c[4 * e4], c[4 * e4 + 1], c[4 * e4 + 2], c[4 * e4 + 3]);
+      if (add) {
+        const float4 old = *(const float4 *)(to + at);
+        v.x += old.x, v.y += old.y, v.z += old.z, v.w += old.w;
+      }
+      *(float4 *)(to + at) = v;
     }
 }
 
 // dx of a piece: C^T[d, rows] += W_piece^T dz^T.  One split of a single piece: straight to dx; else into
-// acc[split], continued over the pieces, joined by k_ce_dx_join.
+// acc[split], added to over the pieces, joined by k_ce_dx_join.
 template <class T, class C>
 __global__ __launch_bounds__(C::THREADS, C::THREADS == 512 ? 2 : 1) void k_ce_dx(const CeArgs a, int whole) {
   using G = Gemm<T, C, false, true>;
@@ -538,23 +544,6 @@ __global__ __launch_bounds__(C::THREADS, C::THREADS == 512 ? 2 : 1) void k_ce_dx
   const int m0 = c0 + wave / C::WN * (C::BM / C::WM), n0 = wave % C::WN * (C::BN / C::WN);
   acc16 acc[C::MB][C::NB];
   G::clear(acc);
-  if (!a.first) {
-#pragma unroll
-    for (int j = 0; j < C::NB; ++j) {
-      const int r = r0 + n0 + 32 * j + (lane & 31);
-      const float *old = a.acc + ((long long)split * a.n + r) * a.dk;
-#pragma unroll
-      for (int i = 0; i < C::MB; ++i)
-#pragma unroll
-        for (int e4 = 0; e4 < 4; ++e4) {
-          const int c = m0 + 32 * i + 8 * e4 + 4 * h;
-          if (r < rows && c < a.dk) {
-            const float4 v = *(const float4 *)(old + c);
-            acc[i][j][4 * e4] = v.x, acc[i][j][4 * e4 + 1] = v.y, acc[i][j][4 * e4 + 2] = v.z, acc[i][j][4 * e4 + 3] = v.w;
-          }
-        }
-    }
-  }
   const int steps = (a.vn + C::BK - 1) / C::BK, per = (steps + a.splits - 1) / a.splits;
   const int ka = min(a.vn, split * per * C::BK), kb = min(a.vn, (split + 1) * per * C::BK);
   G::run({(const T *)a.w + (long long)(a.v0 + ka) * a.dk + c0, a.dk - c0, (unsigned)(a.dk * sizeof(T))},
@@ -571,7 +560,7 @@ __global__ __launch_bounds__(C::THREADS, C::THREADS == 512 ? 2 : 1) void k_ce_dx
 #pragma unroll
   for (int j = 0; j < C::NB; ++j) {
     const int r = r0 + n0 + 32 * j + (lane & 31);
-    if (r < rows) store_sums<C>(a.acc + ((long long)split * a.n + r) * a.dk, acc, j, m0, a.dk, h);
+    if (r < rows) store_sums<C>(a.acc + ((long long)split * a.n + r) * a.dk, acc, j, m0, a.dk, h, !a.first);
   }
 }
 // dx[list[r]] = sum over the splits, in order
@@ -623,7 +612,7 @@ __global__ __launch_bounds__(C::THREADS, C::THREADS == 512 ? 2 : 1) void k_ce_dw
 #pragma unroll
   for (int j = 0; j < C::NB; ++j) {
     const int p = p0 + n0 + 32 * j + (lane & 31);
-    if (p < a.vn) store_sums<C>(a.acc + ((long long)split * a.ldz + p) * a.dk, acc, j, m0, a.dk, h);
+    if (p < a.vn) store_sums<C>(a.acc + ((long long)split * a.ldz + p) * a.dk, acc, j, m0, a.dk, h, false);
   }
 }
 template <class T>
@@ -694,8 +683,10 @@ static CePlan ce_plan(int dtype, int n, int classes, int d, const void *x, const
   p.piece = ceil_div(ceil_div(classes, ceil_div(classes, cols)), class_tile) * class_tile;
   p.pieces = ceil_div(classes, p.piece);
   // enough workgroups for every compute unit: split the long axis while tiles are few
-  auto splits = [](long long tiles, int steps) {
+  // float: a sum of 10^5 terms in one accumulator has lost three of its seven digits, so none is longer than 4096
+  auto splits = [&](long long tiles, int steps) {
     long long s = tiles > 0 ? 512 / tiles : 1;
+    if (dtype == DGNN_F32 && s < (steps + 63) / 64) s = (steps + 63) / 64;
     if (s > steps / 4) s = steps / 4;
     return (int)(s < 1 ? 1 : s > 64 ? 64 : s);
   };

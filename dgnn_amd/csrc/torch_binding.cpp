@@ -1060,41 +1060,45 @@ AttnCall attn_call(const Tensor &q, const Tensor &k, const Tensor &v, const Tens
 }
 Tensor cut(const Tensor &t, int64_t d) { return t.size(2) == d ? t : t.narrow(2, 0, d).contiguous(); }
 
-// -> (out [rows, heads, dim], lse [heads, rows])
-std::tuple<Tensor, Tensor> attention_forward(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &row_ptr,
-                                             const Tensor &col_ptr, double scale, bool causal) {
+// -> (out [rows, heads, dim], lse [heads, rows], out_rest like out or None)
+std::tuple<Tensor, Tensor, py::object> attention_forward(const Tensor &q, const Tensor &k, const Tensor &v,
+                                                         const Tensor &row_ptr, const Tensor &col_ptr, double scale,
+                                                         bool causal, bool rest) {
   c10::DeviceGuard guard(q.device());
   const AttnCall c = attn_call(q, k, v, row_ptr, col_ptr);
   Tensor out = at::empty({c.tq, c.hq, c.width}, q.options()), lse = new_f32({c.hq, c.tq}, q);
+  Tensor low = rest && c.dtype != DGNN_F32 ? at::empty_like(out) : Tensor();
   const size_t nb = API(dgnn_attn_forward_workspace_bytes)(c.nseq, c.tq, c.tk, c.hq, c.hk, c.d);
   Tensor ws = workspace(nb, q);
   check_rc(API(dgnn_attn_forward)(c.dtype, c.nseq, c.tq, c.tk, c.hq, c.hk, c.d, causal, (float)scale, cv(c.q), cv(c.k),
-                                  cv(c.v), c.strides, ip(row_ptr), ip(col_ptr), vo(out), fo(lse), vo(ws), nb, stream_of(q)),
+                                  cv(c.v), c.strides, ip(row_ptr), ip(col_ptr), vo(out), vo(low), fo(lse), vo(ws), nb,
+                                  stream_of(q)),
            "dgnn_attn_forward");
-  return std::make_tuple(cut(out, q.size(2)), lse);
+  return std::make_tuple(cut(out, q.size(2)), lse, low.defined() ? py::cast(cut(low, q.size(2))) : py::object(py::none()));
 }
 
 // -> (dq, dk, dv)
 std::tuple<Tensor, Tensor, Tensor> attention_backward(const Tensor &q, const Tensor &k, const Tensor &v,
                                                       const Tensor &row_ptr, const Tensor &col_ptr, double scale,
                                                       bool causal, const Tensor &out, const Tensor &lse,
-                                                      const Tensor &grad) {
+                                                      const Tensor &grad, const OptTensor &out_rest) {
   c10::DeviceGuard guard(q.device());
   const AttnCall c = attn_call(q, k, v, row_ptr, col_ptr);
   like(out, q, "out", "q"), like(grad, q, "grad", "q"), f32(lse, "lse", 2);
   if (out.sizes() != q.sizes() || grad.sizes() != q.sizes()) fail("out and grad must have q's shape ", q.sizes());
+  if (given(out_rest) && (like(*out_rest, q, "out_rest", "q").sizes() != q.sizes())) fail("out_rest must have q's shape ", q.sizes());
   if (lse.size(0) != c.hq || lse.size(1) != c.tq || lse.device() != q.device()) fail("lse must be the forward's [heads, rows]");
   const int64_t d = q.size(2);
   auto dense = [&](const Tensor &t) {
     return d == c.width && t.is_contiguous() && (uintptr_t)t.data_ptr() % 16 == 0 ? t : padded(t, c.width);
   };
-  const Tensor o = dense(out), g = dense(grad);
+  const Tensor o = dense(out), g = dense(grad), low = given(out_rest) ? dense(*out_rest) : Tensor();
   Tensor dq = at::empty({c.tq, c.hq, c.width}, q.options()), dk = at::empty({c.tk, c.hk, c.width}, q.options()),
          dv = at::empty({c.tk, c.hk, c.width}, q.options());
   const size_t nb = API(dgnn_attn_backward_workspace_bytes)(c.nseq, c.tq, c.tk, c.hq, c.hk, c.d);
   Tensor ws = workspace(nb, q);
   check_rc(API(dgnn_attn_backward)(c.dtype, c.nseq, c.tq, c.tk, c.hq, c.hk, c.d, causal, (float)scale, cv(c.q), cv(c.k),
-                                   cv(c.v), c.strides, ip(row_ptr), ip(col_ptr), cv(o), fp(lse), cv(g), vo(dq), vo(dk),
+                                   cv(c.v), c.strides, ip(row_ptr), ip(col_ptr), cv(o), cv(low), fp(lse), cv(g), vo(dq), vo(dk),
                                    vo(dv), vo(ws), nb, stream_of(q)),
            "dgnn_attn_backward");
   return std::make_tuple(cut(dq, d), cut(dk, d), cut(dv, d));
@@ -1418,12 +1422,12 @@ PYBIND11_MODULE(fused_attention, m) {
   py::options options;
   options.disable_function_signatures();
   init(m, "Packed attention: every row to every key of its own sequence (no reference module).");
-  def(m, "attention_forward", &attention_forward, "q, k, v, row_ptr, col_ptr, scale, causal",
-      "-> (out [rows, heads, dim], lse [heads, rows])", arg("q"), arg("k"), arg("v"), arg("row_ptr"), arg("col_ptr"),
-      arg("scale"), arg("causal"));
-  def(m, "attention_backward", &attention_backward, "q, k, v, row_ptr, col_ptr, scale, causal, out, lse, grad",
+  def(m, "attention_forward", &attention_forward, "q, k, v, row_ptr, col_ptr, scale, causal, rest=False",
+      "-> (out [rows, heads, dim], lse [heads, rows], what rounding took from out with rest=True, else None)", arg("q"), arg("k"), arg("v"), arg("row_ptr"), arg("col_ptr"),
+      arg("scale"), arg("causal"), arg("rest") = false);
+  def(m, "attention_backward", &attention_backward, "q, k, v, row_ptr, col_ptr, scale, causal, out, lse, grad, out_rest=None",
       "-> (dq, dk, dv), deterministic", arg("q"), arg("k"), arg("v"), arg("row_ptr"), arg("col_ptr"), arg("scale"),
-      arg("causal"), arg("out"), arg("lse"), arg("grad"));
+      arg("causal"), arg("out"), arg("lse"), arg("grad"), arg("out_rest") = py::none());
 }
 
 PYBIND11_MODULE(fused_cross_entropy, m) {

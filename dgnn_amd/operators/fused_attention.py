@@ -32,15 +32,16 @@ def PackedAttentionFuse(q, k, v, row_ptr, col_ptr=None, causal=False, scale=None
 class PackedAttentionFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, row_ptr, col_ptr, causal, scale):
-        out, lse = fused_attention.attention_forward(q, k, v, row_ptr, col_ptr, scale, causal)
-        ctx.save_for_backward(q, k, v, row_ptr, col_ptr, out, lse)
+        # rest: what rounding took from a 16-bit out (None for float32); the backward's <grad, out> needs it
+        out, lse, rest = fused_attention.attention_forward(q, k, v, row_ptr, col_ptr, scale, causal, rest=True)
+        ctx.save_for_backward(q, k, v, row_ptr, col_ptr, out, lse, rest)
         ctx.causal, ctx.scale = causal, scale
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad_out):
-        q, k, v, row_ptr, col_ptr, out, lse = ctx.saved_tensors
+        q, k, v, row_ptr, col_ptr, out, lse, rest = ctx.saved_tensors
         dq, dk, dv = fused_attention.attention_backward(q, k, v, row_ptr, col_ptr, ctx.scale, ctx.causal, out, lse,
-                                                        grad_out)
+                                                        grad_out, out_rest=rest)
         return dq, dk, dv, None, None, None, None

@@ -509,6 +509,8 @@ int dgnn_embedding_backward(int dtype, int idx_bytes, int n, int rows, int dim, 
  * col_ptr[s+1] - 1 (int32 device arrays of nseq + 1 ascending offsets; pass the same array twice for self
  * attention).  causal: query i of a sequence sees its keys j <= i + keys - queries, else all of them.
  *   out [tq,hq,d] = softmax(scale q k^T) v;  lse [hq,tq] natural logarithm of the softmax's sum (may be NULL)
+ *   out_rest [tq,hq,d] what rounding took from out, in the same type (may be NULL; kept for the backward, whose
+ *   <grad, out> needs more digits of a 16-bit out than out has)
  * A row that sees no key -- masked, an empty sequence, a row in front of the first or behind the
  * last sequence -- gives out = 0, lse = -inf and has no gradient; rows no sequence holds are never read.
  * strides: HOST array {q_token, q_head, k_token, k_head, v_token, v_head} in elements, the last
@@ -517,14 +519,15 @@ int dgnn_embedding_backward(int dtype, int idx_bytes, int n, int rows, int dim, 
 size_t dgnn_attn_forward_workspace_bytes(int nseq, int tq, int tk, int hq, int hk, int d);
 int dgnn_attn_forward(int dtype, int nseq, int tq, int tk, int hq, int hk, int d, int causal, float scale,
                       const void *q, const void *k, const void *v, const long long *strides, const int *row_ptr,
-                      const int *col_ptr, void *out, float *lse, void *workspace, size_t workspace_bytes, void *stream);
-/* dq [tq,hq,d], dk and dv [tk,hk,d] from grad [tq,hq,d] and the forward's out and lse; fully written.
+                      const int *col_ptr, void *out, void *out_rest, float *lse, void *workspace, size_t workspace_bytes,
+                      void *stream);
+/* dq [tq,hq,d], dk and dv [tk,hk,d] from grad [tq,hq,d] and the forward's out, out_rest (or NULL) and lse; fully written.
  * No atomics: the same bits every time. */
 size_t dgnn_attn_backward_workspace_bytes(int nseq, int tq, int tk, int hq, int hk, int d);
 int dgnn_attn_backward(int dtype, int nseq, int tq, int tk, int hq, int hk, int d, int causal, float scale,
                        const void *q, const void *k, const void *v, const long long *strides, const int *row_ptr,
-                       const int *col_ptr, const void *out, const float *lse, const void *grad, void *dq, void *dk,
-                       void *dv, void *workspace, size_t workspace_bytes, void *stream);
+                       const int *col_ptr, const void *out, const void *out_rest, const float *lse, const void *grad, void *dq,
+                       void *dk, void *dv, void *workspace, size_t workspace_bytes, void *stream);
 
 /* Softmax cross entropy of a linear layer, z = x w^T, without the logits.  x [n,d], w [classes,d]
  * contiguous; label int32 (label_bytes 4) or int64 (8).  A row whose label is ignore_index or outside

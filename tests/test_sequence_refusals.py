@@ -14,10 +14,10 @@ P = 0x10000                      # an aligned address that is never read
 
 
 def attn(dtype=1, nseq=1, tq=8, tk=8, hq=4, hk=2, d=64, q=P, k=P, v=P, strides=None, row_ptr=P, col_ptr=P, out=P,
-         lse=P, ws=P, wsb=1 << 30, null_strides=False):
+         lse=P, rest=None, ws=P, wsb=1 << 30, null_strides=False):
     size = (hq * d, d, hk * d, d, hk * d, d) if strides is None else strides
     arr = None if null_strides else (ctypes.c_longlong * 6)(*size)
-    return _lib.lib().dgnn_attn_forward(dtype, nseq, tq, tk, hq, hk, d, 0, 1.0, q, k, v, arr, row_ptr, col_ptr, out, lse, ws, wsb,
+    return _lib.lib().dgnn_attn_forward(dtype, nseq, tq, tk, hq, hk, d, 0, 1.0, q, k, v, arr, row_ptr, col_ptr, out, rest, lse, ws, wsb,
                                         None)
 
 
@@ -34,7 +34,7 @@ def attn(dtype=1, nseq=1, tq=8, tk=8, hq=4, hk=2, d=64, q=P, k=P, v=P, strides=N
     (dict(strides=(256, 64, 0, 64, 128, 64)), UNSUPPORTED),               # expanded keys
     (dict(strides=(1 << 23, 64, 128, 64, 128, 64)), UNSUPPORTED),
     (dict(q=P + 8), ALIGNMENT), (dict(v=P + 2), ALIGNMENT), (dict(out=P + 4), ALIGNMENT), (dict(row_ptr=P + 2), ALIGNMENT),
-    (dict(lse=P + 1), ALIGNMENT),
+    (dict(lse=P + 1), ALIGNMENT), (dict(rest=P + 8), ALIGNMENT),
     (dict(tk=4096, tq=2, ws=None), WORKSPACE), (dict(tk=4096, tq=2, wsb=4096), WORKSPACE),
     (dict(tk=4096, tq=2, ws=P + 4), ALIGNMENT),                           # single queries: split over the keys
 ])
@@ -42,16 +42,16 @@ def test_attention_forward_refuses(change, code):
     assert attn(**change) == code
 
 
-def attn_bwd(dtype=1, tq=8, tk=8, hq=4, hk=2, d=64, out=P, lse=P, grad=P, dq=P, dk=P, dv=P, ws=P, wsb=1 << 20):
+def attn_bwd(dtype=1, tq=8, tk=8, hq=4, hk=2, d=64, out=P, lse=P, grad=P, dq=P, dk=P, dv=P, rest=None, ws=P, wsb=1 << 20):
     arr = (ctypes.c_longlong * 6)(hq * d, d, hk * d, d, hk * d, d)
-    return _lib.lib().dgnn_attn_backward(dtype, 1, tq, tk, hq, hk, d, 0, 1.0, P, P, P, arr, P, P, out, lse, grad, dq, dk,
+    return _lib.lib().dgnn_attn_backward(dtype, 1, tq, tk, hq, hk, d, 0, 1.0, P, P, P, arr, P, P, out, rest, lse, grad, dq, dk,
                                          dv, ws, wsb, None)
 
 
 @pytest.mark.parametrize("change,code", [
     (dict(out=None), BAD_ARG), (dict(lse=None), BAD_ARG), (dict(grad=None), BAD_ARG), (dict(dq=None), BAD_ARG),
     (dict(dk=None), BAD_ARG), (dict(dv=None), BAD_ARG), (dict(ws=None), WORKSPACE), (dict(wsb=255), WORKSPACE),
-    (dict(grad=P + 8), ALIGNMENT), (dict(dk=P + 8), ALIGNMENT), (dict(ws=P + 2), ALIGNMENT), (dict(lse=P + 2), ALIGNMENT),
+    (dict(grad=P + 8), ALIGNMENT), (dict(dk=P + 8), ALIGNMENT), (dict(ws=P + 2), ALIGNMENT), (dict(lse=P + 2), ALIGNMENT), (dict(rest=P + 4), ALIGNMENT),
     (dict(d=256), UNSUPPORTED),
 ])
 def test_attention_backward_refuses(change, code):
