@@ -58,7 +58,7 @@ __global__ __launch_bounds__(DGNN_BLOCK) void k_embed_fwd(int n, int rows, int d
 }
 
 // ------------------------------------------------------------------ stable radix sort of (row, i)
-constexpr int SORT_TILE = 1024, SORT_BINS = 256, SORT_SMALL = 4096;
+constexpr int SORT_TILE = 1024, SORT_BINS = 256, SORT_SMALL = 8192;
 static inline int sort_tiles(int n) { return (n + SORT_TILE - 1) / SORT_TILE; }
 
 template <class I>
@@ -147,7 +147,7 @@ __device__ __forceinline__ unsigned long long same_digit(int digit, bool on) {
   return same;
 }
 
-// The whole sort of up to SORT_SMALL ids in one workgroup: every wave owns 256 consecutive positions; a
+// The whole sort of up to SORT_SMALL ids in one workgroup: every wave owns 512 consecutive positions; a
 // pass counts the wave's digits, turns the counts into first positions (digit, then wave) and moves
 // the pairs within LDS in order.
 template <class I>
@@ -435,7 +435,9 @@ static int launch_embed_sums(int n, int rows, int dim, float scale, const EmbedP
     DGNN_LAUNCH_CHECK();
   }
   const int lanes = row_lanes(dim, N), groups = DGNN_BLOCK / lanes;
-  const int per_block = groups * 16 > EMBED_ROWS / 2 ? EMBED_ROWS : groups * 16;
+  // as many rows a workgroup as make up for its search, but a thousand workgroups where the rows allow it
+  int per_block = groups * 16 > EMBED_ROWS / 2 ? EMBED_ROWS : groups * 16;
+  if (per_block > (rows + 1023) / 1024) per_block = (rows + 1023) / 1024 > groups ? (rows + 1023) / 1024 : groups;
   hipLaunchKernelGGL((k_embed_rows<T, N>), dim3((unsigned)((rows + (long long)per_block - 1) / per_block)), dim3(DGNN_BLOCK), 0, st, n,
                      rows, dim, lanes, per_block, p.run, scale, key, val, (const T *)grad, part, (T *)out);
   DGNN_LAUNCH_CHECK();
