@@ -373,16 +373,19 @@ __global__ __launch_bounds__(C::THREADS, C::THREADS == 512 ? 2 : 1) void k_ce_fw
 __global__ __launch_bounds__(DGNN_BLOCK) void k_ce_join(const CeArgs a, int tiles) {
   const float *__restrict__ pm = a.part_m, *__restrict__ ps = a.part_s;
   const int n = a.n;
-  __shared__ float sm[32][8], ss[32][8];
+  // doubles: a thread may add some thousand tiles' sums of like size, each rounding the same way
+  __shared__ float sm[32][8];
+  __shared__ double ss[32][8];
   const int c = threadIdx.x & 7, lane = threadIdx.x >> 3, r = blockIdx.x * 8 + c, rows = rows_of(a);
   if ((int)blockIdx.x * 8 >= rows) return;
-  float m = -INFINITY, s = 0.f;
+  float m = -INFINITY;
+  double s = 0.;
   if (r < rows) {
 #pragma unroll 4
     for (int t = lane; t < tiles; t += 32) {
       const float tm = pm[(long long)t * n + r], ts = ps[(long long)t * n + r], top = fmaxf(m, tm);
       const float base = top == -INFINITY ? 0.f : top;
-      s = s * expf(m - base) + ts * expf(tm - base);
+      s = s * (double)expf(m - base) + (double)ts * (double)expf(tm - base);
       m = top;
     }
   }
@@ -392,9 +395,9 @@ __global__ __launch_bounds__(DGNN_BLOCK) void k_ce_join(const CeArgs a, int tile
   float top = sm[0][c];
   for (int w = 1; w < 32; ++w) top = fmaxf(top, sm[w][c]);
   const float base = top == -INFINITY ? 0.f : top;
-  float sum = 0.f;
-  for (int w = 0; w < 32; ++w) sum += ss[w][c] * expf(sm[w][c] - base);
-  const float v = base + logf(sum);
+  double sum = 0.;
+  for (int w = 0; w < 32; ++w) sum += ss[w][c] * (double)expf(sm[w][c] - base);
+  const float v = base + logf((float)sum);
   const int row = row_at(a, r);
   const bool on = a.labels.valid(row);
   a.lse[row] = on ? v : 0.f;

@@ -185,6 +185,32 @@ def test_attention_scales(dtype):
         attention_case(lens, lens, 2, 2, 32, True, dtype, scale=scale)
 
 
+def test_attention_broadcast_inputs_and_gradients():
+    """Expanded keys, values and gradients (strides of zero): values as if they had been copied."""
+    for dtype in DTYPES:
+        ptr = torch.tensor([0, 40, 70], dtype=torch.int32, device=DEV)
+        q = torch.randn(70, 4, 64, device=DEV).to(dtype).requires_grad_()
+        one = torch.randn(70, 1, 64, device=DEV).to(dtype).requires_grad_()          # one key head for all
+        row = torch.randn(1, 4, 64, device=DEV).to(dtype).requires_grad_()           # one value row for all
+        out = PackedAttentionFuse(q, one.expand(70, 4, 64), row.expand(70, 4, 64), ptr, causal=True)
+        got = torch.autograd.grad(out.sum(), [q, one, row])
+        q2, k2, v2 = (t.detach().clone().requires_grad_() for t in (q, one.expand(70, 4, 64), row.expand(70, 4, 64)))
+        out2 = PackedAttentionFuse(q2, k2.contiguous(), v2.contiguous(), ptr, causal=True)
+        want = torch.autograd.grad(out2, [q2, k2, v2], torch.ones_like(out2))
+        assert torch.equal(out, out2) and torch.equal(got[0], want[0])
+        assert torch.equal(got[1], want[1].sum(1, keepdim=True)) and torch.equal(got[2], want[2].sum(0, keepdim=True))
+
+
+def test_second_derivatives_are_refused():
+    ptr = torch.tensor([0, 8], dtype=torch.int32, device=DEV)
+    q = torch.randn(8, 1, 16, device=DEV, requires_grad=True)
+    out = PackedAttentionFuse(q, q, q, ptr)
+    for loss in (out.sum(), out.pow(2).sum()):            # the gradient of out constant, and with a graph of its own
+        g, = torch.autograd.grad(loss, [q], create_graph=True)
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad(g.sum(), [q])
+
+
 def test_attention_nan_stays_in_its_sequence():
     for dtype in DTYPES:
         q, k, v = (torch.randn(200, 2, 64, device=DEV).to(dtype) for _ in range(3))
@@ -323,6 +349,50 @@ def test_cross_entropy_only_one_gradient_and_no_rows():
         assert loss.shape == ((0,) if reduction == "none" else ()) and not loss.any()
         loss.sum().backward()
         assert not w.grad.any() and x.grad.shape == (0, 16)
+
+
+# ------------------------------------------------------------------------------------ beyond 32 bits
+def test_offsets_past_32_bits():
+    """Tables, caches and weights of more than 2^31 elements: the last rows are where they should be."""
+    rows, dim = 34_000_000, 64
+    table = torch.zeros(rows, dim, dtype=torch.bfloat16, device=DEV)
+    at = torch.tensor([0, 1, 33_554_431, 33_554_432, rows - 1], device=DEV)
+    table[at] = torch.randn(5, dim, device=DEV).bfloat16()
+    assert torch.equal(NodeEmbeddingFuse(at, table), table[at])
+    x = torch.randn(40, dim, device=DEV).bfloat16()
+    label = at.repeat(8)
+    w = table.requires_grad_()
+    loss = LinearCrossEntropyFuse(x, w, label, reduction="none")
+    z = x.double() @ table.detach()[at].double().t()
+    total = torch.exp(z).sum(1) + (rows - 5)                      # every other row scores 0
+    want = torch.log(total) - z.gather(1, torch.arange(5, device=DEV).repeat(8).unsqueeze(1))[:, 0]
+    assert (loss.double() - want).abs().max() < 1e-4              # 2^-24 times a sum of 266 k tile terms at most
+    g, = torch.autograd.grad(loss.sum(), w)
+    dw = (torch.softmax(torch.cat([z, torch.log(torch.full_like(total, rows - 5.0)).unsqueeze(1)], 1), 1)[:, :5]
+          - torch.eye(5, device=DEV, dtype=torch.float64).repeat(8, 1)).t() @ x.double()
+    mass = x.double().abs().sum(0)                                # |dz| <= 1, one rounding of dz and one of dw
+    assert ((g[at].double() - dw).abs() <= 2 ** -8 * (mass + dw.abs())).all()
+    del g, w, loss
+    t = table.detach().requires_grad_()
+    go = torch.randn(5, dim, device=DEV).bfloat16()
+    g, = torch.autograd.grad(NodeEmbeddingFuse(at, t), [t], go)
+    assert torch.equal(g[at], go) and int((g != 0).any(1).sum()) == 5
+    del g, t, table
+    # a cache of 1.1 M tokens, 16 heads of 128: one query for each of three sequences, and a prompt at its end
+    tk, h, d = 1_100_000, 16, 128
+    k, v = (torch.randn(tk, h, d, device=DEV, dtype=torch.bfloat16) for _ in range(2))
+    ptr = torch.tensor([0, 300, tk - 700, tk], dtype=torch.int32, device=DEV)
+    for lq, causal in (([1, 1, 1], False), ([0, 0, 200], True)):
+        off = offsets(lq)
+        q = torch.randn(off[-1], h, d, device=DEV, dtype=torch.bfloat16)
+        out = PackedAttentionFuse(q, k, v, torch.tensor(off, dtype=torch.int32, device=DEV), ptr, causal=causal)
+        for s in (0, 2):
+            if lq[s] == 0:
+                continue
+            a, b = [0, 300, tk - 700, tk][s:s + 2]
+            n = b - a
+            want = ref.attention(q[off[s]:off[s + 1]].cpu(), k[a:b].cpu(), v[a:b].cpu(), [0, lq[s]], [0, n], causal, d ** -0.5)
+            ref.check(out[off[s]:off[s + 1]], want["out"], f"sequence {s}")
 
 
 # ------------------------------------------------------------------------------------ together
