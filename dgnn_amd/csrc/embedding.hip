@@ -5,8 +5,8 @@
 // An id outside [0, rows) names no row: zeros out, no gradient.  Both directions are bound by memory.
 // The gradient sorts (id, i) with a stable radix sort, eight bits a pass, so that every row of the
 // table is written exactly once, by the sum of its own run in ascending i: no atomics on floats, no
-// zeroed table, the same bits every time.  Runs longer than RUN (frequent tokens, hub nodes) are
-// summed in pieces first.
+// zeroed table, the same bits every time.  Runs that cross the borders of fixed pieces (all long ones:
+// frequent tokens, hub nodes) are summed a piece at a time first.
 #include "common.hpp"
 
 using namespace dgnn;
@@ -251,24 +251,35 @@ __device__ __forceinline__ int first_not_below_wave(const int *__restrict__ key,
   return lo;
 }
 
-// Sorted positions are cut into pieces of `run`.  A row whose run is longer than that gets one partial
+// Sorted positions are cut into pieces of `run`.  A row whose run crosses a border of pieces gets one partial
 // sum per piece it touches: slot 2 p when its run holds the first position of piece p, slot 2 p + 1
-// when it begins inside (a piece holds the beginning of at most one such run).
+// when it begins inside (and leaves through the end).  Whether a run crosses shows in the keys next to the
+// borders, so nothing is searched.  64 N columns and one piece a workgroup, its positions dealt to four waves.
 template <class T, int N>
-__global__ __launch_bounds__(DGNN_BLOCK) void k_embed_long(int n, int rows, int dim, int run,
-                                                           const int *__restrict__ key, const int *__restrict__ val,
-                                                           const T *__restrict__ grad, float *__restrict__ part) {
+__global__ __launch_bounds__(DGNN_BLOCK) void k_embed_cross(int n, int rows, int dim, int run,
+                                                            const int *__restrict__ key, const int *__restrict__ val,
+                                                            const T *__restrict__ grad, float *__restrict__ part) {
   __shared__ float sums[DGNN_WAVES_PER_BLOCK][DGNN_WAVE * N];
+  __shared__ int counts[2];
   const int lane = lane_id(), wave = wave_in_block();
   const int lo = blockIdx.x * run, hi = min(n, lo + run);
   const int c = (blockIdx.y * DGNN_WAVE + lane) * N;
-  const int ends[2] = {key[lo], key[hi - 1]};
+  const int first = key[lo], last = key[hi - 1];
+  const bool before = lo > 0 && key[lo - 1] == first, behind = hi < n && key[hi] == last;
+  // the run at the front, if it crosses either border, and the one at the end, if it is another and leaves
+  const bool front = first < rows && (before || (behind && first == last)), back = last < rows && behind && first != last;
+  if (!front && !back) return;
+  if (threadIdx.x < 2) counts[threadIdx.x] = 0;
+  __syncthreads();
+  for (int i = lo + wave * DGNN_WAVE; i < hi; i += DGNN_BLOCK) {
+    const int k = i + lane < hi ? key[i + lane] : rows;
+    const int f = __popcll(__ballot(k == first)), b = __popcll(__ballot(k == last));
+    if (lane == 0) atomicAdd(&counts[0], f), atomicAdd(&counts[1], b);
+  }
+  __syncthreads();
   for (int which = 0; which < 2; ++which) {
-    const int k = ends[which];
-    if (k >= rows || (which == 1 && k == ends[0])) continue;
-    const int s = first_not_below_wave(key, n, k), e = first_not_below_wave(key, n, k + 1);
-    if (e - s <= run) continue;
-    const int a = max(s, lo), b = min(e, hi);
+    if (!(which == 0 ? front : back)) continue;
+    const int a = which == 0 ? lo : hi - counts[1], b = which == 0 ? lo + counts[0] : hi;
     float acc[N];
 #pragma unroll
     for (int j = 0; j < N; ++j) acc[j] = 0.f;
@@ -288,7 +299,7 @@ __global__ __launch_bounds__(DGNN_BLOCK) void k_embed_long(int n, int rows, int 
       for (int j = 0; j < N; ++j) {
         float t = 0.f;
         for (int w = 0; w < DGNN_WAVES_PER_BLOCK; ++w) t += sums[w][lane * N + j];
-        part[((long long)(2 * blockIdx.x + (s < lo || s == lo ? 0 : 1))) * dim + c + j] = t;
+        part[(2LL * blockIdx.x + which) * dim + c + j] = t;
       }
     __syncthreads();
   }
@@ -345,7 +356,7 @@ __global__ __launch_bounds__(DGNN_BLOCK) void k_embed_rows(int n, int rows, int 
       float acc[N];
 #pragma unroll
       for (int j = 0; j < N; ++j) acc[j] = 0.f;
-      if (e - s <= run) {
+      if (s / run == (e - 1) / run) {           // inside one piece
 #pragma unroll 8
         for (int i = s; i < e; ++i) {
           const Pack<T, N> p = *(const Pack<T, N> *)(grad + (long long)val[i] * dim + c);
@@ -430,7 +441,7 @@ template <class T, int N>
 static int launch_embed_sums(int n, int rows, int dim, float scale, const EmbedPlan &p, const int *key, const int *val,
                              const void *grad, float *part, void *out, hipStream_t st) {
   if (n > p.run) {
-    hipLaunchKernelGGL((k_embed_long<T, N>), dim3((unsigned)p.pieces, (unsigned)((dim + DGNN_WAVE * N - 1) / (DGNN_WAVE * N))),
+    hipLaunchKernelGGL((k_embed_cross<T, N>), dim3((unsigned)p.pieces, (unsigned)((dim + DGNN_WAVE * N - 1) / (DGNN_WAVE * N))),
                        dim3(DGNN_BLOCK), 0, st, n, rows, dim, p.run, key, val, (const T *)grad, part);
     DGNN_LAUNCH_CHECK();
   }
