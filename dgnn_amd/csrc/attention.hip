@@ -156,7 +156,7 @@ template <class T, int DP, int NW, int HW, int BN, int S>
 __global__ __launch_bounds__(64 * NW * HW, sizeof(T) == 2 ? 2 : 1) void k_attn_fwd(const AttnArgs a) {
   using AT = AttnTile<T, DP, NW, BN, S>;
   DGNN_RING(all, HW * AT::BYTES);
-  const HeadSlot at = head_slot<HW>(a.hk, 1);
+  const HeadSlot at = head_slot<HW>(a.hk, a.nseq, 1);
   if (at.head >= a.hk) return;
   const int kvh = at.head;
   const lds_ptr lds[4] = {all[0] + at.wave * AT::BYTES, all[1] + at.wave * AT::BYTES, all[2] + at.wave * AT::BYTES, all[3] + at.wave * AT::BYTES};
@@ -177,9 +177,9 @@ __global__ __launch_bounds__(64 * NW * HW, sizeof(T) == 2 ? 2 : 1) void k_attn_f
 // tiles of 32, unsplit.
 template <class T, int DP>
 __global__ __launch_bounds__(64, sizeof(T) == 2 ? 2 : 1) void k_attn_split(const AttnArgs a) {
-  using AT = AttnTile<T, DP, 1, 32, DP * sizeof(T) >= 512 ? 3 : 4>;
+  using AT = AttnTile<T, DP, 1, 32, 2>;
   DGNN_RING(lds, AT::BYTES);
-  const int kvh = blockIdx.x % a.hk, slot = blockIdx.x / a.hk, lane = lane_id(), h = lane >> 5;
+  const int kvh = blockIdx.x % a.hk, slot = spread(blockIdx.x / a.hk, (int)gridDim.x / a.hk, a.nseq), lane = lane_id(), h = lane >> 5;
   const Segment seg = find_segment(a.col_ptr, a.nseq, a.tk, 1, a.chunk, slot, false);
   if (seg.tile < 0) return;
   int qs, lq;
@@ -279,11 +279,8 @@ static int launch_fwd(const AttnArgs &a, const AttnPlan &p, hipStream_t st) {
     DGNN_LAUNCH_CHECK();
     return DGNN_OK;
   }
-  switch (rows_kind(a.tq, a.nseq, a.g, a.hk)) {
-    case ROWS_SHORT: return a.hk >= 4 ? launch_rows<T, DP, 1, 4, 32, 1>(a, st) : launch_rows<T, DP, 1, 1, 32, 1>(a, st);
-    case ROWS_FEW: return launch_rows<T, DP, 1, 1, 32, 2>(a, st);
-    default: return launch_rows<T, DP, 4, 1, 64, 2>(a, st);
-  }
+  if (!rows_short(a.tq, a.nseq, a.g)) return launch_rows<T, DP, 4, 1, 64, 2>(a, st);
+  return a.hk >= 4 ? launch_rows<T, DP, 1, 4, 32, 1>(a, st) : launch_rows<T, DP, 1, 1, 32, 1>(a, st);
 }
 template <class T>
 static int launch_fwd_d(const AttnArgs &a, const AttnPlan &p, hipStream_t st) {

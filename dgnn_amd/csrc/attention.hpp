@@ -67,16 +67,22 @@ __device__ __forceinline__ Segment find_segment(const int *__restrict__ ptr, int
 static inline long long tile_slots(int total, int nseq, int g, int rows) {
   return (long long)total * g / rows + nseq + 2;
 }
-// How the rows of an index are dealt out.  Long: four waves share a tile of 128 packed rows and the tiles
-// staged for it.  Short sequences (96 packed rows on average or less): a wave alone has 32 rows, and four
-// waves of a workgroup take four heads, since workgroups are then so many and so brief that starting
-// them counts; one buffer, because more waves on a compute unit hide more than a second buffer (1024
-// graphs of 1 .. 63 nodes, 8 heads of 32, float: forward 38 us with two buffers and 33 with one).  Few: long
-// sequences, but not a workgroup for every compute unit: a wave a workgroup.
-enum RowsKind { ROWS_LONG, ROWS_SHORT, ROWS_FEW };
-static inline RowsKind rows_kind(int total, int nseq, int g, int hk) {
-  if ((long long)total * g <= 96LL * nseq) return ROWS_SHORT;
-  return tile_slots(total, nseq, g, 128) * hk < 256 ? ROWS_FEW : ROWS_LONG;
+// How the rows of an index are dealt out.  Usually four waves share a tile of 128 packed rows and the tiles
+// staged for it (a wave a workgroup is no better where those are fewer than the compute units: 2048 tokens, 8
+// heads of 64, bfloat16, forward 33 us against 40).  Short sequences (96 packed rows on average or less): a wave
+// alone has 32 rows, and four waves of a workgroup take four heads, since workgroups are then so many and so
+// brief that starting them counts; one buffer, because more waves on a compute unit hide more than a
+// second buffer (1024 graphs of 1 .. 63 nodes, 8 heads of 32, float: forward 38 us with two buffers, 33 with one).
+static inline bool rows_short(int total, int nseq, int g) { return (long long)total * g <= 96LL * nseq; }
+// Sequences of equal length leave a spare tile slot at a fixed period, and workgroups are dealt to the XCDs and
+// their shader engines in turn: with every second slot spare, half of the card has all the work.  Every 32
+// slots are therefore taken in an order of their own, rotated by 3 j mod 8 in the j-th 32: for no period
+// up to eight do the rotations and the period cancel, as they would in steps of one for a period of three
+// (training step, 512 sequences of 128 tokens, 8 heads of 64, bfloat16: 546 us without, 346 with; 1024 graphs of
+// 32 nodes, 8 heads of 32, float: 175 and 126; of 64, two tiles and a spare slot: 301 and 303).
+// Only where an eighth of the slots can be spare: long causal sequences are 4 % faster in plain order.
+__device__ __forceinline__ int spread(int slot, int slots, int nseq) {
+  return slots >> 3 < nseq + 2 && (slot | 31) < slots ? (slot & ~31) | ((slot + (3 * (slot >> 5) & 7)) & 31) : slot;
 }
 // Workgroup -> key head and tile slot (and split).  Neighbouring workgroups take neighbouring heads: they go to
 // the eight XCDs in turn, so the tiles of one head meet in few of them.  HW > 1: wave w has the group's w-th head.
@@ -84,10 +90,10 @@ struct HeadSlot {
   int head, slot, split, wave;
 };
 template <int HW>
-__device__ __forceinline__ HeadSlot head_slot(int hk, int splits) {
+__device__ __forceinline__ HeadSlot head_slot(int hk, int nseq, int splits) {
   const int groups = (hk + HW - 1) / HW, wave = HW == 1 ? 0 : uniform_i32(wave_in_block());
   const int rest = blockIdx.x / groups;
-  return {(int)(blockIdx.x % groups) * HW + wave, rest / splits, rest % splits, wave};
+  return {(int)(blockIdx.x % groups) * HW + wave, spread(rest / splits, (int)gridDim.x / groups / splits, nseq), rest % splits, wave};
 }
 // Rows of a segment's sequence in the other index: keys of its queries and the other way round.
 __device__ __forceinline__ void other_side(const int *__restrict__ ptr, const int *__restrict__ own, int nseq, int total,

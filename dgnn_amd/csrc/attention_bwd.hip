@@ -60,7 +60,7 @@ __global__ __launch_bounds__(64 * NW * HW, sizeof(T) == 2 && (NW > 1 || DP < 128
   constexpr int TILE = BQ * TL::ROW_BYTES, STAT = 2 * BQ * 4;
   constexpr int BYTES = 2 * TILE + NW * STAT;
   DGNN_RING(all, HW * BYTES);
-  const HeadSlot at = head_slot<HW>(a.hk, a.splits);
+  const HeadSlot at = head_slot<HW>(a.hk, a.nseq, a.splits);
   if (at.head >= a.hk) return;
   const lds_ptr lds[4] = {all[0] + at.wave * BYTES, all[1] + at.wave * BYTES, all[2] + at.wave * BYTES, all[3] + at.wave * BYTES};
   // Two waves a SIMD leave 256 registers; at DP = 128 the accumulators and both operands take 192, and the
@@ -209,7 +209,7 @@ __global__ __launch_bounds__(64 * NW * HW, sizeof(T) == 2 ? 2 : 1) void k_attn_b
   using SG = Stager<T, DP, BN, THREADS>;
   constexpr int TILE = BN * TL::ROW_BYTES;
   DGNN_RING(all, HW * 2 * TILE);
-  const HeadSlot at = head_slot<HW>(a.hk, 1);
+  const HeadSlot at = head_slot<HW>(a.hk, a.nseq, 1);
   if (at.head >= a.hk) return;
   const lds_ptr lds[4] = {all[0] + at.wave * 2 * TILE, all[1] + at.wave * 2 * TILE, all[2] + at.wave * 2 * TILE, all[3] + at.wave * 2 * TILE};
   const int lane = lane_id(), h = lane >> 5, wave = NW == 1 ? 0 : uniform_i32(wave_in_block());
@@ -296,7 +296,7 @@ __global__ __launch_bounds__(64 * NW * HW, sizeof(T) == 2 ? 2 : 1) void k_attn_b
 // writing and reading dk and dv once each in float: 20 k tokens, 16 / 4 heads of 128, causal, lengths up to
 // 8000: 1.59 ms unsplit.
 static int bwd_splits(int nseq, int tq, int tk, int hq, int hk) {
-  if (nseq <= 0 || tk <= 0 || tq <= 0 || rows_kind(tk, nseq, 1, 1 << 20) == ROWS_SHORT) return 1;
+  if (nseq <= 0 || tk <= 0 || tq <= 0 || rows_short(tk, nseq, 1)) return 1;
   const long long groups = tile_slots(tk, nseq, 1, 128) * hk, steps = (long long)tq / nseq / 32 * (hq / hk);
   long long s = (2047 + groups) / groups;
   if (s > steps / 16) s = steps / 16;
@@ -338,16 +338,14 @@ static int launch_bwd(const AttnArgs &a, const float *lse, hipStream_t st) {
                        (const T *)a.out, (const T *)a.rest, (const T *)a.grad, lse, (float2 *)a.stat);
     DGNN_LAUNCH_CHECK();
   }
-  if (a.tk > 0) switch (a.splits > 1 ? ROWS_LONG : rows_kind(a.tk, a.nseq, 1, a.hk)) {
-      case ROWS_SHORT: rc = a.hk >= 4 ? launch_bwd_kv<T, DP, 1, 4, 1>(a, st) : launch_bwd_kv<T, DP, 1, 1, 1>(a, st); break;
-      case ROWS_FEW: rc = launch_bwd_kv<T, DP, 1, 1, 2>(a, st); break;
-      default: rc = launch_bwd_kv<T, DP, 4, 1, 4>(a, st);
-    }
-  if (rc == DGNN_OK && a.tq > 0) switch (rows_kind(a.tq, a.nseq, a.g, a.hk)) {
-      case ROWS_SHORT: rc = a.hk >= 4 ? launch_bwd_q<T, DP, 1, 4, 1>(a, st) : launch_bwd_q<T, DP, 1, 1, 1>(a, st); break;
-      case ROWS_FEW: rc = launch_bwd_q<T, DP, 1, 1, 2>(a, st); break;
-      default: rc = launch_bwd_q<T, DP, 4, 1, 4>(a, st);
-    }
+  if (a.tk > 0) {
+    if (a.splits > 1 || !rows_short(a.tk, a.nseq, 1)) rc = launch_bwd_kv<T, DP, 4, 1, 4>(a, st);
+    else rc = a.hk >= 4 ? launch_bwd_kv<T, DP, 1, 4, 1>(a, st) : launch_bwd_kv<T, DP, 1, 1, 1>(a, st);
+  }
+  if (rc == DGNN_OK && a.tq > 0) {
+    if (!rows_short(a.tq, a.nseq, a.g)) rc = launch_bwd_q<T, DP, 4, 1, 4>(a, st);
+    else rc = a.hk >= 4 ? launch_bwd_q<T, DP, 1, 4, 1>(a, st) : launch_bwd_q<T, DP, 1, 1, 1>(a, st);
+  }
   return rc;
 }
 template <class T>
