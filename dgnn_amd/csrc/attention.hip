@@ -11,6 +11,12 @@
 // inside the lane (one exchange with lane + 32 for the maximum), the rescaling factor is a lane's scalar,
 // and the 16 weights a lane holds are, unmoved, its operand of the second product (mma.hpp).
 // Key tiles are double buffered, loaded straight to LDS while the previous tile is worked on.
+//
+// Bound by the matrix instructions and, next to them, the exponentials (one a score against 4 d operations), under
+// the power limit that large 16-bit products run into too: 16384 tokens, causal, 16 / 2 heads of 128, float16
+// 1.10 ms, 1000 TFLOP/s (a large matrix product reaches 1125); 32 x 2048 tokens, 8 heads of 64, bfloat16
+// 0.37 - 0.42 ms, 650 - 740 TFLOP/s.  Weights are rounded to T for the second product, half a step each; their sum is
+// of the unrounded ones, in float like every sum here.
 #include "attention.hpp"
 
 using namespace dgnn;
@@ -170,11 +176,12 @@ __global__ __launch_bounds__(64 * NW * HW, sizeof(T) == 2 ? 2 : 1) void k_attn_f
 }
 
 // ------------------------------------------------------------------ few rows, long keys
-// Single queries and poolings: a sequence's first a.few packed rows of a key head are split over chunks of
+// Single queries and poolings, bound by reading the keys and values: a sequence's first a.few packed rows of a key head are split over chunks of
 // a.chunk keys, one wave a chunk, which reads its keys and values once for all query heads of the key
 // head; k_attn_join puts the parts together.  Part (slot, key head) holds {output row, maximum, sum} of
 // each of the rows.  What rows a sequence has beyond those are dealt to its chunks' workgroups in
-// tiles of 32, unsplit.
+// tiles of 32, unsplit.  Two buffers of 32 keys and values: four waves a compute unit keep more loads in flight than
+// two with four buffers (9 sequences of 32768 keys, 32 / 8 heads of 128, bfloat16: 230 us against 245, 5.2 TB/s).
 template <class T, int DP>
 __global__ __launch_bounds__(64, sizeof(T) == 2 ? 2 : 1) void k_attn_split(const AttnArgs a) {
   using AT = AttnTile<T, DP, 1, 32, 2>;
@@ -241,6 +248,10 @@ __global__ __launch_bounds__(DGNN_BLOCK) void k_attn_join(const AttnArgs a) {
 }
 
 // ------------------------------------------------------------------ which kernel
+// Split: at most 32 packed rows a sequence and 256 keys, on average.  Each way, bfloat16, split and unsplit: 16 single
+// queries of 1024 keys 20 and 42 us, 9 of 32768 keys 230 and 1374 us; where the sequences alone fill the card it costs
+// something (256 of 1024 keys 226 and 205 us), but a few long ones among short ones cost more the other way.  A
+// chunk is a 2048th of all keys times heads (9 x 32768: half of it 242 us, twice 272), within 256 .. 2048.
 struct AttnPlan {
   int few, chunk;                       // split: rows kept in parts, keys of a chunk (few = 0: not split)
   long long slots;

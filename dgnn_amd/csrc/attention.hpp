@@ -36,8 +36,9 @@ struct Segment {
 
 // Workgroup -> tile without a list of tiles: segment s owns the tile slots from
 // floor(bound(s) g / rows) + s up to the next segment's, at least as many as it has tiles (the spare
-// ones find nothing to do).  by_row: the segment that holds row `slot` itself.  The segment of a slot is searched with 63 probes a step; the last step's
-// probes are neighbours, so both of its bounds are in two lanes already.
+// ones find nothing to do).  by_row: the segment that holds row `slot` itself.  The segment of a slot is
+// searched with 63 probes a step; the last step's probes are neighbours, so both of its bounds are in two
+// lanes already.
 __device__ __forceinline__ Segment find_segment(const int *__restrict__ ptr, int nseq, int total, int g, int rows,
                                                 int slot, bool last_first, bool by_row = false) {
   int lo = 0, hi = nseq + 2, bound, n, step;

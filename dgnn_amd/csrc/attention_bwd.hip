@@ -7,7 +7,8 @@
 // atomics and results do not depend on the order of workgroups: k_attn_bwd_kv keeps 32 keys a wave
 // with dk^T and dv^T in accumulators and walks the query tiles of all heads that share the key head;
 // k_attn_bwd_q keeps 32 packed query rows a wave and walks the key tiles.  The price is forming z and
-// do v^T twice: seven products instead of five.
+// do v^T twice: seven products instead of five.  p and ds are rounded to T for the products that sum over
+// them, half a step each; everything else is float.
 #include "attention.hpp"
 
 using namespace dgnn;
@@ -15,8 +16,9 @@ using namespace dgnn;
 namespace dgnn {
 
 // stat[head][row] = {lse log2(e), <do, o>}, o with what its rounding took (`rest`): <do, v_j> - <do, o> cancels
-// in rows that see few keys, and half a step of a 16-bit o is all that was left of it; the first is +inf where the row saw no key (p = exp2(z - inf) = 0).
-// One thread per 16-byte chunk, lanes of a row joined by shuffles.
+// in rows that see few keys, and half a step of a 16-bit o is all that was left of it; the first is +inf
+// where the row saw no key (p = exp2(z - inf) = 0).  One thread per 16-byte chunk, lanes of a row joined by
+// shuffles.  Bound by memory: 65536 tokens, 8 heads of 64, bfloat16 35 us, 5.8 TB/s.
 template <class T, int LPR>
 __global__ __launch_bounds__(DGNN_BLOCK) void k_attn_bwd_stat(long long rows, int d, int tq, int hq,
                                                               const T *__restrict__ out, const T *__restrict__ rest,
@@ -51,6 +53,11 @@ __global__ __launch_bounds__(DGNN_BLOCK) void k_attn_bwd_stat(long long rows, in
 template <class T, int DP, int NW>
 constexpr int bwd_rows() { return 32 * DP * (int)sizeof(T) >= 1024 * NW ? 32 : 64; }
 
+// Long sequences: four waves with 32 keys each share the staged tiles of queries and do, a ring of four, since
+// two waves a SIMD (the accumulators' 256 registers) hide little by themselves.  Bound by the matrix instructions
+// under the power limit: 32 x 2048 tokens, 8 heads of 64, bfloat16 0.56 - 0.66 ms, 830 - 980 TFLOP/s; 20 k tokens,
+// causal, 16 / 4 heads of 128, lengths up to 8000, 1.03 ms, 970 TFLOP/s (a large matrix product reaches 1156).
+// 1024 graphs of 1 .. 63 nodes, 8 heads of 32, float: 52 us, waiting for each wave's few loads.
 template <class T, int DP, int NW, int HW, int S>
 __global__ __launch_bounds__(64 * NW * HW, sizeof(T) == 2 && (NW > 1 || DP < 128) ? 2 : 1) void k_attn_bwd_kv(const AttnArgs a) {
   constexpr int BK = 32 * NW, BQ = bwd_rows<T, DP, NW>(), THREADS = 64 * NW;
@@ -202,6 +209,8 @@ __global__ __launch_bounds__(DGNN_BLOCK) void k_attn_bwd_join(const AttnArgs a) 
   *(vec4<T> *)((T *)(c < a.d ? a.dk : a.dv) + row * a.d + (c < a.d ? c : c - a.d)) = o;
 }
 
+// The same with the sides changed, as the forward: a lane has one packed query row.  At the sizes above 0.40 - 0.48 ms,
+// 0.74 ms (1010 TFLOP/s) and 41 us.
 template <class T, int DP, int NW, int HW, int S>
 __global__ __launch_bounds__(64 * NW * HW, sizeof(T) == 2 ? 2 : 1) void k_attn_bwd_q(const AttnArgs a) {
   constexpr int BM = 32 * NW, BN = bwd_rows<T, DP, NW>(), THREADS = 64 * NW;
@@ -294,7 +303,8 @@ __global__ __launch_bounds__(64 * NW * HW, sizeof(T) == 2 ? 2 : 1) void k_attn_b
 // every head that shares the key head, the first ones of a causal sequence all of them: with fewer
 // workgroups than four rounds of the card, the longest of them are most of the time.  The parts cost
 // writing and reading dk and dv once each in float: 20 k tokens, 16 / 4 heads of 128, causal, lengths up to
-// 8000: 1.59 ms unsplit.
+// 8000: 1.59 ms unsplit, 1.03 and 0.05 for the join split; 8192 tokens in one sequence, the whole training step 1.92
+// and 1.29 ms; 2048 tokens, 8 heads of 64, 135 and 119 us.
 static int bwd_splits(int nseq, int tq, int tk, int hq, int hk) {
   if (nseq <= 0 || tk <= 0 || tq <= 0 || rows_short(tk, nseq, 1)) return 1;
   const long long groups = tile_slots(tk, nseq, 1, 128) * hk, steps = (long long)tq / nseq / 32 * (hq / hk);

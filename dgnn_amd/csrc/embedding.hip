@@ -28,7 +28,8 @@ __device__ __forceinline__ int row_of_id(const I *ids, long long i, int rows) {
   return x >= 0 && x < (I)rows ? (int)x : rows;           // rows: names none
 }
 
-// lanes = threads that share a row (a power of two up to 256)
+// lanes = threads that share a row (a power of two up to 256).  65536 ids of 1024 bfloat16 45 us, 5.9 TB/s; 196611 of
+// 100 floats, from 2.4 million rows, 36 us, 4.4 TB/s (a large copy: 5.1).
 template <class T, int N, class I>
 __global__ __launch_bounds__(DGNN_BLOCK) void k_embed_fwd(int n, int rows, int dim, int lanes, float scale,
                                                           const I *__restrict__ ids, const T *__restrict__ table,
@@ -147,9 +148,10 @@ __device__ __forceinline__ unsigned long long same_digit(int digit, bool on) {
   return same;
 }
 
-// The whole sort of up to SORT_SMALL ids in one workgroup: every wave owns 512 consecutive positions; a
-// pass counts the wave's digits, turns the counts into first positions (digit, then wave) and moves
-// the pairs within LDS in order.
+// The whole sort of up to SORT_SMALL ids in one workgroup, since launches are most of a small sort's time (the whole
+// gradient of 2708 rows of 64: 2048 ids 19 us, with three launches a pass 28; 8192 ids 29 and 31): every wave
+// owns 512 consecutive positions; a pass counts the wave's digits, turns the counts into first positions
+// (digit, then wave) and moves the pairs within LDS in order.
 template <class I>
 __global__ __launch_bounds__(1024) void k_sort_small(int n, int rows, int passes, const I *__restrict__ ids,
                                                      int *__restrict__ key, int *__restrict__ val) {
@@ -255,6 +257,8 @@ __device__ __forceinline__ int first_not_below_wave(const int *__restrict__ key,
 // sum per piece it touches: slot 2 p when its run holds the first position of piece p, slot 2 p + 1
 // when it begins inside (and leaves through the end).  Whether a run crosses shows in the keys next to the
 // borders, so nothing is searched.  64 N columns and one piece a workgroup, its positions dealt to four waves.
+// 65536 ids of 1024 bfloat16, most of them frequent ones, 28 us (about 4 TB/s); 196611 of 100 floats 21 us,
+// waiting for key, position and row one after the other.
 template <class T, int N>
 __global__ __launch_bounds__(DGNN_BLOCK) void k_embed_cross(int n, int rows, int dim, int run,
                                                             const int *__restrict__ key, const int *__restrict__ val,
@@ -309,7 +313,8 @@ constexpr int EMBED_ROWS = 256;      // most rows of the table a workgroup write
 
 // A workgroup writes `per_block` consecutive rows.  It finds the sorted positions that name them, marks
 // where each row's run begins and ends, stores zeros to the rows without one as one stream of pieces, and
-// gives every other row to `lanes` threads.
+// gives every other row to `lanes` threads.  2.4 million rows of 100 floats, of which few are named, 231 us, 4.6 TB/s;
+// 50000 rows of 1024 bfloat16 63 us, 3.7 TB/s: the runs there are a few positions long, each a wait of its own.
 template <class T, int N>
 __global__ __launch_bounds__(DGNN_BLOCK) void k_embed_rows(int n, int rows, int dim, int lanes, int per_block, int run, float scale,
                                                            const int *__restrict__ key, const int *__restrict__ val,
