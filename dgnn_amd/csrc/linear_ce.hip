@@ -695,7 +695,8 @@ static CePlan ce_plan(int dtype, int n, int classes, int d, const void *x, const
   p.piece = ceil_div(ceil_div(classes, ceil_div(classes, cols)), class_tile) * class_tile;
   p.pieces = ceil_div(classes, p.piece);
   // enough workgroups for every compute unit: split the long axis while tiles are few
-  // float: a sum of 10^5 terms in one accumulator has lost three of its seven digits, so none is longer than 4096
+  // float: a sum of 10^5 terms in one accumulator has lost three of its seven digits, so none is longer than
+  // 4096 terms, or a 64th of the axis
   auto splits = [&](long long tiles, int steps) {
     long long s = tiles > 0 ? 512 / tiles : 1;
     if (dtype == DGNN_F32 && s < (steps + 63) / 64) s = (steps + 63) / 64;

@@ -265,6 +265,13 @@ def test_attention_few_rows_long_keys(hq, hk, d, causal, dtype):
     attention_case([1], [4000], hq, hk, d, causal, dtype)
 
 
+@pytest.mark.parametrize("dtype", DTYPES, ids=ids_of)
+@pytest.mark.parametrize("rows,keys", [(128, 128), (64, 64), (32, 32), (1, 256), (1, 512)])
+def test_attention_equal_lengths(rows, keys, dtype):
+    """Spare tile slots at a fixed period, which are dealt out in an order of their own."""
+    attention_case([rows] * 71, [keys] * 71, 2, 1, 32, rows == 64, dtype, back=5)
+
+
 def test_attention_many_small_graphs():
     lens = [(i * 7) % 40 for i in range(700)]
     attention_case(lens, lens, 1, 1, 32, False, torch.float32)
@@ -512,3 +519,45 @@ def test_on_a_side_stream():
     side.synchronize()
     for a, b in zip(got, want):
         assert torch.equal(a, b)
+
+
+def test_two_graphs_replayed_at_the_same_time():
+    """Two captured calls of each kind, replayed on two streams: neither finds the other's workspace."""
+    gen = torch.Generator(device=DEV).manual_seed(9)
+    ptr = torch.tensor(offsets([400, 700, 0, 900]), dtype=torch.int32, device=DEV)
+    rows, nodes = 2000, 5000
+
+    def inputs():
+        x = torch.randn(rows, 6, 64, device=DEV, generator=gen).to(torch.bfloat16)
+        w = (torch.randn(nodes, 128, device=DEV, generator=gen) / 8).to(torch.bfloat16)
+        ids = torch.randint(0, nodes, (20000,), device=DEV, generator=gen)
+        return [x.requires_grad_(), w.requires_grad_(), ids, torch.randint(-9, nodes, (rows,), device=DEV, generator=gen)]
+
+    def step(x, w, ids, label):
+        y = PackedAttentionFuse(x[:, :2], x[:, 2:4], x[:, 4:], ptr, causal=True)
+        one = PackedAttentionFuse(x[:4, :2], x[:, 2:4], x[:, 4:], torch.arange(5, dtype=torch.int32, device=DEV), ptr)
+        loss = LinearCrossEntropyFuse(y.flatten(1), w, label) + NodeEmbeddingFuse(ids, w, 0.5).float().mean() + one.float().mean()
+        return [loss.detach()] + list(torch.autograd.grad(loss, [x, w]))
+
+    both, graphs, static, want = [inputs(), inputs()], [], [], []
+    for args in both:
+        want.append([t.clone() for t in step(*args)])
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            step(*args)
+        torch.cuda.current_stream().wait_stream(side)
+        torch.cuda.synchronize()
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            static.append(step(*args))
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(3):
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+                g.replay()
+        torch.cuda.synchronize()
+        for got, ref_ in zip(static, want):
+            for a, b in zip(got, ref_):
+                assert torch.equal(a, b)
