@@ -176,13 +176,142 @@ __global__ __launch_bounds__(64 * NW * HW, sizeof(T) == 2 ? 2 : 1) void k_attn_f
 }
 
 // ------------------------------------------------------------------ few rows, long keys
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+// a 4 x 1 (lane 4 b + i: row i of block b) times 1 x 4 in sixteen blocks; every group of 2^CB blocks takes the
+// first operand of its block BLOCK
+template <int CB, int BLOCK>
+__device__ __forceinline__ f32x4 mma4(float a, float b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_4x4x1f32(a, b, c, CB, BLOCK, 0);
+}
+// The same as AttnTile for up to four rows of floats: its float matrix instructions take 32 rows whether they
+// are there or not, and bound it at half the memory's rate.  Blocks of 4 x 4 lose nothing (single queries of 32 / 8
+// heads of 128: 9 sequences of 32768 keys 418 us against 755, 5.8 TB/s; 16 of 1024 39 against 89).  A tile
+// is 32 keys.  Scores: a lane has a key and half of the dims, so blocks 0 - 7 and 8 - 15 take their own dims of q
+// and the halves are added.  Output: a lane has DP / 64 columns, and the weights, turned in LDS, are the
+// broadcast operand; DP = 32: a column and half of the keys.  Rows lie in the four elements of z and acc.
+template <int DP>
+struct AttnFour {
+  using TL = Tile<float, DP>;
+  using SG = Stager<float, DP, 32, 64>;
+  static constexpr int TILE = 32 * TL::ROW_BYTES, BYTES = 2 * TILE, VC = DP >= 64 ? DP / 64 : 1;
+  static constexpr bool HALVES = DP == 32;      // of the keys, for the output
+  f32x4 acc[VC], m, l;                          // l: this lane's share
+  float c;
+
+  __device__ __forceinline__ void run(const AttnArgs &a, const lds_ptr (&lds)[4], lds_ptr turn, int qs, int lq, int ks, int lk,
+                                      int kvh, int rows, int key0, int key1) {
+    const int lane = lane_id(), h = lane >> 5;
+    const int k_lane = TL::lane_addr(lane & 31, h * (DP / 8)), v_lane = HALVES ? TL::lane_addr(16 * h, (lane & 31) / 4) + lane % 4 * 4 : lane * VC * 4;
+    const int shift = lk - lq;
+    int last[4], seen = 0;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      last[r] = r >= rows ? -1 : a.causal ? min(key1 - 1, r / a.g + shift) : key1 - 1;
+      seen = max(seen, last[r] + 1);
+    }
+    const int tiles = (max(seen - key0, 0) + 31) / 32;
+    c = a.scale * DGNN_LOG2E;
+    const float sign = c > 0.f ? 1.f : c < 0.f ? -1.f : 0.f;         // as in AttnTile (NaN: q and c as they are)
+    c = sign == 0.f ? (c == 0.f ? 1.f : c) : c * sign;
+    float q[DP / 16];
+    {
+      const int r = lane & 3, b = lane >> 2;
+      const float *row = (const float *)a.q + (qs + (long long)(r / a.g)) * a.q_tok + (long long)(kvh * a.g + r % a.g) * a.q_head;
+#pragma unroll
+      for (int j = 0; j < DP / 16; ++j) {
+        const int at = (DP / 2) * (b >> 3) + 8 * j + (b & 7);
+        q[j] = r < rows && at < a.d ? row[at] * sign : 0.f;
+      }
+    }
+    const unsigned k_stride = (unsigned)(a.k_tok * 4), v_stride = (unsigned)(a.v_tok * 4), row_bytes = a.d * 4u;
+    const float *kbase = (const float *)a.k + (ks + (long long)key0) * a.k_tok + (long long)kvh * a.k_head;
+    const float *vbase = (const float *)a.v + (ks + (long long)key0) * a.v_tok + (long long)kvh * a.v_head;
+    SG st_k, st_v;
+    st_k.init(k_stride, a.d);
+    st_v.init(v_stride, a.d);
+    auto stage = [&](int t, auto i) {
+      const int n = t < tiles ? min(32, key1 - key0 - t * 32) : 0;
+      st_k.load(lds[i.value], buffer_over(kbase + (long long)t * 32 * a.k_tok, span_bytes(n, k_stride, row_bytes)));
+      st_v.load(lds[i.value] + TILE, buffer_over(vbase + (long long)t * 32 * a.v_tok, span_bytes(n, v_stride, row_bytes)));
+    };
+#pragma unroll
+    for (int v = 0; v < VC; ++v) acc[v] = f32x4{0.f, 0.f, 0.f, 0.f};
+    m = f32x4{-INFINITY, -INFINITY, -INFINITY, -INFINITY}, l = f32x4{0.f, 0.f, 0.f, 0.f};
+    auto work = [&](int t, auto i) {
+      const lds_ptr kt = lds[i.value], vt = kt + TILE;
+      const int key = key0 + 32 * t + (lane & 31);
+      f32x4 z[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
+      unrolled<0, DP / 8>([&](auto n) {
+        constexpr int C = n.value;
+        const f32x4 k = *(const DGNN_LDS f32x4 *)TL::at(kt, k_lane, 0, C);
+        unrolled<0, 4>([&](auto e) { z[e.value & 1] = mma4<3, 4 * (C & 1) + e.value>(q[C / 2], k[e.value], z[e.value & 1]); });
+      });
+      f32x4 p;
+      bool above = false;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const float s = z[0][r] + z[1][r], both = s + __shfl_xor(s, 32, 64);
+        p[r] = key <= last[r] ? both : -INFINITY;
+        above |= (p[r] - m[r]) * c > 8.f;
+      }
+      if (__any(above)) {                       // a reference near the maximum, as in AttnTile
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float top = wave_max(fmaxf(m[r], p[r])), by = top == m[r] ? 1.f : exp2_fast((m[r] - top) * c);
+          m[r] = top, l[r] *= by;
+#pragma unroll
+          for (int v = 0; v < VC; ++v) acc[v][r] *= by;
+        }
+      }
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const float mc = m[r] == -INFINITY ? 0.f : m[r] * c;
+        p[r] = exp2_fast(fmaf(p[r], c, -mc));
+        l[r] += p[r];
+      }
+      wave_lds_sync();
+      if (h == 0) *(DGNN_LDS f32x4 *)(turn + lane * 16) = p;
+      wave_lds_sync();
+      constexpr int KEYS = HALVES ? 16 : 32, GROUP = KEYS / 2;         // a lane's keys; of one register of weights
+      const lds_ptr own = turn + (HALVES ? 256 * h + lane % 32 * 4 : lane * 4);
+      const float w[2] = {*(const DGNN_LDS float *)own, *(const DGNN_LDS float *)(own + 16 * GROUP)};
+      unrolled<0, KEYS>([&](auto n) {
+        constexpr int K = n.value;
+        const lds_ptr at = TL::at(vt, v_lane, K, 0);
+        unrolled<0, VC>([&](auto v) {
+          acc[v.value] = mma4<HALVES ? 3 : 4, K % GROUP>(w[K / GROUP], *(const DGNN_LDS float *)(at + 4 * v.value), acc[v.value]);
+        });
+      });
+    };
+    ring<2, 2 * SG::LOADS, true>(tiles, stage, work);
+    if (HALVES) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) acc[0][r] += __shfl_xor(acc[0][r], 32, 64);
+    }
+  }
+  // the parts of the rows: {maximum, sum, -, -, output}
+  __device__ __forceinline__ void store(const AttnArgs &a, float *part, int rows) const {
+    const int lane = lane_id(), col = lane * VC;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const float sum = wave_sum(lane < 32 ? l[r] : 0.f);
+      if (r >= rows) continue;
+      float *to = part + r * (a.d + 4);
+      if (lane == 0) to[0] = m[r] == -INFINITY ? -INFINITY : m[r] * c, to[1] = sum;
+#pragma unroll
+      for (int v = 0; v < VC; ++v)
+        if (col + v < a.d) to[4 + col + v] = acc[v][r];             // (DP = 32: d is at most 32)
+    }
+  }
+};
+
 // Single queries and poolings, bound by reading the keys and values: a sequence's first a.few packed rows of a key head are split over chunks of
 // a.chunk keys, one wave a chunk, which reads its keys and values once for all query heads of the key
 // head; k_attn_join puts the parts together.  Part (slot, key head) holds {output row, maximum, sum} of
 // each of the rows.  What rows a sequence has beyond those are dealt to its chunks' workgroups in
 // tiles of 32, unsplit.  Two buffers of 32 keys and values: four waves a compute unit keep more loads in flight than
 // two with four buffers (9 sequences of 32768 keys, 32 / 8 heads of 128, bfloat16: 230 us against 245, 5.2 TB/s).
-template <class T, int DP>
+template <class T, int DP, bool FOUR>
 __global__ __launch_bounds__(64, sizeof(T) == 2 ? 2 : 1) void k_attn_split(const AttnArgs a) {
   using AT = AttnTile<T, DP, 1, 32, 2>;
   DGNN_RING(lds, AT::BYTES);
@@ -193,12 +322,21 @@ __global__ __launch_bounds__(64, sizeof(T) == 2 ? 2 : 1) void k_attn_split(const
   other_side(a.row_ptr, a.col_ptr, a.nseq, a.tq, seg, &qs, &lq);
   const long long rows = (long long)lq * a.g;
   const int chunks = (seg.len + a.chunk - 1) / a.chunk;
+  float *part = a.part + ((long long)slot * a.hk + kvh) * a.few * (a.d + 4);
   AT t;
-  if (rows > 0) {
+  if constexpr (FOUR) {
+    __shared__ __align__(16) char turn[512];
+    if (rows > 0) {
+      AttnFour<DP> f;
+      const int n = (int)min(rows, 4LL);
+      f.run(a, lds, (lds_ptr)turn, qs, lq, seg.start, seg.len, kvh, n, seg.tile * a.chunk, min(seg.len, (seg.tile + 1) * a.chunk));
+      f.store(a, part, n);
+    }
+  } else if (rows > 0) {
     t.run(a, lds, qs, lq, seg.start, seg.len, kvh, 0, min(rows, (long long)a.few), seg.tile * a.chunk,
           min(seg.len, (seg.tile + 1) * a.chunk));
     if (t.valid) {
-      float *part = a.part + (((long long)slot * a.hk + kvh) * a.few + (lane & 31)) * (a.d + 4);
+      part += (lane & 31) * (a.d + 4);
       store_row<float, DP>(part + 4, t.acc, 1.f, a.d, h);
       if (h == 0) part[0] = t.m == -INFINITY ? -INFINITY : t.m * t.c, part[1] = t.l;
     }
@@ -282,7 +420,12 @@ template <class T, int DP>
 static int launch_fwd(const AttnArgs &a, const AttnPlan &p, hipStream_t st) {
   if (p.few > 0) {
     if (p.slots * a.hk > 0x7fffffffLL) return DGNN_ERR_UNSUPPORTED;
-    hipLaunchKernelGGL((k_attn_split<T, DP>), dim3((unsigned)(p.slots * a.hk)), dim3(64), 0, st, a);
+    const dim3 grid((unsigned)(p.slots * a.hk));
+    const bool four = sizeof(T) == 4 && p.few == 4;
+    if constexpr (sizeof(T) == 4) {
+      if (four) hipLaunchKernelGGL((k_attn_split<T, DP, true>), grid, dim3(64), 0, st, a);
+    }
+    if (!four) hipLaunchKernelGGL((k_attn_split<T, DP, false>), grid, dim3(64), 0, st, a);
     DGNN_LAUNCH_CHECK();
     const long long rows = (long long)a.tq * a.hq;
     hipLaunchKernelGGL(k_attn_join<T>, dim3((unsigned)((rows + DGNN_WAVES_PER_BLOCK - 1) / DGNN_WAVES_PER_BLOCK)),

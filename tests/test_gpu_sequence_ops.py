@@ -265,6 +265,17 @@ def test_attention_few_rows_long_keys(hq, hk, d, causal, dtype):
     attention_case([1], [4000], hq, hk, d, causal, dtype)
 
 
+@pytest.mark.parametrize("scale", [None, -0.3, 0.0], ids=["scale", "negative", "zero"])
+@pytest.mark.parametrize("causal", [False, True], ids=["full", "causal"])
+@pytest.mark.parametrize("hq,hk,d", [(4, 1, 128), (6, 3, 100), (3, 3, 64), (8, 2, 33), (4, 4, 20)])
+def test_attention_four_rows_of_floats(hq, hk, d, causal, scale):
+    """The split forward of at most four rows a sequence on average: fewer rows, more rows, none, ragged keys."""
+    lq, lk = [1, 1, 0, 1, 1, 1, 1], [300, 31, 257, 0, 2049, 1, 1000]
+    attention_case(lq, lk, hq, hk, d, causal, torch.float32, front=1, back=3, poison=True, scale=scale, grads=False)
+    if hq == hk:
+        attention_case([9, 0, 1, 2], [700, 512, 640, 5], hq, hk, d, causal, torch.float32, scale=scale)
+
+
 @pytest.mark.parametrize("dtype", DTYPES, ids=ids_of)
 @pytest.mark.parametrize("rows,keys", [(128, 128), (64, 64), (32, 32), (1, 256), (1, 512)])
 def test_attention_equal_lengths(rows, keys, dtype):
