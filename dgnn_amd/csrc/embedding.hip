@@ -541,6 +541,7 @@ int dgnn_embedding_backward(int dtype, int idx_bytes, int n, int rows, int dim, 
                             const void *grad, void *grad_table, void *workspace, size_t workspace_bytes, void *stream) {
   int rc = embed_check(dtype, idx_bytes, n, rows, dim);
   if (rc != DGNN_OK) return rc;
+  if (n > (1 << 30)) return DGNN_ERR_UNSUPPORTED;            // positions and steps past them are ints
   if (rows == 0 || dim == 0) return DGNN_OK;
   if (!grad_table || (n > 0 && (!ids || !grad))) return DGNN_ERR_BAD_ARG;
   const int size = dtype == DGNN_F32 ? 4 : 2;

@@ -499,7 +499,8 @@ int dgnn_gat_epilogue_backward(int n, int hf, int activation, float act_param, c
 int dgnn_embedding_forward(int dtype, int idx_bytes, int n, int rows, int dim, float scale, const void *ids,
                            const void *table, void *out, void *stream);
 /* grad_table [rows,dim] = scale * sum of grad[i,:] over the i that name the row, in ascending i; fully
- * written (rows nobody names: zeros).  Deterministic: a stable sort of the ids, no float atomics. */
+ * written (rows nobody names: zeros).  Deterministic: a stable sort of the ids, no float atomics.
+ * n > 2^30: DGNN_ERR_UNSUPPORTED. */
 size_t dgnn_embedding_backward_workspace_bytes(int n, int rows, int dim);
 int dgnn_embedding_backward(int dtype, int idx_bytes, int n, int rows, int dim, float scale, const void *ids,
                             const void *grad, void *grad_table, void *workspace, size_t workspace_bytes, void *stream);

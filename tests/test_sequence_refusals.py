@@ -73,6 +73,7 @@ def embed_bwd(dtype=0, idx=8, n=4, rows=5, dim=6, ids=P, grad=P, out=P, ws=P, ws
     (embed_bwd, dict(ids=None), BAD_ARG), (embed_bwd, dict(grad=None), BAD_ARG), (embed_bwd, dict(out=None), BAD_ARG),
     (embed_bwd, dict(ws=None), WORKSPACE), (embed_bwd, dict(wsb=100), WORKSPACE), (embed_bwd, dict(ws=P + 4), ALIGNMENT),
     (embed_bwd, dict(grad=P + 1), ALIGNMENT), (embed_bwd, dict(dtype=-1), BAD_ARG),
+    (embed_bwd, dict(n=(1 << 30) + 1), UNSUPPORTED),
 ])
 def test_embedding_refuses(call, change, code):
     assert call(**change) == code
