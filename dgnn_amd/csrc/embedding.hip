@@ -22,6 +22,19 @@ struct __align__(sizeof(T) * N) Pack {
   T v[N];
 };
 
+// PAST: around the caches (accesses of 16 bytes)
+template <bool PAST, class T, int N>
+__device__ __forceinline__ void store_pack(T *to, const Pack<T, N> &p) {
+  if constexpr (PAST) {
+    typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+    u32x4 v;
+    __builtin_memcpy(&v, &p, 16);
+    __builtin_nontemporal_store(v, (u32x4 *)to);
+  } else {
+    *(Pack<T, N> *)to = p;
+  }
+}
+
 template <class I>
 __device__ __forceinline__ int row_of_id(const I *ids, long long i, int rows) {
   const I x = ids[i];
@@ -29,7 +42,7 @@ __device__ __forceinline__ int row_of_id(const I *ids, long long i, int rows) {
 }
 
 // lanes = threads that share a row (a power of two up to 256).  65536 ids of 1024 bfloat16 45 us, 5.9 TB/s; 196611 of
-// 100 floats, from 2.4 million rows, 36 us, 4.4 TB/s (a large copy: 5.1).
+// 100 floats, from 2.4 million rows, 24 - 36 us, 4.4 TB/s and more (a large copy: 5.1).
 template <class T, int N, class I>
 __global__ __launch_bounds__(DGNN_BLOCK) void k_embed_fwd(int n, int rows, int dim, int lanes, float scale,
                                                           const I *__restrict__ ids, const T *__restrict__ table,
@@ -257,7 +270,7 @@ __device__ __forceinline__ int first_not_below_wave(const int *__restrict__ key,
 // sum per piece it touches: slot 2 p when its run holds the first position of piece p, slot 2 p + 1
 // when it begins inside (and leaves through the end).  Whether a run crosses shows in the keys next to the
 // borders, so nothing is searched.  64 N columns and one piece a workgroup, its positions dealt to four waves.
-// 65536 ids of 1024 bfloat16, most of them frequent ones, 28 us (about 4 TB/s); 196611 of 100 floats 21 us,
+// 65536 ids of 1024 bfloat16, most of them frequent ones, 28 us (about 4 TB/s); 196611 of 100 floats 14 us,
 // waiting for key, position and row one after the other.
 template <class T, int N>
 __global__ __launch_bounds__(DGNN_BLOCK) void k_embed_cross(int n, int rows, int dim, int run,
@@ -313,9 +326,11 @@ constexpr int EMBED_ROWS = 256;      // most rows of the table a workgroup write
 
 // A workgroup writes `per_block` consecutive rows.  It finds the sorted positions that name them, marks
 // where each row's run begins and ends, stores zeros to the rows without one as one stream of pieces, and
-// gives every other row to `lanes` threads.  2.4 million rows of 100 floats, of which few are named, 231 us, 4.6 TB/s;
-// 50000 rows of 1024 bfloat16 63 us, 3.7 TB/s: the runs there are a few positions long, each a wait of its own.
-template <class T, int N>
+// gives every other row to `lanes` threads.  A table larger than the 256 MB of cache (PAST) is written around it, so
+// that keys and gradients stay in: 2.4 million rows of 100 floats, of which few are named, 203 us, 5.2 TB/s,
+// against 231, and the kernels next to it find more in the caches (the whole step 302 and 339 us).  50000 rows of 1024 bfloat16 63 us, 3.7 TB/s: the runs there are a few positions long, each a
+// wait of its own.
+template <class T, int N, bool PAST>
 __global__ __launch_bounds__(DGNN_BLOCK) void k_embed_rows(int n, int rows, int dim, int lanes, int per_block, int run, float scale,
                                                            const int *__restrict__ key, const int *__restrict__ val,
                                                            const T *__restrict__ grad, const float *__restrict__ part,
@@ -380,7 +395,7 @@ __global__ __launch_bounds__(DGNN_BLOCK) void k_embed_rows(int n, int rows, int 
       Pack<T, N> p;
 #pragma unroll
       for (int j = 0; j < N; ++j) p.v[j] = (T)(acc[j] * scale);
-      *(Pack<T, N> *)(to + c) = p;
+      store_pack<PAST>(to + c, p);
     }
   }
   // last, so that the stores drain while the next workgroup searches
@@ -391,7 +406,7 @@ __global__ __launch_bounds__(DGNN_BLOCK) void k_embed_rows(int n, int rows, int 
     Pack<T, N> p;
 #pragma unroll
     for (int j = 0; j < N; ++j) p.v[j] = (T)0.f;
-    *(Pack<T, N> *)(out + (long long)row0 * dim + (long long)u * N) = p;
+    store_pack<PAST>(out + (long long)row0 * dim + (long long)u * N, p);
   }
 }
 
@@ -454,8 +469,11 @@ static int launch_embed_sums(int n, int rows, int dim, float scale, const EmbedP
   // as many rows a workgroup as make up for its search, but a thousand workgroups where the rows allow it
   int per_block = groups * 16 > EMBED_ROWS / 2 ? EMBED_ROWS : groups * 16;
   if (per_block > (rows + 1023) / 1024) per_block = (rows + 1023) / 1024 > groups ? (rows + 1023) / 1024 : groups;
-  hipLaunchKernelGGL((k_embed_rows<T, N>), dim3((unsigned)((rows + (long long)per_block - 1) / per_block)), dim3(DGNN_BLOCK), 0, st, n,
-                     rows, dim, lanes, per_block, p.run, scale, key, val, (const T *)grad, part, (T *)out);
+  auto kernel = k_embed_rows<T, N, false>;
+  if constexpr (sizeof(T) * N == 16)
+    if ((double)rows * dim * sizeof(T) > 256e6) kernel = k_embed_rows<T, N, true>;
+  hipLaunchKernelGGL(kernel, dim3((unsigned)((rows + (long long)per_block - 1) / per_block)), dim3(DGNN_BLOCK), 0, st, n, rows, dim,
+                     lanes, per_block, p.run, scale, key, val, (const T *)grad, (const float *)part, (T *)out);
   DGNN_LAUNCH_CHECK();
   return DGNN_OK;
 }
