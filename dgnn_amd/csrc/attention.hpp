@@ -10,7 +10,7 @@ struct AttnArgs {
   const void *q, *k, *v, *out, *grad;         // grad: of the output
   void *o, *dq, *dk, *dv;
   void *rest;                                 // [tq, hq, d], what rounding took from the output (may be NULL)
-  float *lse;                                 // [hq, tq], natural logarithm
+  float *lse;                                 // [hq, tq], natural logarithm (backward: read)
   float *stat;                                // backward: [hq, tq] pairs {lse log2(e) (+inf for an empty row), <grad, out>}
   float *part;                                // partial rows (split forward) or gradients (split backward)
   int few, chunk, splits;

@@ -15,40 +15,6 @@ using namespace dgnn;
 
 namespace dgnn {
 
-// stat[head][row] = {lse log2(e), <do, o>}, o with what its rounding took (`rest`): <do, v_j> - <do, o> cancels
-// in rows that see few keys, and half a step of a 16-bit o is all that was left of it; the first is +inf
-// where the row saw no key (p = exp2(z - inf) = 0).  One thread per 16-byte chunk, lanes of a row joined by
-// shuffles.  Bound by memory: 65536 tokens, 8 heads of 64, bfloat16 35 us, 5.8 TB/s.
-template <class T, int LPR>
-__global__ __launch_bounds__(DGNN_BLOCK) void k_attn_bwd_stat(long long rows, int d, int tq, int hq,
-                                                              const T *__restrict__ out, const T *__restrict__ rest,
-                                                              const T *__restrict__ grad,
-                                                              const float *__restrict__ lse, float2 *__restrict__ stat) {
-  constexpr int VEC = 16 / sizeof(T);
-  const long long r = (blockIdx.x * (long long)DGNN_BLOCK + threadIdx.x) / LPR;
-  const int c = (threadIdx.x % LPR) * VEC;
-  float sum = 0.f;
-  if (r < rows && c < d) {
-    T o[VEC], g[VEC];
-    *(u32x4 *)o = *(const u32x4 *)(out + r * d + c);
-    *(u32x4 *)g = *(const u32x4 *)(grad + r * d + c);
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) sum = fmaf((float)o[j], (float)g[j], sum);
-    if (rest != nullptr) {
-      *(u32x4 *)o = *(const u32x4 *)(rest + r * d + c);
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) sum = fmaf((float)o[j], (float)g[j], sum);
-    }
-  }
-#pragma unroll
-  for (int w = LPR / 2; w > 0; w >>= 1) sum += __shfl_xor(sum, w, 64);
-  if (r < rows && threadIdx.x % LPR == 0) {
-    const long long tok = r / hq, head = r % hq, at = head * tq + tok;
-    const float x = lse[at];
-    stat[at] = make_float2(x == -INFINITY ? INFINITY : x * DGNN_LOG2E, sum);
-  }
-}
-
 // Rows of a staged tile: 32, or 64 where 32 are too few bytes for one load of every wave.
 template <class T, int DP, int NW>
 constexpr int bwd_rows() { return 32 * DP * (int)sizeof(T) >= 1024 * NW ? 32 : 64; }
@@ -210,7 +176,8 @@ __global__ __launch_bounds__(DGNN_BLOCK) void k_attn_bwd_join(const AttnArgs a) 
 }
 
 // The same with the sides changed, as the forward: a lane has one packed query row.  At the sizes above 0.40 - 0.48 ms,
-// 0.74 ms (1010 TFLOP/s) and 41 us.
+// 0.74 ms (1010 TFLOP/s) and 41 us.  It runs first and leaves {lse log2(e), <do, o>} of every row for the
+// other: a kernel of its own for them read grad a second time, 35 to 48 us of the first two steps, 9 of the last.
 template <class T, int DP, int NW, int HW, int S>
 __global__ __launch_bounds__(64 * NW * HW, sizeof(T) == 2 ? 2 : 1) void k_attn_bwd_q(const AttnArgs a) {
   constexpr int BM = 32 * NW, BN = bwd_rows<T, DP, NW>(), THREADS = 64 * NW;
@@ -246,8 +213,27 @@ __global__ __launch_bounds__(64 * NW * HW, sizeof(T) == 2 ? 2 : 1) void k_attn_b
   frag8<T> qf[DP / 16], gf[DP / 16];
   load_row_frags<T, DP>(qf, (const T *)a.q + tok * a.q_tok + (long long)head * a.q_head, a.d, h, valid);
   load_row_frags<T, DP>(gf, (const T *)a.grad + (tok * a.hq + head) * a.d, a.d, h, valid);
-  const float2 stat = valid ? ((const float2 *)a.stat)[(long long)head * a.tq + tok] : make_float2(INFINITY, 0.f);
-  const float lse = stat.x, delta = stat.y;
+  // <do, o>, o with what its rounding took (`rest`): <do, v_j> - <do, o> cancels in rows that see few keys, and half a
+  // step of a 16-bit o is all that was left of it
+  float delta = 0.f;
+  {
+    const long long at = (tok * a.hq + head) * a.d;
+    frag8<T> o[DP / 16];
+    auto add = [&](const void *from) {
+      load_row_frags<T, DP>(o, (const T *)from + at, a.d, h, valid);
+#pragma unroll
+      for (int s = 0; s < DP / 16; ++s)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) delta = fmaf((float)o[s][j], (float)gf[s][j], delta);
+    };
+    add(a.out);
+    if (a.rest != nullptr) add(a.rest);
+    delta += __shfl_xor(delta, 32, 64);
+  }
+  // a row that saw no key: p = exp2(z - inf) = 0
+  float lse = valid ? a.lse[(long long)head * a.tq + tok] : -INFINITY;
+  lse = lse == -INFINITY ? INFINITY : lse * DGNN_LOG2E;
+  if (valid && h == 0) ((float2 *)a.stat)[(long long)head * a.tq + tok] = make_float2(lse, delta);
   const float c = a.scale * DGNN_LOG2E;
 
   const unsigned k_stride = (unsigned)(a.k_tok * sizeof(T)), v_stride = (unsigned)(a.v_tok * sizeof(T));
@@ -337,32 +323,23 @@ static int launch_bwd_q(const AttnArgs &a, hipStream_t st) {
   return DGNN_OK;
 }
 template <class T, int DP>
-static int launch_bwd(const AttnArgs &a, const float *lse, hipStream_t st) {
-  const long long rows = (long long)a.tq * a.hq;
+static int launch_bwd(const AttnArgs &a, hipStream_t st) {
   int rc = DGNN_OK;
-  if (rows > 0) {
-    constexpr int LPR = DP * (int)sizeof(T) / 16;
-    const long long blocks = (rows * LPR + DGNN_BLOCK - 1) / DGNN_BLOCK;
-    if (blocks > 0x7fffffffLL) return DGNN_ERR_UNSUPPORTED;
-    hipLaunchKernelGGL((k_attn_bwd_stat<T, LPR>), dim3((unsigned)blocks), dim3(DGNN_BLOCK), 0, st, rows, a.d, a.tq, a.hq,
-                       (const T *)a.out, (const T *)a.rest, (const T *)a.grad, lse, (float2 *)a.stat);
-    DGNN_LAUNCH_CHECK();
-  }
-  if (a.tk > 0) {
-    if (a.splits > 1 || !rows_short(a.tk, a.nseq, 1)) rc = launch_bwd_kv<T, DP, 4, 1, 4>(a, st);
-    else rc = a.hk >= 4 ? launch_bwd_kv<T, DP, 1, 4, 1>(a, st) : launch_bwd_kv<T, DP, 1, 1, 1>(a, st);
-  }
-  if (rc == DGNN_OK && a.tq > 0) {
+  if (a.tq > 0) {
     if (!rows_short(a.tq, a.nseq, a.g)) rc = launch_bwd_q<T, DP, 4, 1, 4>(a, st);
     else rc = a.hk >= 4 ? launch_bwd_q<T, DP, 1, 4, 1>(a, st) : launch_bwd_q<T, DP, 1, 1, 1>(a, st);
+  }
+  if (rc == DGNN_OK && a.tk > 0) {
+    if (a.splits > 1 || !rows_short(a.tk, a.nseq, 1)) rc = launch_bwd_kv<T, DP, 4, 1, 4>(a, st);
+    else rc = a.hk >= 4 ? launch_bwd_kv<T, DP, 1, 4, 1>(a, st) : launch_bwd_kv<T, DP, 1, 1, 1>(a, st);
   }
   return rc;
 }
 template <class T>
-static int launch_bwd_d(const AttnArgs &a, const float *lse, hipStream_t st) {
-  if (a.d <= 32) return launch_bwd<T, 32>(a, lse, st);
-  if (a.d <= 64) return launch_bwd<T, 64>(a, lse, st);
-  return launch_bwd<T, 128>(a, lse, st);
+static int launch_bwd_d(const AttnArgs &a, hipStream_t st) {
+  if (a.d <= 32) return launch_bwd<T, 32>(a, st);
+  if (a.d <= 64) return launch_bwd<T, 64>(a, st);
+  return launch_bwd<T, 128>(a, st);
 }
 
 }  // namespace dgnn
@@ -390,14 +367,14 @@ int dgnn_attn_backward(int dtype, int nseq, int tq, int tk, int hq, int hk, int 
   if (workspace_bytes < dgnn_attn_backward_workspace_bytes(nseq, tq, tk, hq, hk, d) || (tq > 0 && !workspace)) return DGNN_ERR_WORKSPACE;
   if (((uintptr_t)workspace & 15) || ((uintptr_t)lse & 3)) return DGNN_ERR_ALIGNMENT;
   if ((long long)hq * d * (dtype == DGNN_F32 ? 4 : 2) >= (1LL << 31) / 128) return DGNN_ERR_UNSUPPORTED;
-  a.out = out, a.rest = (void *)out_rest, a.grad = grad, a.dq = dq, a.dk = dk, a.dv = dv;
+  a.out = out, a.lse = (float *)lse, a.rest = (void *)out_rest, a.grad = grad, a.dq = dq, a.dk = dk, a.dv = dv;
   a.stat = (float *)workspace;
   a.splits = bwd_splits(nseq, tq, tk, hq, hk);
   a.part = (float *)((char *)workspace + align256(2 * sizeof(float) * (size_t)tq * (size_t)hq));
   hipStream_t st = (hipStream_t)stream;
-  if (dtype == DGNN_F32) return launch_bwd_d<float>(a, lse, st);
-  if (dtype == DGNN_BF16) return launch_bwd_d<bf16_t>(a, lse, st);
-  return launch_bwd_d<half_t>(a, lse, st);
+  if (dtype == DGNN_F32) return launch_bwd_d<float>(a, st);
+  if (dtype == DGNN_BF16) return launch_bwd_d<bf16_t>(a, st);
+  return launch_bwd_d<half_t>(a, st);
 }
 
 }  // extern "C"
