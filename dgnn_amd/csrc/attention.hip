@@ -162,7 +162,8 @@ template <class T, int DP, int NW, int HW, int BN, int S>
 __global__ __launch_bounds__(64 * NW * HW, sizeof(T) == 2 ? 2 : 1) void k_attn_fwd(const AttnArgs a) {
   using AT = AttnTile<T, DP, NW, BN, S>;
   DGNN_RING(all, HW * AT::BYTES);
-  const HeadSlot at = head_slot<HW>(a.hk, a.nseq, 1);
+  const int splits = NW > 1 ? a.splits : 1;
+  const HeadSlot at = head_slot<HW>(a.hk, a.nseq, splits);
   if (at.head >= a.hk) return;
   const int kvh = at.head;
   const lds_ptr lds[4] = {all[0] + at.wave * AT::BYTES, all[1] + at.wave * AT::BYTES, all[2] + at.wave * AT::BYTES, all[3] + at.wave * AT::BYTES};
@@ -170,9 +171,46 @@ __global__ __launch_bounds__(64 * NW * HW, sizeof(T) == 2 ? 2 : 1) void k_attn_f
   if (seg.tile < 0) return;
   int ks, lk;
   other_side(a.col_ptr, a.row_ptr, a.nseq, a.tk, seg, &ks, &lk);
+  const long long row0 = (long long)seg.tile * 32 * NW, rows = (long long)seg.len * a.g;
+  int key0 = 0, key1 = lk;
+  if (NW > 1 && splits > 1) {                   // an equal share of the keys that the tile's last row sees
+    const int seen = a.causal ? min(lk, (int)((min(rows, row0 + 32 * NW) - 1) / a.g) + lk - seg.len + 1) : lk;
+    const int per = ((max(seen, 0) + BN - 1) / BN + splits - 1) / splits * BN;
+    key0 = uniform_i32(min(at.split * per, lk)), key1 = uniform_i32(min(lk, key0 + per));
+  }
   AT t;
-  t.run(a, lds, seg.start, seg.len, ks, lk, kvh, (long long)seg.tile * 32 * NW, (long long)seg.len * a.g, 0, lk);
-  t.finish(a, lk);
+  t.run(a, lds, seg.start, seg.len, ks, lk, kvh, row0, rows, key0, key1);
+  if (NW == 1 || splits == 1) {
+    t.finish(a, lk);
+    return;
+  }
+  if (!t.valid) return;
+  float *part = a.part + (((long long)at.split * a.tq + t.tok) * a.hq + t.head) * (a.d + 4);
+  store_row<float, DP>(part + 4, t.acc, 1.f, a.d, lane_id() >> 5);
+  if (lane_id() < 32) part[0] = t.m == -INFINITY ? -INFINITY : t.m * t.c, part[1] = t.l, part[2] = t.limit >= 0 && lk > 0 ? 1.f : 0.f;
+}
+// out and lse from the splits' {maximum, sum, whether the row sees a key, -, output}, in order.  One wave a row.
+template <class T>
+__global__ __launch_bounds__(DGNN_BLOCK) void k_attn_merge(const AttnArgs a) {
+  const int lane = lane_id();
+  const long long r = (long long)blockIdx.x * DGNN_WAVES_PER_BLOCK + uniform_i32(wave_in_block()), stride = (long long)a.tq * a.hq * (a.d + 4);
+  if (r >= (long long)a.tq * a.hq) return;
+  const float *part = a.part + r * (a.d + 4);
+  float top = -INFINITY, sum = 0.f;
+  for (int j = 0; j < a.splits; ++j) top = fmaxf(top, part[j * stride]);
+  const float base = top == -INFINITY ? 0.f : top;
+  for (int j = 0; j < a.splits; ++j) sum = fmaf(part[j * stride + 1], exp2_fast(part[j * stride] - base), sum);
+  const bool any = part[2] != 0.f;
+  T *out = (T *)a.o + r * a.d;
+  for (int c = lane; c < a.d; c += 64) {
+    float x = 0.f;
+    for (int j = 0; j < a.splits; ++j) x = fmaf(part[j * stride + 4 + c], exp2_fast(part[j * stride] - base), x);
+    x = any ? x / sum : 0.f;
+    out[c] = (T)x;
+    if (a.rest != nullptr) ((T *)a.rest)[r * a.d + c] = (T)(x - (float)(T)x);
+  }
+  if (a.lse != nullptr && lane == 0)
+    a.lse[r % a.hq * a.tq + r / a.hq] = any ? (base + __builtin_amdgcn_logf(sum)) * DGNN_LN2 : -INFINITY;
 }
 
 // ------------------------------------------------------------------ few rows, long keys
@@ -392,14 +430,24 @@ __global__ __launch_bounds__(DGNN_BLOCK) void k_attn_join(const AttnArgs a) {
 // chunk is a 2048th of all keys times heads (9 x 32768: half of it 242 us, twice 272), within 256 .. 2048.
 struct AttnPlan {
   int few, chunk;                       // split: rows kept in parts, keys of a chunk (few = 0: not split)
+  int splits;                           // tiles of rows: into how many parts the keys are split
   long long slots;
   size_t bytes;
 };
 static AttnPlan attn_plan(int nseq, int tq, int tk, int hq, int hk, int d) {
-  AttnPlan p = {0, 0, 0, 0};
+  AttnPlan p = {0, 0, 1, 0, 0};
   const long long g = hq / hk, rows = nseq > 0 ? ((long long)tq * g + nseq - 1) / nseq : 0;     // of a sequence, on average
   const long long keys = nseq > 0 ? tk / nseq : 0;
-  if (rows == 0 || rows > 32 || keys < 256) return p;
+  if (rows == 0) return p;
+  if (rows > 32) {
+    const long long tiles = ((long long)tq * g / 128 + nseq) * hk;
+    long long s = 512 / tiles;
+    if (s > keys / 512) s = keys / 512;
+    p.splits = (int)(s < 1 ? 1 : s > 16 ? 16 : s);
+    if (p.splits > 1) p.bytes = sizeof(float) * (size_t)p.splits * tq * hq * (d + 4);
+    return p;
+  }
+  if (keys < 256) return p;
   p.few = rows <= 4 ? 4 : rows <= 8 ? 8 : rows <= 16 ? 16 : 32;
   long long c = ((long long)tk * hk / 2048 + 63) / 64 * 64;
   p.chunk = (int)(c < 256 ? 256 : c > 2048 ? 2048 : c);
@@ -410,10 +458,16 @@ static AttnPlan attn_plan(int nseq, int tq, int tk, int hq, int hk, int d) {
 
 template <class T, int DP, int NW, int HW, int BN, int S>
 static int launch_rows(const AttnArgs &a, hipStream_t st) {
-  const long long groups = tile_slots(a.tq, a.nseq, a.g, 32 * NW) * ((a.hk + HW - 1) / HW);
+  const long long groups = tile_slots(a.tq, a.nseq, a.g, 32 * NW) * ((a.hk + HW - 1) / HW) * a.splits;
   if (groups > 0x7fffffffLL) return DGNN_ERR_UNSUPPORTED;
   hipLaunchKernelGGL((k_attn_fwd<T, DP, NW, HW, BN, S>), dim3((unsigned)groups), dim3(64 * NW * HW), 0, st, a);
   DGNN_LAUNCH_CHECK();
+  if (a.splits > 1) {
+    const long long rows = (long long)a.tq * a.hq;
+    hipLaunchKernelGGL(k_attn_merge<T>, dim3((unsigned)((rows + DGNN_WAVES_PER_BLOCK - 1) / DGNN_WAVES_PER_BLOCK)),
+                       dim3(DGNN_BLOCK), 0, st, a);
+    DGNN_LAUNCH_CHECK();
+  }
   return DGNN_OK;
 }
 template <class T, int DP>
@@ -433,7 +487,7 @@ static int launch_fwd(const AttnArgs &a, const AttnPlan &p, hipStream_t st) {
     DGNN_LAUNCH_CHECK();
     return DGNN_OK;
   }
-  if (!rows_short(a.tq, a.nseq, a.g)) return launch_rows<T, DP, 4, 1, 64, 2>(a, st);
+  if (p.splits > 1 || !rows_short(a.tq, a.nseq, a.g)) return launch_rows<T, DP, 4, 1, 64, 2>(a, st);
   return a.hk >= 4 ? launch_rows<T, DP, 1, 4, 32, 1>(a, st) : launch_rows<T, DP, 1, 1, 32, 1>(a, st);
 }
 template <class T>
@@ -501,7 +555,7 @@ int dgnn_attn_forward(int dtype, int nseq, int tq, int tk, int hq, int hk, int d
   a.o = out;
   a.rest = out_rest;
   a.lse = lse;
-  a.part = (float *)workspace, a.few = p.few, a.chunk = p.chunk;
+  a.part = (float *)workspace, a.few = p.few, a.chunk = p.chunk, a.splits = p.splits;
   hipStream_t st = (hipStream_t)stream;
   if (dtype == DGNN_F32) return launch_fwd_d<float>(a, p, st);
   if (dtype == DGNN_BF16) return launch_fwd_d<bf16_t>(a, p, st);

@@ -283,6 +283,16 @@ def test_attention_equal_lengths(rows, keys, dtype):
     attention_case([rows] * 71, [keys] * 71, 2, 1, 32, rows == 64, dtype, back=5)
 
 
+@pytest.mark.parametrize("dtype", DTYPES, ids=ids_of)
+@pytest.mark.parametrize("causal", [False, True], ids=["full", "causal"])
+@pytest.mark.parametrize("hq,hk,d", [(1, 1, 32), (6, 2, 64), (4, 1, 128), (3, 3, 41)])
+def test_attention_few_tiles_long_keys(hq, hk, d, causal, dtype):
+    """Tiles of rows whose keys are split and joined: ragged, no rows, fewer keys than rows, no keys."""
+    attention_case([140, 0, 300, 7, 90], [3000, 700, 1501, 5000, 40], hq, hk, d, causal, dtype, front=2, back=70, poison=True)
+    attention_case([1200, 33], [1200, 0], hq, hk, d, causal, dtype)
+    attention_case([70], [4097], hq, hk, d, causal, dtype, scale=-0.2, grads=False)
+
+
 def test_attention_many_small_graphs():
     lens = [(i * 7) % 40 for i in range(700)]
     attention_case(lens, lens, 1, 1, 32, False, torch.float32)
