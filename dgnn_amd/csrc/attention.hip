@@ -428,6 +428,12 @@ __global__ __launch_bounds__(DGNN_BLOCK) void k_attn_join(const AttnArgs a) {
 // queries of 1024 keys 20 and 42 us, 9 of 32768 keys 230 and 1374 us; where the sequences alone fill the card it costs
 // something (256 of 1024 keys 226 and 205 us), but a few long ones among short ones cost more the other way.  A
 // chunk is a 2048th of all keys times heads (9 x 32768: half of it 242 us, twice 272), within 256 .. 2048.
+//
+// More rows, but tiles of them for less than half of 512 workgroups: the keys of every tile are split into parts of
+// at least 512, by as many as fill those, and joined by k_attn_merge.  Split and unsplit: 4 x 64 rows against 16384
+// keys, 32 / 8 heads of 128, causal, bfloat16, 143 and 317 us; 512 rows against as many 194 and 313; 2 x 40 rows
+// against 3000 keys, 4 heads of 64, float 55 and 263 us; 2048 x 2048, 8 heads of 64, bfloat16 33 and 33, causal 31
+// and 33 (in three parts 36 and 30, 1024 workgroups 43 and 38).
 struct AttnPlan {
   int few, chunk;                       // split: rows kept in parts, keys of a chunk (few = 0: not split)
   int splits;                           // tiles of rows: into how many parts the keys are split
@@ -443,6 +449,7 @@ static AttnPlan attn_plan(int nseq, int tq, int tk, int hq, int hk, int d) {
     const long long tiles = ((long long)tq * g / 128 + nseq) * hk;
     long long s = 512 / tiles;
     if (s > keys / 512) s = keys / 512;
+    if (s < 4 && rows > 128 && s > keys / 1024) s = keys / 1024;     // many rows: writing the parts costs more
     p.splits = (int)(s < 1 ? 1 : s > 16 ? 16 : s);
     if (p.splits > 1) p.bytes = sizeof(float) * (size_t)p.splits * tq * hq * (d + 4);
     return p;
