@@ -239,7 +239,7 @@ struct AttnFour {
   __device__ __forceinline__ void run(const AttnArgs &a, const lds_ptr (&lds)[4], lds_ptr turn, int qs, int lq, int ks, int lk,
                                       int kvh, int rows, int key0, int key1) {
     const int lane = lane_id(), h = lane >> 5;
-    const int k_lane = TL::lane_addr(lane & 31, h * (DP / 8)), v_lane = HALVES ? TL::lane_addr(16 * h, (lane & 31) / 4) + lane % 4 * 4 : lane * VC * 4;
+    const int k_lane = TL::chunk_addr(lane & 31, h * (DP / 8)), v_lane = HALVES ? TL::chunk_addr(16 * h, (lane & 31) / 4) + lane % 4 * 4 : lane * VC * 4;
     const int shift = lk - lq;
     int last[4], seen = 0;
 #pragma unroll

@@ -663,8 +663,8 @@ struct CePlan {
 // Wide tiles halve what every product reads from LDS, but there have to be enough of them for 256 compute
 // units.  bfloat16, both directions with Wide and with Plain: 8192 x 50000 x 1024 3.64 and 4.16 ms (the forward
 // 874 and 956 us), 2048 x 50000 x 512 579 and 625 us.
-static CeShape ce_shape(int dtype, long long m, long long n, long long splits) {
-  const long long wide = ((m + 255) / 256) * ((n + 255) / 256) * splits;
+static CeShape ce_shape(int dtype, long long m, long long n) {
+  const long long wide = ((m + 255) / 256) * ((n + 255) / 256);
   return dtype != DGNN_F32 && wide >= 256 ? CE_WIDE : CE_PLAIN;
 }
 static CePlan ce_plan(int dtype, int n, int classes, int d, const void *x, const void *w) {
@@ -678,7 +678,7 @@ static CePlan ce_plan(int dtype, int n, int classes, int d, const void *x, const
   // up to about 1e9 operations finding the labelled rows costs more than scoring all: 4096 x 41 x 64 float 8.7 us
   // against 19, 1024 x 1000 x 256 bfloat16 14.6 against 19.5; 4096 x 1000 x 128 float 30.4 both
   p.all = !p.gather && 2.0 * n * classes * d <= 1e9;
-  p.z = classes <= 64 ? CE_NARROW : n <= 32 ? CE_THIN : ce_shape(dtype, classes, n, 1);
+  p.z = classes <= 64 ? CE_NARROW : n <= 32 ? CE_THIN : ce_shape(dtype, classes, n);
   const int class_tile = p.z == CE_NARROW ? 64 : p.z == CE_PLAIN ? 128 : 256;
   p.tiles = ceil_div(classes, class_tile);
   p.list = align256(sizeof(int) * ((size_t)n + 1));

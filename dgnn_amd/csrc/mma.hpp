@@ -27,7 +27,6 @@ typedef _Float16 half_t;
 typedef __bf16 bf16_t;
 typedef float acc16 __attribute__((ext_vector_type(16)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
-typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 
 // Pointers into LDS carry their address space: a generic pointer is only proven to be one where the
@@ -103,10 +102,9 @@ struct Tile {
   static constexpr int CPR = COLS / CHUNK;                   // chunks of a row
   static constexpr int ROW_BYTES = COLS * (int)sizeof(T);
   static_assert(CPR == 4 || CPR == 8 || CPR >= 16, "rows of at least four chunks");
-  __device__ static __forceinline__ int swizzle(int row) {
-    if (CPR >= 16) return ((row & 7) << 1) | ((row >> 3) & 1);
-    if (CPR == 8) return (((row >> 1) & 3) << 1) | ((row >> 3) & 1);
-    return (((row >> 2) & 1) << 1) | ((row >> 3) & 1);
+  __device__ static constexpr __forceinline__ int swizzle(int row) {
+    return CPR >= 16 ? ((row & 7) << 1) | ((row >> 3) & 1)
+           : CPR == 8 ? (((row >> 1) & 3) << 1) | ((row >> 3) & 1) : (((row >> 2) & 1) << 1) | ((row >> 3) & 1);
   }
   __device__ static __forceinline__ int chunk_addr(int row, int chunk) {
     return row * ROW_BYTES + ((chunk ^ swizzle(row)) << 4);
@@ -115,18 +113,13 @@ struct Tile {
   // bits of row and chunk, so where a row is the sum of a lane's and a constant row with no bit in common
   //   addr = (lane's row bytes | lane's chunk ^ swizzle) ^ (constant chunk ^ swizzle) + constant row bytes,
   // one exclusive or a read.
-  __device__ static __forceinline__ int lane_addr(int row, int chunk) { return chunk_addr(row, chunk); }
-  __device__ static constexpr __forceinline__ int const_swizzle(int row) {
-    return CPR >= 16 ? ((row & 7) << 1) | ((row >> 3) & 1)
-           : CPR == 8 ? (((row >> 1) & 3) << 1) | ((row >> 3) & 1) : (((row >> 2) & 1) << 1) | ((row >> 3) & 1);
-  }
   __device__ static __forceinline__ lds_ptr at(lds_ptr tile, int lane_part, int row, int chunk) {
-    return tile + (lane_part ^ ((const_swizzle(row) ^ chunk) << 4)) + row * ROW_BYTES;
+    return tile + (lane_part ^ ((swizzle(row) ^ chunk) << 4)) + row * ROW_BYTES;
   }
   // A lane's k elements of a product that sums over the columns: eight consecutive ones, of row
   // row0 + lane % 32 (row0 a multiple of 32) from column k0 + 8 (lane / 32).
   __device__ static __forceinline__ int row_lane(int lane) {
-    return lane_addr(lane & 31, (lane >> 5) * (8 / CHUNK));
+    return chunk_addr(lane & 31, (lane >> 5) * (8 / CHUNK));
   }
   __device__ static __forceinline__ frag8<T> row_frag(lds_ptr tile, int part, int row0, int k0) {
     if constexpr (sizeof(T) == 2) {
@@ -140,7 +133,7 @@ struct Tile {
   // The same in the order of the column reads below, columns k0 + 8 (j / 4) + 4 (lane / 32) + j % 4: the other
   // operand of a product with one of those.
   __device__ static __forceinline__ int row_lane_split(int lane) {
-    return sizeof(T) == 2 ? lane_addr(lane & 31, 0) + (lane >> 5) * 8 : lane_addr(lane & 31, lane >> 5);
+    return sizeof(T) == 2 ? chunk_addr(lane & 31, 0) + (lane >> 5) * 8 : chunk_addr(lane & 31, lane >> 5);
   }
   __device__ static __forceinline__ frag8<T> row_frag_split(lds_ptr tile, int part, int row0, int k0) {
     const vec4<T> a = *(const DGNN_LDS vec4<T> *)at(tile, part, row0, k0 / CHUNK);
@@ -153,8 +146,8 @@ struct Tile {
   // of row i / 4, columns 4 (i % 4) ...
   __device__ static __forceinline__ int col_lane(int lane) {
     if (sizeof(T) == 2)
-      return lane_addr(4 * (lane >> 5) + ((lane & 15) >> 2), 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) + (lane & 1) * 8;
-    return lane_addr(4 * (lane >> 5), (lane & 31) >> 2) + (lane & 3) * 4;
+      return chunk_addr(4 * (lane >> 5) + ((lane & 15) >> 2), 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) + (lane & 1) * 8;
+    return chunk_addr(4 * (lane >> 5), (lane & 31) >> 2) + (lane & 3) * 4;
   }
   __device__ static __forceinline__ frag8<T> col_frag(lds_ptr tile, int part, int row0, int col0) {
     if constexpr (sizeof(T) == 2) {
