@@ -169,6 +169,15 @@ def test_attention_layouts(layout, d, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=ids_of)
+@pytest.mark.parametrize("layout", ["heads", "last", "offset"])
+@pytest.mark.parametrize("d", [32, 64, 108])
+def test_attention_layouts_of_split_keys(layout, d, dtype):
+    """The same where the keys are split: single queries and few tiles of rows."""
+    attention_case([1, 2, 0], [600, 257, 300], 4, 2, d, True, dtype, layout=layout)
+    attention_case([100, 40], [2100, 900], 4, 2, d, True, dtype, layout=layout)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=ids_of)
 @pytest.mark.parametrize("causal", [False, True], ids=["full", "causal"])
 def test_attention_rows_of_no_sequence(causal, dtype):
     """Padding in front and behind: never read (it holds NaN and infinities), zeros come back."""
