@@ -11,7 +11,7 @@ struct AttnArgs {
   void *o, *dq, *dk, *dv;
   void *rest;                                 // [tq, hq, d], what rounding took from the output (may be NULL)
   float *lse;                                 // [hq, tq], natural logarithm (backward: read)
-  float *stat;                                // backward: [hq, tq] pairs {lse log2(e) (+inf for an empty row), <grad, out>}
+  float *stat;                                // backward: [hq, tq] pairs {lse log2(e) - p_shift (+inf for an empty row), <grad, out>}
   float *part;                                // partial rows (split forward) or gradients (split backward)
   int few, chunk, splits;
   const int *row_ptr, *col_ptr;

@@ -9,6 +9,13 @@
 // k_attn_bwd_q keeps 32 packed query rows a wave and walks the key tiles.  The price is forming z and
 // do v^T twice: seven products instead of five.  p and ds are rounded to T for the products that sum over
 // them, half a step each; everything else is float.
+//
+// float16 has neither the range for p of long rows nor for ds = p (<do, v> - delta), whose size is that of the incoming
+// gradient divided by the keys: from 2^-14 down every bit of size costs one of precision, below 2^-25 nothing is left
+// (4096 keys and gradients of 1e-4: three steps of the type).  p is therefore rounded as 2^12 p, and ds times a
+// power of two of the lane's own row (or key), lowered whenever a term outgrows it, like the softmax's running
+// maximum (DsScale); both come out of the float sums at the end.  It costs 4 % of a training step of 32 x 2048 tokens, 8
+// heads of 64 (1440 us, 1378 without).  bfloat16 has float's range.
 #include "attention.hpp"
 
 using namespace dgnn;
@@ -18,6 +25,39 @@ namespace dgnn {
 // Rows of a staged tile: 32, or 64 where 32 are too few bytes for one load of every wave.
 template <class T, int DP, int NW>
 constexpr int bwd_rows() { return 32 * DP * (int)sizeof(T) >= 1024 * NW ? 32 : 64; }
+
+template <class T> constexpr bool scaled() { return std::is_same<T, half_t>::value; }
+template <class T> constexpr float p_shift() { return scaled<T>() ? 12.f : 0.f; }        // p is kept times 2^p_shift
+
+// The running power of two of a lane's column of ds (lanes l and l + 32 share one).  It starts above any use, so that
+// the first terms set it: the largest term so far lies below 2^15, and was below 2^12 when the factor was set.
+template <bool ON>
+struct DsScale {
+  static constexpr float START = 0x1p60f;       // ds < 2^52 from float16 operands of 128 elements: no overflow
+  float by = ON ? START : 1.f;
+  // ds holds terms times `by`; sums are what was added up of such terms
+  template <int N>
+  __device__ __forceinline__ void fit(acc16 &ds, acc16 (&sums)[N]) {
+    if constexpr (ON) {
+      float top = 0.f;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) top = fmaxf(top, fabsf(ds[r]));
+      if (__any(top > 32768.f)) {
+        top = fmaxf(top, __shfl_xor(top, 32, 64));
+        // an infinite term stays infinite whatever the factor
+        const float change = top > 32768.f && top < INFINITY ? ldexpf(1.f, 12 - __builtin_amdgcn_frexp_expf(top)) : 1.f;
+        by *= change;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) ds[r] *= change;
+#pragma unroll
+        for (int b = 0; b < N; ++b)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) sums[b][r] *= change;
+      }
+    }
+  }
+  __device__ __forceinline__ float out() const { return ON ? 1.f / by : 1.f; }
+};
 
 // Long sequences: four waves with 32 keys each share the staged tiles of queries and do, a ring of four, since
 // two waves a SIMD (the accumulators' 256 registers) hide little by themselves.  Bound by the matrix instructions
@@ -37,9 +77,12 @@ __global__ __launch_bounds__(64 * NW * HW, sizeof(T) == 2 && (NW > 1 || DP < 128
   if (at.head >= a.hk) return;
   const lds_ptr lds[4] = {all[0] + at.wave * BYTES, all[1] + at.wave * BYTES, all[2] + at.wave * BYTES, all[3] + at.wave * BYTES};
   // Two waves a SIMD leave 256 registers; at DP = 128 the accumulators and both operands take 192, and the
-  // last fragments of k did not fit (a spill to memory whose wait drains the ring).  They live in LDS.
-  constexpr int PARK = DP == 128 && sizeof(T) == 2 && NW > 1 ? 2 : 0, KEPT = DP / 16 - PARK;
-  __shared__ __align__(16) char parked[PARK ? PARK * THREADS * 16 : 16];
+  // last fragments of k did not fit (a spill to memory whose wait drains the ring).  They live in LDS: two of them,
+  // three with the factor of ds, which is what half of a compute unit's LDS holds next to the ring.  At DP = 64 the factor
+  // would cost the third wave of a SIMD, and one of them lives there.
+  constexpr int PARK = DP == 128 && sizeof(T) == 2 && NW > 1 ? (scaled<T>() ? 3 : 2) : DP == 64 && scaled<T>() ? 1 : 0, KEPT = DP / 16 - PARK;
+  constexpr int PARKERS = THREADS * HW;
+  __shared__ __align__(16) char parked[PARK ? PARK * PARKERS * 16 : 16];
   const int lane = lane_id(), h = lane >> 5, wave = NW == 1 ? 0 : uniform_i32(wave_in_block());
   const int row_lane = TL::row_lane(lane), col_lane = TL::col_lane(lane);
   const int kvh = at.head, split = at.split;
@@ -65,7 +108,7 @@ __global__ __launch_bounds__(64 * NW * HW, sizeof(T) == 2 && (NW > 1 || DP < 128
   load_row_frags<T, DP>(kf, (const T *)a.k + tok * a.k_tok + (long long)kvh * a.k_head, a.d, h, valid);
   load_row_frags<T, DP>(vf, (const T *)a.v + tok * a.v_tok + (long long)kvh * a.v_head, a.d, h, valid);
 #pragma unroll
-  for (int k = KEPT; k < DP / 16; ++k) *(frag8<T> *)(parked + ((k - KEPT) * THREADS + threadIdx.x) * 16) = kf[k];
+  for (int k = KEPT; k < DP / 16; ++k) *(frag8<T> *)(parked + ((k - KEPT) * PARKERS + threadIdx.x) * 16) = kf[k];
   const float c = a.scale * DGNN_LOG2E;
 
   const unsigned q_stride = (unsigned)(a.q_tok * sizeof(T)), g_stride = (unsigned)((long long)a.hq * a.d * sizeof(T));
@@ -91,6 +134,7 @@ __global__ __launch_bounds__(64 * NW * HW, sizeof(T) == 2 && (NW > 1 || DP < 128
   acc16 dk[DP / 32], dv[DP / 32];
 #pragma unroll
   for (int b = 0; b < DP / 32; ++b) dk[b] = acc_zero(), dv[b] = acc_zero();
+  DsScale<scaled<T>()> ds_scale;
 
   int w_tile = s_tile;                                       // tile worked on
   auto work = [&](int, auto i) {
@@ -106,7 +150,7 @@ __global__ __launch_bounds__(64 * NW * HW, sizeof(T) == 2 && (NW > 1 || DP < 128
       acc16 s = acc_zero(), dp = acc_zero();
 #pragma unroll
       for (int k = 0; k < DP / 16; ++k) {
-        const frag8<T> kk = k < KEPT ? kf[k] : *(const frag8<T> *)(parked + ((k - KEPT) * THREADS + threadIdx.x) * 16);
+        const frag8<T> kk = k < KEPT ? kf[k] : *(const frag8<T> *)(parked + ((k - KEPT) * PARKERS + threadIdx.x) * 16);
         s = mma(TL::row_frag(qt, rl, 32 * qb, 16 * k), kk, s);
         dp = mma(TL::row_frag(gt, rl, 32 * qb, 16 * k), vf[k], dp);
       }
@@ -119,7 +163,7 @@ __global__ __launch_bounds__(64 * NW * HW, sizeof(T) == 2 && (NW > 1 || DP < 128
         for (int j = 0; j < 4; ++j) {
           const int r = 4 * r4 + j;
           s[r] = exp2_fast(fmaf(s[r], c, -ls[j]));
-          dp[r] = s[r] * (dp[r] - de[j]);
+          dp[r] = scaled<T>() ? s[r] * ds_scale.by * (dp[r] - de[j]) : s[r] * (dp[r] - de[j]);
         }
       }
       if (q0 < wave_all) {                      // the diagonal crosses this block
@@ -130,6 +174,7 @@ __global__ __launch_bounds__(64 * NW * HW, sizeof(T) == 2 && (NW > 1 || DP < 128
           dp[r] = seen ? dp[r] : 0.f;
         }
       }
+      ds_scale.fit(dp, dk);
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
         const frag8<T> p = frag_of<T>(s, 8 * k), ds = frag_of<T>(dp, 8 * k);
@@ -147,14 +192,15 @@ __global__ __launch_bounds__(64 * NW * HW, sizeof(T) == 2 && (NW > 1 || DP < 128
   const int lane2 = opaque(lane), key2 = key0 + (lane2 & 31);
   if (key2 >= lk) return;
   const long long to = ((seg.start + (long long)key2) * a.hk + kvh) * a.d;
+  const float of_p = scaled<T>() ? 1.f / (1 << (int)p_shift<T>()) : 1.f, of_ds = a.scale * of_p * ds_scale.out();
   if (a.splits > 1) {
     float *part = a.part + 2 * ((long long)split * a.tk * a.hk * a.d + to);
-    store_row<float, DP>(part, dk, a.scale, a.d, lane2 >> 5);
-    store_row<float, DP>(part + a.d, dv, 1.f, a.d, lane2 >> 5);
+    store_row<float, DP>(part, dk, of_ds, a.d, lane2 >> 5);
+    store_row<float, DP>(part + a.d, dv, of_p, a.d, lane2 >> 5);
     return;
   }
-  store_row<T, DP>((T *)a.dk + to, dk, a.scale, a.d, lane2 >> 5);
-  store_row<T, DP>((T *)a.dv + to, dv, 1.f, a.d, lane2 >> 5);
+  store_row<T, DP>((T *)a.dk + to, dk, of_ds, a.d, lane2 >> 5);
+  store_row<T, DP>((T *)a.dv + to, dv, of_p, a.d, lane2 >> 5);
 }
 
 // dk and dv of every (key, key head): the sum of the splits' {dk row, dv row}, in order
@@ -233,7 +279,7 @@ __global__ __launch_bounds__(64 * NW * HW, sizeof(T) == 2 ? 2 : 1) void k_attn_b
   // a row that saw no key: p = exp2(z - inf) = 0
   float lse = valid ? a.lse[(long long)head * a.tq + tok] : -INFINITY;
   lse = lse == -INFINITY ? INFINITY : lse * DGNN_LOG2E;
-  if (valid && h == 0) ((float2 *)a.stat)[(long long)head * a.tq + tok] = make_float2(lse, delta);
+  if (valid && h == 0) ((float2 *)a.stat)[(long long)head * a.tq + tok] = make_float2(lse - p_shift<T>(), delta);
   const float c = a.scale * DGNN_LOG2E;
 
   const unsigned k_stride = (unsigned)(a.k_tok * sizeof(T)), v_stride = (unsigned)(a.v_tok * sizeof(T));
@@ -252,6 +298,7 @@ __global__ __launch_bounds__(64 * NW * HW, sizeof(T) == 2 ? 2 : 1) void k_attn_b
   acc16 dq[DP / 32];
 #pragma unroll
   for (int b = 0; b < DP / 32; ++b) dq[b] = acc_zero();
+  DsScale<scaled<T>()> ds_scale;
 
   auto work = [&](int t, auto i) {
     const lds_ptr kt = lds[i.value], vt = kt + TILE;
@@ -267,11 +314,16 @@ __global__ __launch_bounds__(64 * NW * HW, sizeof(T) == 2 ? 2 : 1) void k_attn_b
         dp = mma(TL::row_frag(vt, rl, 32 * kb, 16 * k), gf[k], dp);
       }
 #pragma unroll
-      for (int r = 0; r < 16; ++r) dp[r] = exp2_fast(fmaf(s[r], c, -lse)) * (dp[r] - delta);
+      for (int r = 0; r < 16; ++r) {
+        // (a power of two: the same rounding as the difference's)
+        const float diff = scaled<T>() ? fmaf(dp[r], ds_scale.by, -delta * ds_scale.by) : dp[r] - delta;
+        dp[r] = exp2_fast(fmaf(s[r], c, -lse)) * diff;
+      }
       if (k0 + 31 > wave_all) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) dp[r] = k0 + acc_row(r, h) <= limit ? dp[r] : 0.f;
       }
+      ds_scale.fit(dp, dq);
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
         const frag8<T> ds = frag_of<T>(dp, 8 * k);
@@ -282,7 +334,7 @@ __global__ __launch_bounds__(64 * NW * HW, sizeof(T) == 2 ? 2 : 1) void k_attn_b
   };
   ring<S, 2 * SG::LOADS, NW == 1>(tiles, stage, work);
 
-  if (valid) store_row<T, DP>((T *)a.dq + (tok * a.hq + head) * a.d, dq, a.scale, a.d, h);
+  if (valid) store_row<T, DP>((T *)a.dq + (tok * a.hq + head) * a.d, dq, a.scale * ds_scale.out(), a.d, h);
 }
 
 // Into how many parts the query tiles of a key tile are split.  A key tile's workgroup walks the queries of

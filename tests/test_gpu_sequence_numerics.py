@@ -1,0 +1,67 @@
+"""Digits of the sequence operators where the tolerances of test_gpu_sequence_ops.py leave room for their loss: small
+and large gradients in float16, confident rows of the loss, long runs of one id, and what masked rows hold."""
+import math
+
+import pytest
+import torch
+
+import sequence_ref as ref
+from dgnn_amd.operators import LinearCrossEntropyFuse, NodeEmbeddingFuse, PackedAttentionFuse
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = [torch.float32, torch.bfloat16, torch.float16]
+DEV = "cuda:0"
+
+
+def ids_of(x):
+    return str(x).replace("torch.", "")
+
+
+def offsets(lens):
+    off = [0]
+    for n in lens:
+        off.append(off[-1] + n)
+    return off
+
+
+# ------------------------------------------------------------------------------------ float16 attention
+@pytest.mark.parametrize("size", [2.0 ** -18, 2.0 ** -13, 1.0, 2.0 ** 11], ids=["2^-18", "2^-13", "1", "2^11"])
+@pytest.mark.parametrize("lq,lk,hq,hk,d,causal", [([4173], [4173], 1, 1, 64, False), ([2000, 31], [2000, 31], 2, 1, 32, True),
+                                                  ([3, 1], [8192, 700], 2, 1, 128, False), ([60, 2, 33, 1], [60, 2, 33, 1], 4, 4, 64, False),
+                                                  ([300, 40], [900, 1500], 4, 2, 128, True)], ids=str)
+def test_float16_gradients_keep_their_digits(lq, lk, hq, hk, d, causal, size, monkeypatch):
+    """The bounds without an allowance of the type's smallest step for every pair of a row and a key: p and ds may be off
+    by half a step of their own size, whatever the size of the incoming gradient, and only the results by the
+    type's smallest.  Values equal the keys, so that dq is about scale * grad however many keys there are."""
+    gen = torch.Generator().manual_seed(7)
+    q_off, k_off = offsets(lq), offsets(lk)
+    k = torch.randn(k_off[-1], hk, d, generator=gen).half()
+    q = (torch.randn(q_off[-1], hq, d, generator=gen) * 0.25).half()
+    grad = (torch.randn(q_off[-1], hq, d, generator=gen) * size).half()
+    small = ref.tiny(torch.float16)
+    monkeypatch.setattr(ref, "tiny", lambda dtype: 0.0)
+    scale = 0.5
+    want = ref.attention(q, k, k, q_off, k_off, causal, scale, grad)
+    ptr = [torch.tensor(o, dtype=torch.int32, device=DEV) for o in (q_off, k_off)]
+    leaves = [t.to(DEV).requires_grad_() for t in (q, k, k)]
+    out = PackedAttentionFuse(*leaves, *ptr, causal=causal, scale=scale)
+    got = torch.autograd.grad(out, leaves, grad.to(DEV))
+    for name, x in zip(("dq", "dk", "dv"), got):
+        assert want[name][0].abs().max() < 60000                  # the results themselves have room
+        ref.check(x, (want[name][0], want[name][1] + small), name)
+
+
+def test_float16_gradients_of_large_terms():
+    """Terms past the type's end, 2^17, whose sums times the scale are inside it."""
+    gen = torch.Generator().manual_seed(8)
+    lens, d, scale = [2, 1, 37, 100], 128, 2.0 ** -6
+    off = offsets(lens)
+    q, k, v, grad = (torch.randn(off[-1], 2, d, generator=gen) for _ in range(4))
+    q, k, v, grad = (t.half() for t in (q, k, v * 16, grad * 2 ** 11))
+    want = ref.attention(q, k, v, off, off, False, scale, grad)
+    leaves = [t.to(DEV).requires_grad_() for t in (q, k, v)]
+    out = PackedAttentionFuse(*leaves, torch.tensor(off, dtype=torch.int32, device=DEV), scale=scale)
+    for name, x in zip(("dq", "dk", "dv"), torch.autograd.grad(out, leaves, grad.to(DEV))):
+        assert want[name][0].abs().max() < 60000
+        ref.check(x, want[name], name)
