@@ -31,6 +31,9 @@ struct AttnTile {
   using TL = Tile<T, DP>;
   using SG = Stager<T, DP, BN, 64 * NW>;
   static constexpr int TILE = BN * TL::ROW_BYTES, BYTES = 2 * TILE;
+  // log2 of the weight of a score at the reference.  float16: 7, weights then run up to 2^15 and lose nothing before 2^-21
+  // of it; at 0, 262144 keys 2^-26 below one other vanished in front of the second product, 0.4 % of the row's sum.
+  static constexpr float UP = std::is_same<T, half_t>::value ? 7.f : 0.f;
   static_assert(S == 1 || 2 * SG::LOADS * (S - 2) < 64, "loads in flight are counted in six bits");
 
   acc16 acc[DP / 32];
@@ -117,7 +120,7 @@ struct AttnTile {
         for (int r = 0; r < 16; ++r) top = fmaxf(top, s[b][r]);
       top = fmaxf(top, __shfl_xor(top, 32, 64));
       // m is a reference near the maximum, not the maximum itself: it moves only when a score exceeds it by more
-      // than 8 (in log2), so weights run up to 256, far from any type's end, and most tiles rescale nothing.
+      // than 8 (in log2), so weights run up to 256 (times 2^UP), far from any type's end, and most tiles rescale nothing.
       // With 32 rows a wave one of them has a new maximum in nearly every tile of some thousand keys.
       if (__any((top - m) * c > 8.f)) {
         const float by = top == m ? 1.f : exp2_fast((m - top) * c);     // m = -inf: 0
@@ -128,7 +131,7 @@ struct AttnTile {
 #pragma unroll
           for (int r = 0; r < 16; ++r) acc[b][r] *= by;
       }
-      const float mc = m == -INFINITY ? 0.f : m * c;
+      const float mc = m == -INFINITY ? 0.f : base();
 #pragma unroll
       for (int b = 0; b < BN / 32; ++b)
 #pragma unroll
@@ -147,6 +150,9 @@ struct AttnTile {
     l += __shfl_xor(l, 32, 64);
   }
 
+  // what the scores' exponents are relative to
+  __device__ __forceinline__ float base() const { return m * c - UP; }
+
   __device__ __forceinline__ void finish(const AttnArgs &a, int lk) const {
     if (!valid) return;
     const int h = lane_id() >> 5;
@@ -154,7 +160,7 @@ struct AttnTile {
     const long long to = (tok * a.hq + head) * a.d;
     store_row<T, DP>((T *)a.o + to, acc, none ? 0.f : 1.f / l, a.d, h, a.rest != nullptr ? (T *)a.rest + to : nullptr);
     if (a.lse != nullptr && h == 0)
-      a.lse[(long long)head * a.tq + tok] = none ? -INFINITY : (m * c + __builtin_amdgcn_logf(l)) * DGNN_LN2;
+      a.lse[(long long)head * a.tq + tok] = none ? -INFINITY : (base() + __builtin_amdgcn_logf(l)) * DGNN_LN2;
   }
 };
 
@@ -187,7 +193,7 @@ __global__ __launch_bounds__(64 * NW * HW, sizeof(T) == 2 ? 2 : 1) void k_attn_f
   if (!t.valid) return;
   float *part = a.part + (((long long)at.split * a.tq + t.tok) * a.hq + t.head) * (a.d + 4);
   store_row<float, DP>(part + 4, t.acc, 1.f, a.d, lane_id() >> 5);
-  if (lane_id() < 32) part[0] = t.m == -INFINITY ? -INFINITY : t.m * t.c, part[1] = t.l, part[2] = t.limit >= 0 && lk > 0 ? 1.f : 0.f;
+  if (lane_id() < 32) part[0] = t.m == -INFINITY ? -INFINITY : t.base(), part[1] = t.l, part[2] = t.limit >= 0 && lk > 0 ? 1.f : 0.f;
 }
 // out and lse from the splits' {maximum, sum, whether the row sees a key, -, output}, in order.  One wave a row.
 template <class T>
@@ -376,7 +382,7 @@ __global__ __launch_bounds__(64, sizeof(T) == 2 ? 2 : 1) void k_attn_split(const
     if (t.valid) {
       part += (lane & 31) * (a.d + 4);
       store_row<float, DP>(part + 4, t.acc, 1.f, a.d, h);
-      if (h == 0) part[0] = t.m == -INFINITY ? -INFINITY : t.m * t.c, part[1] = t.l;
+      if (h == 0) part[0] = t.m == -INFINITY ? -INFINITY : t.base(), part[1] = t.l;
     }
   }
   for (long long row0 = a.few + 32LL * seg.tile; row0 < rows; row0 += 32LL * chunks) {

@@ -65,3 +65,17 @@ def test_float16_gradients_of_large_terms():
     for name, x in zip(("dq", "dk", "dv"), torch.autograd.grad(out, leaves, grad.to(DEV))):
         assert want[name][0].abs().max() < 60000
         ref.check(x, want[name], name)
+
+
+def test_float16_weights_far_below_the_largest():
+    """One key 26 powers of two above 262143 others, in tiles of rows that see all keys in one pass.  Weights are kept in
+    steps of 2^-24 at 2^7 for the largest, so each of the others may be off by 2^-32 of it."""
+    rows, keys, d = 128 * 257, 1 << 18, 16
+    q = torch.zeros(rows, 1, d, dtype=torch.float16, device=DEV)
+    k = torch.zeros(keys, 1, d, dtype=torch.float16, device=DEV)
+    v = torch.ones(keys, 1, d, dtype=torch.float16, device=DEV)
+    q[:, :, 0], k[0, 0, 0], v[0] = 1, 18.015625, 0
+    ptr = [torch.tensor([0, n], dtype=torch.int32, device=DEV) for n in (rows, keys)]
+    out = PackedAttentionFuse(q, k, v, *ptr, scale=1.0).double()
+    want = (keys - 1) / (keys - 1 + math.exp(18.015625))
+    assert (out - want).abs().max() <= keys * 2.0 ** -32 + 2 * ref.half_step(torch.float16) * want
