@@ -153,10 +153,14 @@ struct AttnTile {
   // what the scores' exponents are relative to
   __device__ __forceinline__ float base() const { return m * c - UP; }
 
-  __device__ __forceinline__ void finish(const AttnArgs &a, int lk) const {
+  __device__ __forceinline__ void finish(const AttnArgs &a, int lk) {
     if (!valid) return;
     const int h = lane_id() >> 5;
     const bool none = limit < 0 || lk == 0;
+    if (none) {                                 // not by a factor: weights of zero times a NaN of a row nobody sees is one
+#pragma unroll
+      for (int b = 0; b < DP / 32; ++b) acc[b] = acc_zero();
+    }
     const long long to = (tok * a.hq + head) * a.d;
     store_row<T, DP>((T *)a.o + to, acc, none ? 0.f : 1.f / l, a.d, h, a.rest != nullptr ? (T *)a.rest + to : nullptr);
     if (a.lse != nullptr && h == 0)

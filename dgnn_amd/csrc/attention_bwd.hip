@@ -91,6 +91,9 @@ __global__ __launch_bounds__(64 * NW * HW, sizeof(T) == 2 && (NW > 1 || DP < 128
   int qs, lq;
   other_side(a.row_ptr, a.col_ptr, a.nseq, a.tq, seg, &qs, &lq);
   const int lk = seg.len;
+  // causal: the first rows of a sequence with more rows than keys see none; what they hold must not be read
+  const int blind = a.causal ? max(0, lq - lk) : 0;
+  qs += blind, lq -= blind;
 
   const int key0 = seg.tile * BK + wave * 32, key = key0 + (lane & 31);
   const bool valid = key < lk;
@@ -334,6 +337,10 @@ __global__ __launch_bounds__(64 * NW * HW, sizeof(T) == 2 ? 2 : 1) void k_attn_b
   };
   ring<S, 2 * SG::LOADS, NW == 1>(tiles, stage, work);
 
+  if (limit < 0) {                              // sees no key: no gradient, whatever the keys hold
+#pragma unroll
+    for (int b = 0; b < DP / 32; ++b) dq[b] = acc_zero();
+  }
   if (valid) store_row<T, DP>((T *)a.dq + (tok * a.hq + head) * a.d, dq, a.scale * ds_scale.out(), a.d, h);
 }
 

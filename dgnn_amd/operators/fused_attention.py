@@ -18,8 +18,9 @@ def PackedAttentionFuse(q, k, v, row_ptr, col_ptr=None, causal=False, scale=None
     scale defaults to dim ** -0.5.
 
     A row that sees no key (masked, empty sequence, in front of or behind the sequences) gives zeros and no
-    gradient.  Values do not cross sequences, not even NaN; inside one, a NaN or infinity in a key or
-    value may reach rows that the causal mask keeps from it, as a weight of zero times it does."""
+    gradient, whatever it and the keys hold.  Values do not cross sequences, not even NaN; inside one, a NaN or
+    infinity in a key or value may reach rows that the causal mask keeps from it (and one in a row or its
+    gradient the gradients of keys that it does not see), as a weight of zero times it does."""
     if scale is None:
         scale = q.size(-1) ** -0.5
     if col_ptr is None:

@@ -79,3 +79,38 @@ def test_float16_weights_far_below_the_largest():
     out = PackedAttentionFuse(q, k, v, *ptr, scale=1.0).double()
     want = (keys - 1) / (keys - 1 + math.exp(18.015625))
     assert (out - want).abs().max() <= keys * 2.0 ** -32 + 2 * ref.half_step(torch.float16) * want
+
+
+# ------------------------------------------------------------------------------------ rows that see no key
+@pytest.mark.parametrize("dtype", DTYPES, ids=ids_of)
+@pytest.mark.parametrize("lq,lk,hq,hk", [([100, 7], [40, 7], 4, 2), ([20, 3, 40], [5, 3, 0], 4, 4), ([9, 1, 1], [5, 1000, 700], 1, 1),
+                                         ([40, 1], [5, 900], 4, 2), ([700, 200], [100, 9000], 2, 1), ([2000], [1500], 1, 1)], ids=str)
+def test_rows_that_see_no_key(lq, lk, hq, hk, dtype):
+    """Causal sequences with more rows than keys: the first rows give zeros and take no gradient although the keys and
+    values hold NaN and infinities, and nothing they hold themselves reaches the other rows or the keys."""
+    gen = torch.Generator().manual_seed(11)
+    d, q_off, k_off = 64, offsets(lq), offsets(lk)
+    q, k, v, grad = (torch.randn(t, h, d, generator=gen).to(dtype) for t, h in
+                     ((q_off[-1], hq), (k_off[-1], hk), (k_off[-1], hk), (q_off[-1], hq)))
+    blind = torch.zeros(q_off[-1], dtype=torch.bool)
+    for s in range(len(lq)):
+        blind[q_off[s]:q_off[s] + max(0, lq[s] - lk[s])] = True
+    ptr = [torch.tensor(o, dtype=torch.int32, device=DEV) for o in (q_off, k_off)]
+
+    def step(q, k, v, grad):
+        leaves = [t.to(DEV).requires_grad_() for t in (q, k, v)]
+        out = PackedAttentionFuse(*leaves, *ptr, causal=True)
+        return [out.detach().cpu()] + [t.cpu() for t in torch.autograd.grad(out, leaves, grad.to(DEV))]
+
+    clean = step(q, k, v, grad)
+    for t in (clean[0], clean[1]):
+        assert not t[blind].any() and t[~blind].any()
+    for what in (float("nan"), float("inf")):
+        bad_q, bad_grad = q.clone(), grad.clone()
+        bad_q[blind], bad_grad[blind] = what, what
+        for a, b in zip(step(bad_q, k, v, bad_grad), clean):
+            assert torch.equal(a, b)
+        bad_k, bad_v = k.clone(), v.clone()
+        bad_k[::3], bad_v[::2] = what, what
+        out, dq, _, _ = step(q, bad_k, bad_v, grad)
+        assert not out[blind].any() and not dq[blind].any()
