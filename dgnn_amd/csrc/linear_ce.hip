@@ -161,7 +161,7 @@ __global__ __launch_bounds__(1024) void k_ce_rows(int n, int classes, long long 
       if (i + k < n) {
         if (class_of(label, i + k, classes, ignore) >= 0) on |= 1u << k;
         else if (lse) {
-          lse[i + k] = 0.f;
+          lse[i + k] = lse[n + i + k] = 0.f;
           if (loss) loss[i + k] = 0.f;
         }
       }
@@ -236,7 +236,7 @@ struct CeArgs {
   int n, classes, d, dk;          // dk = d rounded up to whole chunks
   float *part_m, *part_s;         // [class tiles, n]
   float *z_label;                 // [n], by gathered row
-  float *lse, *loss;              // [n], by original row
+  float *lse, *loss;              // by original row, loss [n], lse [2, n]: log-sum and what its rounding to float took
   const float *grad;              // of the loss: n values or one
   int grad_rows, mean;
   const float *grad_top;          // one gradient a row: the largest magnitude
@@ -249,6 +249,16 @@ struct CeArgs {
 
 __device__ __forceinline__ int rows_of(const CeArgs &a) { return a.count ? min(a.n, *a.count) : a.n; }
 __device__ __forceinline__ int row_at(const CeArgs &a, int r) { return a.list ? a.list[r] : r; }
+// A labelled row's results from its largest logit, the log of its sum of exp(z - top) and its label's logit.  top + log
+// is never rounded to float before a logit is taken off: with logits of 400 that alone is 1.5e-5, the whole loss and gradient
+// of a row that is sure of its label.  The backward gets both parts.
+__device__ __forceinline__ void store_row_loss(const CeArgs &a, int row, bool on, float top, double log_sum, float z_label) {
+  const double v = (double)top + log_sum;
+  const float hi = (float)v;
+  a.lse[row] = on ? hi : 0.f;
+  a.lse[a.n + row] = on && fabsf(hi) < INFINITY ? (float)(v - (double)hi) : 0.f;
+  a.loss[row] = on ? (float)((double)top - (double)z_label + log_sum) : 0.f;
+}
 // dz is kept in T as (softmax - onehot) g_i / unit and the products carry the factor unit, the largest |g|
 // (with the mean's division).  A common factor kept out of dz costs no rounding: rounded into it, one
 // g for all rows would put the same error, up to half a step of T, on every gradient.  float16 also has too
@@ -341,12 +351,17 @@ __global__ __launch_bounds__(C::THREADS, C::THREADS == 512 ? 2 : 1) void k_ce_fw
 #pragma unroll
       for (int e = 0; e < 16; ++e) top = fmaxf(top, acc[i][j][e]);
     top = fmaxf(top, __shfl_xor(top, 32, 64));
-    const float base = top == -INFINITY ? 0.f : top * DGNN_LOG2E;
+    // the difference first: the largest logit then adds exactly one.  Blocks of sixteen are summed by themselves, or
+    // a hundred small terms would each be rounded against that one.
+    const float base = top == -INFINITY ? 0.f : top;
     float sum = 0.f;
 #pragma unroll
-    for (int i = 0; i < C::MB; ++i)
+    for (int i = 0; i < C::MB; ++i) {
+      float block = 0.f;
 #pragma unroll
-      for (int e = 0; e < 16; ++e) sum += __builtin_amdgcn_exp2f(fmaf(acc[i][j][e], DGNN_LOG2E, -base));
+      for (int e = 0; e < 16; ++e) block += __builtin_amdgcn_exp2f((acc[i][j][e] - base) * DGNN_LOG2E);
+      sum += block;
+    }
     sum += __shfl_xor(sum, 32, 64);
     if (h == 0) sm[wm][col] = top, ss[wm][col] = sum;
   }
@@ -360,10 +375,7 @@ __global__ __launch_bounds__(C::THREADS, C::THREADS == 512 ? 2 : 1) void k_ce_fw
     for (int w = 0; w < C::WM; ++w) s += ss[w][threadIdx.x] * __builtin_amdgcn_exp2f((sm[w][threadIdx.x] - base) * DGNN_LOG2E);
     if (a.part_m == nullptr) {                  // one tile of classes: this is all there is
       const int row = r0 + threadIdx.x;
-      const bool on = a.labels.valid(row);
-      const float lse = base + logf(s);
-      a.lse[row] = on ? lse : 0.f;
-      a.loss[row] = on ? lse - zl[threadIdx.x] : 0.f;
+      store_row_loss(a, row, a.labels.valid(row), base, (double)logf(s), zl[threadIdx.x]);
       return;
     }
     const long long at = (long long)tile.m * a.n + r0 + threadIdx.x;
@@ -400,11 +412,8 @@ __global__ __launch_bounds__(DGNN_BLOCK) void k_ce_join(const CeArgs a, int tile
   const float base = top == -INFINITY ? 0.f : top;
   double sum = 0.;
   for (int w = 0; w < 32; ++w) sum += ss[w][c] * (double)expf(sm[w][c] - base);
-  const float v = base + logf((float)sum);
   const int row = row_at(a, r);
-  const bool on = a.labels.valid(row);
-  a.lse[row] = on ? v : 0.f;
-  a.loss[row] = on ? v - a.z_label[r] : 0.f;
+  store_row_loss(a, row, a.labels.valid(row), base, log(sum), a.z_label[r]);
 }
 // out[0] = sum of the losses (/ labelled rows), in a fixed order; no labelled row: 0
 __global__ __launch_bounds__(1024) void k_ce_reduce(const CeArgs a, int mean, const float *__restrict__ loss, float *__restrict__ out) {
@@ -496,22 +505,24 @@ __global__ __launch_bounds__(C::THREADS, C::THREADS == 512 ? 2 : 1) void k_ce_dz
          rows_operand<T, G>(a, r0, rows), a.dk, lds, acc);
   const int lane = lane_id(), wave = uniform_i32(wave_in_block()), n0 = wave % C::WN * (C::BN / C::WN);
   const CeScale scale = ce_scale<T>(a, rows);
-  float lse[C::NB], g[C::NB];
+  // exp(z - lse) = exp2(z log2e - c) f, c the product with the whole lse rounded to float, f what that took
+  float c[C::NB], fg[C::NB], g[C::NB];
   int want[C::NB];
 #pragma unroll
   for (int j = 0; j < C::NB; ++j) {
     const int r = r0 + n0 + 32 * j + (lane & 31), row = r < rows ? a.list[r] : a.list[0];
     want[j] = (int)(a.labels.at(row) - v0);
-    lse[j] = a.lse[row] * DGNN_LOG2E;
+    const double t = ((double)a.lse[row] + (double)a.lse[a.n + row]) * (double)DGNN_LOG2E;
+    c[j] = (float)t;
     g[j] = a.grad[a.grad_rows ? row : 0] * scale.by;
+    fg[j] = g[j] * __builtin_amdgcn_exp2f(fabsf(c[j]) < INFINITY ? (float)((double)c[j] - t) : 0.f);
   }
   const int left = a.vn - p0;                   // classes of this tile
   rows_of_tile<T, C>(
       lds,
       [&](int i, int j, int e, int m) {
-        float y = __builtin_amdgcn_exp2f(fmaf(acc[i][j][e], DGNN_LOG2E, -lse[j]));
-        y = m == want[j] ? y - 1.f : y;
-        return (T)(m < left ? y * g[j] : 0.f);
+        const float y = __builtin_amdgcn_exp2f(fmaf(acc[i][j][e], DGNN_LOG2E, -c[j]));
+        return (T)(m < left ? fmaf(y, fg[j], m == want[j] ? -g[j] : 0.f) : 0.f);
       },
       [&](int row, int col, u32x4 piece) {
         if (r0 + row < rows) *(u32x4 *)((T *)a.dz + (long long)(r0 + row) * a.ldz + p0 + col) = piece;

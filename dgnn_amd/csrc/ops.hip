@@ -731,7 +731,7 @@ __global__ __launch_bounds__(256) void k_edgeconv_bwd_gather(long long total, in
 
 extern "C" {
 
-int dgnn_abi_version(void) { return 2; }   // 2: out_neg / a_neg in the fused GAT entry points
+int dgnn_abi_version(void) { return 3; }   // 2: out_neg / a_neg in the fused GAT entry points, 3: lse [2,n] of the linear cross entropy
 
 const char *dgnn_error_string(int code) {
   switch (code) {

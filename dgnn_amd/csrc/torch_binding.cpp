@@ -1122,12 +1122,12 @@ CeCall ce_call(const Tensor &feat, const Tensor &weight, const Tensor &label, in
   return c;
 }
 
-// -> (loss [rows] or [], lse [rows])
+// -> (loss [rows] or [], lse [2, rows])
 std::tuple<Tensor, Tensor> linear_ce_forward(const Tensor &feat, const Tensor &weight, const Tensor &label,
                                              int64_t ignore_index, int64_t reduction) {
   const CeCall c = ce_call(feat, weight, label, reduction);
   c10::DeviceGuard guard(feat.device());
-  Tensor loss = reduction == 0 ? new_f32({c.n}, feat) : new_f32({}, feat), lse = new_f32({c.n}, feat);
+  Tensor loss = reduction == 0 ? new_f32({c.n}, feat) : new_f32({}, feat), lse = new_f32({2, c.n}, feat);
   const size_t nb = API(dgnn_linear_ce_workspace_bytes)(c.dtype, c.n, c.classes, c.d, 0);
   Tensor ws = workspace(nb, feat);
   check_rc(API(dgnn_linear_ce_forward)(c.dtype, c.label_bytes, c.n, c.classes, c.d, ignore_index, (int)reduction, cv(feat),
@@ -1141,8 +1141,8 @@ std::tuple<py::object, py::object> linear_ce_backward(const Tensor &feat, const 
                                                       int64_t ignore_index, int64_t reduction, const Tensor &lse,
                                                       const Tensor &grad, bool want_feat, bool want_weight) {
   const CeCall c = ce_call(feat, weight, label, reduction);
-  f32(lse, "lse", 1), f32(grad, "grad");
-  if (lse.size(0) != c.n || lse.device() != feat.device()) fail("lse must be the forward's [rows]");
+  f32(lse, "lse", 2), f32(grad, "grad");
+  if (lse.size(0) != 2 || lse.size(1) != c.n || lse.device() != feat.device()) fail("lse must be the forward's [2, rows]");
   if (grad.numel() != (reduction == 0 ? c.n : 1) || grad.device() != feat.device())
     fail("grad must be the gradient of the loss, got shape ", grad.sizes());
   c10::DeviceGuard guard(feat.device());
@@ -1435,7 +1435,7 @@ PYBIND11_MODULE(fused_cross_entropy, m) {
   options.disable_function_signatures();
   init(m, "Cross entropy of a linear layer without its logits (no reference module).");
   def(m, "linear_ce_forward", &linear_ce_forward, "feat, weight, label, ignore_index=-100, reduction=1",
-      "-> (loss, lse [rows]); reduction 0: loss [rows], 1: mean over the labelled rows, 2: sum", arg("feat"),
+      "-> (loss, lse [2, rows]: log-sum and what its rounding took); reduction 0: loss [rows], 1: mean over the labelled rows, 2: sum", arg("feat"),
       arg("weight"), arg("label"), arg("ignore_index") = -100, arg("reduction") = 1);
   def(m, "linear_ce_backward", &linear_ce_backward,
       "feat, weight, label, ignore_index, reduction, lse, grad, want_feat=True, want_weight=True",

@@ -534,7 +534,8 @@ int dgnn_attn_backward(int dtype, int nseq, int tq, int tk, int hq, int hk, int 
  * contiguous; label int32 (label_bytes 4) or int64 (8).  A row whose label is ignore_index or outside
  * [0, classes) has no label: loss 0, no gradient, whatever the row holds (NaN too).
  *   reduction 0: loss [n]; 1: loss [1], the mean over the labelled rows (0 when there are none); 2: [1], the sum
- *   lse [n]: log of the softmax's sum (0 for rows without a label), kept for the backward
+ *   lse [2,n]: log of the softmax's sum and what its rounding to float took (0 for rows without a label), kept for
+ *   the backward (ABI 3; [n] before)
  * backward: grad is d / d loss, [n] for reduction 0, else [1]; dx [n,d] and dw [classes,d], either may be NULL.
  * Limits: n <= 2^22, d <= 65536, classes <= 2^30 (DGNN_ERR_UNSUPPORTED). */
 size_t dgnn_linear_ce_workspace_bytes(int dtype, int n, int classes, int d, int backward);

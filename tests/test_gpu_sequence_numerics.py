@@ -114,3 +114,50 @@ def test_rows_that_see_no_key(lq, lk, hq, hk, dtype):
         bad_k[::3], bad_v[::2] = what, what
         out, dq, _, _ = step(q, bad_k, bad_v, grad)
         assert not out[blind].any() and not dq[blind].any()
+
+
+# ------------------------------------------------------------------------------------ loss
+@pytest.mark.parametrize("dtype", DTYPES, ids=ids_of)
+@pytest.mark.parametrize("top", [50.0, 400.0, -272.0])
+@pytest.mark.parametrize("n,classes,dim", [(60, 41, 64), (33, 41, 33), (20, 3000, 64), (100, 1000, 128), (120, 1000, 129),
+                                           (520, 33000, 528)], ids=str)
+def test_loss_of_confident_rows(n, classes, dim, top, dtype):
+    """The label's logit leads all others by 14, with logits of hundreds: the loss is (classes - 1) exp(-14) and the gradient
+    of the label's logit about as small.  Logits are exact (one product each), so what is left is the sum of exp(z - top):
+    one term of 1, at most 25 additions it takes part in (16 of a block, 4 blocks, 1 of the other half, 4 waves), the others
+    2 * 14 + 8 roundings each."""
+    lead = 14.0
+    gen = torch.Generator().manual_seed(n)
+    at = torch.randint(0, classes, (dim,), generator=gen)
+    weight = torch.full((classes, dim), top - lead)
+    weight[at, torch.arange(dim)] = top
+    x, w = torch.eye(n, dim).to(DEV, dtype).requires_grad_(), weight.to(DEV, dtype).requires_grad_()
+    assert torch.equal(w.detach().cpu().float(), weight)
+    label = at[:n].to(DEV)
+    loss = LinearCrossEntropyFuse(x, w, label, reduction="none")
+    one = math.exp(-lead)
+    rest = (classes - 1) * one
+    want = math.log1p(rest)
+    assert loss.min() >= 0
+    assert (loss.double() - want).abs().max() <= (25 + (2 * lead + 8) * rest + want) * ref.U
+    dw, = torch.autograd.grad(loss.sum(), w)
+    e, t0 = ref.half_step(dtype), ref.tiny(dtype)
+    dz = torch.full((classes, n), one / (1 + rest), dtype=torch.float64, device=DEV)
+    bound = dz * ((25 + 2 * lead + 16) * ref.U + 2 * e) + t0
+    pick = (label, torch.arange(n, device=DEV))
+    dz[pick] = -rest / (1 + rest)
+    bound[pick] = 32 * ref.U + 2 * e * rest + t0
+    ref.check(dw[:, :n], (dz, bound), "dw")
+    assert not dw[:, n:].any()
+
+
+def test_loss_backward_refuses_half_of_the_log_sum():
+    from dgnn_amd._lib import DgnnError
+    from dgnn_amd.native import fused_cross_entropy as ext
+    x, w = torch.randn(8, 16, device=DEV), torch.randn(5, 16, device=DEV)
+    label, grad = torch.arange(8, device=DEV) % 5, torch.ones((), device=DEV)
+    _, lse = ext.linear_ce_forward(x, w, label, -100, 1)
+    assert lse.shape == (2, 8)
+    for bad in (lse[0], lse[:1], lse[:, :4].contiguous()):
+        with pytest.raises(DgnnError, match="lse"):
+            ext.linear_ce_backward(x, w, label, -100, 1, bad, grad)
