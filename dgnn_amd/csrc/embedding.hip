@@ -384,13 +384,33 @@ __global__ __launch_bounds__(DGNN_BLOCK) void k_embed_rows(int n, int rows, int 
           for (int j = 0; j < N; ++j) acc[j] += (float)p.v[j];
         }
       } else {
+        // in double: the pieces of a long run are many (4 sqrt(n) of them if one id is all there is), of like size, and
+        // each rounding in float would go the same way (2^20 ids, one row, gradients of 0.1: 4e-5 off).  Four at a time are
+        // joined in float first: eight doubled rows in flight take the registers of two waves a SIMD (step above 343 us)
         const int q0 = s / run, q1 = (e - 1) / run;
-#pragma unroll 8
-        for (int q = q0; q <= q1; ++q) {
-          const float *src = part + (long long)(2 * q + (q == q0 && s != q * run ? 1 : 0)) * dim + c;
+        auto at = [&](int q) { return part + (long long)(2 * q + (q == q0 && s != q * run ? 1 : 0)) * dim + c; };
+        double sum[N];
 #pragma unroll
-          for (int j = 0; j < N; ++j) acc[j] += src[j];
+        for (int j = 0; j < N; ++j) sum[j] = 0.;
+        int q = q0;
+        for (; q + 8 <= q1 + 1; q += 8) {
+          float four[2][N];
+#pragma unroll
+          for (int x = 0; x < 8; ++x) {
+            const float *src = at(q + x);
+#pragma unroll
+            for (int j = 0; j < N; ++j) four[x / 4][j] = x % 4 ? four[x / 4][j] + src[j] : src[j];
+          }
+#pragma unroll
+          for (int j = 0; j < N; ++j) sum[j] += (double)four[0][j] + (double)four[1][j];
         }
+        for (; q <= q1; ++q) {
+          const float *src = at(q);
+#pragma unroll
+          for (int j = 0; j < N; ++j) sum[j] += (double)src[j];
+        }
+#pragma unroll
+        for (int j = 0; j < N; ++j) acc[j] = (float)sum[j];
       }
       Pack<T, N> p;
 #pragma unroll
@@ -410,7 +430,8 @@ __global__ __launch_bounds__(DGNN_BLOCK) void k_embed_rows(int n, int rows, int 
   }
 }
 
-// pieces of about sqrt(n) / 4: the longest run possible is summed in two steps of some hundred terms
+// pieces of sqrt(n) / 4 .. sqrt(n) / 2, at least 64: the longest run possible is summed in float over a quarter of a piece
+// by each of four waves (a whole piece where a run stays inside one), then in double over 2 .. 4 sqrt(n) pieces
 static inline int embed_run(int n) {
   int r = 64;
   while (16LL * r * r < n) r <<= 1;

@@ -161,3 +161,42 @@ def test_loss_backward_refuses_half_of_the_log_sum():
     for bad in (lse[0], lse[:1], lse[:, :4].contiguous()):
         with pytest.raises(DgnnError, match="lse"):
             ext.linear_ce_backward(x, w, label, -100, 1, bad, grad)
+
+
+# ------------------------------------------------------------------------------------ embedding
+def piece(n):
+    """Sorted positions that one float sum runs over at most."""
+    r = 64
+    while 16 * r * r < n:
+        r *= 2
+    return r
+
+
+@pytest.mark.parametrize("n,rows,dim", [(1 << 20, 1, 16), (1 << 20, 2, 6), (1 << 20, 3, 3), (400003, 1, 64), (70001, 1, 100), (9000, 2, 5)])
+def test_embedding_gradient_of_long_runs(n, rows, dim):
+    """One id named by all positions but a few, gradients of one value: every rounding goes the same way.  A quarter of a
+    piece is added up in float, four waves are joined, the piece and the result are rounded: the number of pieces has no part in it."""
+    ids = torch.zeros(n, dtype=torch.int64, device=DEV)
+    ids[::997] = rows - 1
+    table = torch.zeros(rows, dim, device=DEV, requires_grad=True)
+    grad = torch.full((n, dim), 0.1, device=DEV)
+    got, = torch.autograd.grad(NodeEmbeddingFuse(ids, table), [table], grad)
+    want = torch.bincount(ids, minlength=rows).double()[:, None].expand(rows, dim) * grad[0, 0].double()
+    # (the short runs of the last row may lie inside a piece: one wave adds them up)
+    depth = torch.full((rows, 1), piece(n) / 4 + 8, dtype=torch.float64, device=DEV)
+    depth[rows - 1] = max(depth[rows - 1], piece(n)) if rows > 1 else depth[rows - 1]
+    ref.check(got, (want, depth * ref.U * want), "grad_table")
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=ids_of)
+@pytest.mark.parametrize("n,rows,dim", [(70001, 7, 33), (300000, 40, 8), (8193, 3, 129), (8192, 5, 20), (1 << 20, 1000, 4)])
+def test_embedding_gradient_of_whole_numbers(n, rows, dim, dtype):
+    """Whole numbers whose sums are exact: no term is dropped or taken twice in runs of any length."""
+    gen = torch.Generator(device=DEV).manual_seed(n)
+    ids = (torch.rand(n, device=DEV, generator=gen, dtype=torch.float64) ** 4 * (rows + 1)).long() - 1
+    grad = torch.randint(-8, 9, (n, dim), device=DEV, generator=gen).to(dtype)
+    table = torch.zeros(rows, dim, device=DEV, dtype=dtype, requires_grad=True)
+    got, = torch.autograd.grad(NodeEmbeddingFuse(ids, table), [table], grad)
+    good = ids >= 0
+    want = torch.zeros(rows, dim, device=DEV, dtype=torch.float64).index_add_(0, ids[good], grad[good].double())
+    assert torch.equal(got, want.to(dtype))
