@@ -3,6 +3,7 @@ edges, dgNN/operators/fused_gatconv.py; this one over all pairs of a graph, a wa
 import torch
 
 from ..native import fused_attention
+from ._autograd import differentiated
 
 
 def PackedAttentionFuse(q, k, v, row_ptr, col_ptr=None, causal=False, scale=None):
@@ -25,7 +26,7 @@ def PackedAttentionFuse(q, k, v, row_ptr, col_ptr=None, causal=False, scale=None
         scale = q.size(-1) ** -0.5
     if col_ptr is None:
         col_ptr = row_ptr
-    if not (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)):
+    if not differentiated(q, k, v):
         return fused_attention.attention_forward(q, k, v, row_ptr, col_ptr, scale, causal)[0]
     return PackedAttentionFunction.apply(q, k, v, row_ptr, col_ptr, causal, scale)
 

@@ -4,6 +4,7 @@ import torch
 
 from .._lib import DgnnError
 from ..native import fused_cross_entropy
+from ._autograd import differentiated
 
 _REDUCTION = {"none": 0, "mean": 1, "sum": 2}
 
@@ -20,7 +21,7 @@ def LinearCrossEntropyFuse(feat, weight, label, ignore_index=-100, reduction="me
     time; both gradients are summed in float32 in a fixed order."""
     if reduction not in _REDUCTION:
         raise DgnnError(f"reduction must be 'none', 'mean' or 'sum', got {reduction!r}")
-    if not (torch.is_grad_enabled() and (feat.requires_grad or weight.requires_grad)):
+    if not differentiated(feat, weight):
         return fused_cross_entropy.linear_ce_forward(feat.contiguous(), weight.contiguous(), label.contiguous(),
                                                      ignore_index, _REDUCTION[reduction])[0]
     return LinearCrossEntropyFunction.apply(feat, weight, label, ignore_index, _REDUCTION[reduction])

@@ -2,6 +2,7 @@
 import torch
 
 from ..native import fused_embedding
+from ._autograd import differentiated
 
 
 def NodeEmbeddingFuse(ids, table, scale=1.0):
@@ -10,7 +11,7 @@ def NodeEmbeddingFuse(ids, table, scale=1.0):
     ids (int32 or int64, any shape) outside [0, rows) -- padding -- give rows of zeros and no gradient.
     table is [rows, dim], float32, bfloat16 or float16.  Its gradient is dense, summed in float32
     in the order of the ids (sorted, no atomics: the same bits every time)."""
-    if not (torch.is_grad_enabled() and table.requires_grad):        # a lookup alone: no graph to build
+    if not differentiated(table):        # a lookup alone: no graph to build
         return fused_embedding.embedding_forward(ids.contiguous(), table.detach().contiguous(), scale)
     return NodeEmbeddingFunction.apply(ids, table, scale)
 

@@ -200,3 +200,22 @@ def test_embedding_gradient_of_whole_numbers(n, rows, dim, dtype):
     good = ids >= 0
     want = torch.zeros(rows, dim, device=DEV, dtype=torch.float64).index_add_(0, ids[good], grad[good].double())
     assert torch.equal(got, want.to(dtype))
+
+
+# ------------------------------------------------------------------------------------ forward mode
+@pytest.mark.parametrize("grad", [True, False], ids=["grad", "no_grad"])
+def test_forward_mode_is_refused(grad):
+    """A tangent is not dropped: none of the operators has a forward-mode derivative, and all say so."""
+    import torch.autograd.forward_ad as fwd
+    ptr = torch.tensor([0, 8], dtype=torch.int32, device=DEV)
+    x, w, table = torch.randn(8, 2, 16, device=DEV), torch.randn(5, 16, device=DEV), torch.randn(9, 16, device=DEV)
+    ids, label = torch.arange(8, device=DEV), torch.arange(8, device=DEV) % 5
+    flat = x[:, 0].contiguous()
+    calls = [lambda d: PackedAttentionFuse(d(x), x, x, ptr), lambda d: PackedAttentionFuse(x, d(x), x, ptr),
+             lambda d: PackedAttentionFuse(x, x, d(x), ptr), lambda d: NodeEmbeddingFuse(ids, d(table)),
+             lambda d: LinearCrossEntropyFuse(d(flat), w, label), lambda d: LinearCrossEntropyFuse(flat, d(w), label)]
+    with torch.set_grad_enabled(grad), fwd.dual_level():
+        for call in calls:
+            with pytest.raises(NotImplementedError):
+                call(lambda t: fwd.make_dual(t, torch.ones_like(t)))
+            assert not call(lambda t: t).requires_grad            # inside a level, without a tangent
