@@ -23,7 +23,7 @@ def PackedAttentionFuse(q, k, v, row_ptr, col_ptr=None, causal=False, scale=None
     infinity in a key or value may reach rows that the causal mask keeps from it (and one in a row or its
     gradient the gradients of keys that it does not see), as a weight of zero times it does."""
     if scale is None:
-        scale = q.size(-1) ** -0.5
+        scale = max(q.size(-1), 1) ** -0.5                # (a dim of 0 is refused below)
     if col_ptr is None:
         col_ptr = row_ptr
     if not differentiated(q, k, v):
