@@ -400,7 +400,7 @@ __global__ __launch_bounds__(64, sizeof(T) == 2 ? 2 : 1) void k_attn_split(const
 template <class T>
 __global__ __launch_bounds__(DGNN_BLOCK) void k_attn_join(const AttnArgs a) {
   const int lane = lane_id();
-  const long long r = (long long)blockIdx.x * DGNN_WAVES_PER_BLOCK + uniform_i32(wave_in_block());
+  const long long r = (long long)group_in_rows() * DGNN_WAVES_PER_BLOCK + uniform_i32(wave_in_block());
   if (r >= (long long)a.tq * a.hq) return;
   const int tok = (int)(r / a.hq), head = (int)(r % a.hq);
   const Segment seg = find_segment(a.row_ptr, a.nseq, a.tq, 1, 1, tok, false, true);   // the row's sequence
@@ -476,11 +476,11 @@ static AttnPlan attn_plan(int nseq, int tq, int tk, int hq, int hk, int d) {
 template <class T, int DP, int NW, int HW, int BN, int S>
 static int launch_rows(const AttnArgs &a, hipStream_t st) {
   const long long groups = tile_slots(a.tq, a.nseq, a.g, 32 * NW) * ((a.hk + HW - 1) / HW) * a.splits;
-  if (groups > 0x7fffffffLL) return DGNN_ERR_UNSUPPORTED;
+  const long long rows = (long long)a.tq * a.hq;
+  if (!launchable(groups, 64 * NW * HW) || (a.splits > 1 && !launchable(rows, 64))) return DGNN_ERR_UNSUPPORTED;
   hipLaunchKernelGGL((k_attn_fwd<T, DP, NW, HW, BN, S>), dim3((unsigned)groups), dim3(64 * NW * HW), 0, st, a);
   DGNN_LAUNCH_CHECK();
   if (a.splits > 1) {
-    const long long rows = (long long)a.tq * a.hq;
     hipLaunchKernelGGL(k_attn_merge<T>, dim3((unsigned)((rows + DGNN_WAVES_PER_BLOCK - 1) / DGNN_WAVES_PER_BLOCK)),
                        dim3(DGNN_BLOCK), 0, st, a);
     DGNN_LAUNCH_CHECK();
@@ -490,7 +490,7 @@ static int launch_rows(const AttnArgs &a, hipStream_t st) {
 template <class T, int DP>
 static int launch_fwd(const AttnArgs &a, const AttnPlan &p, hipStream_t st) {
   if (p.few > 0) {
-    if (p.slots * a.hk > 0x7fffffffLL) return DGNN_ERR_UNSUPPORTED;
+    if (!launchable(p.slots * a.hk, 64)) return DGNN_ERR_UNSUPPORTED;
     const dim3 grid((unsigned)(p.slots * a.hk));
     const bool four = sizeof(T) == 4 && p.few == 4;
     if constexpr (sizeof(T) == 4) {
@@ -499,8 +499,7 @@ static int launch_fwd(const AttnArgs &a, const AttnPlan &p, hipStream_t st) {
     if (!four) hipLaunchKernelGGL((k_attn_split<T, DP, false>), grid, dim3(64), 0, st, a);
     DGNN_LAUNCH_CHECK();
     const long long rows = (long long)a.tq * a.hq;
-    hipLaunchKernelGGL(k_attn_join<T>, dim3((unsigned)((rows + DGNN_WAVES_PER_BLOCK - 1) / DGNN_WAVES_PER_BLOCK)),
-                       dim3(DGNN_BLOCK), 0, st, a);
+    hipLaunchKernelGGL(k_attn_join<T>, grid_in_rows((rows + DGNN_WAVES_PER_BLOCK - 1) / DGNN_WAVES_PER_BLOCK), dim3(DGNN_BLOCK), 0, st, a);
     DGNN_LAUNCH_CHECK();
     return DGNN_OK;
   }

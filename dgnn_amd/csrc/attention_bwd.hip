@@ -16,6 +16,8 @@
 // power of two of the lane's own row (or key), lowered whenever a term outgrows it, like the softmax's running
 // maximum (DsScale); both come out of the float sums at the end.  It costs 4 % of a training step of 32 x 2048 tokens, 8
 // heads of 64 (1440 us, 1378 without).  bfloat16 has float's range.
+#include <utility>
+
 #include "attention.hpp"
 
 using namespace dgnn;
@@ -209,7 +211,7 @@ __global__ __launch_bounds__(64 * NW * HW, sizeof(T) == 2 && (NW > 1 || DP < 128
 // dk and dv of every (key, key head): the sum of the splits' {dk row, dv row}, in order
 template <class T>
 __global__ __launch_bounds__(DGNN_BLOCK) void k_attn_bwd_join(const AttnArgs a) {
-  const long long rows = (long long)a.tk * a.hk, per = a.d / 4, u = blockIdx.x * (long long)DGNN_BLOCK + threadIdx.x;
+  const long long rows = (long long)a.tk * a.hk, per = a.d / 4, u = group_in_rows() * (long long)DGNN_BLOCK + threadIdx.x;
   if (u >= rows * per * 2) return;
   const long long row = u / (per * 2);
   const int c = (int)(u % (per * 2)) * 4;
@@ -359,24 +361,27 @@ static int bwd_splits(int nseq, int tq, int tk, int hq, int hk) {
 }
 static size_t align256(size_t x) { return (x + 255) / 256 * 256; }
 
+static long long bwd_kv_groups(const AttnArgs &a, int nw, int hw) {
+  return tile_slots(a.tk, a.nseq, 1, 32 * nw) * ((a.hk + hw - 1) / hw) * a.splits;
+}
+static long long bwd_q_groups(const AttnArgs &a, int nw, int hw) {
+  return tile_slots(a.tq, a.nseq, a.g, 32 * nw) * ((a.hk + hw - 1) / hw);
+}
 template <class T, int DP, int NW, int HW, int S>
 static int launch_bwd_kv(const AttnArgs &a, hipStream_t st) {
-  const long long groups = tile_slots(a.tk, a.nseq, 1, 32 * NW) * ((a.hk + HW - 1) / HW) * a.splits;
-  if (groups > 0x7fffffffLL) return DGNN_ERR_UNSUPPORTED;
+  const long long groups = bwd_kv_groups(a, NW, HW);
   hipLaunchKernelGGL((k_attn_bwd_kv<T, DP, NW, HW, S>), dim3((unsigned)groups), dim3(64 * NW * HW), 0, st, a);
   DGNN_LAUNCH_CHECK();
   if (a.splits > 1) {
     const long long blocks = ((long long)a.tk * a.hk * (a.d / 2) + DGNN_BLOCK - 1) / DGNN_BLOCK;
-    if (blocks > 0x7fffffffLL) return DGNN_ERR_UNSUPPORTED;
-    hipLaunchKernelGGL(k_attn_bwd_join<T>, dim3((unsigned)blocks), dim3(DGNN_BLOCK), 0, st, a);
+    hipLaunchKernelGGL(k_attn_bwd_join<T>, grid_in_rows(blocks), dim3(DGNN_BLOCK), 0, st, a);
     DGNN_LAUNCH_CHECK();
   }
   return DGNN_OK;
 }
 template <class T, int DP, int NW, int HW, int S>
 static int launch_bwd_q(const AttnArgs &a, hipStream_t st) {
-  const long long groups = tile_slots(a.tq, a.nseq, a.g, 32 * NW) * ((a.hk + HW - 1) / HW);
-  if (groups > 0x7fffffffLL) return DGNN_ERR_UNSUPPORTED;
+  const long long groups = bwd_q_groups(a, NW, HW);
   hipLaunchKernelGGL((k_attn_bwd_q<T, DP, NW, HW, S>), dim3((unsigned)groups), dim3(64 * NW * HW), 0, st, a);
   DGNN_LAUNCH_CHECK();
   return DGNN_OK;
@@ -384,12 +389,18 @@ static int launch_bwd_q(const AttnArgs &a, hipStream_t st) {
 template <class T, int DP>
 static int launch_bwd(const AttnArgs &a, hipStream_t st) {
   int rc = DGNN_OK;
+  const bool few_q = rows_short(a.tq, a.nseq, a.g), few_k = a.splits <= 1 && rows_short(a.tk, a.nseq, 1);
+  // both of them before either runs
+  for (const auto &[few, groups] : {std::pair(few_q, &bwd_q_groups), std::pair(few_k, &bwd_kv_groups)}) {
+    const int nw = few ? 1 : 4, hw = few && a.hk >= 4 ? 4 : 1;
+    if (!launchable(groups(a, nw, hw), 64 * nw * hw)) return DGNN_ERR_UNSUPPORTED;
+  }
   if (a.tq > 0) {
-    if (!rows_short(a.tq, a.nseq, a.g)) rc = launch_bwd_q<T, DP, 4, 1, 4>(a, st);
+    if (!few_q) rc = launch_bwd_q<T, DP, 4, 1, 4>(a, st);
     else rc = a.hk >= 4 ? launch_bwd_q<T, DP, 1, 4, 1>(a, st) : launch_bwd_q<T, DP, 1, 1, 1>(a, st);
   }
   if (rc == DGNN_OK && a.tk > 0) {
-    if (a.splits > 1 || !rows_short(a.tk, a.nseq, 1)) rc = launch_bwd_kv<T, DP, 4, 1, 4>(a, st);
+    if (!few_k) rc = launch_bwd_kv<T, DP, 4, 1, 4>(a, st);
     else rc = a.hk >= 4 ? launch_bwd_kv<T, DP, 1, 4, 1>(a, st) : launch_bwd_kv<T, DP, 1, 1, 1>(a, st);
   }
   return rc;

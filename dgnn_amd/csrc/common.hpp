@@ -21,6 +21,16 @@
 
 namespace dgnn {
 
+// A dimension of a launch holds fewer than 2^32 work items, whatever the workgroups are.
+static inline bool launchable(long long groups, int threads) { return groups * threads < (1LL << 32); }
+// More workgroups than that: rows of 2^22 of them, workgroup blockIdx.y * gridDim.x + blockIdx.x.  There may be up to a row
+// too many, which the kernel has to find out.
+static inline dim3 grid_in_rows(long long groups) {
+  const long long row = groups < 1 ? 1 : groups < (1 << 22) ? groups : 1 << 22;
+  return dim3((unsigned)row, (unsigned)((groups + row - 1) / row));
+}
+__device__ __forceinline__ unsigned group_in_rows() { return blockIdx.y * gridDim.x + blockIdx.x; }
+
 __device__ __forceinline__ int lane_id() { return threadIdx.x & (DGNN_WAVE - 1); }
 __device__ __forceinline__ int wave_in_block() { return threadIdx.x >> 6; }
 

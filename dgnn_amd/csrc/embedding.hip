@@ -48,7 +48,7 @@ __global__ __launch_bounds__(DGNN_BLOCK) void k_embed_fwd(int n, int rows, int d
                                                           const I *__restrict__ ids, const T *__restrict__ table,
                                                           T *__restrict__ out) {
   const int per = DGNN_BLOCK / lanes;
-  const long long i = (long long)blockIdx.x * per + threadIdx.x / lanes;
+  const long long i = (long long)group_in_rows() * per + threadIdx.x / lanes;
   if (i >= n) return;
   const int r = row_of_id(ids, i, rows);
   for (int c = (threadIdx.x & (lanes - 1)) * N; c < dim; c += lanes * N) {
@@ -463,6 +463,9 @@ static int access_bytes(int dim, int size, const void *a, const void *b) {
     if (x % w == 0) return w;
   return size;
 }
+static int access_elements(int bytes, int size) {           // as DGNN_EMBED_DISPATCH has it
+  return size == 4 || bytes == 16 ? bytes / size : bytes >= 4 ? 2 : 1;
+}
 static int row_lanes(int dim, int per) {
   int l = 1;
   while (l < DGNN_BLOCK && l * per < dim) l <<= 1;
@@ -473,10 +476,16 @@ template <class T, int N, class I>
 static int launch_embed_fwd(int n, int rows, int dim, float scale, const void *ids, const void *table, void *out,
                             hipStream_t st) {
   const int lanes = row_lanes(dim, N), per = DGNN_BLOCK / lanes;
-  hipLaunchKernelGGL((k_embed_fwd<T, N, I>), dim3((unsigned)((n + (long long)per - 1) / per)), dim3(DGNN_BLOCK), 0, st, n, rows,
+  hipLaunchKernelGGL((k_embed_fwd<T, N, I>), grid_in_rows((n + (long long)per - 1) / per), dim3(DGNN_BLOCK), 0, st, n, rows,
                      dim, lanes, scale, (const I *)ids, (const T *)table, (T *)out);
   DGNN_LAUNCH_CHECK();
   return DGNN_OK;
+}
+// as many rows a workgroup as make up for its search, but a thousand workgroups where the rows allow it
+static int rows_per_block(int rows, int lanes) {
+  const int groups = DGNN_BLOCK / lanes, thousandth = (rows + 1023) / 1024;
+  const int most = groups * 16 > EMBED_ROWS / 2 ? EMBED_ROWS : groups * 16;
+  return most <= thousandth ? most : thousandth > groups ? thousandth : groups;
 }
 template <class T, int N>
 static int launch_embed_sums(int n, int rows, int dim, float scale, const EmbedPlan &p, const int *key, const int *val,
@@ -486,10 +495,7 @@ static int launch_embed_sums(int n, int rows, int dim, float scale, const EmbedP
                        dim3(DGNN_BLOCK), 0, st, n, rows, dim, p.run, key, val, (const T *)grad, part);
     DGNN_LAUNCH_CHECK();
   }
-  const int lanes = row_lanes(dim, N), groups = DGNN_BLOCK / lanes;
-  // as many rows a workgroup as make up for its search, but a thousand workgroups where the rows allow it
-  int per_block = groups * 16 > EMBED_ROWS / 2 ? EMBED_ROWS : groups * 16;
-  if (per_block > (rows + 1023) / 1024) per_block = (rows + 1023) / 1024 > groups ? (rows + 1023) / 1024 : groups;
+  const int lanes = row_lanes(dim, N), per_block = rows_per_block(rows, lanes);
   auto kernel = k_embed_rows<T, N, false>;
   if constexpr (sizeof(T) * N == 16)
     if ((double)rows * dim * sizeof(T) > 256e6) kernel = k_embed_rows<T, N, true>;
@@ -527,6 +533,7 @@ static int sort_ids(int n, int rows, const void *ids, const EmbedPlan &p, char *
 
 static int embed_check(int dtype, int idx_bytes, int n, int rows, int dim) {
   if (dtype < 0 || dtype > 2 || (idx_bytes != 4 && idx_bytes != 8) || n < 0 || rows < 0 || dim < 0) return DGNN_ERR_BAD_ARG;
+  if (dim > (1 << 30)) return DGNN_ERR_UNSUPPORTED;          // columns and steps past them are ints
   return DGNN_OK;
 }
 static bool aligned_to(const void *p, int bytes) { return (uintptr_t)p % bytes == 0; }
@@ -585,6 +592,11 @@ int dgnn_embedding_backward(int dtype, int idx_bytes, int n, int rows, int dim, 
   if (!grad_table || (n > 0 && (!ids || !grad))) return DGNN_ERR_BAD_ARG;
   const int size = dtype == DGNN_F32 ? 4 : 2;
   if (!aligned_to(ids, idx_bytes) || !aligned_to(grad, size) || !aligned_to(grad_table, size)) return DGNN_ERR_ALIGNMENT;
+  // (columns are the second dimension of a launch, and a workgroup's rows times their pieces are an int)
+  const int bytes = access_bytes(dim, size, grad, grad_table), per = access_elements(bytes, size);
+  if (dim / (DGNN_WAVE * per) >= 65535 ||
+      !launchable(((long long)rows + DGNN_BLOCK) / rows_per_block(rows, row_lanes(dim, per)), DGNN_BLOCK))
+    return DGNN_ERR_UNSUPPORTED;
   const EmbedPlan p = embed_plan(n > 0 ? n : 1, rows, dim);
   if (n > 0 && (!workspace || workspace_bytes < p.total)) return DGNN_ERR_WORKSPACE;
   if (n > 0 && !aligned_to(workspace, 16)) return DGNN_ERR_ALIGNMENT;
@@ -597,7 +609,6 @@ int dgnn_embedding_backward(int dtype, int idx_bytes, int n, int rows, int dim, 
     if (rc != DGNN_OK) return rc;
     part = (float *)((char *)workspace + 4 * p.pairs + p.counts);
   }
-  const int bytes = access_bytes(dim, size, grad, grad_table);
   DGNN_EMBED_DISPATCH(dtype, bytes, (launch_embed_sums<T, N>(n, rows, dim, scale, p, key, val, grad, part, grad_table, st)));
 }
 

@@ -314,7 +314,7 @@ __global__ __launch_bounds__(C::THREADS, C::THREADS == 512 ? 2 : 1) void k_ce_fw
   DGNN_RING(lds, G::BYTES);
   __shared__ float sm[C::WM][C::BN], ss[C::WM][C::BN], zl[C::BN];
   const int rows = rows_of(a);
-  const TileAt tile = tile_at(blockIdx.x, (a.classes + C::BM - 1) / C::BM, (rows + C::BN - 1) / C::BN);
+  const TileAt tile = tile_at(group_in_rows(), (a.classes + C::BM - 1) / C::BM, (rows + C::BN - 1) / C::BN);
   if (tile.n < 0) return;
   const int v0 = tile.m * C::BM, r0 = tile.n * C::BN;
   acc16 acc[C::MB][C::NB];
@@ -496,7 +496,7 @@ __global__ __launch_bounds__(C::THREADS, C::THREADS == 512 ? 2 : 1) void k_ce_dz
   static_assert(32 * C::BM * sizeof(T) <= G::BYTES && C::WN <= 4, "the tile as rows fits the ring");
   DGNN_RING(lds, G::BYTES);
   const int rows = rows_of(a);
-  const TileAt tile = tile_at(blockIdx.x, a.ldz / C::BM, (rows + C::BN - 1) / C::BN);
+  const TileAt tile = tile_at(group_in_rows(), a.ldz / C::BM, (rows + C::BN - 1) / C::BN);
   if (tile.n < 0) return;
   const int p0 = tile.m * C::BM, v0 = a.v0 + p0, r0 = tile.n * C::BN;
   acc16 acc[C::MB][C::NB];
@@ -556,9 +556,10 @@ __global__ __launch_bounds__(C::THREADS, C::THREADS == 512 ? 2 : 1) void k_ce_dx
   using G = Gemm<T, C, false, true>;
   DGNN_RING(lds, G::BYTES);
   const int rows = rows_of(a), ms = (a.dk + C::BM - 1) / C::BM, ns = (rows + C::BN - 1) / C::BN;
-  const int split = ns > 0 ? blockIdx.x / (ms * ns) : a.splits;
+  const unsigned id = group_in_rows();
+  const int split = ns > 0 ? id / (unsigned)(ms * ns) : a.splits;
   if (split >= a.splits) return;
-  const TileAt tile = tile_at(blockIdx.x % (ms * ns), ms, ns);
+  const TileAt tile = tile_at(id % (unsigned)(ms * ns), ms, ns);
   const int c0 = tile.m * C::BM, r0 = tile.n * C::BN;
   const int lane = lane_id(), h = lane >> 5, wave = uniform_i32(wave_in_block());
   const int m0 = c0 + wave / C::WN * (C::BM / C::WM), n0 = wave % C::WN * (C::BN / C::WN);
@@ -609,8 +610,10 @@ __global__ __launch_bounds__(C::THREADS, C::THREADS == 512 ? 2 : 1) void k_ce_dw
   using G = Gemm<T, C, false, false>;
   DGNN_RING(lds, G::BYTES);
   const int ms = (a.dk + C::BM - 1) / C::BM, ns = (a.vn + C::BN - 1) / C::BN;
-  const int split = blockIdx.x / (ms * ns);
-  const TileAt tile = tile_at(blockIdx.x % (ms * ns), ms, ns);
+  const unsigned id = group_in_rows();
+  const int split = id / (unsigned)(ms * ns);
+  if (split >= a.splits) return;
+  const TileAt tile = tile_at(id % (unsigned)(ms * ns), ms, ns);
   const int c0 = tile.m * C::BM, p0 = tile.n * C::BN;
   const int rows = rows_of(a);
   acc16 acc[C::MB][C::NB];
@@ -778,7 +781,7 @@ static int ce_prepare(const CePlan &p, int n, int classes, int d, bool all, bool
   do {                                                                                                         \
     const long long grid_ = (long long)ceil_div(ms, C::BM) * ceil_div(ns, C::BN) * (splits);                    \
     if (grid_ > 0x7fffffffLL) return DGNN_ERR_UNSUPPORTED;                                                     \
-    hipLaunchKernelGGL((KERNEL<T, C>), dim3((unsigned)grid_), dim3(C::THREADS), 0, st, __VA_ARGS__);           \
+    hipLaunchKernelGGL((KERNEL<T, C>), grid_in_rows(grid_), dim3(C::THREADS), 0, st, __VA_ARGS__);           \
     DGNN_LAUNCH_CHECK();                                                                                       \
   } while (0)
 

@@ -35,7 +35,7 @@ extern "C" {
 #define DGNN_ERR_BAD_ARG (-1)       /* negative size, NULL where a tensor is required     */
 #define DGNN_ERR_UNSUPPORTED (-2)   /* shape outside what the kernels implement           */
 #define DGNN_ERR_WORKSPACE (-3)     /* workspace NULL or smaller than *_workspace_bytes() */
-#define DGNN_ERR_ALIGNMENT (-4)     /* a pointer is not 4-byte aligned                    */
+#define DGNN_ERR_ALIGNMENT (-4)     /* a pointer is not aligned: to 4 bytes, or as the sequence operators ask */
 #define DGNN_ERR_TOO_LARGE (-5)     /* beyond the static scratch of dgnn_gat_forward_noalloc */
 
 /* element types of the dense operators */
@@ -492,15 +492,18 @@ int dgnn_gat_epilogue_backward(int n, int hf, int activation, float act_param, c
  * No counterpart in the reference.  Node-id embedding, attention of every node to every node of its
  * own graph (or walk, or prompt), and a cross entropy over many classes: what a model on sequences of
  * nodes trains with next to the sparse operators above.  Tensors are DGNN_F32, DGNN_BF16 or
- * DGNN_F16 (all of one call alike); sums, softmax statistics and losses are float. */
+ * DGNN_F16 (all of one call alike); sums, softmax statistics and losses are float.  Alignment: every tensor to its
+ * elements; attention's tensors and all workspaces to 16 bytes.  DGNN_ERR_UNSUPPORTED is answered before anything is
+ * launched, also where a launch would have 2^32 work items or more in a dimension. */
 
 /* out[i,:] = scale * table[ids[i],:]; table [rows,dim], out [n,dim], contiguous, any dim.  ids int32
- * (idx_bytes 4) or int64 (8); an id outside [0, rows) names no row: zeros out, no gradient. */
+ * (idx_bytes 4) or int64 (8); an id outside [0, rows) names no row: zeros out, no gradient.  dim > 2^30:
+ * DGNN_ERR_UNSUPPORTED. */
 int dgnn_embedding_forward(int dtype, int idx_bytes, int n, int rows, int dim, float scale, const void *ids,
                            const void *table, void *out, void *stream);
 /* grad_table [rows,dim] = scale * sum of grad[i,:] over the i that name the row, in ascending i; fully
  * written (rows nobody names: zeros).  Deterministic: a stable sort of the ids, no float atomics.
- * n > 2^30: DGNN_ERR_UNSUPPORTED. */
+ * DGNN_ERR_UNSUPPORTED: n > 2^30, or dim of 65535 x 64 accesses and more (4 million elements of 2 bytes at the narrowest). */
 size_t dgnn_embedding_backward_workspace_bytes(int n, int rows, int dim);
 int dgnn_embedding_backward(int dtype, int idx_bytes, int n, int rows, int dim, float scale, const void *ids,
                             const void *grad, void *grad_table, void *workspace, size_t workspace_bytes, void *stream);
@@ -516,7 +519,8 @@ int dgnn_embedding_backward(int dtype, int idx_bytes, int n, int rows, int dim, 
  * last sequence -- gives out = 0, lse = -inf and has no gradient; rows no sequence holds are never read.
  * strides: HOST array {q_token, q_head, k_token, k_head, v_token, v_head} in elements, the last
  * dimension contiguous.  DGNN_ERR_UNSUPPORTED: d > 128, or rows that are not whole 16-byte chunks (d and
- * every stride), or a token stride under d or of 16 MB and more.  The other tensors are contiguous. */
+ * every stride), or a token stride under d or of 16 MB and more, or tq hq or tk hk of 2^31, or about 2^24 tiles of 128
+ * rows (tq hq / 128 + nseq hk, and the same of the keys).  The other tensors are contiguous. */
 size_t dgnn_attn_forward_workspace_bytes(int nseq, int tq, int tk, int hq, int hk, int d);
 int dgnn_attn_forward(int dtype, int nseq, int tq, int tk, int hq, int hk, int d, int causal, float scale,
                       const void *q, const void *k, const void *v, const long long *strides, const int *row_ptr,
@@ -537,7 +541,7 @@ int dgnn_attn_backward(int dtype, int nseq, int tq, int tk, int hq, int hk, int 
  *   lse [2,n]: log of the softmax's sum and what its rounding to float took (0 for rows without a label), kept for
  *   the backward (ABI 3; [n] before)
  * backward: grad is d / d loss, [n] for reduction 0, else [1]; dx [n,d] and dw [classes,d], either may be NULL.
- * Limits: n <= 2^22, d <= 65536, classes <= 2^30 (DGNN_ERR_UNSUPPORTED). */
+ * Limits: n <= 2^22, d <= 65536, classes <= 2^30, n classes <= 2^44 (DGNN_ERR_UNSUPPORTED). */
 size_t dgnn_linear_ce_workspace_bytes(int dtype, int n, int classes, int d, int backward);
 int dgnn_linear_ce_forward(int dtype, int label_bytes, int n, int classes, int d, long long ignore_index, int reduction,
                            const void *x, const void *w, const void *label, float *loss, float *lse, void *workspace,
