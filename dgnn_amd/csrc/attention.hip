@@ -442,8 +442,10 @@ __global__ __launch_bounds__(DGNN_BLOCK) void k_attn_join(const AttnArgs a) {
 // More rows, but tiles of them for less than half of 512 workgroups: the keys of every tile are split into parts of
 // at least 512, by as many as fill those, and joined by k_attn_merge.  Split and unsplit: 4 x 64 rows against 16384
 // keys, 32 / 8 heads of 128, causal, bfloat16, 143 and 317 us; 512 rows against as many 194 and 313; 2 x 40 rows
-// against 3000 keys, 4 heads of 64, float 55 and 263 us; 2048 x 2048, 8 heads of 64, bfloat16 33 and 33, causal 31
-// and 33 (in three parts 36 and 30, 1024 workgroups 43 and 38).
+// against 3000 keys, 4 heads of 64, float 55 and 263 us; 1200 x 1200, 4 heads of 128, float 96 and 166; 1100 x 1100, 2 heads of
+// 64, bfloat16 15.3 and 19.6; but 3 x 1024 rows, 4 heads of 64, float16 20.6 and 18.3.  Three parts of many rows
+// would make a round and a half of workgroups, two are taken (two and three): 1900 x 1900, 8 heads of 32, float 50 and 60
+// us; 2048 x 2048, 8 / 2 heads of 64, float 94 and 111, 8 heads of 64, bfloat16 31.6 and 34.9, causal 30.0 and 28.5.
 struct AttnPlan {
   int few, chunk;                       // split: rows kept in parts, keys of a chunk (few = 0: not split)
   int splits;                           // tiles of rows: into how many parts the keys are split
@@ -459,7 +461,7 @@ static AttnPlan attn_plan(int nseq, int tq, int tk, int hq, int hk, int d) {
     const long long tiles = ((long long)tq * g / 128 + nseq) * hk;
     long long s = 512 / tiles;
     if (s > keys / 512) s = keys / 512;
-    if (s < 4 && rows > 128 && s > keys / 1024) s = keys / 1024;     // many rows: writing the parts costs more
+    if (s == 3 && rows > 128) s = 2;      // three parts are a round and a half of workgroups
     p.splits = (int)(s < 1 ? 1 : s > 16 ? 16 : s);
     if (p.splits > 1) p.bytes = sizeof(float) * (size_t)p.splits * tq * hq * (d + 4);
     return p;
