@@ -226,8 +226,8 @@ __global__ __launch_bounds__(DGNN_BLOCK) void k_attn_bwd_join(const AttnArgs a) 
   *(vec4<T> *)((T *)(c < a.d ? a.dk : a.dv) + row * a.d + (c < a.d ? c : c - a.d)) = o;
 }
 
-// The same with the sides changed, as the forward: a lane has one packed query row.  At the sizes above 0.40 - 0.48 ms,
-// 0.74 ms (1010 TFLOP/s) and 41 us.  It runs first and leaves {lse log2(e), <do, o>} of every row for the
+// The same with the sides changed, as the forward: a lane has one packed query row.  At the sizes above 0.40 - 0.49 ms,
+// 0.74 - 0.79 ms (950 - 1010 TFLOP/s) and 45 us.  It runs first and leaves {lse log2(e), <do, o>} of every row for the
 // other: a kernel of its own for them read grad a second time, 35 to 48 us of the first two steps, 9 of the last.
 template <class T, int DP, int NW, int HW, int S>
 __global__ __launch_bounds__(64 * NW * HW, sizeof(T) == 2 ? 2 : 1) void k_attn_bwd_q(const AttnArgs a) {

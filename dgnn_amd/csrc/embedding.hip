@@ -327,8 +327,9 @@ constexpr int EMBED_ROWS = 256;      // most rows of the table a workgroup write
 // A workgroup writes `per_block` consecutive rows.  It finds the sorted positions that name them, marks
 // where each row's run begins and ends, stores zeros to the rows without one as one stream of pieces, and
 // gives every other row to `lanes` threads.  A table larger than the 256 MB of cache (PAST) is written around it, so
-// that keys and gradients stay in: 2.4 million rows of 100 floats, of which few are named, 203 us, 5.2 TB/s,
-// against 231, and the kernels next to it find more in the caches (the whole step 302 and 339 us).  50000 rows of 1024 bfloat16 63 us, 3.7 TB/s: the runs there are a few positions long, each a
+// that keys and gradients stay in: 2.4 million rows of 100 floats, of which few are named, 209 us, 5.1 TB/s
+// (around the cache or not: 203 and 231 before the join in double, the whole step 302 and 339 us, since the kernels next to it
+// find more there).  50000 rows of 1024 bfloat16 63 us, 3.7 TB/s: the runs there are a few positions long, each a
 // wait of its own.
 template <class T, int N, bool PAST>
 __global__ __launch_bounds__(DGNN_BLOCK) void k_embed_rows(int n, int rows, int dim, int lanes, int per_block, int run, float scale,
@@ -386,7 +387,7 @@ __global__ __launch_bounds__(DGNN_BLOCK) void k_embed_rows(int n, int rows, int 
       } else {
         // in double: the pieces of a long run are many (4 sqrt(n) of them if one id is all there is), of like size, and
         // each rounding in float would go the same way (2^20 ids, one row, gradients of 0.1: 4e-5 off).  Four at a time are
-        // joined in float first: eight doubled rows in flight take the registers of two waves a SIMD (step above 343 us)
+        // joined in float first: eight doubled rows in flight take the registers of two waves a SIMD (the step of 309 us takes 343)
         const int q0 = s / run, q1 = (e - 1) / run;
         auto at = [&](int q) { return part + (long long)(2 * q + (q == q0 && s != q * run ? 1 : 0)) * dim + c; };
         double sum[N];

@@ -129,7 +129,8 @@ __device__ __forceinline__ TileAt tile_at(unsigned id, int ms, int ns) {
 
 // Tile shapes.  Wide: 16-bit types with enough tiles for every compute unit; two waves a SIMD, 128 KB of
 // LDS.  Thin: at most 32 rows, bound by reading the weight (8 x 50000 x 1024 float 55 us, Plain 136; bfloat16 28
-// both).  Narrow: at most 64 classes (4096 x 41 x 64 float 8.7 us, Plain 14.3; 65536 x 64 x 256 bfloat16 97 and 104).
+// both).  Narrow: at most 64 classes (4096 x 41 x 64 float 5.4 us, Plain 11.0;
+// 65536 x 64 x 256 bfloat16, both directions, 235 and 260).
 // Plain: the rest, and float, whose matrix instructions are sixteen times slower and bound every shape.
 using Wide = Shape<256, 256, 32, 2, 4, 4>;
 template <class T> using Plain = Shape<128, 128, sizeof(T) == 2 ? 64 : 16, 2, 2, sizeof(T) == 2 ? 2 : 3>;
@@ -689,8 +690,8 @@ static CePlan ce_plan(int dtype, int n, int classes, int d, const void *x, const
   // rows are read where they are if they are whole, aligned chunks within 32-bit offsets
   p.copy_w = p.dk != d || ((uintptr_t)w & 15) != 0;
   p.gather = p.dk != d || ((uintptr_t)x & 15) != 0 || (long long)n * p.dk * size >= 0x7fffffffLL;
-  // up to about 1e9 operations finding the labelled rows costs more than scoring all: 4096 x 41 x 64 float 8.7 us
-  // against 19, 1024 x 1000 x 256 bfloat16 14.6 against 19.5; 4096 x 1000 x 128 float 30.4 both
+  // up to about 1e9 operations finding the labelled rows costs more than scoring all: 4096 x 41 x 64 float 5.4 us
+  // against 16.9, 1024 x 1000 x 256 bfloat16 12.2 against 16.7; 4096 x 1000 x 128 float 27.2 both
   p.all = !p.gather && 2.0 * n * classes * d <= 1e9;
   p.z = classes <= 64 ? CE_NARROW : n <= 32 ? CE_THIN : ce_shape(dtype, classes, n);
   const int class_tile = p.z == CE_NARROW ? 64 : p.z == CE_PLAIN ? 128 : 256;
