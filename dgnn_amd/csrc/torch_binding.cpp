@@ -1054,7 +1054,9 @@ AttnCall attn_call(const Tensor &q, const Tensor &k, const Tensor &v, const Tens
   Tensor *to[3] = {&c.q, &c.k, &c.v};
   for (int i = 0; i < 3; ++i) {
     *to[i] = rows_readable(*in[i], vec) ? *in[i] : padded(*in[i], c.width);
-    c.strides[2 * i] = to[i]->stride(0), c.strides[2 * i + 1] = to[i]->stride(1);
+    // (no rows: strides of the padded width, which the C entry checks whatever they lead to)
+    const bool none = to[i]->numel() == 0;
+    c.strides[2 * i] = none ? to[i]->size(1) * c.width : to[i]->stride(0), c.strides[2 * i + 1] = none ? c.width : to[i]->stride(1);
   }
   return c;
 }

@@ -116,6 +116,20 @@ def test_rows_that_see_no_key(lq, lk, hq, hk, dtype):
         assert not out[blind].any() and not dq[blind].any()
 
 
+@pytest.mark.parametrize("dtype", DTYPES, ids=ids_of)
+@pytest.mark.parametrize("d", [1, 7, 64, 127])
+@pytest.mark.parametrize("tq,tk", [(0, 0), (5, 0), (300, 0), (0, 5), (0, 700)])
+def test_attention_without_rows_or_keys(tq, tk, d, dtype):
+    """Tensors of no rows at all, at head dims that are padded elsewhere: zeros, and gradients of zero."""
+    leaves = [torch.randn(t, h, d, device=DEV).to(dtype).requires_grad_() for t, h in ((tq, 4), (tk, 2), (tk, 2))]
+    for row_off, col_off in (([0, tq], [0, tk]), ([0], [0]), ([0, 0, tq], [0, tk, tk])):
+        ptr = [torch.tensor(o, dtype=torch.int32, device=DEV) for o in (row_off, col_off)]
+        out = PackedAttentionFuse(*leaves, *ptr, causal=len(row_off) == 3)
+        assert out.shape == (tq, 4, d) and not out.any()
+        for g, leaf in zip(torch.autograd.grad(out, leaves, torch.ones_like(out)), leaves):
+            assert g.shape == leaf.shape and not g.any()
+
+
 # ------------------------------------------------------------------------------------ loss
 @pytest.mark.parametrize("dtype", DTYPES, ids=ids_of)
 @pytest.mark.parametrize("top", [50.0, 400.0, -272.0])
