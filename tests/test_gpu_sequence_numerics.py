@@ -130,6 +130,24 @@ def test_attention_without_rows_or_keys(tq, tk, d, dtype):
             assert g.shape == leaf.shape and not g.any()
 
 
+@pytest.mark.parametrize("dtype", DTYPES, ids=ids_of)
+@pytest.mark.parametrize("singles,rows,keys,hq,hk", [(40, 600, 700, 2, 2), (9, 700, 600, 8, 2), (120, 300, 300, 1, 1)])
+def test_attention_of_prompts_and_single_tokens(singles, rows, keys, hq, hk, dtype):
+    """One call with both: whichever way the whole batch is worked on, every sequence is right."""
+    gen = torch.Generator().manual_seed(singles)
+    lq, lk = [1] * singles, [keys - 7 * (i % 30) for i in range(singles)]
+    lq.insert(singles // 2, rows), lk.insert(singles // 2, keys)
+    d, q_off, k_off = 32, offsets(lq), offsets(lk)
+    q, k, v, grad = (torch.randn(t, h, d, generator=gen).to(dtype) for t, h in
+                     ((q_off[-1], hq), (k_off[-1], hk), (k_off[-1], hk), (q_off[-1], hq)))
+    want = ref.attention(q, k, v, q_off, k_off, True, d ** -0.5, grad)
+    leaves = [t.to(DEV).requires_grad_() for t in (q, k, v)]
+    out = PackedAttentionFuse(*leaves, *(torch.tensor(o, dtype=torch.int32, device=DEV) for o in (q_off, k_off)), causal=True)
+    ref.check(out, want["out"], "out")
+    for name, x in zip(("dq", "dk", "dv"), torch.autograd.grad(out, leaves, grad.to(DEV))):
+        ref.check(x, want[name], name)
+
+
 # ------------------------------------------------------------------------------------ loss
 @pytest.mark.parametrize("dtype", DTYPES, ids=ids_of)
 @pytest.mark.parametrize("top", [50.0, 400.0, -272.0])
